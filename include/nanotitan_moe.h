@@ -295,6 +295,104 @@ int nt_router_linear_backward_mixed(int x_dtype, int dx_dtype, const void* x, co
                                     int64_t d, void* dx, float* dW, void* ws, size_t ws_bytes,
                                     hipStream_t stream);
 
+/* ---------------------------------------------------------------- few tokens */
+
+/* A whole MoE layer for T <= NT_FEW_TOKENS_MAX tokens (a decode step): router,
+ * top-k, experts and gate-weighted sum.
+ *   logits = x @ router^T, or given (exactly one of router [E,d] f32 and
+ *   logits [T,E] f32); gates and topk [T,k] as nt_route_topk gives them;
+ *   out[t] = sum_j gates[t,j] * act(x[t] @ w_up[e]) @ w_down[e], e = topk[t,j],
+ * act = silu(x @ w_up[e]) * (x @ w_val[e]), or the erf GELU where w_val is NULL.
+ * x, out [T,d], w_up, w_val [E,d,f], w_down [E,f,d] of dtype (f32, f16, bf16);
+ * the hidden values are rounded to dtype, everything else is float32 up to the
+ * one rounding of out. k <= 32, E <= NT_MAX_EXPERTS. The workspace (16-byte
+ * aligned, contents arbitrary) is written before it is read: calls that cannot
+ * overlap may share one. Replaces, for few tokens, the dataflow of reference
+ * src/model/cuda_backend.py:17-81. */
+#define NT_FEW_TOKENS_MAX 64
+size_t nt_moe_few_tokens_workspace_bytes(int dtype, int64_t T, int32_t E, int32_t k, int64_t d,
+                                         int64_t f);
+int nt_moe_few_tokens(int dtype, const void* x, const float* router, const float* logits,
+                      const void* w_up, const void* w_val, const void* w_down, int64_t T,
+                      int32_t E, int32_t k, int64_t d, int64_t f, float* gates, int32_t* topk,
+                      void* out, void* ws, size_t ws_bytes, hipStream_t stream);
+
+/* ------------------------------------------------------- 8-bit checkpoints */
+
+/* Activations kept in 8 bits for the backward. 32 consecutive columns of a
+ * row (fewer at its end) share a power of two 2^x, x the least integer >= -127
+ * with max|v| < 127.5 * 2^x: codes [rows,f] = the integers nearest to v * 2^-x
+ * (ties to even), exps [rows, nt_checkpoint8_blocks(f)] = x + 127. A block that
+ * holds an infinity or a NaN has exponent 255 and decodes to NaN. x is f32, f16
+ * or bf16; decoding is exact in the type that was kept, but for a value that
+ * rounds past the type's largest: it decodes to that. No counterpart in the
+ * reference, which keeps activations as they are. */
+int64_t nt_checkpoint8_blocks(int64_t f);
+int nt_checkpoint8(int dtype, const void* x, int64_t rows, int64_t f, int8_t* codes,
+                   uint8_t* exps, hipStream_t stream);
+int nt_checkpoint8_decode(int dtype, const int8_t* codes, const uint8_t* exps, int64_t rows,
+                          int64_t f, void* x, hipStream_t stream);
+
+/* act = gelu(h) (erf) and h's checkpoint; and the backward at the values h^
+ * that the checkpoint holds: dh = dact * gelu'(h^), act = gelu(h^) (NULL to
+ * skip). The forward keeps nothing where codes and exps are NULL. dh may
+ * overwrite dact. */
+int nt_gelu_checkpoint8(int dtype, const void* h, int64_t rows, int64_t f, void* act,
+                        int8_t* codes, uint8_t* exps, hipStream_t stream);
+int nt_gelu_backward8(int dtype, const void* dact, const int8_t* codes, const uint8_t* exps,
+                      int64_t rows, int64_t f, void* dh, void* act, hipStream_t stream);
+
+/* hidden = silu(gate) * value and both checkpoints; and the backward at the
+ * values that they hold: dgate = dhidden * value^ * silu'(gate^), dvalue =
+ * dhidden * silu(gate^), hidden = silu(gate^) * value^ (NULL to skip). The
+ * forward keeps nothing where all codes and exps are NULL. dgate or dvalue may
+ * overwrite dhidden. */
+int nt_swiglu_checkpoint8(int dtype, const void* gate, const void* value, int64_t rows, int64_t f,
+                          void* hidden, int8_t* gate_codes, uint8_t* gate_exps,
+                          int8_t* value_codes, uint8_t* value_exps, hipStream_t stream);
+int nt_swiglu_backward8(int dtype, const void* dhidden, const int8_t* gate_codes,
+                        const uint8_t* gate_exps, const int8_t* value_codes,
+                        const uint8_t* value_exps, int64_t rows, int64_t f, void* dgate,
+                        void* dvalue, void* hidden, hipStream_t stream);
+
+/* --------------------------------------------------------------- block norms */
+
+/* Norms before and after a block, with its gate and residual scale.
+ *   rms:   N(v) = v r w,            r = 1 / sqrt(mean v^2 + eps)
+ *   layer: N(v) = (v - mean v) r w + b, r = 1 / sqrt(var v + eps)
+ *   p = N(y; w, b) (p = y where w is NULL),  h = x + scale * gate * p,
+ *   n = N(h; w_next, b_next) of h as stored (not computed where w_next is NULL).
+ * x, h [T,d] of x_dtype (f32, or dtype); y, n [T,d] and gate [T,gate_cols]
+ * (gate_cols 1 or d) of dtype (f32, f16, bf16); w, b, w_next, b_next [d] and
+ * scale [scale_cols] (1 or d) of param_dtype (f32, f16, bf16). gate, scale, b
+ * and b_next may be NULL (1, 1, 0, 0); rms norms take no bias. y NULL: h is x
+ * and not written, n = N(x). stats [T,4] f32 keeps the rows' means and r for
+ * the backward (NULL to skip). d <= 16384. Arithmetic in float32. n may
+ * overwrite y, and h may overwrite x. No counterpart in the reference, whose
+ * layer calls torch's LayerNorm before the block (src/model/model.py:205-211). */
+enum nt_norm_kind { NT_NORM_RMS = 0, NT_NORM_LAYER = 1 };
+int nt_block_norm(int x_dtype, int dtype, int param_dtype, int kind, const void* x, const void* y,
+                  const void* w, const void* b, const void* gate, int64_t gate_cols,
+                  const void* scale, int64_t scale_cols, const void* w_next, const void* b_next,
+                  float eps, int64_t T, int64_t d, void* h, void* n, float* stats,
+                  hipStream_t stream);
+
+/* Gradients of nt_block_norm. h is the forward's h (its x where y is NULL),
+ * dh [T,d] of x_dtype and dn [T,d] of dtype the outputs' gradients (NULL:
+ * zero). Each output may be NULL: dx [T,d] of x_dtype, dy [T,d] and dgate
+ * [T,gate_cols] of dtype, dscale, dw, db, dw_next, db_next like their
+ * parameters. The parameters' gradients are summed over the tokens in
+ * float32, in an order that the sizes alone fix, through the workspace (none
+ * is needed without them). T = 0 writes their zeros. */
+size_t nt_block_norm_backward_workspace_bytes(int64_t T, int64_t d);
+int nt_block_norm_backward(int x_dtype, int dtype, int param_dtype, int kind, const void* h,
+                           const void* y, const void* w, const void* b, const void* gate,
+                           int64_t gate_cols, const void* scale, int64_t scale_cols,
+                           const void* w_next, const float* stats, const void* dh, const void* dn,
+                           int64_t T, int64_t d, void* dx, void* dy, void* dgate, void* dscale,
+                           void* dw, void* db, void* dw_next, void* db_next, void* ws,
+                           size_t ws_bytes, hipStream_t stream);
+
 /* ------------------------------------------------------------- grouped GEMM */
 
 /* Workspace for nt_grouped_gemm_dw and the paired dW + dX calls with these

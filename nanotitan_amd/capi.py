@@ -24,6 +24,8 @@ NT_ERR_LAUNCH = 5
 NT_ERR_TOO_LARGE = 6
 NT_ERR_SCRATCH = 7
 NT_MAX_EXPERTS = 1024
+NT_FEW_TOKENS_MAX = 64
+NT_NORM_RMS, NT_NORM_LAYER = 0, 1
 NT_NOALLOC_SCRATCH_BYTES = 4 << 20
 
 _P = c_void_p  # any device pointer, hipStream_t included
@@ -112,6 +114,39 @@ EXPORTS: dict[str, tuple[object, list[object]]] = {
     "nt_router_linear_backward_mixed": (
         c_int,
         [c_int, c_int, _P, _P, _P, _P, c_int64, c_int32, c_int64, _P, _P, _P, c_size_t, _P],
+    ),
+    "nt_moe_few_tokens_workspace_bytes": (
+        c_size_t,
+        [c_int, c_int64, c_int32, c_int32, c_int64, c_int64],
+    ),
+    "nt_moe_few_tokens": (
+        c_int,
+        [c_int, _P, _P, _P, _P, _P, _P, c_int64, c_int32, c_int32, c_int64, c_int64, _P, _P, _P,
+         _P, c_size_t, _P],
+    ),
+    "nt_checkpoint8_blocks": (c_int64, [c_int64]),
+    "nt_checkpoint8": (c_int, [c_int, _P, c_int64, c_int64, _P, _P, _P]),
+    "nt_checkpoint8_decode": (c_int, [c_int, _P, _P, c_int64, c_int64, _P, _P]),
+    "nt_gelu_checkpoint8": (c_int, [c_int, _P, c_int64, c_int64, _P, _P, _P, _P]),
+    "nt_gelu_backward8": (c_int, [c_int, _P, _P, _P, c_int64, c_int64, _P, _P, _P]),
+    "nt_swiglu_checkpoint8": (
+        c_int,
+        [c_int, _P, _P, c_int64, c_int64, _P, _P, _P, _P, _P, _P],
+    ),
+    "nt_swiglu_backward8": (
+        c_int,
+        [c_int, _P, _P, _P, _P, _P, c_int64, c_int64, _P, _P, _P, _P],
+    ),
+    "nt_block_norm": (
+        c_int,
+        [c_int, c_int, c_int, c_int, _P, _P, _P, _P, _P, c_int64, _P, c_int64, _P, _P, c_float,
+         c_int64, c_int64, _P, _P, _P, _P],
+    ),
+    "nt_block_norm_backward_workspace_bytes": (c_size_t, [c_int64, c_int64]),
+    "nt_block_norm_backward": (
+        c_int,
+        [c_int, c_int, c_int, c_int, _P, _P, _P, _P, _P, c_int64, _P, c_int64, _P, _P, _P, _P,
+         c_int64, c_int64, _P, _P, _P, _P, _P, _P, _P, _P, _P, c_size_t, _P],
     ),
     "nt_grouped_gemm_workspace_bytes": (c_size_t, [c_int, c_int32, c_int64, c_int64, c_int64]),
     "nt_grouped_gemm_tail_workspace_bytes": (

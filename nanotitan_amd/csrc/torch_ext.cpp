@@ -873,6 +873,302 @@ std::tuple<c10::optional<Tensor>, c10::optional<Tensor>> router_linear_backward(
   return {dx, dW};
 }
 
+// ------------------------------------------- few tokens, norms, checkpoints
+
+const float* f32_or_null(const c10::optional<Tensor>& t) {
+  return t ? t->data_ptr<float>() : nullptr;
+}
+const void* ptr_or_null(const c10::optional<Tensor>& t) { return t ? t->data_ptr() : nullptr; }
+void* out_or_null(const c10::optional<Tensor>& t) { return t ? t->data_ptr() : nullptr; }
+
+// moe_few_tokens(x, w_up, w_val, w_down, top_k, router, logits) -> (out, gates,
+// topk): a whole MoE layer for at most NT_FEW_TOKENS_MAX tokens.
+std::tuple<Tensor, Tensor, Tensor> moe_few_tokens(Tensor x, Tensor w_up,
+                                                  c10::optional<Tensor> w_val, Tensor w_down,
+                                                  int64_t top_k, c10::optional<Tensor> router,
+                                                  c10::optional<Tensor> logits) {
+  check_device(x, "x");
+  check_same_device(x, {&w_up, &w_down});
+  TORCH_CHECK(x.dim() == 2 && w_up.dim() == 3 && w_up.size(1) == x.size(1),
+              "expected x [T,d] and up weights [E,d,f]");
+  const int64_t T = x.size(0), d = x.size(1), E = w_up.size(0), f = w_up.size(2);
+  TORCH_CHECK(w_down.dim() == 3 && w_down.size(0) == E && w_down.size(1) == f &&
+                  w_down.size(2) == d, "expected down weights [E,f,d]");
+  TORCH_CHECK(x.is_contiguous() && w_up.is_contiguous() && w_down.is_contiguous(),
+              "inputs must be contiguous");
+  TORCH_CHECK(w_up.scalar_type() == x.scalar_type() && w_down.scalar_type() == x.scalar_type(),
+              "x and the weights must share a dtype");
+  if (w_val) {
+    check_same_device(x, {&*w_val});
+    TORCH_CHECK(w_val->sizes() == w_up.sizes() && w_val->is_contiguous() &&
+                    w_val->scalar_type() == x.scalar_type(),
+                "gate and value weights must be alike");
+  }
+  TORCH_CHECK(router.has_value() != logits.has_value(),
+              "exactly one of the router's weight and logits is needed");
+  const Tensor& r = router ? *router : *logits;
+  check_f32(r, router ? "router weight" : "logits");
+  check_same_device(x, {&r});
+  TORCH_CHECK(r.is_contiguous() && r.dim() == 2 && r.size(0) == (router ? E : T) &&
+                  r.size(1) == (router ? d : E),
+              "expected a contiguous router weight [E,d] or logits [T,E]");
+  TORCH_CHECK(T <= NT_FEW_TOKENS_MAX, "at most ", NT_FEW_TOKENS_MAX, " tokens, got ", T);
+  TORCH_CHECK(top_k >= 1 && top_k <= E, "top_k must be in [1, num_experts]");
+  c10::hip::HIPGuard guard(x.get_device());
+  Tensor out = at::empty_like(x);
+  Tensor gates = at::empty({T, top_k}, x.options().dtype(at::kFloat));
+  Tensor topk = at::empty({T, top_k}, x.options().dtype(at::kInt));
+  const int dt = dtype_code(x);
+  Tensor ws = workspace(
+      x, nt_moe_few_tokens_workspace_bytes(dt, T, (int32_t)E, (int32_t)top_k, d, f));
+  check_status(nt_moe_few_tokens(dt, x.data_ptr(), f32_or_null(router), f32_or_null(logits),
+                                 w_up.data_ptr(), ptr_or_null(w_val), w_down.data_ptr(), T,
+                                 (int32_t)E, (int32_t)top_k, d, f, gates.data_ptr<float>(),
+                                 topk.data_ptr<int32_t>(), out.data_ptr(), ws.data_ptr(),
+                                 ws.numel(), stream_of(x)),
+               "moe_few_tokens");
+  return {out, gates, topk};
+}
+
+// What block_norm and its backward share: shapes, types and devices.
+struct NormShape {
+  int64_t T, d, gate_cols, scale_cols;
+  int x_dtype, dtype, param;
+};
+NormShape check_norm(const Tensor& x, const c10::optional<Tensor>& y,
+                     std::initializer_list<const c10::optional<Tensor>*> params,
+                     const c10::optional<Tensor>& gate, const c10::optional<Tensor>& scale,
+                     at::ScalarType n_dtype) {
+  check_device(x, "x");
+  TORCH_CHECK(x.dim() == 2 && x.is_contiguous(), "x must be a contiguous [T,d]");
+  NormShape s = {x.size(0), x.size(1), 0, 0, dtype_code(x), dtype_code(n_dtype), -1};
+  TORCH_CHECK(s.d >= 1, "x must have at least one column");
+  auto param = [&](const Tensor& t) {
+    check_same_device(x, {&t});
+    const int code = dtype_code(t);
+    TORCH_CHECK(s.param < 0 || s.param == code, "the norms' parameters must share a dtype");
+    s.param = code;
+  };
+  if (y) {
+    check_same_device(x, {&*y});
+    TORCH_CHECK(y->sizes() == x.sizes() && y->is_contiguous(), "y must be contiguous, like x");
+    TORCH_CHECK(y->scalar_type() == n_dtype, "y must be of the block's dtype");
+  }
+  for (const auto* p : params) {
+    if (!p->has_value()) continue;
+    param(**p);
+    TORCH_CHECK((*p)->dim() == 1 && (*p)->numel() == s.d && (*p)->is_contiguous(),
+                "weights and biases must be contiguous [d]");
+  }
+  if (gate) {
+    check_same_device(x, {&*gate});
+    TORCH_CHECK(gate->dim() == 2 && gate->size(0) == s.T && gate->is_contiguous() &&
+                    (gate->size(1) == 1 || gate->size(1) == s.d) &&
+                    gate->scalar_type() == n_dtype,
+                "gate must be a contiguous [T,d] or [T,1] of the block's dtype");
+    s.gate_cols = gate->size(1);
+  }
+  if (scale) {
+    param(*scale);
+    TORCH_CHECK((scale->numel() == 1 || scale->numel() == s.d) && scale->is_contiguous(),
+                "scale must be contiguous, of one value or [d]");
+    s.scale_cols = scale->numel();
+  }
+  if (s.param < 0) s.param = NT_F32;
+  return s;
+}
+
+// block_norm(x, y, w, b, gate, scale, w_next, b_next, layer, eps, dtype, keep) ->
+// (h, n, stats): h without y, n without w_next and stats without keep are None.
+std::tuple<c10::optional<Tensor>, c10::optional<Tensor>, c10::optional<Tensor>> block_norm(
+    Tensor x, c10::optional<Tensor> y, c10::optional<Tensor> w, c10::optional<Tensor> b,
+    c10::optional<Tensor> gate, c10::optional<Tensor> scale, c10::optional<Tensor> w_next,
+    c10::optional<Tensor> b_next, bool layer, double eps, c10::optional<at::ScalarType> dtype,
+    bool keep) {
+  const at::ScalarType nt = y ? y->scalar_type() : dtype.value_or(x.scalar_type());
+  const NormShape s = check_norm(x, y, {&w, &b, &w_next, &b_next}, gate, scale, nt);
+  c10::hip::HIPGuard guard(x.get_device());
+  c10::optional<Tensor> h, n, stats;
+  if (y) h = at::empty_like(x);
+  if (w_next) n = at::empty_like(x, x.options().dtype(nt));
+  if (keep) stats = at::empty({s.T, 4}, x.options().dtype(at::kFloat));
+  check_status(nt_block_norm(s.x_dtype, s.dtype, s.param, layer ? NT_NORM_LAYER : NT_NORM_RMS,
+                             x.data_ptr(), ptr_or_null(y), ptr_or_null(w), ptr_or_null(b),
+                             ptr_or_null(gate), s.gate_cols, ptr_or_null(scale), s.scale_cols,
+                             ptr_or_null(w_next), ptr_or_null(b_next), (float)eps, s.T, s.d,
+                             out_or_null(h), out_or_null(n),
+                             stats ? stats->data_ptr<float>() : nullptr, stream_of(x)),
+               "block_norm");
+  return {h, n, stats};
+}
+
+// block_norm_backward(h, y, w, b, gate, scale, w_next, stats, dh, dn, layer,
+// need) -> (dx, dy, dw, db, dgate, dscale, dw_next, db_next), those that `need`
+// names in this order. h: the forward's (its x without y); db_next's type is
+// the parameters'.
+std::vector<c10::optional<Tensor>> block_norm_backward(
+    Tensor h, c10::optional<Tensor> y, c10::optional<Tensor> w, c10::optional<Tensor> b,
+    c10::optional<Tensor> gate, c10::optional<Tensor> scale, c10::optional<Tensor> w_next,
+    Tensor stats, c10::optional<Tensor> dh, c10::optional<Tensor> dn, bool layer,
+    std::vector<bool> need) {
+  const at::ScalarType nt = y ? y->scalar_type() : dn ? dn->scalar_type() : h.scalar_type();
+  const NormShape s = check_norm(h, y, {&w, &b, &w_next}, gate, scale, nt);
+  TORCH_CHECK(need.size() == 8, "need must name eight gradients");
+  check_f32(stats, "stats");
+  check_same_device(h, {&stats});
+  TORCH_CHECK(stats.is_contiguous() && stats.numel() == 4 * s.T, "stats must be [T,4]");
+  for (const auto* g : {&dh, &dn}) {
+    if (!g->has_value()) continue;
+    check_same_device(h, {&**g});
+    TORCH_CHECK((*g)->sizes() == h.sizes() && (*g)->is_contiguous() &&
+                    (*g)->scalar_type() == (g == &dh ? h.scalar_type() : nt),
+                "gradients must be contiguous and of their outputs' shape and dtype");
+  }
+  c10::hip::HIPGuard guard(h.get_device());
+  std::vector<c10::optional<Tensor>> out(8);
+  const auto like = [&](int i, const c10::optional<Tensor>& t) {
+    if (need[i] && t) out[i] = at::empty_like(*t);
+  };
+  like(0, h), like(1, y), like(2, w), like(4, gate), like(5, scale), like(6, w_next);
+  if (need[3] && w) out[3] = at::empty_like(*w);
+  if (need[7] && w_next) out[7] = at::empty_like(*w_next);
+  const bool params = out[2] || out[3] || out[5] || out[6] || out[7];
+  Tensor ws = workspace(h, params ? nt_block_norm_backward_workspace_bytes(s.T, s.d) : 0);
+  check_status(nt_block_norm_backward(
+                   s.x_dtype, s.dtype, s.param, layer ? NT_NORM_LAYER : NT_NORM_RMS, h.data_ptr(),
+                   ptr_or_null(y), ptr_or_null(w), ptr_or_null(b), ptr_or_null(gate), s.gate_cols,
+                   ptr_or_null(scale), s.scale_cols, ptr_or_null(w_next), stats.data_ptr<float>(),
+                   ptr_or_null(dh), ptr_or_null(dn), s.T, s.d, out_or_null(out[0]),
+                   out_or_null(out[1]), out_or_null(out[4]), out_or_null(out[5]),
+                   out_or_null(out[2]), out_or_null(out[3]), out_or_null(out[6]),
+                   out_or_null(out[7]), ws.data_ptr(), ws.numel(), stream_of(h)),
+               "block_norm_backward");
+  return out;
+}
+
+void check_rows8(const Tensor& x, const char* name) {
+  check_device(x, name);
+  TORCH_CHECK(x.dim() == 2 && x.size(1) >= 1 && x.is_contiguous(), name,
+              " must be a contiguous [rows, columns]");
+  const auto t = x.scalar_type();
+  TORCH_CHECK(t == at::kFloat || t == at::kHalf || t == at::kBFloat16, name,
+              " must be float32, float16 or bfloat16");
+}
+void check_kept8(const Tensor& codes, const Tensor& exps) {
+  check_device(codes, "codes");
+  check_same_device(codes, {&exps});
+  TORCH_CHECK(codes.scalar_type() == at::kChar && exps.scalar_type() == at::kByte,
+              "codes must be int8 and exponents uint8");
+  TORCH_CHECK(codes.dim() == 2 && codes.size(1) >= 1 && exps.dim() == 2 &&
+                  codes.is_contiguous() && exps.is_contiguous() &&
+                  exps.size(0) == codes.size(0) &&
+                  exps.size(1) == nt_checkpoint8_blocks(codes.size(1)),
+              "expected contiguous codes [rows,f] and exponents [rows,ceil(f/32)]");
+}
+using Kept8 = c10::optional<Tensor>;
+std::pair<Kept8, Kept8> empty8(const Tensor& x, bool keep) {
+  if (!keep) return {};
+  return {at::empty(x.sizes(), x.options().dtype(at::kChar)),
+          at::empty({x.size(0), nt_checkpoint8_blocks(x.size(1))}, x.options().dtype(at::kByte))};
+}
+int8_t* codes_of(const std::pair<Kept8, Kept8>& q) {
+  return q.first ? q.first->data_ptr<int8_t>() : nullptr;
+}
+uint8_t* exps_of(const std::pair<Kept8, Kept8>& q) {
+  return q.second ? q.second->data_ptr<uint8_t>() : nullptr;
+}
+
+// checkpoint8(x) -> (codes, exponents) and back.
+std::tuple<Tensor, Tensor> checkpoint8(Tensor x) {
+  check_rows8(x, "x");
+  c10::hip::HIPGuard guard(x.get_device());
+  auto q = empty8(x, true);
+  check_status(nt_checkpoint8(dtype_code(x), x.data_ptr(), x.size(0), x.size(1), codes_of(q),
+                              exps_of(q), stream_of(x)),
+               "checkpoint8");
+  return {*q.first, *q.second};
+}
+Tensor checkpoint8_decode(Tensor codes, Tensor exps, at::ScalarType dtype) {
+  check_kept8(codes, exps);
+  c10::hip::HIPGuard guard(codes.get_device());
+  Tensor x = at::empty(codes.sizes(), codes.options().dtype(dtype));
+  check_status(nt_checkpoint8_decode(dtype_code(x), codes.data_ptr<int8_t>(),
+                                     exps.data_ptr<uint8_t>(), codes.size(0), codes.size(1),
+                                     x.data_ptr(), stream_of(codes)),
+               "checkpoint8_decode");
+  return x;
+}
+
+// gelu_checkpoint8(h) -> (act, codes, exponents); gelu_backward8 -> (dh, act or
+// None) at the checkpoint's values.
+std::tuple<Tensor, Kept8, Kept8> gelu_checkpoint8(Tensor h, bool keep) {
+  check_rows8(h, "h");
+  c10::hip::HIPGuard guard(h.get_device());
+  Tensor act = at::empty_like(h);
+  auto q = empty8(h, keep);
+  check_status(nt_gelu_checkpoint8(dtype_code(h), h.data_ptr(), h.size(0), h.size(1),
+                                   act.data_ptr(), codes_of(q), exps_of(q), stream_of(h)),
+               "gelu_checkpoint8");
+  return {act, q.first, q.second};
+}
+std::tuple<Tensor, c10::optional<Tensor>> gelu_backward8(Tensor dact, Tensor codes, Tensor exps,
+                                                         bool need_act) {
+  check_rows8(dact, "dact");
+  check_kept8(codes, exps);
+  check_same_device(dact, {&codes});
+  TORCH_CHECK(codes.sizes() == dact.sizes(), "codes must be of the gradient's shape");
+  c10::hip::HIPGuard guard(dact.get_device());
+  Tensor dh = at::empty_like(dact);
+  c10::optional<Tensor> act;
+  if (need_act) act = at::empty_like(dact);
+  check_status(nt_gelu_backward8(dtype_code(dact), dact.data_ptr(), codes.data_ptr<int8_t>(),
+                                 exps.data_ptr<uint8_t>(), dact.size(0), dact.size(1),
+                                 dh.data_ptr(), out_or_null(act), stream_of(dact)),
+               "gelu_backward8");
+  return {dh, act};
+}
+
+// swiglu_checkpoint8(gate, value) -> (hidden, gate's codes and exponents,
+// value's); swiglu_backward8 -> (dgate, dvalue, hidden or None).
+std::tuple<Tensor, Kept8, Kept8, Kept8, Kept8> swiglu_checkpoint8(Tensor gate, Tensor value,
+                                                                  bool keep) {
+  check_rows8(gate, "gate");
+  check_rows8(value, "value");
+  check_same_device(gate, {&value});
+  TORCH_CHECK(gate.sizes() == value.sizes() && gate.scalar_type() == value.scalar_type(),
+              "gate and value must be alike");
+  c10::hip::HIPGuard guard(gate.get_device());
+  Tensor hidden = at::empty_like(gate);
+  auto qg = empty8(gate, keep), qv = empty8(value, keep);
+  check_status(nt_swiglu_checkpoint8(dtype_code(gate), gate.data_ptr(), value.data_ptr(),
+                                     gate.size(0), gate.size(1), hidden.data_ptr(), codes_of(qg),
+                                     exps_of(qg), codes_of(qv), exps_of(qv), stream_of(gate)),
+               "swiglu_checkpoint8");
+  return {hidden, qg.first, qg.second, qv.first, qv.second};
+}
+std::tuple<Tensor, Tensor, c10::optional<Tensor>> swiglu_backward8(
+    Tensor dhidden, Tensor gate_codes, Tensor gate_exps, Tensor value_codes, Tensor value_exps,
+    bool need_hidden) {
+  check_rows8(dhidden, "dhidden");
+  check_kept8(gate_codes, gate_exps);
+  check_kept8(value_codes, value_exps);
+  check_same_device(dhidden, {&gate_codes, &value_codes});
+  TORCH_CHECK(gate_codes.sizes() == dhidden.sizes() && value_codes.sizes() == dhidden.sizes(),
+              "codes must be of the gradient's shape");
+  c10::hip::HIPGuard guard(dhidden.get_device());
+  Tensor dgate = at::empty_like(dhidden), dvalue = at::empty_like(dhidden);
+  c10::optional<Tensor> hidden;
+  if (need_hidden) hidden = at::empty_like(dhidden);
+  check_status(
+      nt_swiglu_backward8(dtype_code(dhidden), dhidden.data_ptr(), gate_codes.data_ptr<int8_t>(),
+                          gate_exps.data_ptr<uint8_t>(), value_codes.data_ptr<int8_t>(),
+                          value_exps.data_ptr<uint8_t>(), dhidden.size(0), dhidden.size(1),
+                          dgate.data_ptr(), dvalue.data_ptr(), out_or_null(hidden),
+                          stream_of(dhidden)),
+      "swiglu_backward8");
+  return {dgate, dvalue, hidden};
+}
+
 // stream_copy(dst, src, blocks=0): the library's 16-byte streaming copy of
 // src's bytes into dst (the achievable-bandwidth reference of the benchmark).
 void stream_copy(Tensor dst, Tensor src, int64_t blocks) {
@@ -1212,6 +1508,20 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         "Backward of the router's linear layer for both of its gradients -> (dx, dW)",
         pybind11::arg("x"), pybind11::arg("weight"), pybind11::arg("dl"), pybind11::arg("da"),
         pybind11::arg("need_dx"), pybind11::arg("need_dW"), pybind11::arg("dx_dtype") = pybind11::none());
+  m.def("moe_few_tokens", &moe_few_tokens,
+        "A whole MoE layer for few tokens -> (out [T,d], gates [T,k], topk [T,k])",
+        pybind11::arg("x"), pybind11::arg("w_up"), pybind11::arg("w_val"), pybind11::arg("w_down"),
+        pybind11::arg("top_k"), pybind11::arg("router"), pybind11::arg("logits"));
+  m.def("block_norm", &block_norm,
+        "Norms before and after a block with gate and residual scale -> (h, n, stats)");
+  m.def("block_norm_backward", &block_norm_backward,
+        "Gradients of block_norm -> [dx, dy, dw, db, dgate, dscale, dw_next, db_next]");
+  m.def("checkpoint8", &checkpoint8, "Rows in 8 bits -> (codes int8, exponents uint8)");
+  m.def("checkpoint8_decode", &checkpoint8_decode, "The rows that a checkpoint holds");
+  m.def("gelu_checkpoint8", &gelu_checkpoint8, "GELU with its input kept in 8 bits");
+  m.def("gelu_backward8", &gelu_backward8, "GELU's backward from an 8-bit checkpoint");
+  m.def("swiglu_checkpoint8", &swiglu_checkpoint8, "SwiGLU with its inputs kept in 8 bits");
+  m.def("swiglu_backward8", &swiglu_backward8, "SwiGLU's backward from 8-bit checkpoints");
   m.def("stream_fill", &stream_fill, "16-byte streaming device fill (write bandwidth reference)",
         pybind11::arg("dst"), pybind11::arg("value") = 0);
   m.def("stream_read", &stream_read, "16-byte streaming device read (read bandwidth reference)",

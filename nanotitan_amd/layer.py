@@ -13,9 +13,15 @@
   weights (src/model/feed_fwd.py:39-122), three grouped GEMMs.
 * ``GeluExpertFFN(cfg, spec)`` — the 2-GEMM up -> GELU -> down FFN the
   benchmark configs specify, with the activation fused into the GEMMs.
-* ``MoE(cfg, spec)`` — router + experts + backend (src/model/feed_fwd.py:128-152).
+* ``MoE(cfg, spec)`` — router + experts + backend (src/model/feed_fwd.py:128-152);
+  ``MoE.decode`` runs the layer on the few tokens of a decode step.
+* ``MoEBlock(cfg, spec)`` — the MoE half of a transformer layer: norm, MoE, norm,
+  gate, residual scale and sum (src/model/model.py:205-211).
 * ``route(logits, top_k)`` — fp32 softmax, top-k with ties to the lower
   expert id, renormalised gates, int32 ids.
+
+``cfg.ffn_checkpoint8 = True`` has the experts keep their activations in 8
+bits for the backward.
 
 Only the HIP path exists here; any other ``moe_backend`` raises.
 """
@@ -30,12 +36,17 @@ from torch.profiler import record_function
 
 from nanotitan_amd.moe_ops import (
     combine_inv_fn,
+    grouped_gelu_ffn8_fn,
     grouped_gelu_ffn_fn,
+    moe_few_tokens,
+    post_norm_fn,
+    pre_norm_fn,
     route_dispatch_fn,
     route_fn,
     router_aux_fn,
     router_gate_fn,
     router_stats_fn,
+    swiglu_ffn8_fn,
     swiglu_ffn_fn,
 )
 
@@ -132,7 +143,8 @@ class ExpertFFN(nn.Module):
     def forward(self, packed_X, expert_offset):
         # Gate and value GEMMs in one kernel with silu(gate) * value in its
         # epilogue; the backward fuses the activation's gradient likewise.
-        return swiglu_ffn_fn(packed_X, self.W_gate, self.W_val, self.W_out, expert_offset)
+        ffn = swiglu_ffn8_fn if getattr(self.cfg, "ffn_checkpoint8", False) else swiglu_ffn_fn
+        return ffn(packed_X, self.W_gate, self.W_val, self.W_out, expert_offset)
 
     def parameter_count(self) -> int:
         return sum(p.numel() for p in self.parameters())
@@ -151,7 +163,9 @@ class GeluExpertFFN(nn.Module):
         self.W_down = nn.Parameter(torch.randn(E, f, d).mul_(std).to(cfg.dtype))
 
     def forward(self, packed_X, expert_offset):
-        return grouped_gelu_ffn_fn(packed_X, self.W_up, self.W_down, expert_offset)
+        ffn = (grouped_gelu_ffn8_fn if getattr(self.cfg, "ffn_checkpoint8", False)
+               else grouped_gelu_ffn_fn)
+        return ffn(packed_X, self.W_up, self.W_down, expert_offset)
 
 
 def moe_forward_from_logits(x_flat, logits, experts, num_experts, top_k):
@@ -250,3 +264,70 @@ class MoE(nn.Module):
 
     def forward(self, x):
         return self.moe_backend.forward(x)
+
+    @torch.no_grad()
+    def decode(self, x):
+        """The layer's output for the few tokens (at most 64 in all) of a decode step.
+
+        x [B,S,d] -> [B,S,d], the values of ``forward`` up to the roundings that the one
+        kernel path does not make; no statistics, no gradients.
+        """
+        flat = x.reshape(-1, x.shape[-1]).contiguous()
+        if _plain_router(self.router, flat):
+            route = {"router_weight": self.router.weight}
+        else:
+            logits = self.router(flat.to(self.router.weight.dtype))
+            route = {"logits": logits.float().contiguous()}
+        e = self.experts
+        weights = ((e.W_gate, e.W_val, e.W_out) if isinstance(e, ExpertFFN)
+                   else (e.W_up, e.W_down))
+        return moe_few_tokens(flat, weights, self.cfg.top_k, **route)[0].view(x.shape)
+
+
+class MoEBlock(nn.Module):
+    """The MoE half of a transformer layer, h = x + scale * gate * N(MoE(N(x))).
+
+    The reference's layer is x + ffn(ffn_norm(x)) (src/model/model.py:205-211): ``norm``
+    "layer", ``post_norm`` False. ``norm`` is "rms" or "layer"; ``post_norm`` adds the norm
+    after the MoE; ``residual_scale`` a learned scale per channel of that initial value; a
+    gate is an input of ``forward``. Parameters are of cfg.dtype.
+
+    Blocks that follow each other share a pass: ``forward(x, following=block)`` also
+    returns ``block``'s first norm of h, which goes to it as ``normed``.
+    """
+
+    def __init__(self, cfg, spec=None, ffn: str = "swiglu", norm: str = "rms",
+                 post_norm: bool = True, residual_scale: float | None = None, eps: float = 1e-6):
+        super().__init__()
+        if norm not in ("rms", "layer"):
+            raise ValueError(f"norm={norm!r}: expected 'rms' or 'layer'")
+        self.moe = MoE(cfg, spec, ffn=ffn)
+        self.norm, self.eps = norm, eps
+
+        def param(on, value):
+            return nn.Parameter(torch.full((cfg.d_model,), value, dtype=cfg.dtype)) if on else None
+
+        layer = norm == "layer"
+        self.pre_weight, self.pre_bias = param(True, 1.0), param(layer, 0.0)
+        self.post_weight = param(post_norm, 1.0)
+        self.post_bias = param(post_norm and layer, 0.0)
+        self.scale = param(residual_scale is not None, residual_scale)
+
+    def _run(self, moe, x, normed, gate, following):
+        if normed is None:
+            normed = pre_norm_fn(x, self.pre_weight, self.pre_bias, self.norm, self.eps,
+                                 self.pre_weight.dtype)
+        y, *stats = moe(normed)
+        nxt = (None, None) if following is None else (following.pre_weight, following.pre_bias)
+        h = post_norm_fn(x, y, self.post_weight, self.post_bias, gate=gate, scale=self.scale,
+                         next_weight=nxt[0], next_bias=nxt[1], kind=self.norm, eps=self.eps)
+        return (*(h if following is not None else (h, None)), *stats)
+
+    def forward(self, x, normed=None, gate=None, following=None):
+        """x [B,S,d] -> (h, the following block's normed h or None, MoELayerStats)."""
+        return self._run(self.moe, x, normed, gate, following)
+
+    @torch.no_grad()
+    def decode(self, x, normed=None, gate=None, following=None):
+        """The same for few tokens (``MoE.decode``): (h, the following block's normed h or None)."""
+        return self._run(lambda n: (self.moe.decode(n),), x, normed, gate, following)

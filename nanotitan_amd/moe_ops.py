@@ -30,6 +30,7 @@ from __future__ import annotations
 from typing import Any
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from nanotitan_amd.extension import get_hip_extension
 
@@ -549,3 +550,263 @@ def dispatch_fn(X, topk_weights, topk_experts, num_experts, counted_ws=None):
 
 def combine_inv_fn(packed_expert_outputs, inv, packed_topk_weights, out_dtype=torch.float32):
     return CombineInvFN.apply(packed_expert_outputs, inv, packed_topk_weights, out_dtype)
+
+
+# ------------------------------------------------------------- few tokens
+
+
+def _tracked(*tensors) -> bool:
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
+def moe_few_tokens(x, weights, top_k, router_weight=None, logits=None):
+    """A whole MoE layer for the few tokens (at most 64) of a decode step.
+
+    x [T,d]; weights (W_gate, W_val, W_out) for SwiGLU experts or (W_up, W_down) for GELU
+    ones; either the router's weight [E,d] or its logits [T,E], float32. Returns (out [T,d],
+    gates [T,k] float32, ids [T,k] int32): the values of route_fn, dispatch, the experts'
+    grouped GEMMs and combine (reference src/model/cuda_backend.py:17-81), with only the
+    hidden values rounded to x's dtype on the way. Inference only: it raises where a gradient
+    would be lost.
+    """
+    if len(weights) not in (2, 3):
+        raise RuntimeError("weights are (W_gate, W_val, W_out) or (W_up, W_down)")
+    if _tracked(x, *weights, router_weight, logits):
+        raise RuntimeError("moe_few_tokens has no backward: call it under torch.no_grad()")
+    return get_hip_extension().moe_few_tokens(
+        x, weights[0], weights[1] if len(weights) == 3 else None, weights[-1], top_k,
+        router_weight, logits)
+
+
+# ------------------------------------------------------------ block norms
+
+
+class BlockNormFN(torch.autograd.Function):
+    """Norms before and after a block with its gate and residual scale, rows [T,d].
+
+    p = N(y; w, b) (y itself without w), h = x + scale * gate * p, n = N(h; w_next,
+    b_next) of h as it is held (h is x without y). Returns (h, n), None for what is not
+    computed. Saved for the backward: h, y, gate and four floats a row.
+    """
+
+    @staticmethod
+    def forward(ctx, x, y, w, b, gate, scale, w_next, b_next, layer, eps, dtype):
+        h, n, stats = get_hip_extension().block_norm(x, y, w, b, gate, scale, w_next, b_next,
+                                                     layer, eps, dtype, True)
+        ctx.save_for_backward(x if y is None else h, y, w, b, gate, scale, w_next, stats)
+        ctx.layer, ctx.has_bias = layer, (b is not None, b_next is not None)
+        ctx.set_materialize_grads(False)
+        return h, n
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dh, dn):
+        h, y, w, b, gate, scale, w_next, stats = ctx.saved_tensors
+        if dh is None and dn is None:
+            return (None,) * 11
+        need = list(ctx.needs_input_grad[:8])
+        grads = get_hip_extension().block_norm_backward(
+            h, y, w, b, gate, scale, w_next, stats, None if dh is None else dh.contiguous(),
+            None if dn is None else dn.contiguous(), ctx.layer, need)
+        return (*grads, None, None, None)
+
+
+_NORM_KINDS = {"rms": False, "layer": True}
+
+
+def _rows(t, d):
+    return None if t is None else t.reshape(-1, d).contiguous()
+
+
+def _block_norm(x, y, w, b, gate, scale, w_next, b_next, kind, eps, dtype):
+    if kind not in _NORM_KINDS:
+        raise RuntimeError(f"norm kind {kind!r}: expected 'rms' or 'layer'")
+    d = x.shape[-1]
+    if gate is not None:
+        if gate.shape[:-1] != x.shape[:-1] or gate.shape[-1] not in (1, d):
+            raise RuntimeError("gate must have x's shape, or one column for each of its rows")
+        gate = _rows(gate, gate.shape[-1])
+    if y is not None and y.shape != x.shape:
+        raise RuntimeError("x and y must be of one shape")
+    args = (_rows(x, d), _rows(y, d), w, b, gate, scale, w_next, b_next, _NORM_KINDS[kind], eps,
+            dtype)
+    if _tracked(x, y, w, b, gate, scale, w_next, b_next):
+        h, n = BlockNormFN.apply(*args)
+    else:
+        h, n, _ = get_hip_extension().block_norm(*args, False)
+    return tuple(None if t is None else t.view(x.shape) for t in (h, n))
+
+
+def pre_norm_fn(x, weight, bias=None, kind="rms", eps=1e-6, dtype=None):
+    """The norm before a block: N(x; weight, bias) over the last dimension, in ``dtype``.
+
+    ``kind`` "rms" (no bias) or "layer"; x float32, float16 or bfloat16, and ``dtype`` x's
+    or, for a float32 residual stream, a 16-bit one. Weight and bias [d] share a dtype.
+    """
+    return _block_norm(x, None, None, None, None, None, weight, bias, kind, eps, dtype)[1]
+
+
+def post_norm_fn(x, y, weight=None, bias=None, gate=None, scale=None, next_weight=None,
+                 next_bias=None, kind="rms", eps=1e-6):
+    """After a block with input x and output y: h = x + scale * gate * N(y; weight, bias).
+
+    Without a weight N(y) is y; ``gate`` is of y's shape or one value a row, in y's dtype;
+    ``scale`` [d] or one value. With ``next_weight`` the next block's norm of h comes from
+    the same pass and (h, n) is returned, else h. x is of y's dtype or float32, h of x's, n
+    of y's; the parameters share a dtype and get their gradients in it.
+    """
+    h, n = _block_norm(x, y, weight, bias, gate, scale, next_weight, next_bias, kind, eps, None)
+    return h if next_weight is None else (h, n)
+
+
+# ------------------------------------------------------ 8-bit checkpoints
+
+
+def checkpoint8(x):
+    """(codes int8 [rows,f], exponents uint8 [rows,ceil(f/32)]) of x's rows.
+
+    32 columns share a power of two; a value is off by at most 1/255 of its block's largest.
+    """
+    return get_hip_extension().checkpoint8(x)
+
+
+def checkpoint8_decode(codes, exponents, dtype):
+    """The rows that a checkpoint holds (exact in the dtype that was kept)."""
+    return get_hip_extension().checkpoint8_decode(codes, exponents, dtype)
+
+
+class Gelu8FN(torch.autograd.Function):
+    """gelu(h) (erf), h kept in 8 bits: the backward is gelu' at the value kept."""
+
+    @staticmethod
+    def forward(ctx, h):
+        act, *kept = get_hip_extension().gelu_checkpoint8(h.contiguous(), True)
+        ctx.save_for_backward(*kept)
+        return act
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dact):
+        return get_hip_extension().gelu_backward8(dact.contiguous(), *ctx.saved_tensors, False)[0]
+
+
+class SwiGLU8FN(torch.autograd.Function):
+    """silu(gate) * value, both kept in 8 bits: the backward is taken at the values kept."""
+
+    @staticmethod
+    def forward(ctx, gate, value):
+        hidden, *kept = get_hip_extension().swiglu_checkpoint8(
+            gate.contiguous(), value.contiguous(), True)
+        ctx.save_for_backward(*kept)
+        return hidden
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dhidden):
+        dgate, dvalue, _ = get_hip_extension().swiglu_backward8(
+            dhidden.contiguous(), *ctx.saved_tensors, False)
+        return dgate, dvalue
+
+
+def gelu8_fn(h):
+    if not _tracked(h):  # nothing to keep
+        return get_hip_extension().gelu_checkpoint8(h.contiguous(), False)[0]
+    return Gelu8FN.apply(h)
+
+
+def swiglu8_fn(gate, value):
+    if not _tracked(gate, value):
+        return get_hip_extension().swiglu_checkpoint8(gate.contiguous(), value.contiguous(),
+                                                      False)[0]
+    return SwiGLU8FN.apply(gate, value)
+
+
+class GroupedGeluFFN8_FN(torch.autograd.Function):
+    """GroupedGeluFFN_FN that keeps X and h = X W_up in 8 bits instead of X, gelu(h), gelu'(h).
+
+    The forward is grouped_gemm_fn, gelu, grouped_gemm_fn; the backward recomputes gelu and
+    gelu' from the h kept and takes the weight gradients from the values kept.
+    """
+
+    @staticmethod
+    def forward(ctx, X, expert_offset, W_up, W_down):
+        ext = get_hip_extension()
+        X = X.contiguous()
+        act, *kept = ext.gelu_checkpoint8(ext.grouped_gemm_kernel(X, expert_offset, W_up), True)
+        kept_X = ext.checkpoint8(X) if ctx.needs_input_grad[2] else (None, None)
+        ctx.save_for_backward(expert_offset, W_up, W_down, *kept, *kept_X)
+        return ext.grouped_gemm_kernel(act, expert_offset, W_down)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        ext = get_hip_extension()
+        off, W_up, W_down, codes, exps, *kept_X = ctx.saved_tensors
+        dy = dy.contiguous()
+        need_X, _, need_up, need_down = ctx.needs_input_grad
+        dX = dW_up = dW_down = None
+        dact = ext.bwd_grouped_gemm_dX_kernel(W_down, off, dy)
+        dh, act = ext.gelu_backward8(dact, codes, exps, need_down)
+        if need_down:
+            dW_down = ext.bwd_grouped_gemm_dW_kernel(act, off, dy)
+        if need_up:
+            X = ext.checkpoint8_decode(*kept_X, dy.dtype)
+            if need_X:
+                dW_up, dX = ext.bwd_grouped_gemm_dW_dX(X, W_up, off, dh)
+            else:
+                dW_up = ext.bwd_grouped_gemm_dW_kernel(X, off, dh)
+        elif need_X:
+            dX = ext.bwd_grouped_gemm_dX_kernel(W_up, off, dh)
+        return dX, None, dW_up, dW_down
+
+
+class SwiGLUFFN8_FN(torch.autograd.Function):
+    """SwiGLUFFN_FN that keeps X, gate and value in 8 bits instead of X, hidden, gate, value."""
+
+    @staticmethod
+    def forward(ctx, X, expert_offset, W_gate, W_val, W_out):
+        ext = get_hip_extension()
+        X = X.contiguous()
+        hidden, gate, value = ext.grouped_gemm_swiglu(X, expert_offset, W_gate, W_val)
+        need_W = ctx.needs_input_grad[2] or ctx.needs_input_grad[3]
+        kept_X = ext.checkpoint8(X) if need_W else (None, None)
+        ctx.save_for_backward(expert_offset, W_gate, W_val, W_out, *ext.checkpoint8(gate),
+                              *ext.checkpoint8(value), *kept_X)
+        del gate, value
+        return ext.grouped_gemm_kernel(hidden, expert_offset, W_out)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        ext = get_hip_extension()
+        off, W_gate, W_val, W_out, gc, ge, vc, ve, *kept_X = ctx.saved_tensors
+        dy = dy.contiguous()
+        need_X, _, need_gate, need_val, need_out = ctx.needs_input_grad
+        dX = dW_gate = dW_val = dW_out = None
+        dhidden = ext.bwd_grouped_gemm_dX_kernel(W_out, off, dy)
+        dg, dv, hidden = ext.swiglu_backward8(dhidden, gc, ge, vc, ve, need_out)
+        if need_out:
+            dW_out = ext.bwd_grouped_gemm_dW_kernel(hidden, off, dy)
+        del hidden, dhidden
+        X = ext.checkpoint8_decode(*kept_X, dy.dtype) if need_gate or need_val else None
+        if need_X and need_gate:
+            dW_gate, dX = ext.bwd_grouped_gemm_dW_dX2(X, W_gate, W_val, off, dg, dv)
+        elif need_X:
+            dX = ext.bwd_grouped_gemm_dX2(W_gate, W_val, off, dg, dv)
+        elif need_gate:
+            dW_gate = ext.bwd_grouped_gemm_dW_kernel(X, off, dg)
+        if need_val:
+            dW_val = ext.bwd_grouped_gemm_dW_kernel(X, off, dv)
+        return dX, None, dW_gate, dW_val, dW_out
+
+
+def grouped_gelu_ffn8_fn(X, W_up, W_down, expert_offset):
+    if not _tracked(X, W_up, W_down):
+        return grouped_gelu_ffn_fn(X, W_up, W_down, expert_offset)
+    return GroupedGeluFFN8_FN.apply(X, expert_offset, W_up, W_down)
+
+
+def swiglu_ffn8_fn(X, W_gate, W_val, W_out, expert_offset):
+    if not _tracked(X, W_gate, W_val, W_out):
+        return swiglu_ffn_fn(X, W_gate, W_val, W_out, expert_offset)
+    return SwiGLUFFN8_FN.apply(X, expert_offset, W_gate, W_val, W_out)
