@@ -16,6 +16,7 @@
 // permutes (one per two values): nothing but the tokens is read twice, nothing
 // goes through LDS but the waves' partial sums at the end.
 #include <algorithm>
+#include <type_traits>
 
 #include "common.hpp"
 
@@ -35,6 +36,8 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
+struct LiveExpert;
+
 struct FewArgs {
   const void* x;        // [T, d]
   const float* router;  // [E, d], or null
@@ -46,7 +49,9 @@ struct FewArgs {
   float* gates;    // [T, k]
   int32_t* topk;   // [T, k]
   void* out;       // [T, d]
-  int32_t* inv;    // [T, k]: row of an assignment in hidden and partial
+  int32_t* arrived;    // [ceil(d / 64)]: finished parts of the columns' tiles
+  int32_t* inv;        // [T, k]: row of an assignment in hidden and partial
+  LiveExpert* live;  // the experts that have tokens
   void* hidden;    // [T k, f]
   float* partial;  // [splits][T k][d]
 };
@@ -143,14 +148,19 @@ __global__ void __launch_bounds__(kRouteThreads) few_route_kernel(FewArgs a) {
 
 // ------------------------------------------------------------- expert tiles
 
-// What every workgroup of the expert kernels finds out first: each expert's
-// tokens, the first row of each (rows by expert, then token) and the experts
-// that have any.
+// Which tokens each expert has, the first row of each (rows by expert, then
+// token) and the experts that have any.
 struct Plan {
   uint64_t mask[NT_MAX_EXPERTS];
   uint16_t first[NT_MAX_EXPERTS];
   uint16_t live[NT_MAX_EXPERTS];
   int32_t num_live;
+};
+
+// The same for the down projection, in memory: the number of live experts,
+// then each one's {expert, first row, rows, 0}.
+struct LiveExpert {
+  int32_t expert, first, rows, pad;
 };
 
 __device__ __forceinline__ void make_plan(const FewArgs& a, Plan& s) {
@@ -176,49 +186,66 @@ __device__ __forceinline__ void make_plan(const FewArgs& a, Plan& s) {
   __syncthreads();
 }
 
+// What the down projection reads of it, and its counters cleared.
+__device__ __forceinline__ void write_plan(const FewArgs& a, const Plan& s) {
+  for (int i = threadIdx.x; i < a.T * a.k; i += kThreads) {
+    const int e = a.topk[i], t = i / a.k;
+    a.inv[i] = s.first[e] + popc64(s.mask[e] & ((1ull << t) - 1));
+  }
+  for (int i = threadIdx.x; i < s.num_live; i += kThreads) {
+    const int e = s.live[i];
+    a.live[1 + i] = {e, s.first[e], popc64(s.mask[e]), 0};
+  }
+  if (threadIdx.x == 0) a.live[0] = {s.num_live, 0, 0, 0};
+  for (int i = threadIdx.x; i < ceil_div(a.d, (int64_t)kCols); i += kThreads) a.arrived[i] = 0;
+}
+
 // The r-th token of a mask.
 __device__ __forceinline__ int nth_token(uint64_t mask, int r) {
   for (int i = 0; i < r; ++i) mask &= mask - 1;
   return mask ? __builtin_ctzll(mask) : 0;
 }
 
-template <typename T>
-struct mma;  // eight k values of a lane: products of a 16 x 32 by a 32 x 16 tile
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
+// A buffer of raw words from a uniform address.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_of(const void* base, uint32_t bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, bytes, 0x00027000);
+}
+constexpr int kNonTemporal = 2;  // the instruction's nt bit
 
+// Eight k values of a lane: what the matrix instructions of a step take.
 // 16-bit: four columns of eight rows in 16 registers; the fragment of column c
 // gathers its half-words, two rows at a time.
 template <typename T>
-struct mma16 {
+struct mma {
   struct Weights {
     uint32_t r[8][2];
   };
   struct Tokens {
     uint32_t v[4];
   };
-  __device__ static void column(const Weights& w, int c, uint32_t (&out)[4]) {
+  __device__ static void load_row(__amdgpu_buffer_rsrc_t b, uint32_t off, uint32_t (&out)[2]) {
+    const u32x2 v = __builtin_amdgcn_raw_buffer_load_b64(b, off, 0, kNonTemporal);
+    out[0] = v[0], out[1] = v[1];
+  }
+  __device__ static void load_eight(__amdgpu_buffer_rsrc_t b, uint32_t off, uint32_t (&out)[4]) {
+    const u32x4 v = __builtin_amdgcn_raw_buffer_load_b128(b, off, 0, 0);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) out[i] = v[i];
+  }
+  __device__ static f32x4 run(const Tokens& x, const Weights& w, int c, f32x4 acc) {
+    uint32_t b[4];
 #pragma unroll
     for (int p = 0; p < 4; ++p)
-      out[p] = __builtin_amdgcn_perm(w.r[2 * p + 1][c >> 1], w.r[2 * p][c >> 1],
-                                     (c & 1) ? 0x07060302u : 0x05040100u);
-  }
-};
-template <>
-struct mma<bf16> : mma16<bf16> {
-  __device__ static f32x4 run(const Tokens& x, const Weights& w, int c, f32x4 acc) {
-    uint32_t b[4];
-    column(w, c, b);
-    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, x.v),
-                                                   __builtin_bit_cast(bf16x8, b), acc, 0, 0, 0);
-  }
-};
-template <>
-struct mma<f16> : mma16<f16> {
-  __device__ static f32x4 run(const Tokens& x, const Weights& w, int c, f32x4 acc) {
-    uint32_t b[4];
-    column(w, c, b);
-    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, x.v),
-                                                  __builtin_bit_cast(f16x8, b), acc, 0, 0, 0);
+      b[p] = __builtin_amdgcn_perm(w.r[2 * p + 1][c >> 1], w.r[2 * p][c >> 1],
+                                   (c & 1) ? 0x07060302u : 0x05040100u);
+    if constexpr (std::is_same<T, bf16>::value)
+      return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, x.v),
+                                                     __builtin_bit_cast(bf16x8, b), acc, 0, 0, 0);
+    else
+      return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, x.v),
+                                                    __builtin_bit_cast(f16x8, b), acc, 0, 0, 0);
   }
 };
 // fp32: the eight k values go one by one; which of the 32 a lane group holds
@@ -231,6 +258,19 @@ struct mma<float> {
   struct Tokens {
     float v[8];
   };
+  __device__ static void load_row(__amdgpu_buffer_rsrc_t b, uint32_t off, float (&out)[4]) {
+    const u32x4 v = __builtin_amdgcn_raw_buffer_load_b128(b, off, 0, kNonTemporal);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) out[i] = __uint_as_float(v[i]);
+  }
+  __device__ static void load_eight(__amdgpu_buffer_rsrc_t b, uint32_t off, float (&out)[8]) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const u32x4 v = __builtin_amdgcn_raw_buffer_load_b128(b, off, h * 16, 0);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) out[h * 4 + i] = __uint_as_float(v[i]);
+    }
+  }
   __device__ static f32x4 run(const Tokens& x, const Weights& w, int c, f32x4 acc) {
 #pragma unroll
     for (int i = 0; i < 8; ++i)
@@ -239,71 +279,162 @@ struct mma<float> {
   }
 };
 
-// Rows k0 .. k0 + 7 (the lane's) of columns c0 .. c0 + 3 of a [K, N] matrix.
-// Rows past K and columns past N are zero.
-template <typename T>
-__device__ __forceinline__ void load_weights(const typename elem<T>::storage* w, int64_t K,
-                                             int64_t N, int64_t k0, int64_t c0, bool inside,
-                                             typename mma<T>::Weights& out) {
+// Four columns of eight weight rows for each of MATS matrices, and eight
+// values of each of TL tokens, as a lane holds them for one step.
+template <typename T, int MATS, int TL>
+struct Step {
   typedef typename elem<T>::storage S;
-  if (inside) {
+  typename mma<T>::Weights w[MATS];
+  typename mma<T>::Tokens x[TL];
+
+  // Buffer loads: the step's first row goes into the scalar base and the lane's
+  // eight offsets (bytes, the same for every step and matrix) stay 32-bit: as
+  // 64-bit addresses they took 32 registers more. `left` rows remain from the
+  // step's first; those past them are out of the buffer's range and read as
+  // zero. The weights are read once (non-temporal).
+  __device__ __forceinline__ void load_weights(const S* const (&base)[MATS], int64_t N,
+                                               int64_t start, int64_t step, int64_t left,
+                                               const uint32_t (&off)[8]) {
+    const int64_t size = (left * N - start) * (int64_t)sizeof(S);
+    const uint32_t range = size < 0xffffffffll ? (uint32_t)size : 0xffffffffu;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) __builtin_memcpy(out.r[i], w + (k0 + i) * N + c0, 4 * sizeof(S));
-  } else {
+    for (int i = 0; i < MATS; ++i) {
+      const auto buf = buffer_of(base[i] + step * kStep * N + start, range);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      S v[4];
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        const bool in = k0 + i < K && c0 + c < N;
-        v[c] = in ? w[(k0 + i) * N + c0 + c] : S(0);
-      }
-      __builtin_memcpy(out.r[i], v, sizeof(v));
+      for (int r = 0; r < 8; ++r) mma<T>::load_row(buf, off[r], w[i].r[r]);
     }
   }
-}
-template <typename T>
-__device__ __forceinline__ void load_tokens(const typename elem<T>::storage* row, int64_t K,
-                                            int64_t k0, typename mma<T>::Tokens& out) {
-  typedef typename elem<T>::storage S;
-  if (k0 + 8 <= K) {
-    __builtin_memcpy(out.v, row + k0, 8 * sizeof(S));
-  } else {
-    S v[8];
+  template <int MT>
+  __device__ __forceinline__ void load_tokens(const S* x0, const uint32_t (&row)[MT],
+                                              int64_t step) {
+    const auto buf = buffer_of(x0 + step * kStep, 0xffffffffu);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = k0 + i < K ? row[k0 + i] : S(0);
-    __builtin_memcpy(out.v, v, sizeof(v));
+    for (int m = 0; m < TL; ++m) mma<T>::load_eight(buf, row[m], x[m].v);
   }
-}
-
-// acc += rows (MT x 16 of them, `row[m]` this lane's) x columns [c0, c0 + 64)
-// of MATS [K, N] matrices over this wave's k-steps in [s0, s1).
-template <typename T, int MATS, int MT>
-__device__ __forceinline__ void wave_tile(const typename elem<T>::storage* const (&w)[MATS],
-                                          const typename elem<T>::storage* const (&row)[MT],
-                                          int tiles, int64_t K, int64_t N, int64_t col, int64_t s0,
-                                          int64_t s1, f32x4 (&acc)[MATS][MT][4]) {
-  const int lane = lane_id(), wave = threadIdx.x / kWave;
-  const int64_t c0 = col + (lane & 15) * 4;
-  const bool whole = col + kCols <= N;
-  for (int64_t s = s0 + wave; s < s1; s += kWaves) {
-    const int64_t k0 = s * kStep + (lane >> 4) * 8;
-    const bool inside = whole && s * kStep + kStep <= K;
-    typename mma<T>::Weights wt[MATS];
-    typename mma<T>::Tokens xt[MT];
+  // Past the last whole step: `left` values of each token.
+  template <int MT>
+  __device__ __forceinline__ void load_last_tokens(const S* x0, const uint32_t (&row)[MT],
+                                                   int64_t step, int64_t left) {
+    const int k0 = (lane_id() >> 4) * 8;
 #pragma unroll
-    for (int i = 0; i < MATS; ++i) load_weights<T>(w[i], K, N, k0, c0, inside, wt[i]);
+    for (int m = 0; m < TL; ++m) {
+      S v[8];
 #pragma unroll
-    for (int m = 0; m < MT; ++m)
-      if (m < tiles) load_tokens<T>(row[m], K, k0, xt[m]);
+      for (int r = 0; r < 8; ++r)
+        v[r] = k0 + r < left ? x0[row[m] / sizeof(S) + step * kStep + r] : S(0);
+      __builtin_memcpy(x[m].v, v, sizeof(v));
+    }
+  }
+  // Matrices of fewer than four columns: element by element.
+  __device__ __forceinline__ void load_narrow_weights(const S* const (&base)[MATS], int64_t N,
+                                                      int64_t step, int64_t left) {
+    const int k0 = (lane_id() >> 4) * 8, c0 = (lane_id() & 15) * 4;
+#pragma unroll
+    for (int i = 0; i < MATS; ++i)
+#pragma unroll
+      for (int r = 0; r < 8; ++r) {
+        S v[4];
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+          v[c] = k0 + r < left && c0 + c < N ? base[i][(step * kStep + k0 + r) * N + c0 + c] : S(0);
+        __builtin_memcpy(w[i].r[r], v, sizeof(v));
+      }
+  }
+  template <int MT>
+  __device__ __forceinline__ void multiply(f32x4 (&acc)[MATS][MT][4]) const {
 #pragma unroll
     for (int i = 0; i < MATS; ++i)
 #pragma unroll
       for (int c = 0; c < 4; ++c)
 #pragma unroll
-        for (int m = 0; m < MT; ++m)
-          if (m < tiles) acc[i][m][c] = mma<T>::run(xt[m], wt[i], c, acc[i][m][c]);
+        for (int m = 0; m < TL; ++m) acc[i][m][c] = mma<T>::run(x[m], w[i], c, acc[i][m][c]);
   }
+};
+
+// A tile of 64 columns of [K, N] matrices: its first column, and the lane's
+// first. The last tile of a width reaches back to be whole (its first columns
+// are then another tile's too and not stored); in matrices of fewer than 64
+// columns, lanes past the end repeat the last four.
+struct TileColumns {
+  int64_t start;
+  uint32_t lane;
+  __device__ __forceinline__ TileColumns(int64_t tile, int64_t N) {
+    start = tile * kCols + kCols <= N ? tile * kCols : N > kCols ? N - kCols : 0;
+    const int64_t c = (lane_id() & 15) * 4, most = N - start - 4;
+    lane = (uint32_t)(c <= most || most < 0 ? c : most);
+  }
+};
+
+// acc += TL x 16 token rows (byte row[m] of x0, this lane's) times the tile,
+// over the k-steps [s0, s1): the waves take them in turn, each with the next
+// step's loads in flight while it multiplies.
+template <int TL, bool NARROW, typename T, int MATS, int MT>
+__device__ __forceinline__ void wave_tile(const typename elem<T>::storage* const (&base)[MATS],
+                                          const typename elem<T>::storage* x0,
+                                          const uint32_t (&row)[MT], const TileColumns& tc,
+                                          int64_t K, int64_t N, int64_t s0, int64_t s1,
+                                          f32x4 (&acc)[MATS][MT][4]) {
+  typedef Step<T, MATS, TL> Held;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  int64_t s = s0 + wave;
+  if constexpr (NARROW) {
+    for (; s < s1; s += kWaves) {
+      Held t;
+      t.load_narrow_weights(base, N, s, K - s * kStep);
+      t.load_last_tokens(x0, row, s, K - s * kStep);
+      t.multiply(acc);
+    }
+    return;
+  }
+  uint32_t off[8];
+#pragma unroll
+  for (int r = 0; r < 8; ++r)
+    off[r] = (((uint32_t)(lane_id() >> 4) * 8 + r) * (uint32_t)N + tc.lane) *
+             (uint32_t)sizeof(typename elem<T>::storage);
+  const int64_t whole = s1 < K / kStep ? s1 : K / kStep;
+  const int n = s < whole ? (int)((whole - s + kWaves - 1) / kWaves) : 0;
+  auto load = [&](Held& t, int i) {
+    const int64_t at = s + (int64_t)i * kWaves;
+    t.load_weights(base, N, tc.start, at, K - at * kStep, off);
+    t.load_tokens(x0, row, at);
+  };
+  Held even, odd;
+  if (n > 0) load(even, 0);
+  for (int i = 1; i < n; i += 2) {
+    load(odd, i);
+    even.multiply(acc);
+    if (i + 1 < n) load(even, i + 1);
+    odd.multiply(acc);
+  }
+  if (n & 1) even.multiply(acc);
+  s += (int64_t)n * kWaves;
+  if (s < s1) {
+    Held t;
+    t.load_weights(base, N, tc.start, s, K - s * kStep, off);
+    t.load_last_tokens(x0, row, s, K - s * kStep);
+    t.multiply(acc);
+  }
+}
+
+// The same for any number of row tiles up to MT.
+template <bool NARROW, typename T, int MATS, int MT>
+__device__ __forceinline__ void wave_tiles(int tiles,
+                                           const typename elem<T>::storage* const (&base)[MATS],
+                                           const typename elem<T>::storage* x0,
+                                           const uint32_t (&row)[MT], const TileColumns& tc,
+                                           int64_t K, int64_t N, int64_t s0, int64_t s1,
+                                           f32x4 (&acc)[MATS][MT][4]) {
+#pragma unroll
+  for (int i = 0; i < MATS; ++i)
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) acc[i][m][c] = f32x4{0.f, 0.f, 0.f, 0.f};
+  if (tiles == 1) wave_tile<1, NARROW, T>(base, x0, row, tc, K, N, s0, s1, acc);
+  if constexpr (MT >= 2)
+    if (tiles == 2) wave_tile<2, NARROW, T>(base, x0, row, tc, K, N, s0, s1, acc);
+  if constexpr (MT == 4)
+    if (tiles > 2) wave_tile<4, NARROW, T>(base, x0, row, tc, K, N, s0, s1, acc);
 }
 
 // The eight waves' sums of row tile m: thread i gets columns 2 (i & 1) of
@@ -334,6 +465,15 @@ __device__ __forceinline__ void fold_waves(const f32x4 (&acc)[MATS][MT][4], int 
     }
   }
 }
+// Where a thread's two values of row tile m lie: row, and column of the tile.
+__device__ __forceinline__ int fold_row(int m) {
+  return m * kRowsMma + (((threadIdx.x >> 1) & 63) >> 4) * 4 + (threadIdx.x >> 7);
+}
+template <bool NARROW>
+__device__ __forceinline__ int64_t fold_col(const TileColumns& tc, int64_t N) {
+  const int64_t c = ((threadIdx.x >> 1) & 15) * 4, most = N - tc.start - 4;
+  return tc.start + (NARROW || c <= most ? c : most) + (threadIdx.x & 1) * 2;
+}
 
 __device__ __forceinline__ float few_gelu(float x) {
   return 0.5f * x * (1.f + erff(x * 0.70710678f));
@@ -341,7 +481,7 @@ __device__ __forceinline__ float few_gelu(float x) {
 
 // hidden = act(x W1[, x W2]), one tile of 64 hidden columns of one expert at a
 // time; the waves share the reduction over d.
-template <typename T, bool SWIGLU, int MT>
+template <typename T, bool SWIGLU, int MT, bool NARROW>
 __global__ void __launch_bounds__(kThreads) few_up_kernel(FewArgs a) {
   typedef typename elem<T>::storage S;
   constexpr int MATS = SWIGLU ? 2 : 1;
@@ -349,44 +489,35 @@ __global__ void __launch_bounds__(kThreads) few_up_kernel(FewArgs a) {
   __shared__ __attribute__((aligned(16))) float s_acc[kWaves * MATS * kRowsMma * kCols];
   make_plan(a, s_plan);
   const int lane = lane_id();
-  if (blockIdx.x == 0) {
-    for (int i = threadIdx.x; i < a.T * a.k; i += kThreads) {
-      const int e = a.topk[i], t = i / a.k;
-      a.inv[i] = s_plan.first[e] + popc64(s_plan.mask[e] & ((1ull << t) - 1));
-    }
-  }
+  if (blockIdx.x == 0) write_plan(a, s_plan);
   const int64_t per = ceil_div(a.f, (int64_t)kCols), steps = ceil_div(a.d, (int64_t)kStep);
   const int64_t items = s_plan.num_live * per;
   for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
-    const int e = s_plan.live[item / per];
+    const int e = __builtin_amdgcn_readfirstlane(s_plan.live[item / per]);
     const int64_t col = item % per * kCols;
+    const TileColumns tc(item % per, a.f);
     const uint64_t mask = s_plan.mask[e];
-    const int rows = popc64(mask), tiles = (rows + kRowsMma - 1) / kRowsMma;
-    const S* row[MT];
+    const int rows = __builtin_amdgcn_readfirstlane(popc64(mask));
+    const int tiles = (rows + kRowsMma - 1) / kRowsMma;
+    uint32_t row[MT];
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
       const int r = m * kRowsMma + (lane & 15);
-      row[m] = static_cast<const S*>(a.x) + (int64_t)nth_token(mask, r < rows ? r : 0) * a.d;
+      row[m] = ((uint32_t)nth_token(mask, r < rows ? r : 0) * (uint32_t)a.d + (lane >> 4) * 8) *
+               (uint32_t)sizeof(S);
     }
     const S* w[MATS];
     w[0] = static_cast<const S*>(a.w1) + (int64_t)e * a.d * a.f;
     if constexpr (SWIGLU) w[1] = static_cast<const S*>(a.w2) + (int64_t)e * a.d * a.f;
     f32x4 acc[MATS][MT][4];
-#pragma unroll
-    for (int i = 0; i < MATS; ++i)
-#pragma unroll
-      for (int m = 0; m < MT; ++m)
-#pragma unroll
-        for (int c = 0; c < 4; ++c) acc[i][m][c] = f32x4{0.f, 0.f, 0.f, 0.f};
-    wave_tile<T, MATS, MT>(w, row, tiles, a.d, a.f, col, 0, steps, acc);
+    wave_tiles<NARROW, T>(tiles, w, static_cast<const S*>(a.x), row, tc, a.d, a.f, 0, steps, acc);
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
       if (m >= tiles) break;
       float v[MATS][2];
       fold_waves<MATS, MT>(acc, m, s_acc, v);
-      const int src = (threadIdx.x >> 1) & 63;
-      const int r = m * kRowsMma + (src >> 4) * 4 + (threadIdx.x >> 7);
-      const int64_t c = col + (src & 15) * 4 + (threadIdx.x & 1) * 2;
+      const int r = fold_row(m);
+      const int64_t c = fold_col<NARROW>(tc, a.f);
       if (r < rows) {
         S* h = static_cast<S*>(a.hidden) + (int64_t)(s_plan.first[e] + r) * a.f;
 #pragma unroll
@@ -394,78 +525,90 @@ __global__ void __launch_bounds__(kThreads) few_up_kernel(FewArgs a) {
           float z;
           if constexpr (SWIGLU) z = v[0][j] / (1.f + __expf(-v[0][j])) * v[1][j];
           else z = few_gelu(v[0][j]);
-          if (c + j < a.f) h[c + j] = elem<T>::store(z);
+          if (c + j >= col && c + j < a.f) h[c + j] = elem<T>::store(z);
         }
       }
     }
   }
 }
 
+// out_t = sum_j gates_tj sum_s partial[s][inv_tj] for 64 columns from col, by
+// the workgroup that finished the tile's last part.
+template <typename T>
+__device__ __forceinline__ void combine_tile(const FewArgs& a, int64_t col) {
+  typedef typename elem<T>::storage S;
+  const int64_t stride = (int64_t)a.T * a.k * a.d, c = col + lane_id();
+  if (c >= a.d) return;
+  for (int t = threadIdx.x / kWave; t < a.T; t += kWaves) {
+    float sum = 0.f;
+    for (int j = 0; j < a.k; ++j) {
+      const float* p = a.partial + (int64_t)a.inv[t * a.k + j] * a.d + c;
+      float y = 0.f;
+#pragma unroll 4
+      for (int s = 0; s < a.splits; ++s)
+        y += __hip_atomic_load(p + s * stride, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      sum = fmaf(a.gates[t * a.k + j], y, sum);
+    }
+    static_cast<S*>(a.out)[(int64_t)t * a.d + c] = elem<T>::store(sum);
+  }
+}
+
 // partial[s] = hidden W3 over the s-th part of f, one tile of 64 columns of
-// one expert at a time.
-template <typename T, int MT>
+// one expert at a time; then the gate-weighted sum of the tile's columns by
+// whoever finishes them last. Partials are written and read through the L2s
+// (agent scope: the workgroups run on any XCD); a wave's are complete when its
+// vmcnt is zero, and the counter is touched behind the barrier after that.
+template <typename T, int MT, bool NARROW>
 __global__ void __launch_bounds__(kThreads) few_down_kernel(FewArgs a) {
   typedef typename elem<T>::storage S;
-  __shared__ Plan s_plan;
   __shared__ __attribute__((aligned(16))) float s_acc[kWaves * kRowsMma * kCols];
-  make_plan(a, s_plan);
+  __shared__ int32_t s_last;
   const int lane = lane_id();
+  const int num_live = a.live[0].expert;
   const int64_t per = ceil_div(a.d, (int64_t)kCols), steps = ceil_div(a.f, (int64_t)kStep);
-  const int64_t items = s_plan.num_live * per * a.splits;
+  const int64_t items = num_live * per * a.splits;
   for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
     const int split = (int)(item % a.splits);
-    const int64_t tile = item / a.splits;
-    const int e = s_plan.live[tile / per];
-    const int64_t col = tile % per * kCols;
-    const int rows = popc64(s_plan.mask[e]), tiles = (rows + kRowsMma - 1) / kRowsMma;
-    const int64_t first = s_plan.first[e];
-    const S* row[MT];
+    const int64_t tile = item / a.splits % per, col = tile * kCols;
+    LiveExpert le = a.live[1 + item / a.splits / per];
+    le.expert = __builtin_amdgcn_readfirstlane(le.expert);
+    le.first = __builtin_amdgcn_readfirstlane(le.first);
+    const int rows = __builtin_amdgcn_readfirstlane(le.rows);
+    const int tiles = (rows + kRowsMma - 1) / kRowsMma;
+    const TileColumns tc(tile, a.d);
+    uint32_t row[MT];
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
       const int r = m * kRowsMma + (lane & 15);
-      row[m] = static_cast<const S*>(a.hidden) + (first + (r < rows ? r : 0)) * a.f;
+      row[m] = ((uint32_t)(r < rows ? r : 0) * (uint32_t)a.f + (lane >> 4) * 8) *
+               (uint32_t)sizeof(S);
     }
-    const S* w[1] = {static_cast<const S*>(a.w3) + (int64_t)e * a.f * a.d};
+    const S* hidden = static_cast<const S*>(a.hidden) + (int64_t)le.first * a.f;
+    const S* w[1] = {static_cast<const S*>(a.w3) + (int64_t)le.expert * a.f * a.d};
     f32x4 acc[1][MT][4];
-#pragma unroll
-    for (int m = 0; m < MT; ++m)
-#pragma unroll
-      for (int c = 0; c < 4; ++c) acc[0][m][c] = f32x4{0.f, 0.f, 0.f, 0.f};
-    wave_tile<T, 1, MT>(w, row, tiles, a.f, a.d, col, steps * split / a.splits,
-                        steps * (split + 1) / a.splits, acc);
+    wave_tiles<NARROW, T>(tiles, w, hidden, row, tc, a.f, a.d, steps * split / a.splits,
+                          steps * (split + 1) / a.splits, acc);
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
       if (m >= tiles) break;
       float v[1][2];
       fold_waves<1, MT>(acc, m, s_acc, v);
-      const int src = (threadIdx.x >> 1) & 63;
-      const int r = m * kRowsMma + (src >> 4) * 4 + (threadIdx.x >> 7);
-      const int64_t c = col + (src & 15) * 4 + (threadIdx.x & 1) * 2;
+      const int r = fold_row(m);
+      const int64_t c = fold_col<NARROW>(tc, a.d);
       if (r < rows) {
-        float* p = a.partial + ((int64_t)split * a.T * a.k + first + r) * a.d;
+        float* p = a.partial + ((int64_t)split * a.T * a.k + le.first + r) * a.d;
 #pragma unroll
         for (int j = 0; j < 2; ++j)
-          if (c + j < a.d) p[c + j] = v[0][j];
+          if (c + j >= col && c + j < a.d)
+            __hip_atomic_store(p + c + j, v[0][j], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
       }
     }
+    wait_batch_loads();
+    __syncthreads();
+    if (threadIdx.x == 0) s_last = atomicAdd(&a.arrived[tile], 1) == num_live * a.splits - 1;
+    __syncthreads();
+    if (s_last) combine_tile<T>(a, col);
   }
-}
-
-// out_t = sum_j gates_tj sum_s partial[s][inv_tj].
-template <typename T>
-__global__ void __launch_bounds__(256) few_combine_kernel(FewArgs a) {
-  const int t = blockIdx.y;
-  const int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (c >= a.d) return;
-  const int64_t stride = (int64_t)a.T * a.k * a.d;
-  float sum = 0.f;
-  for (int j = 0; j < a.k; ++j) {
-    const float* p = a.partial + (int64_t)a.inv[t * a.k + j] * a.d + c;
-    float y = 0.f;
-    for (int s = 0; s < a.splits; ++s) y += p[s * stride];
-    sum = fmaf(a.gates[t * a.k + j], y, sum);
-  }
-  static_cast<typename elem<T>::storage*>(a.out)[(int64_t)t * a.d + c] = elem<T>::store(sum);
 }
 
 // Parts of the down projection's reduction: as many as give every slot a tile,
@@ -477,14 +620,17 @@ int32_t few_splits(int64_t T, int32_t k, int32_t E, int64_t d, int64_t f) {
 }
 
 struct Layout {
-  size_t inv, hidden, partial, bytes;
+  size_t arrived, inv, live, hidden, partial, bytes;
 };
 Layout few_layout(int dtype, int64_t T, int32_t k, int32_t E, int64_t d, int64_t f) {
   Layout l;
-  const size_t A = (size_t)T * k;
-  l.inv = 0;
-  l.hidden = (size_t)round_up((int64_t)A * 4, 256);
-  l.partial = l.hidden + (size_t)round_up((int64_t)(A * f) * dtype_bytes(dtype), 256);
+  const int64_t A = T * k;
+  auto after = [](size_t at, int64_t bytes) { return at + (size_t)round_up(bytes, 256); };
+  l.arrived = 0;
+  l.inv = after(l.arrived, ceil_div(d, (int64_t)kCols) * 4);
+  l.live = after(l.inv, A * 4);
+  l.hidden = after(l.live, (1 + std::min<int64_t>(A, E)) * (int64_t)sizeof(LiveExpert));
+  l.partial = after(l.hidden, A * f * dtype_bytes(dtype));
   l.bytes = l.partial + (size_t)few_splits(T, k, E, d, f) * A * d * 4;
   return l;
 }
@@ -497,28 +643,28 @@ int check_few(int dtype, int64_t T, int32_t E, int32_t k, int64_t d, int64_t f) 
   return NT_OK;
 }
 
-template <typename T, int MT>
+template <typename T, int MT, bool NARROW>
 void launch_few(const FewArgs& a, hipStream_t stream) {
   const int64_t most = std::min<int64_t>((int64_t)a.T * a.k, a.E);
   hipLaunchKernelGGL((few_route_kernel<T>), dim3((unsigned)a.T), dim3(kRouteThreads), 0, stream, a);
   const dim3 up((unsigned)std::min<int64_t>(kSlots, most * ceil_div(a.f, (int64_t)kCols)));
   if (a.w2 != nullptr)
-    hipLaunchKernelGGL((few_up_kernel<T, true, MT>), up, dim3(kThreads), 0, stream, a);
+    hipLaunchKernelGGL((few_up_kernel<T, true, MT, NARROW>), up, dim3(kThreads), 0, stream, a);
   else
-    hipLaunchKernelGGL((few_up_kernel<T, false, MT>), up, dim3(kThreads), 0, stream, a);
+    hipLaunchKernelGGL((few_up_kernel<T, false, MT, NARROW>), up, dim3(kThreads), 0, stream, a);
   const dim3 down(
       (unsigned)std::min<int64_t>(kSlots, most * ceil_div(a.d, (int64_t)kCols) * a.splits));
-  hipLaunchKernelGGL((few_down_kernel<T, MT>), down, dim3(kThreads), 0, stream, a);
-  hipLaunchKernelGGL((few_combine_kernel<T>), dim3((unsigned)ceil_div(a.d, (int64_t)256), (unsigned)a.T),
-                     dim3(256), 0, stream, a);
+  hipLaunchKernelGGL((few_down_kernel<T, MT, NARROW>), down, dim3(kThreads), 0, stream, a);
 }
 
 template <typename T>
 void launch_few(const FewArgs& a, hipStream_t stream) {
+  // a lane's four columns have to exist (the loads' width)
+  if (a.d < 4 || a.f < 4) launch_few<T, 4, true>(a, stream);
   // tokens an expert can have at most, in row tiles
-  if (a.T <= kRowsMma) launch_few<T, 1>(a, stream);
-  else if (a.T <= 2 * kRowsMma) launch_few<T, 2>(a, stream);
-  else launch_few<T, 4>(a, stream);
+  else if (a.T <= kRowsMma) launch_few<T, 1, false>(a, stream);
+  else if (a.T <= 2 * kRowsMma) launch_few<T, 2, false>(a, stream);
+  else launch_few<T, 4, false>(a, stream);
 }
 
 }  // namespace
@@ -552,7 +698,9 @@ int nt_moe_few_tokens(int dtype, const void* x, const float* router, const float
   a.T = (int32_t)T, a.E = E, a.k = k, a.d = d, a.f = f;
   a.splits = few_splits(T, k, E, d, f);
   a.gates = gates, a.topk = topk, a.out = out;
+  a.arrived = reinterpret_cast<int32_t*>(base + l.arrived);
   a.inv = reinterpret_cast<int32_t*>(base + l.inv);
+  a.live = reinterpret_cast<LiveExpert*>(base + l.live);
   a.hidden = base + l.hidden;
   a.partial = reinterpret_cast<float*>(base + l.partial);
   if (dtype == NT_F32) launch_few<float>(a, stream);
