@@ -29,7 +29,6 @@ constexpr int kThreads = kWaves * kWave;
 constexpr int kCols = 64;   // columns of a tile: 16 lanes x 4
 constexpr int kRowsMma = 16;
 constexpr int kStep = 32;   // weight rows a wave takes at a time
-constexpr int kSlots = 512;  // workgroups of the expert kernels: two on each of 256 CUs
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
@@ -45,6 +44,8 @@ struct FewArgs {
   const void *w1, *w2;  // [E, d, f]; w2 null for gelu
   const void* w3;       // [E, f, d]
   int32_t T, E, k, splits;
+  int32_t most_live;  // experts that can have tokens, at most
+  bool fused, arrive; // routing in the up projection; gate sum in the down projection
   int64_t d, f;
   float* gates;    // [T, k]
   int32_t* topk;   // [T, k]
@@ -76,33 +77,83 @@ __device__ __forceinline__ uint64_t shfl_xor64(uint64_t v, int o) {
   return ((uint64_t)__shfl_xor((uint32_t)(v >> 32), o, kWave) << 32) | lo;
 }
 
-// One token a workgroup: its logits (a wave takes every sixteenth expert, its
-// lanes the columns), then the top-k by one wave.
+// This wave's part of the sums x[i] . w[i] over the columns [c0, c1), four a
+// lane at a time, all N sums' loads of 512 columns in flight together. Past c1
+// a lane reads the last four again and counts none twice.
+template <typename T, int N>
+__device__ __forceinline__ void dot_part(const typename elem<T>::storage* const (&x)[N],
+                                         const float* const (&w)[N], int64_t c0, int64_t c1,
+                                         float (&sum)[N]) {
+  typedef typename elem<T>::storage S;
+#pragma unroll
+  for (int i = 0; i < N; ++i) sum[i] = 0.f;
+  if (c1 - c0 < 4) {
+    if (c0 + lane_id() < c1)
+      for (int i = 0; i < N; ++i)
+        sum[i] = elem<T>::load(x[i][c0 + lane_id()]) * w[i][c0 + lane_id()];
+  } else {
+    typedef float W4 __attribute__((ext_vector_type(4), aligned(4)));
+    typedef S X4 __attribute__((ext_vector_type(4), aligned(sizeof(S))));
+    for (int64_t b = c0; b < c1; b += 2 * kWave * 4) {
+      W4 wv[2][N];
+      X4 xv[2][N];
+      int skip[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int64_t c = b + (h * kWave + lane_id()) * 4, at = c + 4 <= c1 ? c : c1 - 4;
+        skip[h] = c - at < 4 ? (int)(c - at) : 4;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          wv[h][i] = *reinterpret_cast<const W4*>(w[i] + at);
+          xv[h][i] = *reinterpret_cast<const X4*>(x[i] + at);
+        }
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            sum[i] = j >= skip[h] ? fmaf(elem<T>::load(xv[h][i][j]), wv[h][i][j], sum[i]) : sum[i];
+    }
+  }
+#pragma unroll
+  for (int o = kWave / 2; o >= 1; o >>= 1)
+#pragma unroll
+    for (int i = 0; i < N; ++i) sum[i] += __shfl_xor(sum[i], o, kWave);
+}
+
+// One token a workgroup: its logits (each wave an expert, or a part of one's
+// columns where there are fewer experts than waves), then the top-k by one
+// wave.
 constexpr int kRouteThreads = 1024;
+constexpr int kRouteWaves = kRouteThreads / kWave;
 template <typename T>
 __global__ void __launch_bounds__(kRouteThreads) few_route_kernel(FewArgs a) {
   typedef typename elem<T>::storage S;
   __shared__ float s_logit[NT_MAX_EXPERTS];
+  __shared__ float s_part[kRouteWaves];
   const int t = blockIdx.x, lane = lane_id(), wave = threadIdx.x / kWave;
   if (a.router != nullptr) {
     const S* x = static_cast<const S*>(a.x) + (int64_t)t * a.d;
-    for (int e = wave; e < a.E; e += kRouteThreads / kWave) {
-      const float* w = a.router + (int64_t)e * a.d;
-      float sum = 0.f;
-      for (int64_t c = lane * 4; c < a.d; c += kWave * 4) {
-        if (c + 4 <= a.d) {
-          float wv[4];
-          S xv[4];
-          __builtin_memcpy(wv, w + c, sizeof(wv));
-          __builtin_memcpy(xv, x + c, sizeof(xv));
-#pragma unroll
-          for (int i = 0; i < 4; ++i) sum = fmaf(elem<T>::load(xv[i]), wv[i], sum);
-        } else {
-          for (int64_t i = c; i < a.d; ++i) sum = fmaf(elem<T>::load(x[i]), w[i], sum);
-        }
+    int parts = 1;
+    while (2 * parts * a.E <= kRouteWaves) parts *= 2;
+    const int64_t width = round_up(ceil_div(a.d, (int64_t)parts), 4);
+    for (int i = wave; i < a.E * parts; i += kRouteWaves) {
+      const int64_t c0 = (i % parts) * width, c1 = c0 + width < a.d ? c0 + width : a.d;
+      const S* const xs[1] = {x};
+      const float* const ws[1] = {a.router + (int64_t)(i / parts) * a.d};
+      float sum[1];
+      dot_part<T, 1>(xs, ws, c0, c1, sum);
+      if (lane == 0) (parts > 1 ? s_part : s_logit)[i] = sum[0];
+    }
+    if (parts > 1) {
+      __syncthreads();
+      if ((int)threadIdx.x < a.E) {
+        float sum = 0.f;
+        for (int p = 0; p < parts; ++p) sum += s_part[threadIdx.x * parts + p];
+        s_logit[threadIdx.x] = sum;
       }
-      sum = wave_sum(sum);
-      if (lane == 0) s_logit[e] = sum;
     }
   } else {
     for (int e = threadIdx.x; e < a.E; e += kRouteThreads) s_logit[e] = a.logits[(int64_t)t * a.E + e];
@@ -146,6 +197,58 @@ __global__ void __launch_bounds__(kRouteThreads) few_route_kernel(FewArgs a) {
   }
 }
 
+// The same for all tokens in one workgroup of the up projection, which every
+// workgroup repeats: worth it while it costs less than the launch (4.7 us and
+// its gap) that it saves. A choice's place is the number of logits ahead of
+// it, so that no selection waits for another: s_topk and s_value [T k].
+constexpr int kFusedLogits = 512;
+template <typename T>
+__device__ __forceinline__ void route_here(const FewArgs& a, float* s_logit, int32_t* s_topk,
+                                           float* s_value) {
+  typedef typename elem<T>::storage S;
+  const int n = a.T * a.E;
+  if (a.router != nullptr) {
+    constexpr int N = 4;
+    for (int i0 = threadIdx.x / kWave; i0 < n; i0 += N * kWaves) {
+      const S* xs[N];
+      const float* ws[N];
+      float sum[N];
+#pragma unroll
+      for (int q = 0; q < N; ++q) {
+        const int i = i0 + q * kWaves < n ? i0 + q * kWaves : i0;
+        xs[q] = static_cast<const S*>(a.x) + (int64_t)(i / a.E) * a.d;
+        ws[q] = a.router + (int64_t)(i % a.E) * a.d;
+      }
+      dot_part<T, N>(xs, ws, 0, a.d, sum);
+#pragma unroll
+      for (int q = 0; q < N; ++q)
+        if (lane_id() == 0 && i0 + q * kWaves < n) s_logit[i0 + q * kWaves] = sum[q];
+    }
+  } else {
+    for (int i = threadIdx.x; i < n; i += kThreads) s_logit[i] = a.logits[i];
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < n; i += kThreads) {
+    const int t = i / a.E, e = i - t * a.E;
+    const uint64_t key = choice_key(s_logit[i], e);
+    int ahead = 0;
+    for (int o = 0; o < a.E; ++o) ahead += choice_key(s_logit[t * a.E + o], o) > key;
+    if (ahead < a.k) {
+      s_topk[t * a.k + ahead] = e;
+      s_value[t * a.k + ahead] = s_logit[i];
+    }
+  }
+  __syncthreads();
+  if (blockIdx.x != 0) return;
+  for (int i = threadIdx.x; i < a.T * a.k; i += kThreads) {
+    const float* v = s_value + i / a.k * a.k;
+    float den = 0.f;
+    for (int j = 0; j < a.k; ++j) den += expf(v[j] - v[0]);
+    a.gates[i] = expf(s_value[i] - v[0]) * (1.f / den);
+    a.topk[i] = s_topk[i];
+  }
+}
+
 // ------------------------------------------------------------- expert tiles
 
 // Which tokens each expert has, the first row of each (rows by expert, then
@@ -163,11 +266,11 @@ struct LiveExpert {
   int32_t expert, first, rows, pad;
 };
 
-__device__ __forceinline__ void make_plan(const FewArgs& a, Plan& s) {
+__device__ __forceinline__ void make_plan(const FewArgs& a, const int32_t* topk, Plan& s) {
   for (int e = threadIdx.x; e < a.E; e += kThreads) s.mask[e] = 0;
   __syncthreads();
   for (int i = threadIdx.x; i < a.T * a.k; i += kThreads)
-    atomicOr(reinterpret_cast<unsigned long long*>(&s.mask[a.topk[i]]), 1ull << (i / a.k));
+    atomicOr(reinterpret_cast<unsigned long long*>(&s.mask[topk[i]]), 1ull << (i / a.k));
   __syncthreads();
   if (threadIdx.x < kWave) {
     int row = 0, live = 0;
@@ -187,9 +290,9 @@ __device__ __forceinline__ void make_plan(const FewArgs& a, Plan& s) {
 }
 
 // What the down projection reads of it, and its counters cleared.
-__device__ __forceinline__ void write_plan(const FewArgs& a, const Plan& s) {
+__device__ __forceinline__ void write_plan(const FewArgs& a, const int32_t* topk, const Plan& s) {
   for (int i = threadIdx.x; i < a.T * a.k; i += kThreads) {
-    const int e = a.topk[i], t = i / a.k;
+    const int e = topk[i], t = i / a.k;
     a.inv[i] = s.first[e] + popc64(s.mask[e] & ((1ull << t) - 1));
   }
   for (int i = threadIdx.x; i < s.num_live; i += kThreads) {
@@ -366,19 +469,18 @@ struct TileColumns {
 };
 
 // acc += TL x 16 token rows (byte row[m] of x0, this lane's) times the tile,
-// over the k-steps [s0, s1): the waves take them in turn, each with the next
-// step's loads in flight while it multiplies.
-template <int TL, bool NARROW, typename T, int MATS, int MT>
+// over the k-steps [s0, s1): the tile's KW waves take them in turn, each with
+// the next step's loads in flight while it multiplies.
+template <int TL, int KW, bool NARROW, typename T, int MATS, int MT>
 __device__ __forceinline__ void wave_tile(const typename elem<T>::storage* const (&base)[MATS],
                                           const typename elem<T>::storage* x0,
                                           const uint32_t (&row)[MT], const TileColumns& tc,
                                           int64_t K, int64_t N, int64_t s0, int64_t s1,
                                           f32x4 (&acc)[MATS][MT][4]) {
   typedef Step<T, MATS, TL> Held;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-  int64_t s = s0 + wave;
+  int64_t s = s0 + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave % KW);
   if constexpr (NARROW) {
-    for (; s < s1; s += kWaves) {
+    for (; s < s1; s += KW) {
       Held t;
       t.load_narrow_weights(base, N, s, K - s * kStep);
       t.load_last_tokens(x0, row, s, K - s * kStep);
@@ -392,22 +494,37 @@ __device__ __forceinline__ void wave_tile(const typename elem<T>::storage* const
     off[r] = (((uint32_t)(lane_id() >> 4) * 8 + r) * (uint32_t)N + tc.lane) *
              (uint32_t)sizeof(typename elem<T>::storage);
   const int64_t whole = s1 < K / kStep ? s1 : K / kStep;
-  const int n = s < whole ? (int)((whole - s + kWaves - 1) / kWaves) : 0;
+  const int n = s < whole ? (int)((whole - s + KW - 1) / KW) : 0;
   auto load = [&](Held& t, int i) {
-    const int64_t at = s + (int64_t)i * kWaves;
+    const int64_t at = s + (int64_t)i * KW;
     t.load_weights(base, N, tc.start, at, K - at * kStep, off);
     t.load_tokens(x0, row, at);
   };
-  Held even, odd;
-  if (n > 0) load(even, 0);
-  for (int i = 1; i < n; i += 2) {
-    load(odd, i);
-    even.multiply(acc);
-    if (i + 1 < n) load(even, i + 1);
-    odd.multiply(acc);
+  // The loads of the loop are unconditional: behind a branch, the wait for an
+  // older step's registers would be for the newer ones too. (Two steps in
+  // flight beside the one multiplied: 143 -> 179 us for 33 tokens, 128 experts
+  // of 2048 x 768.)
+  Held t0, t1;
+  if constexpr (sizeof(typename elem<T>::storage) == 4 && TL * MATS >= 4) {
+    // float32 weights and these many sums fill the registers: one step at a time
+    for (int i = 0; i < n; ++i) {
+      load(t0, i);
+      t0.multiply(acc);
+    }
+  } else if (n > 0) {
+    load(t0, 0);
+    int i = 1;
+    for (; i + 1 < n; i += 2) {
+      load(t1, i);
+      t0.multiply(acc);
+      load(t0, i + 1);
+      t1.multiply(acc);
+    }
+    if (i < n) load(t1, i);
+    t0.multiply(acc);
+    if (i < n) t1.multiply(acc);
   }
-  if (n & 1) even.multiply(acc);
-  s += (int64_t)n * kWaves;
+  s += (int64_t)n * KW;
   if (s < s1) {
     Held t;
     t.load_weights(base, N, tc.start, s, K - s * kStep, off);
@@ -417,7 +534,7 @@ __device__ __forceinline__ void wave_tile(const typename elem<T>::storage* const
 }
 
 // The same for any number of row tiles up to MT.
-template <bool NARROW, typename T, int MATS, int MT>
+template <int KW, bool NARROW, typename T, int MATS, int MT>
 __device__ __forceinline__ void wave_tiles(int tiles,
                                            const typename elem<T>::storage* const (&base)[MATS],
                                            const typename elem<T>::storage* x0,
@@ -430,69 +547,96 @@ __device__ __forceinline__ void wave_tiles(int tiles,
     for (int m = 0; m < MT; ++m)
 #pragma unroll
       for (int c = 0; c < 4; ++c) acc[i][m][c] = f32x4{0.f, 0.f, 0.f, 0.f};
-  if (tiles == 1) wave_tile<1, NARROW, T>(base, x0, row, tc, K, N, s0, s1, acc);
+  if (tiles == 1) wave_tile<1, KW, NARROW, T>(base, x0, row, tc, K, N, s0, s1, acc);
   if constexpr (MT >= 2)
-    if (tiles == 2) wave_tile<2, NARROW, T>(base, x0, row, tc, K, N, s0, s1, acc);
+    if (tiles == 2) wave_tile<2, KW, NARROW, T>(base, x0, row, tc, K, N, s0, s1, acc);
   if constexpr (MT == 4)
-    if (tiles > 2) wave_tile<4, NARROW, T>(base, x0, row, tc, K, N, s0, s1, acc);
+    if (tiles > 2) wave_tile<4, KW, NARROW, T>(base, x0, row, tc, K, N, s0, s1, acc);
 }
 
-// The eight waves' sums of row tile m: thread i gets columns 2 (i & 1) of
-// lane (i >> 1) & 63's four, of that lane's row i >> 7, of every matrix.
-template <int MATS, int MT>
+// The sums of a tile's KW waves for row tile m. A thread gets 16 / KW columns
+// of one row (fold_row, fold_col) for every matrix; a wave alone with its tile
+// keeps its own, four columns at a time (`part` 0..3).
+template <int KW, int MATS, int MT>
 __device__ __forceinline__ void fold_waves(const f32x4 (&acc)[MATS][MT][4], int m, float* s_acc,
-                                           float (&v)[MATS][2]) {
+                                           float (&v)[MATS][16 / KW]) {
+  constexpr int N = 16 / KW;
   const int lane = lane_id(), wave = threadIdx.x / kWave;
-  __syncthreads();
+  if constexpr (KW == 1) {
 #pragma unroll
-  for (int i = 0; i < MATS; ++i)
+    for (int i = 0; i < MATS; ++i)
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      f32x4 t;
+      for (int r = 0; r < 4; ++r)
 #pragma unroll
-      for (int c = 0; c < 4; ++c) t[c] = acc[i][m][c][r];
-      *reinterpret_cast<f32x4*>(s_acc + (((wave * MATS + i) * 4 + r) * kWave + lane) * 4) = t;
-    }
-  __syncthreads();
+        for (int c = 0; c < 4; ++c) v[i][r * 4 + c] = acc[i][m][c][r];
+  } else {
+    __syncthreads();
 #pragma unroll
-  for (int i = 0; i < MATS; ++i) {
-    v[i][0] = v[i][1] = 0.f;
+    for (int i = 0; i < MATS; ++i)
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) {
-      const float* p = s_acc + (w * MATS + i) * 4 * kWave * 4 + threadIdx.x * 2;
-      v[i][0] += p[0];
-      v[i][1] += p[1];
+      for (int r = 0; r < 4; ++r) {
+        f32x4 t;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) t[c] = acc[i][m][c][r];
+        *reinterpret_cast<f32x4*>(s_acc + (((wave * MATS + i) * 4 + r) * kWave + lane) * 4) = t;
+      }
+    __syncthreads();
+    const float* s = s_acc + wave / KW * KW * MATS * 1024 + threadIdx.x % (KW * kWave) * N;
+#pragma unroll
+    for (int i = 0; i < MATS; ++i) {
+#pragma unroll
+      for (int j = 0; j < N; ++j) v[i][j] = 0.f;
+#pragma unroll
+      for (int w = 0; w < KW; ++w)
+#pragma unroll
+        for (int j = 0; j < N; ++j) v[i][j] += s[(w * MATS + i) * 1024 + j];
     }
   }
 }
-// Where a thread's two values of row tile m lie: row, and column of the tile.
-__device__ __forceinline__ int fold_row(int m) {
-  return m * kRowsMma + (((threadIdx.x >> 1) & 63) >> 4) * 4 + (threadIdx.x >> 7);
+// Where value j of a thread lies: the row of row tile m and the column of the
+// matrix. The tile's sums are [4][64 lanes][4 columns], lane l's rows 4 (l / 16).
+template <int KW>
+__device__ __forceinline__ int fold_row(int m, int j) {
+  const int at = KW == 1 ? j / 4 * 256 + lane_id() * 4 : threadIdx.x % (KW * kWave) * (16 / KW);
+  return m * kRowsMma + (at >> 2 & 63) / 16 * 4 + at / 256;
 }
-template <bool NARROW>
-__device__ __forceinline__ int64_t fold_col(const TileColumns& tc, int64_t N) {
-  const int64_t c = ((threadIdx.x >> 1) & 15) * 4, most = N - tc.start - 4;
-  return tc.start + (NARROW || c <= most ? c : most) + (threadIdx.x & 1) * 2;
+template <int KW, bool NARROW>
+__device__ __forceinline__ int64_t fold_col(const TileColumns& tc, int64_t N, int j) {
+  const int at = KW == 1 ? j / 4 * 256 + lane_id() * 4 + j % 4
+                         : threadIdx.x % (KW * kWave) * (16 / KW) + j;
+  const int64_t c = (at >> 2 & 15) * 4, most = N - tc.start - 4;
+  return tc.start + (NARROW || c <= most ? c : most) + (at & 3);
 }
 
 __device__ __forceinline__ float few_gelu(float x) {
   return 0.5f * x * (1.f + erff(x * 0.70710678f));
 }
 
-// hidden = act(x W1[, x W2]), one tile of 64 hidden columns of one expert at a
-// time; the waves share the reduction over d.
-template <typename T, bool SWIGLU, int MT, bool NARROW>
+// hidden = act(x W1[, x W2]), one tile of 64 hidden columns of one expert for
+// KW waves at a time.
+template <typename T, bool SWIGLU, int MT, int KW, bool NARROW>
 __global__ void __launch_bounds__(kThreads) few_up_kernel(FewArgs a) {
   typedef typename elem<T>::storage S;
-  constexpr int MATS = SWIGLU ? 2 : 1;
+  constexpr int MATS = SWIGLU ? 2 : 1, kTiles = kWaves / KW, N = 16 / KW;
   __shared__ Plan s_plan;
-  __shared__ __attribute__((aligned(16))) float s_acc[kWaves * MATS * kRowsMma * kCols];
-  make_plan(a, s_plan);
+  __shared__ __attribute__((aligned(16))) float
+      s_acc[KW == 1 ? 3 * kFusedLogits : kWaves * MATS * kRowsMma * kCols];
+  const int32_t* topk = a.topk;
+  if (a.fused) {
+    int32_t* s_topk = reinterpret_cast<int32_t*>(s_acc + kFusedLogits);
+    route_here<T>(a, s_acc, s_topk, s_acc + 2 * kFusedLogits);
+    topk = s_topk;
+  }
+  make_plan(a, topk, s_plan);
   const int lane = lane_id();
-  if (blockIdx.x == 0) write_plan(a, s_plan);
+  if (blockIdx.x == 0) write_plan(a, topk, s_plan);
   const int64_t per = ceil_div(a.f, (int64_t)kCols), steps = ceil_div(a.d, (int64_t)kStep);
   const int64_t items = s_plan.num_live * per;
-  for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
+  const int group = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave / KW);
+  for (int64_t first = (int64_t)blockIdx.x * kTiles; first < items;
+       first += (int64_t)gridDim.x * kTiles) {
+    // past the last tile, a group repeats it and stores nothing
+    const int64_t item = first + group < items ? first + group : items - 1;
     const int e = __builtin_amdgcn_readfirstlane(s_plan.live[item / per]);
     const int64_t col = item % per * kCols;
     const TileColumns tc(item % per, a.f);
@@ -510,70 +654,91 @@ __global__ void __launch_bounds__(kThreads) few_up_kernel(FewArgs a) {
     w[0] = static_cast<const S*>(a.w1) + (int64_t)e * a.d * a.f;
     if constexpr (SWIGLU) w[1] = static_cast<const S*>(a.w2) + (int64_t)e * a.d * a.f;
     f32x4 acc[MATS][MT][4];
-    wave_tiles<NARROW, T>(tiles, w, static_cast<const S*>(a.x), row, tc, a.d, a.f, 0, steps, acc);
+    wave_tiles<KW, NARROW, T>(tiles, w, static_cast<const S*>(a.x), row, tc, a.d, a.f, 0, steps,
+                              acc);
+    S* hidden = static_cast<S*>(a.hidden) + (int64_t)s_plan.first[e] * a.f;
+    // groups may have different numbers of row tiles: the barriers of the fold
+    // are the same for all
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
-      if (m >= tiles) break;
-      float v[MATS][2];
-      fold_waves<MATS, MT>(acc, m, s_acc, v);
-      const int r = fold_row(m);
-      const int64_t c = fold_col<NARROW>(tc, a.f);
-      if (r < rows) {
-        S* h = static_cast<S*>(a.hidden) + (int64_t)(s_plan.first[e] + r) * a.f;
+      if (KW == 8 && m >= tiles) break;
+      if (KW == 1 && m >= tiles) break;
+      float v[MATS][N];
+      fold_waves<KW, MATS, MT>(acc, m, s_acc, v);
+      if (item != first + group) continue;
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          float z;
-          if constexpr (SWIGLU) z = v[0][j] / (1.f + __expf(-v[0][j])) * v[1][j];
-          else z = few_gelu(v[0][j]);
-          if (c + j >= col && c + j < a.f) h[c + j] = elem<T>::store(z);
-        }
+      for (int j = 0; j < N; ++j) {
+        const int r = fold_row<KW>(m, j);
+        const int64_t c = fold_col<KW, NARROW>(tc, a.f, j);
+        float z;
+        if constexpr (SWIGLU) z = v[0][j] / (1.f + __expf(-v[0][j])) * v[1][j];
+        else z = few_gelu(v[0][j]);
+        if (r < rows && c >= col && c < a.f) hidden[(int64_t)r * a.f + c] = elem<T>::store(z);
       }
     }
   }
 }
 
-// out_t = sum_j gates_tj sum_s partial[s][inv_tj] for 64 columns from col, by
-// the workgroup that finished the tile's last part.
-template <typename T>
-__device__ __forceinline__ void combine_tile(const FewArgs& a, int64_t col) {
-  typedef typename elem<T>::storage S;
-  const int64_t stride = (int64_t)a.T * a.k * a.d, c = col + lane_id();
-  if (c >= a.d) return;
-  for (int t = threadIdx.x / kWave; t < a.T; t += kWaves) {
-    float sum = 0.f;
-    for (int j = 0; j < a.k; ++j) {
-      const float* p = a.partial + (int64_t)a.inv[t * a.k + j] * a.d + c;
-      float y = 0.f;
+// out_t = sum_j gates_tj sum_s partial[s][inv_tj], column c of token t. SHARED:
+// written by workgroups of this launch.
+template <typename T, bool SHARED>
+__device__ __forceinline__ void combine_at(const FewArgs& a, int t, int64_t c) {
+  const int64_t stride = (int64_t)a.T * a.k * a.d;
+  float sum = 0.f;
 #pragma unroll 4
-      for (int s = 0; s < a.splits; ++s)
-        y += __hip_atomic_load(p + s * stride, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-      sum = fmaf(a.gates[t * a.k + j], y, sum);
-    }
-    static_cast<S*>(a.out)[(int64_t)t * a.d + c] = elem<T>::store(sum);
+  for (int j = 0; j < a.k; ++j) {
+    const float* p = a.partial + (int64_t)a.inv[t * a.k + j] * a.d + c;
+    float y = 0.f;
+#pragma unroll 4
+    for (int s = 0; s < a.splits; ++s)
+      y += SHARED ? __hip_atomic_load(p + s * stride, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)
+                  : p[s * stride];
+    sum = fmaf(a.gates[t * a.k + j], y, sum);
   }
+  static_cast<typename elem<T>::storage*>(a.out)[(int64_t)t * a.d + c] = elem<T>::store(sum);
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256) few_combine_kernel(FewArgs a) {
+  const int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (c < a.d) combine_at<T, false>(a, blockIdx.y, c);
 }
 
 // partial[s] = hidden W3 over the s-th part of f, one tile of 64 columns of
-// one expert at a time; then the gate-weighted sum of the tile's columns by
-// whoever finishes them last. Partials are written and read through the L2s
+// one expert for KW waves at a time. Where a workgroup has a tile alone (KW =
+// 8) and at most one, whoever finishes the last part of a tile's columns also
+// sums them over the experts: partials are written and read through the L2s
 // (agent scope: the workgroups run on any XCD); a wave's are complete when its
 // vmcnt is zero, and the counter is touched behind the barrier after that.
-template <typename T, int MT, bool NARROW>
+// Elsewhere a launch of its own sums them: with eight tiles a workgroup the
+// waits cost 30 us of 90 (33 tokens, 128 experts of 768 x 2048).
+template <typename T, int MT, int KW, bool NARROW>
 __global__ void __launch_bounds__(kThreads) few_down_kernel(FewArgs a) {
   typedef typename elem<T>::storage S;
-  __shared__ __attribute__((aligned(16))) float s_acc[kWaves * kRowsMma * kCols];
+  constexpr int kTiles = kWaves / KW, N = 16 / KW;
+  __shared__ __attribute__((aligned(16))) float s_acc[KW == 1 ? 4 : kWaves * kRowsMma * kCols];
   __shared__ int32_t s_last;
   const int lane = lane_id();
-  const int num_live = a.live[0].expert;
   const int64_t per = ceil_div(a.d, (int64_t)kCols), steps = ceil_div(a.f, (int64_t)kStep);
-  const int64_t items = num_live * per * a.splits;
-  for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
-    const int split = (int)(item % a.splits);
-    const int64_t tile = item / a.splits % per, col = tile * kCols;
-    LiveExpert le = a.live[1 + item / a.splits / per];
+  const int64_t most = (int64_t)a.most_live * per * a.splits;
+  const int group = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave / KW);
+  for (int64_t start = (int64_t)blockIdx.x * kTiles; start < most;
+       start += (int64_t)gridDim.x * kTiles) {
+    // the entry and the number of entries in one wait: past the number it is
+    // arbitrary, but there
+    const int64_t at = start + group < most ? start + group : most - 1;
+    const int num_live = __builtin_amdgcn_readfirstlane(a.live[0].expert);
+    LiveExpert le = a.live[1 + at / a.splits / per];
+    const int64_t items = num_live * per * a.splits;
+    if (start >= items) return;
+    const bool mine = start + group < items;
+    const int64_t item = mine ? start + group : items - 1;
+    if (!mine) le = a.live[num_live];
     le.expert = __builtin_amdgcn_readfirstlane(le.expert);
     le.first = __builtin_amdgcn_readfirstlane(le.first);
     const int rows = __builtin_amdgcn_readfirstlane(le.rows);
+    const int split = (int)(item % a.splits);
+    const int64_t tile = item / a.splits % per, col = tile * kCols;
     const int tiles = (rows + kRowsMma - 1) / kRowsMma;
     const TileColumns tc(tile, a.d);
     uint32_t row[MT];
@@ -586,37 +751,59 @@ __global__ void __launch_bounds__(kThreads) few_down_kernel(FewArgs a) {
     const S* hidden = static_cast<const S*>(a.hidden) + (int64_t)le.first * a.f;
     const S* w[1] = {static_cast<const S*>(a.w3) + (int64_t)le.expert * a.f * a.d};
     f32x4 acc[1][MT][4];
-    wave_tiles<NARROW, T>(tiles, w, hidden, row, tc, a.f, a.d, steps * split / a.splits,
-                          steps * (split + 1) / a.splits, acc);
+    wave_tiles<KW, NARROW, T>(tiles, w, hidden, row, tc, a.f, a.d, steps * split / a.splits,
+                              steps * (split + 1) / a.splits, acc);
+    float* out = a.partial + ((int64_t)split * a.T * a.k + le.first) * a.d;
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
-      if (m >= tiles) break;
-      float v[1][2];
-      fold_waves<1, MT>(acc, m, s_acc, v);
-      const int r = fold_row(m);
-      const int64_t c = fold_col<NARROW>(tc, a.d);
-      if (r < rows) {
-        float* p = a.partial + ((int64_t)split * a.T * a.k + le.first + r) * a.d;
+      if (KW == 8 && m >= tiles) break;
+      if (KW == 1 && m >= tiles) break;
+      float v[1][N];
+      fold_waves<KW, 1, MT>(acc, m, s_acc, v);
+      if (!mine) continue;
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
-          if (c + j >= col && c + j < a.d)
-            __hip_atomic_store(p + c + j, v[0][j], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      for (int j = 0; j < N; ++j) {
+        const int r = fold_row<KW>(m, j);
+        const int64_t c = fold_col<KW, NARROW>(tc, a.d, j);
+        if (r >= rows || c < col || c >= a.d) continue;
+        float* p = out + (int64_t)r * a.d + c;
+        if (KW == 8 && a.arrive)
+          __hip_atomic_store(p, v[0][j], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        else
+          *p = v[0][j];
       }
     }
-    wait_batch_loads();
-    __syncthreads();
-    if (threadIdx.x == 0) s_last = atomicAdd(&a.arrived[tile], 1) == num_live * a.splits - 1;
-    __syncthreads();
-    if (s_last) combine_tile<T>(a, col);
+    if (KW == 8 && a.arrive) {
+      wait_batch_loads();
+      __syncthreads();
+      if (threadIdx.x == 0) s_last = atomicAdd(&a.arrived[tile], 1) == num_live * a.splits - 1;
+      __syncthreads();
+      if (s_last && col + lane < a.d)
+        for (int t = threadIdx.x / kWave; t < a.T; t += kWaves)
+          combine_at<T, true>(a, t, col + lane);
+    }
   }
 }
+
+// Waves of the chip that the expert kernels are laid out for (256 CUs): 16 a CU
+// with one row tile, 8 with more (their accumulators take the registers).
+int64_t few_waves(int64_t T) { return T <= kRowsMma ? 4096 : 2048; }
 
 // Parts of the down projection's reduction: as many as give every slot a tile,
 // each with a k-step for every wave.
 int32_t few_splits(int64_t T, int32_t k, int32_t E, int64_t d, int64_t f) {
   const int64_t tiles = std::min<int64_t>(T * k, E) * ceil_div(d, (int64_t)kCols);
   const int64_t most = std::max<int64_t>(1, ceil_div(f, (int64_t)kStep) / kWaves);
-  return (int32_t)std::max<int64_t>(1, std::min(most, kSlots / std::max<int64_t>(1, tiles)));
+  return (int32_t)std::max<int64_t>(1, std::min(most, few_waves(T) / kWaves / std::max<int64_t>(1, tiles)));
+}
+
+// Waves of a tile: as many as leave every tile its place at once. Fewer waves
+// a tile means fewer of the folds and barriers that end one; with more tiles
+// than waves a wave takes several in turn.
+int few_tile_waves(int64_t T, int64_t tiles) {
+  int w = kWaves;
+  while (w > 1 && tiles * w > few_waves(T)) w /= 2;
+  return w;
 }
 
 struct Layout {
@@ -643,18 +830,51 @@ int check_few(int dtype, int64_t T, int32_t E, int32_t k, int64_t d, int64_t f) 
   return NT_OK;
 }
 
-template <typename T, int MT, bool NARROW>
-void launch_few(const FewArgs& a, hipStream_t stream) {
-  const int64_t most = std::min<int64_t>((int64_t)a.T * a.k, a.E);
-  hipLaunchKernelGGL((few_route_kernel<T>), dim3((unsigned)a.T), dim3(kRouteThreads), 0, stream, a);
-  const dim3 up((unsigned)std::min<int64_t>(kSlots, most * ceil_div(a.f, (int64_t)kCols)));
+template <typename T, int MT, int KW, bool NARROW>
+void launch_up(const FewArgs& a, int64_t tiles, hipStream_t stream) {
+  const dim3 grid((unsigned)std::min<int64_t>(few_waves(a.T) / kWaves, ceil_div(tiles * KW, (int64_t)kWaves)));
   if (a.w2 != nullptr)
-    hipLaunchKernelGGL((few_up_kernel<T, true, MT, NARROW>), up, dim3(kThreads), 0, stream, a);
+    hipLaunchKernelGGL((few_up_kernel<T, true, MT, KW, NARROW>), grid, dim3(kThreads), 0, stream, a);
   else
-    hipLaunchKernelGGL((few_up_kernel<T, false, MT, NARROW>), up, dim3(kThreads), 0, stream, a);
-  const dim3 down(
-      (unsigned)std::min<int64_t>(kSlots, most * ceil_div(a.d, (int64_t)kCols) * a.splits));
-  hipLaunchKernelGGL((few_down_kernel<T, MT, NARROW>), down, dim3(kThreads), 0, stream, a);
+    hipLaunchKernelGGL((few_up_kernel<T, false, MT, KW, NARROW>), grid, dim3(kThreads), 0, stream, a);
+}
+template <typename T, int MT, int KW, bool NARROW>
+void launch_down(const FewArgs& a, int64_t tiles, hipStream_t stream) {
+  const dim3 grid((unsigned)std::min<int64_t>(few_waves(a.T) / kWaves, ceil_div(tiles * KW, (int64_t)kWaves)));
+  hipLaunchKernelGGL((few_down_kernel<T, MT, KW, NARROW>), grid, dim3(kThreads), 0, stream, a);
+}
+
+template <typename T, int MT, bool NARROW>
+void launch_few(FewArgs a, hipStream_t stream) {
+  // Routing inside the up projection while it is short (see route_here): at
+  // most 256 multiply-adds or 128 comparisons a thread.
+  const int64_t n = (int64_t)a.T * a.E;
+  a.fused = n <= kFusedLogits && a.T * a.k <= kFusedLogits && n * a.E <= 1 << 16 &&
+            (a.router == nullptr || n * a.d <= 1 << 17);
+  if (!a.fused)
+    hipLaunchKernelGGL((few_route_kernel<T>), dim3((unsigned)a.T), dim3(kRouteThreads), 0, stream, a);
+  const int64_t up = a.most_live * ceil_div(a.f, (int64_t)kCols);
+  const int64_t down = a.most_live * ceil_div(a.d, (int64_t)kCols) * a.splits;
+  const int up_waves = NARROW ? kWaves : few_tile_waves(a.T, up);
+  const int down_waves = NARROW ? kWaves : few_tile_waves(a.T, down);
+  a.arrive = down_waves == kWaves && down <= few_waves(a.T) / kWaves;
+  if constexpr (NARROW) {
+    launch_up<T, MT, 8, true>(a, up, stream);
+    launch_down<T, MT, 8, true>(a, down, stream);
+  } else {
+    if (up_waves == 8) launch_up<T, MT, 8, false>(a, up, stream);
+    else if (up_waves == 4) launch_up<T, MT, 4, false>(a, up, stream);
+    else if (up_waves == 2) launch_up<T, MT, 2, false>(a, up, stream);
+    else launch_up<T, MT, 1, false>(a, up, stream);
+    if (down_waves == 8) launch_down<T, MT, 8, false>(a, down, stream);
+    else if (down_waves == 4) launch_down<T, MT, 4, false>(a, down, stream);
+    else if (down_waves == 2) launch_down<T, MT, 2, false>(a, down, stream);
+    else launch_down<T, MT, 1, false>(a, down, stream);
+  }
+  if (!a.arrive)
+    hipLaunchKernelGGL((few_combine_kernel<T>),
+                       dim3((unsigned)ceil_div(a.d, (int64_t)256), (unsigned)a.T), dim3(256), 0,
+                       stream, a);
 }
 
 template <typename T>
@@ -697,6 +917,7 @@ int nt_moe_few_tokens(int dtype, const void* x, const float* router, const float
   a.x = x, a.router = router, a.logits = logits, a.w1 = w_up, a.w2 = w_val, a.w3 = w_down;
   a.T = (int32_t)T, a.E = E, a.k = k, a.d = d, a.f = f;
   a.splits = few_splits(T, k, E, d, f);
+  a.most_live = (int32_t)std::min<int64_t>(T * k, E);
   a.gates = gates, a.topk = topk, a.out = out;
   a.arrived = reinterpret_cast<int32_t*>(base + l.arrived);
   a.inv = reinterpret_cast<int32_t*>(base + l.inv);
