@@ -34,7 +34,7 @@ EXT = PKG / "_nanotitan_hip.so"
 
 HIP_SOURCES = ["library.hip", "router.hip", "router_linear.hip", "dispatch.hip",
                "combine.hip", "grouped_gemm.hip", "staged_gemm.hip", "block_norm.hip",
-               "checkpoint8.hip", "few_tokens.hip"]
+               "block_norm_backward.hip", "checkpoint8.hip", "few_tokens.hip"]
 OFFLOAD_ARCH = "gfx950"
 ROCM = Path(os.environ.get("ROCM_PATH", "/opt/rocm"))
 

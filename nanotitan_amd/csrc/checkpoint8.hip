@@ -13,27 +13,21 @@
 // The activation kernels read an expert FFN's pre-activations once, write its
 // hidden values and the checkpoint; their backwards read the checkpoint and
 // the hidden gradient, and write the pre-activations' gradients and, for the
-// down projection's weight gradient, the hidden values again. All of it is
-// bound by HBM; a lane holds eight columns, four lanes a block.
+// down projection's weight gradient, the hidden values again. HBM bounds all
+// of it as long as the arithmetic stays near 30 instructions a value, which is
+// why erf, the division and the conversions are written out below.
 #include <algorithm>
 
+#include "bits.hpp"
 #include "common.hpp"
 
 namespace nt {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kVec = 8;
+constexpr int kVec = 16;  // columns of a lane: 16 bytes of codes
 constexpr int kBlock = 32;
 constexpr int kLanes = kBlock / kVec;  // lanes of a block
-
-__device__ __forceinline__ uint32_t dpp_max(uint32_t v) {
-  // over the four lanes of a quad: lane ^ 1, then lane ^ 2
-  const uint32_t a = __builtin_amdgcn_mov_dpp(v, 0xB1, 0xF, 0xF, true);
-  v = v > a ? v : a;
-  const uint32_t b = __builtin_amdgcn_mov_dpp(v, 0x4E, 0xF, 0xF, true);
-  return v > b ? v : b;
-}
 
 // The shared exponent's byte from the bits of max|v|.
 __device__ __forceinline__ uint32_t block_byte(uint32_t most) {
@@ -49,83 +43,118 @@ __device__ __forceinline__ float up_scale(uint32_t byte) {
   return __uint_as_float(byte == 255u ? 0x7fc00000u : byte == 0u ? 0x400000u : byte << 23);
 }
 
-// A wave's place: the row and chunk (eight columns) of each lane. Chunks per
-// row are a multiple of four, so that a block's lanes are one quad; rows are
-// counted in 64 bits per workgroup and in 32 inside it.
+// A lane's row and its first column. Chunks per row are a multiple of two, so
+// that a block's lanes are neighbours. The workgroup's first row is 64-bit and
+// the same for all its lanes; from there on 32 bits do.
 struct Place {
   int64_t row;
   int32_t c0;
   bool live;
 };
-__device__ __forceinline__ Place place(int64_t rows, int32_t chunks, int64_t item) {
+__device__ __forceinline__ Place place(int64_t rows, int32_t chunks) {
+  const int64_t first = (int64_t)blockIdx.x * kThreads, row0 = first / chunks;
+  const uint32_t at = (uint32_t)(first - row0 * chunks) + threadIdx.x;
+  const uint32_t down = at / (uint32_t)chunks;
   Place p;
-  p.row = item / chunks;
-  p.c0 = (int32_t)(item - p.row * chunks) * kVec;
+  p.row = row0 + down;
+  p.c0 = (int32_t)(at - down * (uint32_t)chunks) * kVec;
   p.live = p.row < rows;
   return p;
 }
 
+// A lane's sixteen values as they are stored, zeros past the row's end.
 template <typename T>
-__device__ __forceinline__ void load8(const typename elem<T>::storage* p, int64_t row, int32_t c0,
-                                      int32_t f, bool live, float (&v)[kVec]) {
-  typename elem<T>::storage s[kVec];
-  if (live && c0 + kVec <= f) {
-    __builtin_memcpy(s, p + row * f + c0, sizeof(s));
+struct Values {
+  typedef typename elem<T>::storage S;
+  typedef S V __attribute__((ext_vector_type(kVec), aligned(sizeof(S))));
+  V v;
+  __device__ __forceinline__ void load(const void* rows, const Place& p, int32_t f) {
+    const S* at = static_cast<const S*>(rows) + p.row * f + p.c0;
+    if (p.live && p.c0 + kVec <= f) {
+      v = __builtin_nontemporal_load(reinterpret_cast<const V*>(at));
+    } else {
 #pragma unroll
-    for (int i = 0; i < kVec; ++i) v[i] = elem<T>::load(s[i]);
-  } else {
-#pragma unroll
-    for (int i = 0; i < kVec; ++i)
-      v[i] = live && c0 + i < f ? elem<T>::load(p[row * f + c0 + i]) : 0.f;
+      for (int i = 0; i < kVec; ++i) v[i] = p.live && p.c0 + i < f ? at[i] : S(0);
+    }
   }
-}
-template <typename T>
-__device__ __forceinline__ void store8(typename elem<T>::storage* p, int64_t row, int32_t c0,
-                                       int32_t f, bool live, const float (&v)[kVec]) {
-  typename elem<T>::storage s[kVec];
+  __device__ __forceinline__ float operator[](int i) const { return elem<T>::load(v[i]); }
+  __device__ __forceinline__ void set(int i, float x) { v[i] = to_bits<T>(x); }
+  __device__ __forceinline__ void store(void* rows, const Place& p, int32_t f) const {
+    S* at = static_cast<S*>(rows) + p.row * f + p.c0;
+    if (p.live && p.c0 + kVec <= f) {
+      *reinterpret_cast<V*>(at) = v;
+    } else if (p.live) {
 #pragma unroll
-  for (int i = 0; i < kVec; ++i) s[i] = elem<T>::store(v[i]);
-  if (live && c0 + kVec <= f) {
-    __builtin_memcpy(p + row * f + c0, s, sizeof(s));
-  } else if (live) {
-#pragma unroll
-    for (int i = 0; i < kVec; ++i)
-      if (c0 + i < f) p[row * f + c0 + i] = s[i];
+      for (int i = 0; i < kVec; ++i)
+        if (p.c0 + i < f) at[i] = v[i];
+    }
   }
-}
+  // Bits of the largest magnitude as a float; an infinity or a NaN is above
+  // all others. 16-bit values are compared as pairs of integers.
+  __device__ __forceinline__ uint32_t most() const {
+    if constexpr (sizeof(S) == 4) {
+      uint32_t m = 0;
+#pragma unroll
+      for (int i = 0; i < kVec; ++i) {
+        const uint32_t b = __float_as_uint(v[i]) & 0x7fffffffu;
+        m = b > m ? b : m;
+      }
+      return m;
+    } else {
+      typedef uint16_t U2 __attribute__((ext_vector_type(2)));
+      U2 m = {0, 0};
+#pragma unroll
+      for (int i = 0; i < kVec; i += 2) {
+        const U2 b = U2{v[i], v[i + 1]} & U2{0x7fff, 0x7fff};
+        m = __builtin_elementwise_max(m, b);
+      }
+      return __float_as_uint(elem<T>::load(m[0] > m[1] ? m[0] : m[1]));
+    }
+  }
+};
 
-// The checkpoint of the lane's eight values (zeros past the row's end).
-__device__ __forceinline__ void keep8(const float (&v)[kVec], int8_t* codes, uint8_t* bytes,
-                                      int64_t row, int32_t c0, int32_t f, int32_t chunks,
-                                      bool live) {
-  uint32_t most = 0;
-#pragma unroll
-  for (int i = 0; i < kVec; ++i) {
-    const uint32_t b = __float_as_uint(v[i]) & 0x7fffffffu;
-    most = b > most ? b : most;
-  }
-  const uint32_t byte = block_byte(dpp_max(most));
+typedef uint32_t Codes __attribute__((ext_vector_type(kVec / 4), aligned(1)));
+
+// The checkpoint of the lane's values. Adding 1.5 * 2^23 rounds v 2^-x to an
+// integer (ties to even) and leaves it in the sum's low byte.
+template <typename T>
+__device__ __forceinline__ void keep8(const Values<T>& v, int8_t* codes, uint8_t* bytes,
+                                      const Place& p, int32_t f, int32_t chunks) {
+  uint32_t most = v.most();
+  const uint32_t other = __builtin_amdgcn_mov_dpp(most, 0xB1, 0xF, 0xF, true);  // lane ^ 1
+  most = most > other ? most : other;
+  const uint32_t byte = block_byte(most);
   const float s = down_scale(byte);
-  int8_t q[kVec];
+  Codes q;
 #pragma unroll
-  for (int i = 0; i < kVec; ++i) q[i] = byte == 255u ? 0 : (int8_t)(int)rintf(v[i] * s);
-  if (!live) return;
-  if (c0 + kVec <= f) {
-    __builtin_memcpy(codes + row * f + c0, q, sizeof(q));
+  for (int i = 0; i < kVec / 4; ++i) {
+    uint32_t b[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) b[j] = __float_as_uint(fmaf(v[i * 4 + j], s, 12582912.f));
+    const uint32_t lo = __builtin_amdgcn_perm(b[1], b[0], 0x0c0c0400u);
+    const uint32_t hi = __builtin_amdgcn_perm(b[3], b[2], 0x04000c0cu);
+    q[i] = byte == 255u ? 0u : lo | hi;
+  }
+  if (!p.live) return;
+  int8_t* at = codes + p.row * f + p.c0;
+  if (p.c0 + kVec <= f) {
+    *reinterpret_cast<Codes*>(at) = q;
   } else {
 #pragma unroll
     for (int i = 0; i < kVec; ++i)
-      if (c0 + i < f) codes[row * f + c0 + i] = q[i];
+      if (p.c0 + i < f) at[i] = (int8_t)(q[i / 4] >> (8 * (i % 4)));
   }
-  if ((lane_id() & (kLanes - 1)) == 0) bytes[row * (chunks / kLanes) + c0 / kBlock] = (uint8_t)byte;
+  if ((lane_id() & (kLanes - 1)) == 0)
+    bytes[p.row * (chunks / kLanes) + p.c0 / kBlock] = (uint8_t)byte;
 }
 
-// The largest finite value of T, and the byte of the blocks that can round past
-// it: 64 units, next to the largest value, are a power of two out of range.
+// The largest finite value of T, and the byte from which a block can round past
+// it (64 units, next to the largest value, are a power of two out of range) or
+// 128 of its units pass float32's.
 template <typename T>
 struct range {
   static constexpr uint32_t most = sizeof(typename elem<T>::storage) == 4 ? 0x7f7fffffu : 0x7f7f0000u;
-  static constexpr uint32_t byte = 249;
+  static constexpr uint32_t byte = 248;
 };
 template <>
 struct range<f16> {
@@ -133,29 +162,64 @@ struct range<f16> {
   static constexpr uint32_t byte = 137;
 };
 
-template <typename T>
-__device__ __forceinline__ void held8(const int8_t* codes, const uint8_t* bytes, int64_t row,
-                                      int32_t c0, int32_t f, int32_t chunks, bool live,
-                                      float (&v)[kVec]) {
-  int8_t q[kVec];
-  if (live && c0 + kVec <= f) {
-    __builtin_memcpy(q, codes + row * f + c0, sizeof(q));
-  } else {
+// What a checkpoint holds: with the sign bit flipped a code is an unsigned
+// byte, 128 above, which one instruction turns into a float.
+struct Held {
+  Codes q;
+  uint32_t byte;
+  __device__ __forceinline__ void load(const int8_t* codes, const uint8_t* bytes, const Place& p,
+                                       int32_t f, int32_t chunks) {
+    const int8_t* at = codes + p.row * f + p.c0;
+    if (p.live && p.c0 + kVec <= f) {
+      q = __builtin_nontemporal_load(reinterpret_cast<const Codes*>(at));
+    } else {
 #pragma unroll
-    for (int i = 0; i < kVec; ++i) q[i] = live && c0 + i < f ? codes[row * f + c0 + i] : 0;
+      for (int i = 0; i < kVec / 4; ++i) q[i] = 0;
+#pragma unroll
+      for (int i = 0; i < kVec; ++i)
+        if (p.live && p.c0 + i < f) q[i / 4] |= (uint32_t)(uint8_t)at[i] << (8 * (i % 4));
+    }
+    byte = p.live ? bytes[p.row * (chunks / kLanes) + p.c0 / kBlock] : 0u;
   }
-  const uint32_t byte = live ? bytes[row * (chunks / kLanes) + c0 / kBlock] : 0u;
-  const float s = up_scale(byte);
+  template <typename T>
+  __device__ __forceinline__ void values(float (&v)[kVec]) const {
+    const float s = up_scale(byte), off = -128.f * s;
 #pragma unroll
-  for (int i = 0; i < kVec; ++i) v[i] = (float)q[i] * s;
-  if (byte >= range<T>::byte) {
-    const float most = __uint_as_float(range<T>::most);
+    for (int i = 0; i < kVec; ++i) {
+      const uint32_t w = q[i / 4] ^ 0x80808080u;
+      v[i] = fmaf((float)((w >> (8 * (i % 4))) & 0xffu), s, off);
+    }
+    if (byte >= range<T>::byte) {
+      const float most = __uint_as_float(range<T>::most);
 #pragma unroll
-    for (int i = 0; i < kVec; ++i) v[i] = v[i] > most ? most : v[i] < -most ? -most : v[i];  // NaN stays
+      for (int i = 0; i < kVec; ++i) {
+        const float x = (float)(int8_t)(q[i / 4] >> (8 * (i % 4))) * s;
+        v[i] = x > most ? most : x < -most ? -most : x;  // NaN stays
+      }
+    }
   }
+};
+
+// 1 / (1 + e^-x): the reciprocal is within an ulp, the exponential's argument
+// within half an ulp of x.
+__device__ __forceinline__ float sigmoid(float x) {
+  return __builtin_amdgcn_rcpf(1.f + __expf(-x));
 }
 
-__device__ __forceinline__ float sigmoid(float x) { return 1.f / (1.f + __expf(-x)); }
+// The normal distribution's Phi(x), and e^(-x^2 / 2) on the way, by Abramowitz
+// and Stegun's 7.1.26: erfc(z) = (a1 t + ... + a5 t^5) e^(-z^2), t = 1 / (1 +
+// 0.3275911 z), z = |x| / sqrt(2), within 1.5e-7. The exponential is the one
+// that gelu's slope needs, and small Phi stay relatively exact.
+__device__ __forceinline__ float normal_cdf(float x, float& bell) {
+  bell = __expf(-0.5f * x * x);
+  const float t = __builtin_amdgcn_rcpf(fmaf(0.3275911f * 0.70710678f, fabsf(x), 1.f));
+  float p = fmaf(1.061405429f, t, -1.453152027f);
+  p = fmaf(p, t, 1.421413741f);
+  p = fmaf(p, t, -0.284496736f);
+  p = fmaf(p, t, 0.254829592f);
+  const float tail = 0.5f * p * t * bell;
+  return x < 0.f ? tail : 1.f - tail;
+}
 
 struct Act8Args {
   const void *a, *b;        // pre-activation (gate), value; backward: the hidden gradient in a
@@ -171,58 +235,64 @@ enum { kCopy8 = 0, kGelu8 = 1, kSwiGLU8 = 2 };
 // Forward: out = act(a[, b]) (kCopy8: none) and the checkpoints of a and b.
 template <typename T, int ACT>
 __global__ void __launch_bounds__(kThreads) keep8_kernel(Act8Args g) {
-  typedef typename elem<T>::storage S;
-  const Place p = place(g.rows, g.chunks, (int64_t)blockIdx.x * kThreads + threadIdx.x);
-  float a[kVec], b[kVec], o[kVec];
-  load8<T>(static_cast<const S*>(g.a), p.row, p.c0, g.f, p.live, a);
-  if constexpr (ACT == kSwiGLU8) load8<T>(static_cast<const S*>(g.b), p.row, p.c0, g.f, p.live, b);
+  const Place p = place(g.rows, g.chunks);
+  Values<T> a, b, o;
+  a.load(g.a, p, g.f);
+  if constexpr (ACT == kSwiGLU8) b.load(g.b, p, g.f);
   if constexpr (ACT != kCopy8) {
 #pragma unroll
-    for (int i = 0; i < kVec; ++i)
-      o[i] = ACT == kSwiGLU8 ? a[i] * sigmoid(a[i]) * b[i]
-                             : 0.5f * a[i] * (1.f + erff(a[i] * 0.70710678f));
-    store8<T>(static_cast<S*>(g.out), p.row, p.c0, g.f, p.live, o);
+    for (int i = 0; i < kVec; ++i) {
+      float bell;
+      o.set(i, ACT == kSwiGLU8 ? a[i] * sigmoid(a[i]) * b[i] : a[i] * normal_cdf(a[i], bell));
+    }
+    o.store(g.out, p, g.f);
   }
   if (g.qa == nullptr) return;  // the activation alone
-  keep8(a, g.qa, g.xa, p.row, p.c0, g.f, g.chunks, p.live);
-  if constexpr (ACT == kSwiGLU8) keep8(b, g.qb, g.xb, p.row, p.c0, g.f, g.chunks, p.live);
+  keep8<T>(a, g.qa, g.xa, p, g.f, g.chunks);
+  if constexpr (ACT == kSwiGLU8) keep8<T>(b, g.qb, g.xb, p, g.f, g.chunks);
 }
 
 // Backward at the checkpoint's values: da (and db) from the hidden gradient
 // in a, and the hidden values again where out is wanted. kCopy8: decode to out.
 template <typename T, int ACT>
 __global__ void __launch_bounds__(kThreads) held8_kernel(Act8Args g) {
-  typedef typename elem<T>::storage S;
-  const Place p = place(g.rows, g.chunks, (int64_t)blockIdx.x * kThreads + threadIdx.x);
-  float a[kVec], b[kVec], d[kVec], o[kVec];
-  held8<T>(g.qa, g.xa, p.row, p.c0, g.f, g.chunks, p.live, a);
+  const Place p = place(g.rows, g.chunks);
+  Held ha, hb;
+  ha.load(g.qa, g.xa, p, g.f, g.chunks);
+  if constexpr (ACT == kSwiGLU8) hb.load(g.qb, g.xb, p, g.f, g.chunks);
+  float a[kVec], b[kVec];
   if constexpr (ACT == kCopy8) {
-    store8<T>(static_cast<S*>(g.out), p.row, p.c0, g.f, p.live, a);
+    Values<T> x;
+    ha.values<T>(a);
+#pragma unroll
+    for (int i = 0; i < kVec; ++i) x.set(i, a[i]);
+    x.store(g.out, p, g.f);
     return;
   }
-  load8<T>(static_cast<const S*>(g.a), p.row, p.c0, g.f, p.live, d);
+  Values<T> d, da, db, o;
+  d.load(g.a, p, g.f);
+  ha.values<T>(a);
   if constexpr (ACT == kSwiGLU8) {
-    held8<T>(g.qb, g.xb, p.row, p.c0, g.f, g.chunks, p.live, b);
+    hb.values<T>(b);
 #pragma unroll
     for (int i = 0; i < kVec; ++i) {
       const float s = sigmoid(a[i]), silu = a[i] * s;
-      o[i] = silu * b[i];
-      b[i] *= d[i] * s * (1.f + a[i] * (1.f - s));  // the gate's gradient
-      d[i] *= silu;                                 // the value's
+      o.set(i, silu * b[i]);
+      da.set(i, d[i] * b[i] * fmaf(silu, 1.f - s, s));  // silu' = s + silu (1 - s)
+      db.set(i, d[i] * silu);
     }
-    store8<T>(static_cast<S*>(g.da), p.row, p.c0, g.f, p.live, b);
-    store8<T>(static_cast<S*>(g.db), p.row, p.c0, g.f, p.live, d);
+    db.store(g.db, p, g.f);
   } else {
 #pragma unroll
     for (int i = 0; i < kVec; ++i) {
-      const float cdf = 0.5f * (1.f + erff(a[i] * 0.70710678f));
-      const float pdf = __expf(-0.5f * a[i] * a[i]) * 0.39894228f;
-      o[i] = a[i] * cdf;
-      d[i] *= cdf + a[i] * pdf;
+      float bell;
+      const float cdf = normal_cdf(a[i], bell);
+      o.set(i, a[i] * cdf);
+      da.set(i, d[i] * fmaf(a[i] * 0.39894228f, bell, cdf));
     }
-    store8<T>(static_cast<S*>(g.da), p.row, p.c0, g.f, p.live, d);
   }
-  if (g.out != nullptr) store8<T>(static_cast<S*>(g.out), p.row, p.c0, g.f, p.live, o);
+  da.store(g.da, p, g.f);
+  if (g.out != nullptr) o.store(g.out, p, g.f);
 }
 
 int check8(int dtype, int64_t rows, int64_t f) {

@@ -581,60 +581,14 @@ def moe_few_tokens(x, weights, top_k, router_weight=None, logits=None):
 # ------------------------------------------------------------ block norms
 
 
-class BlockNormFN(torch.autograd.Function):
-    """Norms before and after a block with its gate and residual scale, rows [T,d].
-
-    p = N(y; w, b) (y itself without w), h = x + scale * gate * p, n = N(h; w_next,
-    b_next) of h as it is held (h is x without y). Returns (h, n), None for what is not
-    computed. Saved for the backward: h, y, gate and four floats a row.
-    """
-
-    @staticmethod
-    def forward(ctx, x, y, w, b, gate, scale, w_next, b_next, layer, eps, dtype):
-        h, n, stats = get_hip_extension().block_norm(x, y, w, b, gate, scale, w_next, b_next,
-                                                     layer, eps, dtype, True)
-        ctx.save_for_backward(x if y is None else h, y, w, b, gate, scale, w_next, stats)
-        ctx.layer, ctx.has_bias = layer, (b is not None, b_next is not None)
-        ctx.set_materialize_grads(False)
-        return h, n
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dh, dn):
-        h, y, w, b, gate, scale, w_next, stats = ctx.saved_tensors
-        if dh is None and dn is None:
-            return (None,) * 11
-        need = list(ctx.needs_input_grad[:8])
-        grads = get_hip_extension().block_norm_backward(
-            h, y, w, b, gate, scale, w_next, stats, None if dh is None else dh.contiguous(),
-            None if dn is None else dn.contiguous(), ctx.layer, need)
-        return (*grads, None, None, None)
-
-
 _NORM_KINDS = {"rms": False, "layer": True}
-
-
-def _rows(t, d):
-    return None if t is None else t.reshape(-1, d).contiguous()
 
 
 def _block_norm(x, y, w, b, gate, scale, w_next, b_next, kind, eps, dtype):
     if kind not in _NORM_KINDS:
         raise RuntimeError(f"norm kind {kind!r}: expected 'rms' or 'layer'")
-    d = x.shape[-1]
-    if gate is not None:
-        if gate.shape[:-1] != x.shape[:-1] or gate.shape[-1] not in (1, d):
-            raise RuntimeError("gate must have x's shape, or one column for each of its rows")
-        gate = _rows(gate, gate.shape[-1])
-    if y is not None and y.shape != x.shape:
-        raise RuntimeError("x and y must be of one shape")
-    args = (_rows(x, d), _rows(y, d), w, b, gate, scale, w_next, b_next, _NORM_KINDS[kind], eps,
-            dtype)
-    if _tracked(x, y, w, b, gate, scale, w_next, b_next):
-        h, n = BlockNormFN.apply(*args)
-    else:
-        h, n, _ = get_hip_extension().block_norm(*args, False)
-    return tuple(None if t is None else t.view(x.shape) for t in (h, n))
+    return get_hip_extension().block_norm_fn(x, y, w, b, gate, scale, w_next, b_next,
+                                             _NORM_KINDS[kind], eps, dtype)
 
 
 def pre_norm_fn(x, weight, bias=None, kind="rms", eps=1e-6, dtype=None):
@@ -675,50 +629,14 @@ def checkpoint8_decode(codes, exponents, dtype):
     return get_hip_extension().checkpoint8_decode(codes, exponents, dtype)
 
 
-class Gelu8FN(torch.autograd.Function):
-    """gelu(h) (erf), h kept in 8 bits: the backward is gelu' at the value kept."""
-
-    @staticmethod
-    def forward(ctx, h):
-        act, *kept = get_hip_extension().gelu_checkpoint8(h.contiguous(), True)
-        ctx.save_for_backward(*kept)
-        return act
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dact):
-        return get_hip_extension().gelu_backward8(dact.contiguous(), *ctx.saved_tensors, False)[0]
-
-
-class SwiGLU8FN(torch.autograd.Function):
-    """silu(gate) * value, both kept in 8 bits: the backward is taken at the values kept."""
-
-    @staticmethod
-    def forward(ctx, gate, value):
-        hidden, *kept = get_hip_extension().swiglu_checkpoint8(
-            gate.contiguous(), value.contiguous(), True)
-        ctx.save_for_backward(*kept)
-        return hidden
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dhidden):
-        dgate, dvalue, _ = get_hip_extension().swiglu_backward8(
-            dhidden.contiguous(), *ctx.saved_tensors, False)
-        return dgate, dvalue
-
-
 def gelu8_fn(h):
-    if not _tracked(h):  # nothing to keep
-        return get_hip_extension().gelu_checkpoint8(h.contiguous(), False)[0]
-    return Gelu8FN.apply(h)
+    """gelu(h) (erf) with h kept in 8 bits: the backward is gelu' at the value kept."""
+    return get_hip_extension().gelu8_fn(h)
 
 
 def swiglu8_fn(gate, value):
-    if not _tracked(gate, value):
-        return get_hip_extension().swiglu_checkpoint8(gate.contiguous(), value.contiguous(),
-                                                      False)[0]
-    return SwiGLU8FN.apply(gate, value)
+    """silu(gate) * value with both kept in 8 bits: the backward is taken at the values kept."""
+    return get_hip_extension().swiglu8_fn(gate, value)
 
 
 class GroupedGeluFFN8_FN(torch.autograd.Function):
