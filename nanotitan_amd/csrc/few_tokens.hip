@@ -18,14 +18,17 @@
 #include <algorithm>
 #include <type_traits>
 
+#include "bits.hpp"
 #include "common.hpp"
 
 namespace nt {
 namespace {
 
 constexpr int kMaxTokens = NT_FEW_TOKENS_MAX;
-constexpr int kWaves = 8;
-constexpr int kThreads = kWaves * kWave;
+// Waves of a workgroup whose tiles take KW waves each: small workgroups fill the
+// registers of a CU better (12 waves of 156 registers fit, or one workgroup of 8).
+constexpr int group_waves(int tile_waves) { return tile_waves > 4 ? tile_waves : 4; }
+constexpr int kMaxTileWaves = 8;
 constexpr int kCols = 64;   // columns of a tile: 16 lanes x 4
 constexpr int kRowsMma = 16;
 constexpr int kStep = 32;   // weight rows a wave takes at a time
@@ -209,26 +212,27 @@ __device__ __forceinline__ void route_here(const FewArgs& a, float* s_logit, int
   const int n = a.T * a.E;
   if (a.router != nullptr) {
     constexpr int N = 4;
-    for (int i0 = threadIdx.x / kWave; i0 < n; i0 += N * kWaves) {
+    const int waves = blockDim.x / kWave;
+    for (int i0 = threadIdx.x / kWave; i0 < n; i0 += N * waves) {
       const S* xs[N];
       const float* ws[N];
       float sum[N];
 #pragma unroll
       for (int q = 0; q < N; ++q) {
-        const int i = i0 + q * kWaves < n ? i0 + q * kWaves : i0;
+        const int i = i0 + q * waves < n ? i0 + q * waves : i0;
         xs[q] = static_cast<const S*>(a.x) + (int64_t)(i / a.E) * a.d;
         ws[q] = a.router + (int64_t)(i % a.E) * a.d;
       }
       dot_part<T, N>(xs, ws, 0, a.d, sum);
 #pragma unroll
       for (int q = 0; q < N; ++q)
-        if (lane_id() == 0 && i0 + q * kWaves < n) s_logit[i0 + q * kWaves] = sum[q];
+        if (lane_id() == 0 && i0 + q * waves < n) s_logit[i0 + q * waves] = sum[q];
     }
   } else {
-    for (int i = threadIdx.x; i < n; i += kThreads) s_logit[i] = a.logits[i];
+    for (int i = threadIdx.x; i < n; i += blockDim.x) s_logit[i] = a.logits[i];
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < n; i += kThreads) {
+  for (int i = threadIdx.x; i < n; i += blockDim.x) {
     const int t = i / a.E, e = i - t * a.E;
     const uint64_t key = choice_key(s_logit[i], e);
     int ahead = 0;
@@ -240,7 +244,7 @@ __device__ __forceinline__ void route_here(const FewArgs& a, float* s_logit, int
   }
   __syncthreads();
   if (blockIdx.x != 0) return;
-  for (int i = threadIdx.x; i < a.T * a.k; i += kThreads) {
+  for (int i = threadIdx.x; i < a.T * a.k; i += blockDim.x) {
     const float* v = s_value + i / a.k * a.k;
     float den = 0.f;
     for (int j = 0; j < a.k; ++j) den += expf(v[j] - v[0]);
@@ -267,9 +271,9 @@ struct LiveExpert {
 };
 
 __device__ __forceinline__ void make_plan(const FewArgs& a, const int32_t* topk, Plan& s) {
-  for (int e = threadIdx.x; e < a.E; e += kThreads) s.mask[e] = 0;
+  for (int e = threadIdx.x; e < a.E; e += blockDim.x) s.mask[e] = 0;
   __syncthreads();
-  for (int i = threadIdx.x; i < a.T * a.k; i += kThreads)
+  for (int i = threadIdx.x; i < a.T * a.k; i += blockDim.x)
     atomicOr(reinterpret_cast<unsigned long long*>(&s.mask[topk[i]]), 1ull << (i / a.k));
   __syncthreads();
   if (threadIdx.x < kWave) {
@@ -291,16 +295,16 @@ __device__ __forceinline__ void make_plan(const FewArgs& a, const int32_t* topk,
 
 // What the down projection reads of it, and its counters cleared.
 __device__ __forceinline__ void write_plan(const FewArgs& a, const int32_t* topk, const Plan& s) {
-  for (int i = threadIdx.x; i < a.T * a.k; i += kThreads) {
+  for (int i = threadIdx.x; i < a.T * a.k; i += blockDim.x) {
     const int e = topk[i], t = i / a.k;
     a.inv[i] = s.first[e] + popc64(s.mask[e] & ((1ull << t) - 1));
   }
-  for (int i = threadIdx.x; i < s.num_live; i += kThreads) {
+  for (int i = threadIdx.x; i < s.num_live; i += blockDim.x) {
     const int e = s.live[i];
     a.live[1 + i] = {e, s.first[e], popc64(s.mask[e]), 0};
   }
   if (threadIdx.x == 0) a.live[0] = {s.num_live, 0, 0, 0};
-  for (int i = threadIdx.x; i < ceil_div(a.d, (int64_t)kCols); i += kThreads) a.arrived[i] = 0;
+  for (int i = threadIdx.x; i < ceil_div(a.d, (int64_t)kCols); i += blockDim.x) a.arrived[i] = 0;
 }
 
 // The r-th token of a mask.
@@ -382,6 +386,21 @@ struct mma<float> {
   }
 };
 
+// A tile of 64 columns of [K, N] matrices: its first column, and the lane's
+// first. The last tile of a width reaches back to be whole (its first columns
+// are then another tile's too and not stored); in matrices of fewer than 64
+// columns, lanes past the end repeat the last four.
+struct TileColumns {
+  int64_t start;
+  uint32_t lane;
+  TileColumns() = default;
+  __device__ __forceinline__ TileColumns(int64_t col, int64_t N) {
+    start = col + kCols <= N ? col : N > kCols ? N - kCols : 0;
+    const int64_t c = (lane_id() & 15) * 4, most = N - start - 4;
+    lane = (uint32_t)(c <= most || most < 0 ? c : most);
+  }
+};
+
 // Four columns of eight weight rows for each of MATS matrices, and eight
 // values of each of TL tokens, as a lane holds them for one step.
 template <typename T, int MATS, int TL>
@@ -396,13 +415,13 @@ struct Step {
   // step's first; those past them are out of the buffer's range and read as
   // zero. The weights are read once (non-temporal).
   __device__ __forceinline__ void load_weights(const S* const (&base)[MATS], int64_t N,
-                                               int64_t start, int64_t step, int64_t left,
-                                               const uint32_t (&off)[8]) {
-    const int64_t size = (left * N - start) * (int64_t)sizeof(S);
-    const uint32_t range = size < 0xffffffffll ? (uint32_t)size : 0xffffffffu;
+                                               const TileColumns (&tc)[MATS], int64_t step,
+                                               int64_t left, const uint32_t (&off)[8]) {
 #pragma unroll
     for (int i = 0; i < MATS; ++i) {
-      const auto buf = buffer_of(base[i] + step * kStep * N + start, range);
+      const int64_t size = (left * N - tc[i].start) * (int64_t)sizeof(S);
+      const auto buf = buffer_of(base[i] + step * kStep * N + tc[i].start,
+                                 size < 0xffffffffll ? (uint32_t)size : 0xffffffffu);
 #pragma unroll
       for (int r = 0; r < 8; ++r) mma<T>::load_row(buf, off[r], w[i].r[r]);
     }
@@ -454,28 +473,14 @@ struct Step {
   }
 };
 
-// A tile of 64 columns of [K, N] matrices: its first column, and the lane's
-// first. The last tile of a width reaches back to be whole (its first columns
-// are then another tile's too and not stored); in matrices of fewer than 64
-// columns, lanes past the end repeat the last four.
-struct TileColumns {
-  int64_t start;
-  uint32_t lane;
-  __device__ __forceinline__ TileColumns(int64_t tile, int64_t N) {
-    start = tile * kCols + kCols <= N ? tile * kCols : N > kCols ? N - kCols : 0;
-    const int64_t c = (lane_id() & 15) * 4, most = N - start - 4;
-    lane = (uint32_t)(c <= most || most < 0 ? c : most);
-  }
-};
-
 // acc += TL x 16 token rows (byte row[m] of x0, this lane's) times the tile,
 // over the k-steps [s0, s1): the tile's KW waves take them in turn, each with
 // the next step's loads in flight while it multiplies.
 template <int TL, int KW, bool NARROW, typename T, int MATS, int MT>
 __device__ __forceinline__ void wave_tile(const typename elem<T>::storage* const (&base)[MATS],
                                           const typename elem<T>::storage* x0,
-                                          const uint32_t (&row)[MT], const TileColumns& tc,
-                                          int64_t K, int64_t N, int64_t s0, int64_t s1,
+                                          const uint32_t (&row)[MT],
+                                          const TileColumns (&tc)[MATS], int64_t K, int64_t N, int64_t s0, int64_t s1,
                                           f32x4 (&acc)[MATS][MT][4]) {
   typedef Step<T, MATS, TL> Held;
   int64_t s = s0 + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave % KW);
@@ -491,13 +496,13 @@ __device__ __forceinline__ void wave_tile(const typename elem<T>::storage* const
   uint32_t off[8];
 #pragma unroll
   for (int r = 0; r < 8; ++r)
-    off[r] = (((uint32_t)(lane_id() >> 4) * 8 + r) * (uint32_t)N + tc.lane) *
+    off[r] = (((uint32_t)(lane_id() >> 4) * 8 + r) * (uint32_t)N + tc[0].lane) *
              (uint32_t)sizeof(typename elem<T>::storage);
   const int64_t whole = s1 < K / kStep ? s1 : K / kStep;
   const int n = s < whole ? (int)((whole - s + KW - 1) / KW) : 0;
   auto load = [&](Held& t, int i) {
     const int64_t at = s + (int64_t)i * KW;
-    t.load_weights(base, N, tc.start, at, K - at * kStep, off);
+    t.load_weights(base, N, tc, at, K - at * kStep, off);
     t.load_tokens(x0, row, at);
   };
   // The loads of the loop are unconditional: behind a branch, the wait for an
@@ -527,19 +532,19 @@ __device__ __forceinline__ void wave_tile(const typename elem<T>::storage* const
   s += (int64_t)n * KW;
   if (s < s1) {
     Held t;
-    t.load_weights(base, N, tc.start, s, K - s * kStep, off);
+    t.load_weights(base, N, tc, s, K - s * kStep, off);
     t.load_last_tokens(x0, row, s, K - s * kStep);
     t.multiply(acc);
   }
 }
 
-// The same for any number of row tiles up to MT.
+// The same for any number of row tiles up to MT (none: zeros).
 template <int KW, bool NARROW, typename T, int MATS, int MT>
 __device__ __forceinline__ void wave_tiles(int tiles,
                                            const typename elem<T>::storage* const (&base)[MATS],
                                            const typename elem<T>::storage* x0,
-                                           const uint32_t (&row)[MT], const TileColumns& tc,
-                                           int64_t K, int64_t N, int64_t s0, int64_t s1,
+                                           const uint32_t (&row)[MT],
+                                           const TileColumns (&tc)[MATS], int64_t K, int64_t N, int64_t s0, int64_t s1,
                                            f32x4 (&acc)[MATS][MT][4]) {
 #pragma unroll
   for (int i = 0; i < MATS; ++i)
@@ -612,12 +617,13 @@ __device__ __forceinline__ float few_gelu(float x) {
   return 0.5f * x * (1.f + erff(x * 0.70710678f));
 }
 
-// hidden = act(x W1[, x W2]), one tile of 64 hidden columns of one expert for
-// KW waves at a time.
-template <typename T, bool SWIGLU, int MT, int KW, bool NARROW>
-__global__ void __launch_bounds__(kThreads) few_up_kernel(FewArgs a) {
+// hidden = act(x W1[, x W2]), one tile of 64 hidden columns of one expert (or
+// HALVES = 2 neighbouring ones of a single matrix: as much in flight a wave as
+// with two matrices) for KW waves at a time.
+template <typename T, bool SWIGLU, int HALVES, int MT, int KW, bool NARROW>
+__global__ void __launch_bounds__(group_waves(KW) * kWave) few_up_kernel(FewArgs a) {
   typedef typename elem<T>::storage S;
-  constexpr int MATS = SWIGLU ? 2 : 1, kTiles = kWaves / KW, N = 16 / KW;
+  constexpr int MATS = SWIGLU ? 2 : HALVES, kWaves = group_waves(KW), kTiles = kWaves / KW, N = 16 / KW;
   __shared__ Plan s_plan;
   __shared__ __attribute__((aligned(16))) float
       s_acc[KW == 1 ? 3 * kFusedLogits : kWaves * MATS * kRowsMma * kCols];
@@ -630,7 +636,7 @@ __global__ void __launch_bounds__(kThreads) few_up_kernel(FewArgs a) {
   make_plan(a, topk, s_plan);
   const int lane = lane_id();
   if (blockIdx.x == 0) write_plan(a, topk, s_plan);
-  const int64_t per = ceil_div(a.f, (int64_t)kCols), steps = ceil_div(a.d, (int64_t)kStep);
+  const int64_t per = ceil_div(a.f, (int64_t)kCols * HALVES), steps = ceil_div(a.d, (int64_t)kStep);
   const int64_t items = s_plan.num_live * per;
   const int group = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave / KW);
   for (int64_t first = (int64_t)blockIdx.x * kTiles; first < items;
@@ -638,43 +644,57 @@ __global__ void __launch_bounds__(kThreads) few_up_kernel(FewArgs a) {
     // past the last tile, a group repeats it and stores nothing
     const int64_t item = first + group < items ? first + group : items - 1;
     const int e = __builtin_amdgcn_readfirstlane(s_plan.live[item / per]);
-    const int64_t col = item % per * kCols;
-    const TileColumns tc(item % per, a.f);
+    const int64_t col = item % per * HALVES * kCols;
+    TileColumns tc[MATS];
+#pragma unroll
+    for (int i = 0; i < MATS; ++i) tc[i] = TileColumns(col + i * (HALVES - 1) * kCols, a.f);
     const uint64_t mask = s_plan.mask[e];
     const int rows = __builtin_amdgcn_readfirstlane(popc64(mask));
-    const int tiles = (rows + kRowsMma - 1) / kRowsMma;
+    const S* w[MATS];
+    w[0] = static_cast<const S*>(a.w1) + (int64_t)e * a.d * a.f;
+    if constexpr (MATS == 2)
+      w[1] = static_cast<const S*>(SWIGLU ? a.w2 : a.w1) + (int64_t)e * a.d * a.f;
+    S* hidden = static_cast<S*>(a.hidden) + (int64_t)s_plan.first[e] * a.f;
+    // MT x 16 rows at a time. Two groups in a workgroup may have different
+    // numbers of rows: the barriers of the fold are the same for both.
+    int most = rows;
+    if constexpr (kTiles > 1 && KW > 1)
+      for (int g = 0; g < kTiles; ++g) {
+        const int64_t i = first + g < items ? first + g : items - 1;
+        most = max(most, popc64(s_plan.mask[s_plan.live[i / per]]));
+      }
+    most = __builtin_amdgcn_readfirstlane(most);
+    for (int r0 = 0; r0 < most; r0 += MT * kRowsMma) {
+    const int tiles = min((rows - r0 + kRowsMma - 1) / kRowsMma, MT);
     uint32_t row[MT];
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
-      const int r = m * kRowsMma + (lane & 15);
+      const int r = r0 + m * kRowsMma + (lane & 15);
       row[m] = ((uint32_t)nth_token(mask, r < rows ? r : 0) * (uint32_t)a.d + (lane >> 4) * 8) *
                (uint32_t)sizeof(S);
     }
-    const S* w[MATS];
-    w[0] = static_cast<const S*>(a.w1) + (int64_t)e * a.d * a.f;
-    if constexpr (SWIGLU) w[1] = static_cast<const S*>(a.w2) + (int64_t)e * a.d * a.f;
     f32x4 acc[MATS][MT][4];
     wave_tiles<KW, NARROW, T>(tiles, w, static_cast<const S*>(a.x), row, tc, a.d, a.f, 0, steps,
                               acc);
-    S* hidden = static_cast<S*>(a.hidden) + (int64_t)s_plan.first[e] * a.f;
-    // groups may have different numbers of row tiles: the barriers of the fold
-    // are the same for all
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
-      if (KW == 8 && m >= tiles) break;
-      if (KW == 1 && m >= tiles) break;
+      if ((kTiles == 1 || KW == 1) && m >= tiles) break;
       float v[MATS][N];
       fold_waves<KW, MATS, MT>(acc, m, s_acc, v);
       if (item != first + group) continue;
 #pragma unroll
-      for (int j = 0; j < N; ++j) {
-        const int r = fold_row<KW>(m, j);
-        const int64_t c = fold_col<KW, NARROW>(tc, a.f, j);
-        float z;
-        if constexpr (SWIGLU) z = v[0][j] / (1.f + __expf(-v[0][j])) * v[1][j];
-        else z = few_gelu(v[0][j]);
-        if (r < rows && c >= col && c < a.f) hidden[(int64_t)r * a.f + c] = elem<T>::store(z);
-      }
+      for (int h = 0; h < HALVES; ++h)
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+          const int r = r0 + fold_row<KW>(m, j);
+          const int64_t c = fold_col<KW, NARROW>(tc[h], a.f, j);
+          float z;
+          if constexpr (SWIGLU) z = v[0][j] / (1.f + __expf(-v[0][j])) * v[1][j];
+          else z = few_gelu(v[h][j]);
+          if (r < rows && c >= col + h * kCols && c < a.f)
+            hidden[(int64_t)r * a.f + c] = to_bits<T>(z);
+        }
+    }
     }
   }
 }
@@ -695,7 +715,7 @@ __device__ __forceinline__ void combine_at(const FewArgs& a, int t, int64_t c) {
                   : p[s * stride];
     sum = fmaf(a.gates[t * a.k + j], y, sum);
   }
-  static_cast<typename elem<T>::storage*>(a.out)[(int64_t)t * a.d + c] = elem<T>::store(sum);
+  static_cast<typename elem<T>::storage*>(a.out)[(int64_t)t * a.d + c] = to_bits<T>(sum);
 }
 
 template <typename T>
@@ -712,14 +732,15 @@ __global__ void __launch_bounds__(256) few_combine_kernel(FewArgs a) {
 // vmcnt is zero, and the counter is touched behind the barrier after that.
 // Elsewhere a launch of its own sums them: with eight tiles a workgroup the
 // waits cost 30 us of 90 (33 tokens, 128 experts of 768 x 2048).
-template <typename T, int MT, int KW, bool NARROW>
-__global__ void __launch_bounds__(kThreads) few_down_kernel(FewArgs a) {
+template <typename T, int HALVES, int MT, int KW, bool NARROW>
+__global__ void __launch_bounds__(group_waves(KW) * kWave) few_down_kernel(FewArgs a) {
   typedef typename elem<T>::storage S;
-  constexpr int kTiles = kWaves / KW, N = 16 / KW;
-  __shared__ __attribute__((aligned(16))) float s_acc[KW == 1 ? 4 : kWaves * kRowsMma * kCols];
+  constexpr int kWaves = group_waves(KW), kTiles = kWaves / KW, N = 16 / KW;
+  __shared__ __attribute__((aligned(16))) float 
+      s_acc[KW == 1 ? 4 : kWaves * HALVES * kRowsMma * kCols];
   __shared__ int32_t s_last;
   const int lane = lane_id();
-  const int64_t per = ceil_div(a.d, (int64_t)kCols), steps = ceil_div(a.f, (int64_t)kStep);
+  const int64_t per = ceil_div(a.d, (int64_t)kCols * HALVES), steps = ceil_div(a.f, (int64_t)kStep);
   const int64_t most = (int64_t)a.most_live * per * a.splits;
   const int group = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave / KW);
   for (int64_t start = (int64_t)blockIdx.x * kTiles; start < most;
@@ -738,42 +759,57 @@ __global__ void __launch_bounds__(kThreads) few_down_kernel(FewArgs a) {
     le.first = __builtin_amdgcn_readfirstlane(le.first);
     const int rows = __builtin_amdgcn_readfirstlane(le.rows);
     const int split = (int)(item % a.splits);
-    const int64_t tile = item / a.splits % per, col = tile * kCols;
-    const int tiles = (rows + kRowsMma - 1) / kRowsMma;
-    const TileColumns tc(tile, a.d);
+    const int64_t tile = item / a.splits % per, col = tile * HALVES * kCols;
+    TileColumns tc[HALVES];
+#pragma unroll
+    for (int h = 0; h < HALVES; ++h) tc[h] = TileColumns(col + h * kCols, a.d);
+    const S* hidden = static_cast<const S*>(a.hidden) + (int64_t)le.first * a.f;
+    const S* w[HALVES];
+#pragma unroll
+    for (int h = 0; h < HALVES; ++h)
+      w[h] = static_cast<const S*>(a.w3) + (int64_t)le.expert * a.f * a.d;
+    float* out = a.partial + ((int64_t)split * a.T * a.k + le.first) * a.d;
+    int most_rows = rows;
+    if constexpr (kTiles > 1 && KW > 1)
+      for (int g = 0; g < kTiles; ++g) {
+        const int64_t i = start + g < items ? start + g : items - 1;
+        most_rows = max(most_rows, a.live[1 + i / a.splits / per].rows);
+      }
+    most_rows = __builtin_amdgcn_readfirstlane(most_rows);
+    for (int r0 = 0; r0 < most_rows; r0 += MT * kRowsMma) {
+    const int tiles = min((rows - r0 + kRowsMma - 1) / kRowsMma, MT);
     uint32_t row[MT];
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
-      const int r = m * kRowsMma + (lane & 15);
+      const int r = r0 + m * kRowsMma + (lane & 15);
       row[m] = ((uint32_t)(r < rows ? r : 0) * (uint32_t)a.f + (lane >> 4) * 8) *
                (uint32_t)sizeof(S);
     }
-    const S* hidden = static_cast<const S*>(a.hidden) + (int64_t)le.first * a.f;
-    const S* w[1] = {static_cast<const S*>(a.w3) + (int64_t)le.expert * a.f * a.d};
-    f32x4 acc[1][MT][4];
+    f32x4 acc[HALVES][MT][4];
     wave_tiles<KW, NARROW, T>(tiles, w, hidden, row, tc, a.f, a.d, steps * split / a.splits,
                               steps * (split + 1) / a.splits, acc);
-    float* out = a.partial + ((int64_t)split * a.T * a.k + le.first) * a.d;
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
-      if (KW == 8 && m >= tiles) break;
-      if (KW == 1 && m >= tiles) break;
-      float v[1][N];
-      fold_waves<KW, 1, MT>(acc, m, s_acc, v);
+      if ((kTiles == 1 || KW == 1) && m >= tiles) break;
+      float v[HALVES][N];
+      fold_waves<KW, HALVES, MT>(acc, m, s_acc, v);
       if (!mine) continue;
 #pragma unroll
-      for (int j = 0; j < N; ++j) {
-        const int r = fold_row<KW>(m, j);
-        const int64_t c = fold_col<KW, NARROW>(tc, a.d, j);
-        if (r >= rows || c < col || c >= a.d) continue;
-        float* p = out + (int64_t)r * a.d + c;
-        if (KW == 8 && a.arrive)
-          __hip_atomic_store(p, v[0][j], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        else
-          *p = v[0][j];
-      }
+      for (int h = 0; h < HALVES; ++h)
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+          const int r = r0 + fold_row<KW>(m, j);
+          const int64_t c = fold_col<KW, NARROW>(tc[h], a.d, j);
+          if (r >= rows || c < col + h * kCols || c >= a.d) continue;
+          float* p = out + (int64_t)r * a.d + c;
+          if (KW == 8 && HALVES == 1 && a.arrive)
+            __hip_atomic_store(p, v[h][j], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+          else
+            *p = v[h][j];
+        }
     }
-    if (KW == 8 && a.arrive) {
+    }
+    if (KW == 8 && HALVES == 1 && a.arrive) {
       wait_batch_loads();
       __syncthreads();
       if (threadIdx.x == 0) s_last = atomicAdd(&a.arrived[tile], 1) == num_live * a.splits - 1;
@@ -785,25 +821,43 @@ __global__ void __launch_bounds__(kThreads) few_down_kernel(FewArgs a) {
   }
 }
 
-// Waves of the chip that the expert kernels are laid out for (256 CUs): 16 a CU
-// with one row tile, 8 with more (their accumulators take the registers).
-int64_t few_waves(int64_t T) { return T <= kRowsMma ? 4096 : 2048; }
-
-// Parts of the down projection's reduction: as many as give every slot a tile,
-// each with a k-step for every wave.
-int32_t few_splits(int64_t T, int32_t k, int32_t E, int64_t d, int64_t f) {
-  const int64_t tiles = std::min<int64_t>(T * k, E) * ceil_div(d, (int64_t)kCols);
-  const int64_t most = std::max<int64_t>(1, ceil_div(f, (int64_t)kStep) / kWaves);
-  return (int32_t)std::max<int64_t>(1, std::min(most, few_waves(T) / kWaves / std::max<int64_t>(1, tiles)));
+// Waves that fit the chip (256 CUs) by the kernels' registers: with one row tile
+// sixteen a CU, twelve for two matrices, else twelve and eight.
+int64_t few_waves(int row_tiles, int mats) {
+  return 256 * (16 - 4 * (mats - 1) - (row_tiles == 1 ? 0 : 4));
 }
 
-// Waves of a tile: as many as leave every tile its place at once. Fewer waves
-// a tile means fewer of the folds and barriers that end one; with more tiles
-// than waves a wave takes several in turn.
-int few_tile_waves(int64_t T, int64_t tiles) {
-  int w = kWaves;
-  while (w > 1 && tiles * w > few_waves(T)) w /= 2;
-  return w;
+// Parts of the down projection's reduction: as many as give every CU two
+// tiles, each with a k-step for every wave.
+int32_t few_splits(int64_t T, int32_t k, int32_t E, int64_t d, int64_t f) {
+  const int64_t tiles = std::min<int64_t>(T * k, E) * ceil_div(d, (int64_t)kCols);
+  const int64_t most = std::max<int64_t>(1, ceil_div(f, (int64_t)kStep) / kMaxTileWaves);
+  return (int32_t)std::max<int64_t>(1, std::min(most, 512 / std::max<int64_t>(1, tiles)));
+}
+
+// How an expert kernel's tiles lie: as many waves each as leave every tile its
+// place at once. Fewer waves a tile means fewer of the folds and barriers that
+// end one; with more tiles than waves a wave takes several in turn. One matrix
+// over a long reduction is taken 128 columns at a time by eight waves where
+// those tiles fill whole rounds of the CUs: twice as much in flight a wave (16
+// tokens, 14,336 x 4,096: 157 -> 138 us; with three steps a wave instead, 33
+// tokens, 768 x 2,048, 58 -> 62).
+struct FewTiles {
+  int halves, waves;
+  int64_t count;
+};
+FewTiles few_tiles(int row_tiles, int64_t experts, int64_t K, int64_t N, int64_t parts, int mats,
+                   bool pairs) {
+  FewTiles t = {1, kMaxTileWaves, experts * ceil_div(N, (int64_t)kCols) * parts};
+  const int64_t paired = experts * ceil_div(N, (int64_t)2 * kCols) * parts;
+  if (pairs && mats == 1 && K / parts >= 16 * kMaxTileWaves * kStep &&
+      paired * 20 >= ceil_div(paired, 256) * 256 * 17) {
+    t.halves = 2;
+    t.count = paired;
+  } else {
+    while (t.waves > 1 && t.count * t.waves > few_waves(row_tiles, mats)) t.waves /= 2;
+  }
+  return t;
 }
 
 struct Layout {
@@ -830,22 +884,33 @@ int check_few(int dtype, int64_t T, int32_t E, int32_t k, int64_t d, int64_t f) 
   return NT_OK;
 }
 
-template <typename T, int MT, int KW, bool NARROW>
-void launch_up(const FewArgs& a, int64_t tiles, hipStream_t stream) {
-  const dim3 grid((unsigned)std::min<int64_t>(few_waves(a.T) / kWaves, ceil_div(tiles * KW, (int64_t)kWaves)));
-  if (a.w2 != nullptr)
-    hipLaunchKernelGGL((few_up_kernel<T, true, MT, KW, NARROW>), grid, dim3(kThreads), 0, stream, a);
-  else
-    hipLaunchKernelGGL((few_up_kernel<T, false, MT, KW, NARROW>), grid, dim3(kThreads), 0, stream, a);
+// f(halves, waves of a tile) as constants. Two 64-column tiles side by side are
+// for the 16-bit types (float32's would not fit the registers).
+template <typename T, bool NARROW, typename F>
+void by_tiles(const FewTiles& t, F&& f) {
+  const auto one = std::integral_constant<int, 1>();
+  const auto eight = std::integral_constant<int, 8>();
+  if constexpr (NARROW) {
+    f(one, eight);
+  } else {
+    if (t.halves == 2) {
+      if constexpr (sizeof(typename elem<T>::storage) == 2) f(std::integral_constant<int, 2>(), eight);
+    } else if (t.waves == 8) f(one, eight);
+    else if (t.waves == 4) f(one, std::integral_constant<int, 4>());
+    else if (t.waves == 2) f(one, std::integral_constant<int, 2>());
+    else f(one, one);
+  }
 }
-template <typename T, int MT, int KW, bool NARROW>
-void launch_down(const FewArgs& a, int64_t tiles, hipStream_t stream) {
-  const dim3 grid((unsigned)std::min<int64_t>(few_waves(a.T) / kWaves, ceil_div(tiles * KW, (int64_t)kWaves)));
-  hipLaunchKernelGGL((few_down_kernel<T, MT, KW, NARROW>), grid, dim3(kThreads), 0, stream, a);
+// A workgroup for every group_waves / KW tiles, up to eight on each CU: past
+// that they take several in turn.
+dim3 few_grid(int64_t tiles, int tile_waves) {
+  return dim3((unsigned)std::min<int64_t>(
+      8192 / group_waves(tile_waves), ceil_div(tiles * tile_waves, (int64_t)group_waves(tile_waves))));
 }
 
 template <typename T, int MT, bool NARROW>
 void launch_few(FewArgs a, hipStream_t stream) {
+  constexpr bool kPairs = sizeof(typename elem<T>::storage) == 2;
   // Routing inside the up projection while it is short (see route_here): at
   // most 256 multiply-adds or 128 comparisons a thread.
   const int64_t n = (int64_t)a.T * a.E;
@@ -853,24 +918,25 @@ void launch_few(FewArgs a, hipStream_t stream) {
             (a.router == nullptr || n * a.d <= 1 << 17);
   if (!a.fused)
     hipLaunchKernelGGL((few_route_kernel<T>), dim3((unsigned)a.T), dim3(kRouteThreads), 0, stream, a);
-  const int64_t up = a.most_live * ceil_div(a.f, (int64_t)kCols);
-  const int64_t down = a.most_live * ceil_div(a.d, (int64_t)kCols) * a.splits;
-  const int up_waves = NARROW ? kWaves : few_tile_waves(a.T, up);
-  const int down_waves = NARROW ? kWaves : few_tile_waves(a.T, down);
-  a.arrive = down_waves == kWaves && down <= few_waves(a.T) / kWaves;
-  if constexpr (NARROW) {
-    launch_up<T, MT, 8, true>(a, up, stream);
-    launch_down<T, MT, 8, true>(a, down, stream);
-  } else {
-    if (up_waves == 8) launch_up<T, MT, 8, false>(a, up, stream);
-    else if (up_waves == 4) launch_up<T, MT, 4, false>(a, up, stream);
-    else if (up_waves == 2) launch_up<T, MT, 2, false>(a, up, stream);
-    else launch_up<T, MT, 1, false>(a, up, stream);
-    if (down_waves == 8) launch_down<T, MT, 8, false>(a, down, stream);
-    else if (down_waves == 4) launch_down<T, MT, 4, false>(a, down, stream);
-    else if (down_waves == 2) launch_down<T, MT, 2, false>(a, down, stream);
-    else launch_down<T, MT, 1, false>(a, down, stream);
-  }
+  const bool swiglu = a.w2 != nullptr;
+  const FewTiles up = few_tiles(MT, a.most_live, a.d, a.f, 1, swiglu ? 2 : 1, kPairs);
+  by_tiles<T, NARROW>(up, [&](auto halves, auto waves) {
+    constexpr int H = decltype(halves)::value, KW = decltype(waves)::value;
+    const dim3 grid = few_grid(up.count, KW), block(group_waves(KW) * kWave);
+    if (swiglu && H == 1)
+      hipLaunchKernelGGL((few_up_kernel<T, true, 1, MT, KW, NARROW>), grid, block, 0, stream, a);
+    if (!swiglu)
+      hipLaunchKernelGGL((few_up_kernel<T, false, H, MT, KW, NARROW>), grid, block, 0, stream, a);
+  });
+  const FewTiles down = few_tiles(MT, a.most_live, a.f, a.d, a.splits, 1, kPairs);
+  // 16 arrivals on a counter cost less than a launch, 40 do not
+  a.arrive = down.halves == 1 && down.waves == kMaxTileWaves && down.count <= 512 &&
+             a.most_live * a.splits <= 16;
+  by_tiles<T, NARROW>(down, [&](auto halves, auto waves) {
+    constexpr int H = decltype(halves)::value, KW = decltype(waves)::value;
+    hipLaunchKernelGGL((few_down_kernel<T, H, MT, KW, NARROW>), few_grid(down.count, KW),
+                       dim3(group_waves(KW) * kWave), 0, stream, a);
+  });
   if (!a.arrive)
     hipLaunchKernelGGL((few_combine_kernel<T>),
                        dim3((unsigned)ceil_div(a.d, (int64_t)256), (unsigned)a.T), dim3(256), 0,
@@ -881,8 +947,11 @@ template <typename T>
 void launch_few(const FewArgs& a, hipStream_t stream) {
   // a lane's four columns have to exist (the loads' width)
   if (a.d < 4 || a.f < 4) launch_few<T, 4, true>(a, stream);
-  // tokens an expert can have at most, in row tiles
-  else if (a.T <= kRowsMma) launch_few<T, 1, false>(a, stream);
+  // Row tiles taken at once: those of the most tokens that an expert can have;
+  // one where experts have few tokens on average (one that has more reads its
+  // weights again for every 16), since more take the registers that hold twice
+  // the waves (33 tokens, top-8 of 128: 143 -> 131 us).
+  else if (a.T <= kRowsMma || a.T * a.k <= 4 * a.E) launch_few<T, 1, false>(a, stream);
   else if (a.T <= 2 * kRowsMma) launch_few<T, 2, false>(a, stream);
   else launch_few<T, 4, false>(a, stream);
 }
