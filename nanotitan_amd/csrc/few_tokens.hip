@@ -40,6 +40,9 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 struct LiveExpert;
 
+// Routing in a launch of its own, or in every workgroup of the up projection.
+enum { kRouteApart = 0, kRouteFused = 1, kRouteSmall = 2 };
+
 struct FewArgs {
   const void* x;        // [T, d]
   const float* router;  // [E, d], or null
@@ -48,7 +51,8 @@ struct FewArgs {
   const void* w3;       // [E, f, d]
   int32_t T, E, k, splits;
   int32_t most_live;  // experts that can have tokens, at most
-  bool fused, arrive; // routing in the up projection; gate sum in the down projection
+  int32_t route;      // where the routing is done
+  bool arrive;        // gate sum in the down projection
   int64_t d, f;
   float* gates;    // [T, k]
   int32_t* topk;   // [T, k]
@@ -205,33 +209,40 @@ __global__ void __launch_bounds__(kRouteThreads) few_route_kernel(FewArgs a) {
 // its gap) that it saves. A choice's place is the number of logits ahead of
 // it, so that no selection waits for another: s_topk and s_value [T k].
 constexpr int kFusedLogits = 512;
-template <typename T>
-__device__ __forceinline__ void route_here(const FewArgs& a, float* s_logit, int32_t* s_topk,
-                                           float* s_value) {
+template <typename T, int N>
+__device__ __forceinline__ void router_here(const FewArgs& a, float* s_logit) {
   typedef typename elem<T>::storage S;
-  const int n = a.T * a.E;
-  if (a.router != nullptr) {
-    constexpr int N = 4;
-    const int waves = blockDim.x / kWave;
-    for (int i0 = threadIdx.x / kWave; i0 < n; i0 += N * waves) {
-      const S* xs[N];
-      const float* ws[N];
-      float sum[N];
+  const int n = a.T * a.E, waves = blockDim.x / kWave;
+  for (int i0 = threadIdx.x / kWave; i0 < n; i0 += N * waves) {
+    const S* xs[N];
+    const float* ws[N];
+    float sum[N];
 #pragma unroll
-      for (int q = 0; q < N; ++q) {
-        const int i = i0 + q * waves < n ? i0 + q * waves : i0;
-        xs[q] = static_cast<const S*>(a.x) + (int64_t)(i / a.E) * a.d;
-        ws[q] = a.router + (int64_t)(i % a.E) * a.d;
-      }
-      dot_part<T, N>(xs, ws, 0, a.d, sum);
-#pragma unroll
-      for (int q = 0; q < N; ++q)
-        if (lane_id() == 0 && i0 + q * waves < n) s_logit[i0 + q * waves] = sum[q];
+    for (int q = 0; q < N; ++q) {
+      const int i = i0 + q * waves < n ? i0 + q * waves : i0;
+      xs[q] = static_cast<const S*>(a.x) + (int64_t)(i / a.E) * a.d;
+      ws[q] = a.router + (int64_t)(i % a.E) * a.d;
     }
+    dot_part<T, N>(xs, ws, 0, a.d, sum);
+#pragma unroll
+    for (int q = 0; q < N; ++q)
+      if (lane_id() == 0 && i0 + q * waves < n) s_logit[i0 + q * waves] = sum[q];
+  }
+}
+template <typename T>
+__device__ __forceinline__ void logits_here(const FewArgs& a, float* s_logit) {
+  if (a.router == nullptr) {
+    for (int i = threadIdx.x; i < a.T * a.E; i += blockDim.x) s_logit[i] = a.logits[i];
+  } else if (a.T * a.E * kWave <= 2 * (int)blockDim.x) {
+    router_here<T, 2>(a, s_logit);
   } else {
-    for (int i = threadIdx.x; i < n; i += blockDim.x) s_logit[i] = a.logits[i];
+    router_here<T, 4>(a, s_logit);
   }
   __syncthreads();
+}
+__device__ __forceinline__ void route_here(const FewArgs& a, const float* s_logit, int32_t* s_topk,
+                                           float* s_value) {
+  const int n = a.T * a.E;
   for (int i = threadIdx.x; i < n; i += blockDim.x) {
     const int t = i / a.E, e = i - t * a.E;
     const uint64_t key = choice_key(s_logit[i], e);
@@ -306,6 +317,66 @@ __device__ __forceinline__ void write_plan(const FewArgs& a, const int32_t* topk
   if (threadIdx.x == 0) a.live[0] = {s.num_live, 0, 0, 0};
   for (int i = threadIdx.x; i < ceil_div(a.d, (int64_t)kCols); i += blockDim.x) a.arrived[i] = 0;
 }
+
+// The same for at most eight tokens and 64 experts, by every wave on its own and
+// in registers (lane e: expert e), with one barrier where the plan in LDS takes
+// six: latency is all that such a call costs.
+constexpr int kSmallTokens = 8;
+struct SmallPlan {
+  uint32_t mask, first;  // of expert lane_id()
+  uint64_t live;
+
+  __device__ __forceinline__ void make(const FewArgs& a, const float* s_logit, int32_t* s_topk,
+                                       float* s_value) {
+    const int e = lane_id();
+    const bool writer = blockIdx.x == 0 && threadIdx.x < kWave;
+    mask = 0;
+    for (int t = 0; t < a.T; ++t) {
+      const float z = e < a.E ? s_logit[t * a.E + e] : 0.f;
+      const uint64_t key = e < a.E ? choice_key(z, e) : 0ull;
+      const uint32_t lo = (uint32_t)key, hi = (uint32_t)(key >> 32);
+      int ahead = 0;
+      for (int o = 0; o < a.E; ++o) {
+        const uint64_t other = ((uint64_t)(uint32_t)__builtin_amdgcn_readlane(hi, o) << 32) |
+                               (uint32_t)__builtin_amdgcn_readlane(lo, o);
+        ahead += other > key;
+      }
+      if (e < a.E && ahead < a.k) {
+        mask |= 1u << t;
+        if (writer) {
+          s_topk[t * a.k + ahead] = e;
+          s_value[t * a.k + ahead] = z;
+        }
+      }
+    }
+    const int n = __popc(mask);
+    first = (uint32_t)(wave_incl_scan(n) - n);
+    live = ballot(n > 0);
+    if (!writer) return;
+    lds_wave_sync();
+    for (int i = lane_id(); i < ((a.T * a.k + kWave - 1) & -kWave); i += kWave) {
+      const bool in = i < a.T * a.k;
+      const int t = in ? i / a.k : 0, c = in ? s_topk[i] : 0;
+      const uint32_t its_first = __shfl(first, c, kWave), its_mask = __shfl(mask, c, kWave);
+      if (!in) continue;
+      const float* v = s_value + t * a.k;
+      float den = 0.f;
+      for (int j = 0; j < a.k; ++j) den += expf(v[j] - v[0]);
+      a.gates[i] = expf(s_value[i] - v[0]) * (1.f / den);
+      a.topk[i] = c;
+      a.inv[i] = (int32_t)its_first + __popc(its_mask & ((1u << t) - 1));
+    }
+    if (n > 0) a.live[1 + popc64(live & lanemask_lt())] = {e, (int32_t)first, n, 0};
+    if (lane_id() == 0) a.live[0] = {popc64(live), 0, 0, 0};
+    for (int i = lane_id(); i < ceil_div(a.d, (int64_t)kCols); i += kWave) a.arrived[i] = 0;
+  }
+  // The i-th live expert (uniform).
+  __device__ __forceinline__ int expert(int i) const {
+    uint64_t m = live;
+    for (; i > 0; --i) m &= m - 1;
+    return __builtin_ctzll(m);
+  }
+};
 
 // The r-th token of a mask.
 __device__ __forceinline__ int nth_token(uint64_t mask, int r) {
@@ -627,34 +698,49 @@ __global__ void __launch_bounds__(group_waves(KW) * kWave) few_up_kernel(FewArgs
   __shared__ Plan s_plan;
   __shared__ __attribute__((aligned(16))) float
       s_acc[KW == 1 ? 3 * kFusedLogits : kWaves * MATS * kRowsMma * kCols];
-  const int32_t* topk = a.topk;
-  if (a.fused) {
-    int32_t* s_topk = reinterpret_cast<int32_t*>(s_acc + kFusedLogits);
-    route_here<T>(a, s_acc, s_topk, s_acc + 2 * kFusedLogits);
-    topk = s_topk;
-  }
-  make_plan(a, topk, s_plan);
   const int lane = lane_id();
-  if (blockIdx.x == 0) write_plan(a, topk, s_plan);
+  const bool small = KW == kMaxTileWaves && a.route == kRouteSmall;
+  SmallPlan here = {};
+  int num_live;
+  if (small) {
+    logits_here<T>(a, s_acc);
+    here.make(a, s_acc, reinterpret_cast<int32_t*>(s_acc + kFusedLogits), s_acc + 2 * kFusedLogits);
+    num_live = popc64(here.live);
+  } else {
+    const int32_t* topk = a.topk;
+    if (a.route == kRouteFused) {
+      int32_t* s_topk = reinterpret_cast<int32_t*>(s_acc + kFusedLogits);
+      logits_here<T>(a, s_acc);
+      route_here(a, s_acc, s_topk, s_acc + 2 * kFusedLogits);
+      topk = s_topk;
+    }
+    make_plan(a, topk, s_plan);
+    if (blockIdx.x == 0) write_plan(a, topk, s_plan);
+    num_live = s_plan.num_live;
+  }
   const int64_t per = ceil_div(a.f, (int64_t)kCols * HALVES), steps = ceil_div(a.d, (int64_t)kStep);
-  const int64_t items = s_plan.num_live * per;
+  const int64_t items = num_live * per;
   const int group = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave / KW);
   for (int64_t first = (int64_t)blockIdx.x * kTiles; first < items;
        first += (int64_t)gridDim.x * kTiles) {
     // past the last tile, a group repeats it and stores nothing
     const int64_t item = first + group < items ? first + group : items - 1;
-    const int e = __builtin_amdgcn_readfirstlane(s_plan.live[item / per]);
+    const int e = __builtin_amdgcn_readfirstlane(small ? here.expert((int)(item / per))
+                                                      : s_plan.live[item / per]);
     const int64_t col = item % per * HALVES * kCols;
     TileColumns tc[MATS];
 #pragma unroll
     for (int i = 0; i < MATS; ++i) tc[i] = TileColumns(col + i * (HALVES - 1) * kCols, a.f);
-    const uint64_t mask = s_plan.mask[e];
+    const uint64_t mask =
+        small ? (uint32_t)__builtin_amdgcn_readlane(here.mask, e) : s_plan.mask[e];
+    const int first_row =
+        small ? __builtin_amdgcn_readlane(here.first, e) : (int)s_plan.first[e];
     const int rows = __builtin_amdgcn_readfirstlane(popc64(mask));
     const S* w[MATS];
     w[0] = static_cast<const S*>(a.w1) + (int64_t)e * a.d * a.f;
     if constexpr (MATS == 2)
       w[1] = static_cast<const S*>(SWIGLU ? a.w2 : a.w1) + (int64_t)e * a.d * a.f;
-    S* hidden = static_cast<S*>(a.hidden) + (int64_t)s_plan.first[e] * a.f;
+    S* hidden = static_cast<S*>(a.hidden) + (int64_t)first_row * a.f;
     // MT x 16 rows at a time. Two groups in a workgroup may have different
     // numbers of rows: the barriers of the fold are the same for both.
     int most = rows;
@@ -914,12 +1000,15 @@ void launch_few(FewArgs a, hipStream_t stream) {
   // Routing inside the up projection while it is short (see route_here): at
   // most 256 multiply-adds or 128 comparisons a thread.
   const int64_t n = (int64_t)a.T * a.E;
-  a.fused = n <= kFusedLogits && a.T * a.k <= kFusedLogits && n * a.E <= 1 << 16 &&
-            (a.router == nullptr || n * a.d <= 1 << 17);
-  if (!a.fused)
-    hipLaunchKernelGGL((few_route_kernel<T>), dim3((unsigned)a.T), dim3(kRouteThreads), 0, stream, a);
   const bool swiglu = a.w2 != nullptr;
   const FewTiles up = few_tiles(MT, a.most_live, a.d, a.f, 1, swiglu ? 2 : 1, kPairs);
+  a.route = kRouteApart;
+  if (n <= kFusedLogits && a.T * a.k <= kFusedLogits && n * a.E <= 1 << 16 &&
+      (a.router == nullptr || n * a.d <= 1 << 17))
+    a.route = a.T <= kSmallTokens && a.E <= kWave && up.waves == kMaxTileWaves ? kRouteSmall
+                                                                               : kRouteFused;
+  if (a.route == kRouteApart)
+    hipLaunchKernelGGL((few_route_kernel<T>), dim3((unsigned)a.T), dim3(kRouteThreads), 0, stream, a);
   by_tiles<T, NARROW>(up, [&](auto halves, auto waves) {
     constexpr int H = decltype(halves)::value, KW = decltype(waves)::value;
     const dim3 grid = few_grid(up.count, KW), block(group_waves(KW) * kWave);

@@ -109,6 +109,58 @@ def test_all_tokens_on_one_expert(ext, dtype, T):
     _check(x, None, logits.cuda(), weights, 2)
 
 
+# T, d, f, E, k, skew: by the number of column tiles, 8, 4, 2 and 1 waves take one; long
+# reductions take 128 columns at a time; an expert past 16 tokens among many with few
+# takes its weights more than once.
+LAYOUTS = [(64, 72, 1000, 24, 1, False), (64, 72, 1000, 48, 2, True), (40, 72, 1000, 64, 2, True),
+           (64, 72, 1000, 128, 2, True), (12, 1000, 72, 128, 4, False), (33, 1000, 72, 128, 2, True),
+           (5, 8192, 4096, 4, 2, False), (30, 8192, 4096, 4, 2, False), (64, 8000, 4100, 4, 3, False),
+           (20, 4100, 8000, 4, 2, False), (3, 4096, 8192, 4, 4, False), (9, 64, 4096, 32, 2, False)]
+
+
+@pytest.mark.parametrize("dtype,ffn", [("bf16", "swiglu"), ("fp16", "gelu"), ("fp32", "swiglu")])
+@pytest.mark.parametrize("T,d,f,E,k,skew", LAYOUTS)
+def test_every_tile_layout(ext, dtype, ffn, T, d, f, E, k, skew):
+    dt = TYPES[dtype]
+    g = torch.Generator(device="cuda").manual_seed(T + E)
+
+    def t(*shape, std):
+        return (torch.empty(shape, device="cuda").normal_(0, std, generator=g)).to(dt)
+
+    x = t(T, d, std=1.0)
+    up = [t(E, d, f, std=d**-0.5) for _ in range(2 if ffn == "swiglu" else 1)]
+    weights = (*up, t(E, f, d, std=f**-0.5))
+    logits = torch.empty(T, E, device="cuda").normal_(generator=g)
+    if skew:
+        logits[:, E // 3] += 50.0
+        logits[: T // 2, E - 1] += 40.0
+    with torch.no_grad():
+        out, gates, ids = moe_few_tokens(x, weights, k, logits=logits)
+    want_gates, want_ids = route_fn(logits, k)
+    assert torch.equal(ids, want_ids)
+    want = torch.zeros(T, d, device="cuda", dtype=torch.float64)
+    for e in torch.unique(ids).tolist():
+        tok, j = torch.nonzero(ids == e, as_tuple=True)
+        a = x[tok].double()
+        z = a @ weights[0][e].double()
+        if ffn == "swiglu":
+            h = torch.nn.functional.silu(z) * (a @ weights[1][e].double())
+        else:
+            h = torch.nn.functional.gelu(z)
+        w = want_gates[tok, j].double().unsqueeze(1)
+        want.index_add_(0, tok, w * (h @ weights[-1][e].double()))
+    # the roundings of the output and of the hidden values, half a step of the norm each at
+    # most; float32 sums of d terms, then f, in chains of at most K / 32 + 8 additions, whose
+    # errors add up like those of independent roundings
+    ulps = (max(d, f) / 32 + 8) * U
+    eps = torch.finfo(dt).eps if dt != torch.float32 else 0.0
+    err = (out.double() - want).norm(dim=1)
+    assert bool((err <= (eps + 8 * ulps) * want.norm(dim=1)).all()), float(
+        (err / want.norm(dim=1)).max())
+    with torch.no_grad():
+        assert torch.equal(moe_few_tokens(x, weights, k, logits=logits)[0], out)
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 def test_any_alignment(ext, dtype):
     for shift in (1, 2, 3):
