@@ -146,13 +146,24 @@ __global__ void __launch_bounds__(kRouteThreads) few_route_kernel(FewArgs a) {
     int parts = 1;
     while (2 * parts * a.E <= kRouteWaves) parts *= 2;
     const int64_t width = round_up(ceil_div(a.d, (int64_t)parts), 4);
-    for (int i = wave; i < a.E * parts; i += kRouteWaves) {
-      const int64_t c0 = (i % parts) * width, c1 = c0 + width < a.d ? c0 + width : a.d;
-      const S* const xs[1] = {x};
-      const float* const ws[1] = {a.router + (int64_t)(i / parts) * a.d};
-      float sum[1];
-      dot_part<T, 1>(xs, ws, c0, c1, sum);
-      if (lane == 0) (parts > 1 ? s_part : s_logit)[i] = sum[0];
+    constexpr int N = 4;
+    for (int i0 = wave; i0 < a.E * parts; i0 += N * kRouteWaves) {
+      const int64_t c0 = i0 % parts * width, c1 = c0 + width < a.d ? c0 + width : a.d;
+      const S* xs[N];
+      const float* ws[N];
+      float sum[N];
+#pragma unroll
+      for (int q = 0; q < N; ++q) {  // (with parts > 1 there is one each)
+        const int i = i0 + q * kRouteWaves < a.E * parts ? i0 + q * kRouteWaves : i0;
+        xs[q] = x;
+        ws[q] = a.router + (int64_t)(i / parts) * a.d;
+      }
+      dot_part<T, N>(xs, ws, c0, c1, sum);
+#pragma unroll
+      for (int q = 0; q < N; ++q) {
+        const int i = i0 + q * kRouteWaves;
+        if (lane == 0 && i < a.E * parts) (parts > 1 ? s_part : s_logit)[i] = sum[q];
+      }
     }
     if (parts > 1) {
       __syncthreads();
@@ -913,12 +924,23 @@ int64_t few_waves(int row_tiles, int mats) {
   return 256 * (16 - 4 * (mats - 1) - (row_tiles == 1 ? 0 : 4));
 }
 
-// Parts of the down projection's reduction: as many as give every CU two
-// tiles, each with a k-step for every wave.
+// Row tiles taken at once: those of the most tokens that an expert can have; one
+// where experts have few tokens on average (one that has more reads its weights
+// again for every 16), since more take the registers that hold twice the waves
+// (33 tokens, top-8 of 128: 143 -> 131 us).
+int few_row_tiles(int64_t T, int32_t k, int32_t E) {
+  if (T <= kRowsMma || T * k <= 4 * E) return 1;
+  return T <= 2 * kRowsMma ? 2 : 4;
+}
+
+// Parts of the down projection's reduction: as many as give every CU the
+// workgroups that it holds (two with one row tile), each with two k-steps for
+// every wave (one token of 512: 17.3 us, with one k-step 17.9).
 int32_t few_splits(int64_t T, int32_t k, int32_t E, int64_t d, int64_t f) {
   const int64_t tiles = std::min<int64_t>(T * k, E) * ceil_div(d, (int64_t)kCols);
-  const int64_t most = std::max<int64_t>(1, ceil_div(f, (int64_t)kStep) / kMaxTileWaves);
-  return (int32_t)std::max<int64_t>(1, std::min(most, 512 / std::max<int64_t>(1, tiles)));
+  const int64_t most = std::max<int64_t>(1, ceil_div(f, (int64_t)kStep) / (2 * kMaxTileWaves));
+  const int64_t slots = few_row_tiles(T, k, E) == 1 ? 512 : 256;
+  return (int32_t)std::max<int64_t>(1, std::min(most, slots / std::max<int64_t>(1, tiles)));
 }
 
 // How an expert kernel's tiles lie: as many waves each as leave every tile its
@@ -998,13 +1020,14 @@ template <typename T, int MT, bool NARROW>
 void launch_few(FewArgs a, hipStream_t stream) {
   constexpr bool kPairs = sizeof(typename elem<T>::storage) == 2;
   // Routing inside the up projection while it is short (see route_here): at
-  // most 256 multiply-adds or 128 comparisons a thread.
+  // most 128 comparisons a thread, and eight of the router's sums a wave
+  // (with 32, in workgroups of four waves, 8 tokens took 40 us for 28).
   const int64_t n = (int64_t)a.T * a.E;
   const bool swiglu = a.w2 != nullptr;
   const FewTiles up = few_tiles(MT, a.most_live, a.d, a.f, 1, swiglu ? 2 : 1, kPairs);
   a.route = kRouteApart;
   if (n <= kFusedLogits && a.T * a.k <= kFusedLogits && n * a.E <= 1 << 16 &&
-      (a.router == nullptr || n * a.d <= 1 << 17))
+      (a.router == nullptr || (n <= 8 * up.waves && n * a.d <= 1 << 15)))
     a.route = a.T <= kSmallTokens && a.E <= kWave && up.waves == kMaxTileWaves ? kRouteSmall
                                                                                : kRouteFused;
   if (a.route == kRouteApart)
@@ -1018,9 +1041,11 @@ void launch_few(FewArgs a, hipStream_t stream) {
       hipLaunchKernelGGL((few_up_kernel<T, false, H, MT, KW, NARROW>), grid, block, 0, stream, a);
   });
   const FewTiles down = few_tiles(MT, a.most_live, a.f, a.d, a.splits, 1, kPairs);
-  // 16 arrivals on a counter cost less than a launch, 40 do not
+  // 16 arrivals on a counter and the sum of a few tokens by one workgroup cost
+  // less than a launch (one token of 512: 17 against 19 us); 40 arrivals, or 32
+  // tokens, do not (25 against 22)
   a.arrive = down.halves == 1 && down.waves == kMaxTileWaves && down.count <= 512 &&
-             a.most_live * a.splits <= 16;
+             a.most_live * a.splits <= 16 && a.T <= kSmallTokens;
   by_tiles<T, NARROW>(down, [&](auto halves, auto waves) {
     constexpr int H = decltype(halves)::value, KW = decltype(waves)::value;
     hipLaunchKernelGGL((few_down_kernel<T, H, MT, KW, NARROW>), few_grid(down.count, KW),
@@ -1036,12 +1061,9 @@ template <typename T>
 void launch_few(const FewArgs& a, hipStream_t stream) {
   // a lane's four columns have to exist (the loads' width)
   if (a.d < 4 || a.f < 4) launch_few<T, 4, true>(a, stream);
-  // Row tiles taken at once: those of the most tokens that an expert can have;
-  // one where experts have few tokens on average (one that has more reads its
-  // weights again for every 16), since more take the registers that hold twice
-  // the waves (33 tokens, top-8 of 128: 143 -> 131 us).
-  else if (a.T <= kRowsMma || a.T * a.k <= 4 * a.E) launch_few<T, 1, false>(a, stream);
-  else if (a.T <= 2 * kRowsMma) launch_few<T, 2, false>(a, stream);
+  else if (const int tiles = few_row_tiles(a.T, a.k, a.E); tiles == 1)
+    launch_few<T, 1, false>(a, stream);
+  else if (tiles == 2) launch_few<T, 2, false>(a, stream);
   else launch_few<T, 4, false>(a, stream);
 }
 
