@@ -279,8 +279,12 @@ class MoE(nn.Module):
             logits = self.router(flat.to(self.router.weight.dtype))
             route = {"logits": logits.float().contiguous()}
         e = self.experts
-        weights = ((e.W_gate, e.W_val, e.W_out) if isinstance(e, ExpertFFN)
-                   else (e.W_up, e.W_down))
+        if type(e) is ExpertFFN:
+            weights = (e.W_gate, e.W_val, e.W_out)
+        elif type(e) is GeluExpertFFN:
+            weights = (e.W_up, e.W_down)
+        else:
+            raise RuntimeError(f"decode runs this package's experts, not {type(e).__name__}")
         return moe_few_tokens(flat, weights, self.cfg.top_k, **route)[0].view(x.shape)
 
 
@@ -314,6 +318,8 @@ class MoEBlock(nn.Module):
         self.scale = param(residual_scale is not None, residual_scale)
 
     def _run(self, moe, x, normed, gate, following):
+        if following is not None and (following.norm, following.eps) != (self.norm, self.eps):
+            raise ValueError("a following block's norm must be of this block's kind and eps")
         if normed is None:
             normed = pre_norm_fn(x, self.pre_weight, self.pre_bias, self.norm, self.eps,
                                  self.pre_weight.dtype)

@@ -1,10 +1,13 @@
 """Few-token layer, block norms and 8-bit checkpoints without a GPU: the 64-bit
 oracle of the checkpoint format, and the refusals of the C ABI and the wrappers."""
 
+from types import SimpleNamespace
+
 import pytest
 import torch
 
 from nanotitan_amd import capi, moe_ops
+from nanotitan_amd.layer import MoE, MoEBlock
 
 
 def kept64(x):
@@ -198,3 +201,31 @@ def test_wrappers_refuse_before_the_extension_runs():
         moe_ops.moe_few_tokens(x.requires_grad_(), (up, down), 1, logits=torch.zeros(4, 2))
     with torch.no_grad(), pytest.raises(RuntimeError, match="GPU tensor"):
         moe_ops.moe_few_tokens(x, (up, down), 1, logits=torch.zeros(4, 2))
+
+
+def _cfg(**over):
+    return SimpleNamespace(**dict(num_experts=2, top_k=1, d_model=8, ffn_in=16, moe_backend="hip",
+                                  dtype=torch.float32, router_alpha=0.01) | over)
+
+
+def test_decode_refuses_foreign_experts():
+    """Their weights may have another layout, or their forward another formula."""
+    class Experts(torch.nn.Module):
+        def __init__(self):
+            super().__init__()
+            self.W_up, self.W_down = torch.zeros(2, 8, 16), torch.zeros(2, 16, 8)
+
+    moe = MoE(_cfg(), ffn="gelu")
+    moe.experts = Experts()
+    with pytest.raises(RuntimeError, match="not Experts"):
+        moe.decode(torch.zeros(1, 2, 8))
+
+
+@pytest.mark.parametrize("other", [dict(norm="layer"), dict(eps=1e-5)])
+def test_block_refuses_to_take_another_norm_along(other):
+    """One pass holds one kind of norm: the following block's would come out wrong."""
+    block, following = MoEBlock(_cfg()), MoEBlock(_cfg(), **other)
+    with pytest.raises(ValueError, match="following block's norm"):
+        block(torch.zeros(1, 2, 8), following=following)
+    with pytest.raises(ValueError, match="following block's norm"):
+        block.decode(torch.zeros(1, 2, 8), following=following)
