@@ -335,8 +335,8 @@ int nt_checkpoint8_decode(int dtype, const int8_t* codes, const uint8_t* exps, i
 
 /* act = gelu(h) (erf) and h's checkpoint; and the backward at the values h^
  * that the checkpoint holds: dh = dact * gelu'(h^), act = gelu(h^) (NULL to
- * skip). The forward keeps nothing where codes and exps are NULL. dh may
- * overwrite dact. */
+ * skip). The forward keeps nothing where codes and exps are NULL. Outputs must
+ * not overlap inputs, here and in the swiglu pair. */
 int nt_gelu_checkpoint8(int dtype, const void* h, int64_t rows, int64_t f, void* act,
                         int8_t* codes, uint8_t* exps, hipStream_t stream);
 int nt_gelu_backward8(int dtype, const void* dact, const int8_t* codes, const uint8_t* exps,
@@ -345,8 +345,7 @@ int nt_gelu_backward8(int dtype, const void* dact, const int8_t* codes, const ui
 /* hidden = silu(gate) * value and both checkpoints; and the backward at the
  * values that they hold: dgate = dhidden * value^ * silu'(gate^), dvalue =
  * dhidden * silu(gate^), hidden = silu(gate^) * value^ (NULL to skip). The
- * forward keeps nothing where all codes and exps are NULL. dgate or dvalue may
- * overwrite dhidden. */
+ * forward keeps nothing where all codes and exps are NULL. */
 int nt_swiglu_checkpoint8(int dtype, const void* gate, const void* value, int64_t rows, int64_t f,
                           void* hidden, int8_t* gate_codes, uint8_t* gate_exps,
                           int8_t* value_codes, uint8_t* value_exps, hipStream_t stream);
@@ -367,9 +366,9 @@ int nt_swiglu_backward8(int dtype, const void* dhidden, const int8_t* gate_codes
  * scale [scale_cols] (1 or d) of param_dtype (f32, f16, bf16). gate, scale, b
  * and b_next may be NULL (1, 1, 0, 0); rms norms take no bias. y NULL: h is x
  * and not written, n = N(x). stats [T,4] f32 keeps the rows' means and r for
- * the backward (NULL to skip). d <= 16384. Arithmetic in float32. n may
- * overwrite y, and h may overwrite x. No counterpart in the reference, whose
- * layer calls torch's LayerNorm before the block (src/model/model.py:205-211). */
+ * the backward (NULL to skip). d <= 16384. Arithmetic in float32. Outputs must
+ * not overlap inputs. No counterpart in the reference, whose layer calls torch's
+ * LayerNorm before the block (src/model/model.py:205-211). */
 enum nt_norm_kind { NT_NORM_RMS = 0, NT_NORM_LAYER = 1 };
 int nt_block_norm(int x_dtype, int dtype, int param_dtype, int kind, const void* x, const void* y,
                   const void* w, const void* b, const void* gate, int64_t gate_cols,

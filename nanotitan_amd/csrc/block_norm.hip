@@ -168,7 +168,8 @@ int nt_block_norm(int x_dtype, int dtype, int param_dtype, int kind, const void*
       norm::by_mode(y != nullptr, gate != nullptr && gate_cols == d && d > 1, [&](auto mode) {
         typedef decltype(shape) SH;
         constexpr int M = decltype(mode)::value;
-        const dim3 grid((unsigned)norm::blocks_of(T, d, kind == NT_NORM_LAYER ? 4 : 6)), block(norm::block_threads(SH::TPR));
+        const dim3 grid((unsigned)norm::blocks_of(T, d, kind == NT_NORM_LAYER ? 4 : 6));
+        const dim3 block(norm::block_threads(SH::TPR));
         if (kind == NT_NORM_LAYER)
           hipLaunchKernelGGL((block_norm_kernel<decltype(tx), decltype(t), SH, true, M>), grid,
                              block, 0, stream, a);

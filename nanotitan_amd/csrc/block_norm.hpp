@@ -186,7 +186,8 @@ inline int64_t blocks_of(int64_t T, int64_t d, int waves) {
   int64_t n = 1;
   by_width(d, [&](auto s) {
     constexpr int TPR = decltype(s)::TPR;
-    n = std::min<int64_t>(waves * 256 * 256 / block_threads(TPR), ceil_div(T, (int64_t)(block_threads(TPR) / TPR)));
+    n = std::min<int64_t>(waves * 256 * 256 / block_threads(TPR),
+                          ceil_div(T, (int64_t)(block_threads(TPR) / TPR)));
   });
   return std::max<int64_t>(1, n);
 }

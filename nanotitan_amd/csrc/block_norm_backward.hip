@@ -33,7 +33,8 @@ struct NormGradArgs {
 };
 
 template <typename TX, typename T, typename SH, bool LAYER, int MODE>
-__global__ void __launch_bounds__(block_threads(SH::TPR)) __attribute__((amdgpu_waves_per_eu(SH::TPR >= 512 ? 4 : 1)))
+__global__ void __launch_bounds__(block_threads(SH::TPR))
+__attribute__((amdgpu_waves_per_eu(SH::TPR >= 512 ? 4 : 1)))
 block_norm_backward_kernel(NormGradArgs a) {
   typedef typename elem<T>::storage S;
   constexpr int V = SH::V, TPR = SH::TPR, CH = SH::CH;
@@ -186,7 +187,8 @@ block_norm_backward_kernel(NormGradArgs a) {
           for (int i = 0; i < V; ++i) {
             float s = 0.f;
 #pragma unroll
-            for (int r = 0; r < kRows; ++r) s += s_fold[(k * V + i) * kThreads + r * TPR + threadIdx.x];
+            for (int r = 0; r < kRows; ++r)
+              s += s_fold[(k * V + i) * kThreads + r * TPR + threadIdx.x];
             acc[q][k][i] = s;
           }
       }
@@ -319,7 +321,8 @@ int nt_block_norm_backward(int x_dtype, int dtype, int param_dtype, int kind, co
   if (T == 0 && a.sums == 0) return NT_OK;  // else one workgroup writes the sums' zeros
   const int rc = norm::by_types(x_dtype, dtype, [&](auto tx, auto t) {
     norm::by_width(d, [&](auto shape) {
-      norm::by_mode(y != nullptr || T == 0, gate != nullptr && gate_cols == d && d > 1, [&](auto mode) {
+      const bool gate_each = gate != nullptr && gate_cols == d && d > 1;
+      norm::by_mode(y != nullptr || T == 0, gate_each, [&](auto mode) {
         typedef decltype(shape) SH;
         constexpr int M = decltype(mode)::value;
         const dim3 grid((unsigned)blocks), block(norm::block_threads(SH::TPR));

@@ -3,9 +3,9 @@
 // 32 consecutive columns of a row share a power of two 2^x, x the least
 // integer (>= -127) with max|v| < 127.5 2^x; a value is kept as the int8
 // nearest to v 2^-x (ties to even) and the block as the byte x + 127. Scaling
-// by a power of two is exact, so a value is off by half a unit at most: 2^-7
-// of the block's largest value, 0.3 to 0.6 % of a normal block's deviation (an
-// 8-bit float with 3 mantissa bits: 2.6 % of each value). Decoding is exact in
+// by a power of two is exact, so a value is off by half a unit at most: 1/127.5
+// of the block's largest value, as a norm 0.5 to 1.1 % of a normal block (an
+// 8-bit float with 3 mantissa bits: 2.6 %). Decoding is exact in
 // every activation type: 7 bits fit bf16's 8. A block with an infinity or a NaN
 // gets the byte 255 and decodes to NaN; a value that rounds past the type's
 // largest decodes to that.
@@ -153,7 +153,8 @@ __device__ __forceinline__ void keep8(const Values<T>& v, int8_t* codes, uint8_t
 // 128 of its units pass float32's.
 template <typename T>
 struct range {
-  static constexpr uint32_t most = sizeof(typename elem<T>::storage) == 4 ? 0x7f7fffffu : 0x7f7f0000u;
+  static constexpr uint32_t most =
+      sizeof(typename elem<T>::storage) == 4 ? 0x7f7fffffu : 0x7f7f0000u;
   static constexpr uint32_t byte = 248;
 };
 template <>

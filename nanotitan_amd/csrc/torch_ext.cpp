@@ -1209,7 +1209,8 @@ struct BlockNormFunction : public torch::autograd::Function<BlockNormFunction> {
                                OptTensor b, OptTensor gate, OptTensor scale, OptTensor w_next,
                                OptTensor b_next, bool layer, double eps,
                                c10::optional<at::ScalarType> dtype) {
-    auto [h, n, stats] = block_norm(x, y, w, b, gate, scale, w_next, b_next, layer, eps, dtype, true);
+    auto [h, n, stats] =
+        block_norm(x, y, w, b, gate, scale, w_next, b_next, layer, eps, dtype, true);
     ctx->save_for_backward({h ? *h : x, defined(y), defined(w), defined(b), defined(gate),
                             defined(scale), defined(w_next), defined(b_next), *stats});
     ctx->saved_data["layer"] = layer;

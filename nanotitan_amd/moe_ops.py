@@ -619,7 +619,8 @@ def post_norm_fn(x, y, weight=None, bias=None, gate=None, scale=None, next_weigh
 def checkpoint8(x):
     """(codes int8 [rows,f], exponents uint8 [rows,ceil(f/32)]) of x's rows.
 
-    32 columns share a power of two; a value is off by at most 1/255 of its block's largest.
+    32 columns share a power of two; a value is off by at most 1/127.5 of its block's
+    largest. A block with an infinity or a NaN decodes to NaN.
     """
     return get_hip_extension().checkpoint8(x)
 
@@ -630,12 +631,12 @@ def checkpoint8_decode(codes, exponents, dtype):
 
 
 def gelu8_fn(h):
-    """gelu(h) (erf) with h kept in 8 bits: the backward is gelu' at the value kept."""
+    """gelu(h) (erf) of rows [rows,f], h kept in 8 bits: the backward is gelu' at the value kept."""
     return get_hip_extension().gelu8_fn(h)
 
 
 def swiglu8_fn(gate, value):
-    """silu(gate) * value with both kept in 8 bits: the backward is taken at the values kept."""
+    """silu(gate) * value of rows [rows,f], both kept in 8 bits for the backward."""
     return get_hip_extension().swiglu8_fn(gate, value)
 
 

@@ -165,6 +165,24 @@ def test_what_is_left_out(ext, kind, gate, scale, post, nxt):
             assert torch.equal(h, h2) and (n is None or torch.equal(n, n2))
 
 
+def test_any_one_input_alone(ext):
+    """Frozen inputs get no gradient, and the others the bits that they get together."""
+    c = _case(40, 264, torch.bfloat16, torch.bfloat16, torch.float32, "layer", "token", "channel",
+              True, True)
+    _, _, full = _run(c, "layer")
+    names = ["x", "y", "w", "b", "gate", "scale", "wn", "bn"]
+    for alone in names:
+        leaf = {n: c[n].cuda().requires_grad_(n == alone) for n in names}
+        h, n = post_norm_fn(leaf["x"], leaf["y"], leaf["w"], leaf["b"], gate=leaf["gate"],
+                            scale=leaf["scale"], next_weight=leaf["wn"], next_bias=leaf["bn"],
+                            kind="layer", eps=EPS)
+        outs = [(h, c["dh"].cuda())] if alone not in ("wn", "bn") else []
+        outs.append((n, c["dn"].cuda()))
+        (g,) = torch.autograd.grad([o for o, _ in outs], [leaf[alone]], [g for _, g in outs])
+        assert torch.equal(g, full[alone]), alone
+        assert all(v.grad is None for v in leaf.values())
+
+
 @pytest.mark.parametrize("dh,dn", [(True, False), (False, True)])
 @pytest.mark.parametrize("d", [72, 1536])
 def test_only_one_output_used(ext, dh, dn, d):
