@@ -10,7 +10,9 @@
 // the sums over the row and their use, the parameters read once per workgroup.
 // The loads of a row go out together; the other waves of a SIMD hide them
 // (with the next row's loads kept in flight instead, fewer waves fit: 122
-// against 112 us at 16,384 x 4,096).
+// against 112 us at 16,384 x 4,096). A workgroup that fills its CU has no others
+// and keeps the next row in flight (8,192 x 8,192, bf16: 156 -> 139 us) unless
+// its rows fill the registers (4,096 x 16,384, float32, layer: 266 -> 347).
 #include "block_norm.hpp"
 
 namespace nt {
@@ -62,6 +64,7 @@ __global__ void __launch_bounds__(block_threads(SH::TPR)) block_norm_kernel(Norm
   constexpr int kThreads = block_threads(TPR), kRows = kThreads / TPR;
   __shared__ float s_red[2 * (kThreads / kWave)];
   RowSum<TPR, 1> sum{s_red};
+  constexpr bool kAhead = TPR >= 1024 && CH == 1;
   Chunk<V> c[CH];
   float sw[CH][V], sb[CH][V], wn[CH][V], bn[CH][V];  // s w, s b, w', b'
   const float width = (float)a.d;
@@ -86,10 +89,11 @@ __global__ void __launch_bounds__(block_threads(SH::TPR)) block_norm_kernel(Norm
       if constexpr (MODE == kGated) rg[k] = load_raw<T, V>(a.gate, base, c[k]);
     }
   };
+  if constexpr (kAhead) load(row);
   for (int64_t first = (int64_t)blockIdx.x * kRows; first < a.T; first += step, row += step) {
     const bool live = row < a.T;  // rows that share a workgroup may be past the end
     const int64_t base = row * a.d;
-    load(row);
+    if constexpr (!kAhead) load(row);
     float h[CH][V], p[CH][V], g[CH][V];
 #pragma unroll
     for (int k = 0; k < CH; ++k) {
@@ -97,6 +101,7 @@ __global__ void __launch_bounds__(block_threads(SH::TPR)) block_norm_kernel(Norm
       if constexpr (MODE != kPre) values<T, V>(ry[k], c[k], p[k]);
       if constexpr (MODE == kGated) values<T, V>(rg[k], c[k], g[k]);
     }
+    if constexpr (kAhead) load(row + step);
     float mean_y = 0.f, r_y = 1.f, mean_h = 0.f, r_h = 1.f;
     if constexpr (MODE != kPre) {
       float g_row = 1.f;

@@ -7,7 +7,9 @@
 // Bound by HBM, as the forward. A thread owns the same columns of every row
 // that its workgroup takes and keeps the parameters' sums over them in
 // registers; the workgroup's rows are added through LDS at the end and the
-// workgroups' sums by a second launch, always in the same order.
+// workgroups' sums by a second launch, always in the same order. Four waves a
+// SIMD have to fit (128 registers): the parameters are parked in LDS (layer
+// norms of 131,072 x 512: 222 -> 160 us, of 16,384 x 4,096: 307 -> 199).
 #include "block_norm.hpp"
 
 namespace nt {
@@ -32,9 +34,30 @@ struct NormGradArgs {
   bool one;  // the single scale's gradient is wanted
 };
 
+// The parameters of a thread's columns, where only it reads them: a row needs
+// them twice for a moment, and the registers go to the sums.
+template <int SETS, int CH, int V, int THREADS>
+struct Parked {
+  static constexpr int W = V % 4 == 0 ? 4 : 1;  // values side by side
+  typedef float F __attribute__((ext_vector_type(W)));
+  static constexpr int kSize = SETS * CH * V / W * THREADS;
+  F* s;
+  __device__ __forceinline__ F* at(int set, int k) const {
+    return s + (set * CH + k) * (V / W) * THREADS + threadIdx.x;
+  }
+  __device__ __forceinline__ void put(int set, int k, const float (&v)[V]) const {
+#pragma unroll
+    for (int i = 0; i < V; i += W) __builtin_memcpy(at(set, k) + i / W * THREADS, v + i, sizeof(F));
+  }
+  __device__ __forceinline__ void get(int set, int k, float (&v)[V]) const {
+#pragma unroll
+    for (int i = 0; i < V; i += W) __builtin_memcpy(v + i, at(set, k) + i / W * THREADS, sizeof(F));
+  }
+};
+
 template <typename TX, typename T, typename SH, bool LAYER, int MODE>
 __global__ void __launch_bounds__(block_threads(SH::TPR))
-__attribute__((amdgpu_waves_per_eu(SH::TPR >= 512 ? 4 : 1)))
+__attribute__((amdgpu_waves_per_eu(LAYER || SH::TPR >= 512 ? 4 : 1)))
 block_norm_backward_kernel(NormGradArgs a) {
   typedef typename elem<T>::storage S;
   constexpr int V = SH::V, TPR = SH::TPR, CH = SH::CH;
@@ -42,16 +65,27 @@ block_norm_backward_kernel(NormGradArgs a) {
   __shared__ float s_red[2 * 3 * (kThreads / kWave)];
   __shared__ float s_fold[kRows > 1 ? kThreads * CH * V : 1];
   RowSum<TPR, 3> sum{s_red};
-  const int sub = threadIdx.x / TPR;
+  enum { kSW, kNext, kSB };
+  constexpr bool kParkSB = LAYER && CH == 1;  // three sets of 16,384 exceed the LDS
+  typedef Parked<kParkSB ? 3 : 2, CH, V, kThreads> Params;
+  __shared__ typename Params::F s_params[Params::kSize];
+  const Params params{s_params};
+  // a wave's rows are one: its addresses stay scalar
+  const int sub =
+      TPR >= kWave ? __builtin_amdgcn_readfirstlane(threadIdx.x / TPR) : threadIdx.x / TPR;
   Chunk<V> c[CH];
-  float acc[kSums][CH][V];
-  float sw[CH][V], sb[CH][V], wn[CH][V];
+  float acc[kSums][CH][V], sb[CH][V];
 #pragma unroll
   for (int k = 0; k < CH; ++k) {
     c[k] = Chunk<V>((k * TPR + threadIdx.x % TPR) * V, a.d);
-    if constexpr (MODE != kPre)
-      load_scaled<V, LAYER>(a.w, a.b, a.scale, a.scale_cols, a.param, c[k], sw[k], sb[k]);
-    load_params<V>(a.w_next, a.param, c[k], 1.f, wn[k]);
+    float sw[V], wn[V];
+    if constexpr (MODE != kPre) {
+      load_scaled<V, LAYER>(a.w, a.b, a.scale, a.scale_cols, a.param, c[k], sw, sb[k]);
+      params.put(kSW, k, sw);
+      if constexpr (kParkSB) params.put(kSB, k, sb[k]);
+    }
+    load_params<V>(a.w_next, a.param, c[k], 1.f, wn);
+    params.put(kNext, k, wn);
 #pragma unroll
     for (int q = 0; q < kSums; ++q)
 #pragma unroll
@@ -81,6 +115,7 @@ block_norm_backward_kernel(NormGradArgs a) {
   for (int64_t first = (int64_t)blockIdx.x * kRows; first < a.T; first += step, row += step) {
     const bool live = row < a.T;  // rows that share a workgroup may be past the end
     const int64_t base = row * a.d;
+    asm volatile("" ::: "memory");  // the parameters stay parked
     load(row);
     const float mean_y = st[0], r_y = st[1], mean_h = st[2], r_h = st[3];
     float D[CH][V], hh[CH][V], u[CH][V], y[CH][V], g[CH][V];
@@ -101,7 +136,9 @@ block_norm_backward_kernel(NormGradArgs a) {
     if (has_dn) {
       float t[3] = {0.f, 0.f, 0.f};
 #pragma unroll
-      for (int k = 0; k < CH; ++k)
+      for (int k = 0; k < CH; ++k) {
+        float wn[V];
+        params.get(kNext, k, wn);
 #pragma unroll
         for (int i = 0; i < V; ++i) {
           hh[k][i] = (hh[k][i] - mean_h) * r_h;
@@ -110,10 +147,11 @@ block_norm_backward_kernel(NormGradArgs a) {
             acc[kSumNext][k][i] = fmaf(u[k][i], hh[k][i], acc[kSumNext][k][i]);
             if constexpr (LAYER) acc[kSumNextBias][k][i] += u[k][i];
           }
-          u[k][i] *= wn[k][i];
+          u[k][i] *= wn[i];
           if constexpr (LAYER) t[0] += u[k][i];
           t[1] = fmaf(u[k][i], hh[k][i], t[1]);
         }
+      }
       sum(t);
       const float m0 = LAYER ? t[0] * inv_d : 0.f, m1 = t[1] * inv_d;
 #pragma unroll
@@ -133,21 +171,23 @@ block_norm_backward_kernel(NormGradArgs a) {
       float t[3] = {0.f, 0.f, 0.f};
 #pragma unroll
       for (int k = 0; k < CH; ++k) {
-        float dg[V];
+        float dg[V], sw[V];
+        params.get(kSW, k, sw);
+        if constexpr (kParkSB) params.get(kSB, k, sb[k]);
 #pragma unroll
         for (int i = 0; i < V; ++i) {
           const float gi = MODE == kGated ? g[k][i] : g_row;
           const float Dv = c[k].owns(i) ? D[k][i] : 0.f;
           y[k][i] = c[k].owns(i) ? (y[k][i] - mean_y) * r_y : 0.f;
           // s g p's derivative by g, and D g: times s w it is u of dN, summed A and B
-          dg[i] = Dv * (LAYER ? fmaf(y[k][i], sw[k][i], sb[k][i]) : y[k][i] * sw[k][i]);
+          dg[i] = Dv * (LAYER ? fmaf(y[k][i], sw[i], sb[k][i]) : y[k][i] * sw[i]);
           if constexpr (MODE == kPost) t[2] += dg[i];
           const float Dg = Dv * gi;
           if (live) {
             acc[kSumA][k][i] = fmaf(Dg, y[k][i], acc[kSumA][k][i]);
             if constexpr (LAYER) acc[kSumB][k][i] += Dg;
           }
-          D[k][i] = Dg * sw[k][i];
+          D[k][i] = Dg * sw[i];
           if constexpr (LAYER) t[0] += D[k][i];
           t[1] = fmaf(D[k][i], y[k][i], t[1]);
         }
