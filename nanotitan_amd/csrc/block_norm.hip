@@ -10,9 +10,17 @@
 // the sums over the row and their use, the parameters read once per workgroup.
 // The loads of a row go out together; the other waves of a SIMD hide them
 // (with the next row's loads kept in flight instead, fewer waves fit: 122
-// against 112 us at 16,384 x 4,096). A workgroup that fills its CU has no others
-// and keeps the next row in flight (8,192 x 8,192, bf16: 156 -> 139 us) unless
-// its rows fill the registers (4,096 x 16,384, float32, layer: 266 -> 347).
+// against 112 us at 16,384 x 4,096). A layer norm's workgroup that has its CU
+// alone keeps the next row in flight (8,192 x 8,192, bf16: 124 -> 104 us), but
+// not where a thread's rows fill the registers (16,384 columns).
+//
+// At 40 instructions a value, 16-bit rows would wait for the vector units: so
+// columns that a thread does not own are cleared two at a time and once, sums
+// go by lane moves, and the root is one instruction.
+//
+// Measured on MI355X (a copy: 5.65 TB/s), bf16, norm, residual and next norm:
+// 16,384 x 4,096 rms 101 us (5.3 TB/s), layer 105 (5.1); 131,072 x 512 108 and
+// 104 (5.0, 5.1); with an elementwise gate 130 and 126 (5.2, 5.3).
 #include "block_norm.hpp"
 
 namespace nt {
@@ -33,7 +41,7 @@ struct NormArgs {
 // mean and r of a row held in v (zeros where a chunk does not own a column).
 template <typename SH, bool LAYER>
 __device__ __forceinline__ void row_stats(const float (&v)[SH::CH][SH::V],
-                                          const Chunk<SH::V> (&c)[SH::CH], float d, float eps,
+                                          const Chunk<SH::V> (&c)[SH::CH], float inv_d, float eps,
                                           RowSum<SH::TPR, 1>& sum, float& mean, float& r) {
   mean = 0.f;
   if constexpr (LAYER) {
@@ -43,7 +51,7 @@ __device__ __forceinline__ void row_stats(const float (&v)[SH::CH][SH::V],
 #pragma unroll
       for (int i = 0; i < SH::V; ++i) t[0] += v[k][i];
     sum(t);
-    mean = t[0] / d;
+    mean = t[0] * inv_d;
   }
   float q[1] = {0.f};
 #pragma unroll
@@ -54,20 +62,24 @@ __device__ __forceinline__ void row_stats(const float (&v)[SH::CH][SH::V],
       q[0] = fmaf(u, u, q[0]);
     }
   sum(q);
-  // the division and the root once a row: full precision costs nothing here
-  r = 1.f / sqrtf(q[0] / d + eps);
+  // The instruction is within one unit in the last place, but for denormals,
+  // which are scaled out of its way. (A root and a division in full were 40
+  // instructions for each thread's eight values.)
+  const float var = fmaf(q[0], inv_d, eps);
+  const bool tiny = var < 0x1p-100f;
+  r = __builtin_amdgcn_rsqf(tiny ? var * 0x1p+60f : var) * (tiny ? 0x1p+30f : 1.f);
 }
 
 template <typename TX, typename T, typename SH, bool LAYER, int MODE>
 __global__ void __launch_bounds__(block_threads(SH::TPR)) block_norm_kernel(NormArgs a) {
   constexpr int V = SH::V, TPR = SH::TPR, CH = SH::CH;
   constexpr int kThreads = block_threads(TPR), kRows = kThreads / TPR;
-  __shared__ float s_red[2 * (kThreads / kWave)];
+  __shared__ float s_red[RowSum<TPR, 1>::kSize];
   RowSum<TPR, 1> sum{s_red};
-  constexpr bool kAhead = TPR >= 1024 && CH == 1;
+  constexpr bool kAhead = LAYER && TPR >= 1024 && CH == 1;
   Chunk<V> c[CH];
   float sw[CH][V], sb[CH][V], wn[CH][V], bn[CH][V];  // s w, s b, w', b'
-  const float width = (float)a.d;
+  const float inv_d = 1.f / (float)a.d;
 #pragma unroll
   for (int k = 0; k < CH; ++k) {
     c[k] = Chunk<V>((k * TPR + threadIdx.x % TPR) * V, a.d);
@@ -99,16 +111,18 @@ __global__ void __launch_bounds__(block_threads(SH::TPR)) block_norm_kernel(Norm
     for (int k = 0; k < CH; ++k) {
       values<TX, V>(rx[k], c[k], h[k]);
       if constexpr (MODE != kPre) values<T, V>(ry[k], c[k], p[k]);
-      if constexpr (MODE == kGated) values<T, V>(rg[k], c[k], g[k]);
+      if constexpr (MODE == kGated) all_values<T, V>(rg[k], g[k]);
     }
     if constexpr (kAhead) load(row + step);
+    // x, y and the parameters are zero where a chunk does not own a column, and so
+    // is h (unless a value overlapped is an infinity or NaN, as is then the row)
     float mean_y = 0.f, r_y = 1.f, mean_h = 0.f, r_h = 1.f;
     if constexpr (MODE != kPre) {
       float g_row = 1.f;
       if (MODE == kPost && a.gate != nullptr)
         g_row = elem<T>::load(
             static_cast<const typename elem<T>::storage*>(a.gate)[live ? row : a.T - 1]);
-      if (a.w != nullptr) row_stats<SH, LAYER>(p, c, width, a.eps, sum, mean_y, r_y);
+      if (a.w != nullptr) row_stats<SH, LAYER>(p, c, inv_d, a.eps, sum, mean_y, r_y);
 #pragma unroll
       for (int k = 0; k < CH; ++k) {
 #pragma unroll
@@ -117,13 +131,12 @@ __global__ void __launch_bounds__(block_threads(SH::TPR)) block_norm_kernel(Norm
           const float v = LAYER ? fmaf(hat, sw[k][i], sb[k][i]) : hat * sw[k][i];
           h[k][i] = elem<TX>::load(
               to_bits<TX>(fmaf(MODE == kGated ? g[k][i] : g_row, v, h[k][i])));
-          if (!c[k].owns(i)) h[k][i] = 0.f;
         }
         if (live) store_chunk<TX, V>(a.h, base, c[k], h[k]);
       }
     }
     if (a.w_next != nullptr) {
-      row_stats<SH, LAYER>(h, c, width, a.eps, sum, mean_h, r_h);
+      row_stats<SH, LAYER>(h, c, inv_d, a.eps, sum, mean_h, r_h);
 #pragma unroll
       for (int k = 0; k < CH; ++k) {
 #pragma unroll
@@ -173,7 +186,11 @@ int nt_block_norm(int x_dtype, int dtype, int param_dtype, int kind, const void*
       norm::by_mode(y != nullptr, gate != nullptr && gate_cols == d && d > 1, [&](auto mode) {
         typedef decltype(shape) SH;
         constexpr int M = decltype(mode)::value;
-        const dim3 grid((unsigned)norm::blocks_of(T, d, kind == NT_NORM_LAYER ? 4 : 6));
+        // Waves a SIMD. Of 6, workgroups of 16 waves would be one and a half a CU
+        // (8,192 x 8,192, bf16, rms: 110 us, against 103); of 8, layer norms' sums
+        // in turn are slower (16,384 x 4,096: 116 against 104).
+        constexpr int kWaves = SH::TPR >= 1024 ? 8 : 6;
+        const dim3 grid((unsigned)norm::blocks_of(T, d, kind == NT_NORM_LAYER ? 4 : kWaves));
         const dim3 block(norm::block_threads(SH::TPR));
         if (kind == NT_NORM_LAYER)
           hipLaunchKernelGGL((block_norm_kernel<decltype(tx), decltype(t), SH, true, M>), grid,

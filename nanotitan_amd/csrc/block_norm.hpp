@@ -42,7 +42,30 @@ __device__ __forceinline__ Raw<T, V> load_raw(const void* rows, int64_t base, co
   return *reinterpret_cast<const Raw<T, V>*>(
       static_cast<const typename elem<T>::storage*>(rows) + base + c.start);
 }
-// The values, zero where the chunk does not own them.
+// The raw values with those that the chunk does not own cleared: 16-bit ones by
+// pairs.
+template <typename T, int V>
+__device__ __forceinline__ Raw<T, V> owned(const Raw<T, V>& raw, const Chunk<V>& c) {
+  Raw<T, V> out = raw;
+  if constexpr (sizeof(raw[0]) == 2 && V % 2 == 0) {
+    typedef uint32_t Pairs __attribute__((ext_vector_type(V / 2)));
+    Pairs p = __builtin_bit_cast(Pairs, raw);
+#pragma unroll
+    for (int i = 0; i < V / 2; ++i)
+      p[i] &= (c.owns(2 * i) ? 0xffffu : 0u) | (c.owns(2 * i + 1) ? 0xffff0000u : 0u);
+    out = __builtin_bit_cast(Raw<T, V>, p);
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) out[i] = c.owns(i) ? raw[i] : 0;
+  }
+  return out;
+}
+// The values as they are, and zero where the chunk does not own them.
+template <typename T, int V>
+__device__ __forceinline__ void all_values(const Raw<T, V>& raw, float (&v)[V]) {
+#pragma unroll
+  for (int i = 0; i < V; ++i) v[i] = elem<T>::load(raw[i]);
+}
 template <typename T, int V>
 __device__ __forceinline__ void values(const Raw<T, V>& raw, const Chunk<V>& c, float (&v)[V]) {
 #pragma unroll
@@ -108,34 +131,62 @@ __device__ __forceinline__ void load_scaled(const void* w, const void* b, const 
   }
 }
 
-// Sums over the TPR threads of a row, every thread receiving them: shuffles
-// inside a wave, then LDS across the row's waves (which have the workgroup
-// alone). Calls alternate between the halves of s_red ([2][N][waves]), so that
-// one barrier each is enough.
-template <int TPR, int N>
+// v plus another lane's, by its place in a row of 16 lanes.
+template <int CTRL, int ROWS = 0xf>
+__device__ __forceinline__ float plus_lane(float v) {
+  return v + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, ROWS, 0xf,
+                                                        ROWS == 0xf));
+}
+// Sum over each LANES neighbouring lanes, which all receive it.
+template <int LANES>
+__device__ __forceinline__ float lanes_sum(float v) {
+  static_assert(LANES <= 16, "a row of lanes");
+  if constexpr (LANES >= 2) v = plus_lane<0xb1>(v);   // lane ^ 1
+  if constexpr (LANES >= 4) v = plus_lane<0x4e>(v);   // lane ^ 2
+  if constexpr (LANES >= 8) v = plus_lane<0x141>(v);  // 7 - lane, of each 8
+  if constexpr (LANES >= 16) v = plus_lane<0x140>(v); // 15 - lane, of each 16
+  return v;
+}
+// Sum over the wave: in its last lane.
+__device__ __forceinline__ float last_lane_sum(float v) {
+  v = lanes_sum<16>(v);
+  v = plus_lane<0x142, 0xa>(v);  // lane 15 of a row to the next, rows 1 and 3
+  return plus_lane<0x143, 0xc>(v);  // lane 31 to rows 2 and 3
+}
+
+// Sums over the TPR threads of a row, every thread receiving them: inside a
+// wave by lane moves (shuffles through LDS took a fifth of a row's
+// instructions), then through LDS across the row's waves, which have the
+// workgroup alone. Calls alternate between the halves of s_red ([2][kMost]
+// [waves]), so that one barrier each is enough.
+template <int TPR, int MOST>
 struct RowSum {
+  static constexpr int W = TPR > kWave ? TPR / kWave : 1;
+  static constexpr int kSize = 2 * MOST * W;
   float* s_red;
   int half = 0;
+  template <int N>
   __device__ __forceinline__ void operator()(float (&v)[N]) {
+    static_assert(N <= MOST && (TPR == 16 || TPR >= kWave), "row sums");
+    if constexpr (TPR == 16) {
 #pragma unroll
-    for (int o = (TPR < kWave ? TPR : kWave) / 2; o >= 1; o >>= 1)
+      for (int i = 0; i < N; ++i) v[i] = lanes_sum<16>(v[i]);
+    } else if constexpr (TPR == kWave) {
 #pragma unroll
-      for (int i = 0; i < N; ++i) v[i] += __shfl_xor(v[i], o, kWave);
-    if constexpr (TPR > kWave) {
-      constexpr int W = TPR / kWave;
-      float* s = s_red + half * N * W;
+      for (int i = 0; i < N; ++i)
+        v[i] = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(last_lane_sum(v[i])), 63));
+    } else {
+      float* s = s_red + half * MOST * W;
       half ^= 1;
-      if (lane_id() == 0) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[i] = last_lane_sum(v[i]);
+      if (lane_id() == kWave - 1) {
 #pragma unroll
         for (int i = 0; i < N; ++i) s[i * W + threadIdx.x / kWave] = v[i];
       }
       __syncthreads();
 #pragma unroll
-      for (int i = 0; i < N; ++i) {
-        v[i] = 0.f;
-#pragma unroll
-        for (int w = 0; w < W; ++w) v[i] += s[i * W + w];
-      }
+      for (int i = 0; i < N; ++i) v[i] = lanes_sum<W>(s[i * W + lane_id() % W]);
     }
   }
 };

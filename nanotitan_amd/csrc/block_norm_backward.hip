@@ -10,6 +10,12 @@
 // workgroups' sums by a second launch, always in the same order. Four waves a
 // SIMD have to fit (128 registers): the parameters are parked in LDS (layer
 // norms of 131,072 x 512: 222 -> 160 us, of 16,384 x 4,096: 307 -> 199).
+//
+// Measured on MI355X (a copy: 5.65 TB/s), bf16: 16,384 x 4,096 rms 160 us
+// (5.0 TB/s), layer 172 (4.7); 131,072 x 512 156 and 161 (5.2, 5.0); the sums'
+// launch is 5 to 8 us of each. Above 8,192 columns a thread holds sixteen and
+// the sums no longer fit its registers: 4,096 x 16,384 rms 210 (3.8), layer 454
+// (1.8).
 #include "block_norm.hpp"
 
 namespace nt {
@@ -62,7 +68,7 @@ block_norm_backward_kernel(NormGradArgs a) {
   typedef typename elem<T>::storage S;
   constexpr int V = SH::V, TPR = SH::TPR, CH = SH::CH;
   constexpr int kThreads = block_threads(TPR), kRows = kThreads / TPR;
-  __shared__ float s_red[2 * 3 * (kThreads / kWave)];
+  __shared__ float s_red[RowSum<TPR, 3>::kSize];
   __shared__ float s_fold[kRows > 1 ? kThreads * CH * V : 1];
   RowSum<TPR, 3> sum{s_red};
   enum { kSW, kNext, kSB };
@@ -118,14 +124,16 @@ block_norm_backward_kernel(NormGradArgs a) {
     asm volatile("" ::: "memory");  // the parameters stay parked
     load(row);
     const float mean_y = st[0], r_y = st[1], mean_h = st[2], r_h = st[3];
+    // Columns that a chunk does not own count in the row's sums with parameters
+    // of zero, and their own sums are not stored.
     float D[CH][V], hh[CH][V], u[CH][V], y[CH][V], g[CH][V];
 #pragma unroll
     for (int k = 0; k < CH; ++k) {
-      values<TX, V>(rd[k], c[k], D[k]);
-      values<TX, V>(rh[k], c[k], hh[k]);
-      values<T, V>(rn[k], c[k], u[k]);
-      if constexpr (MODE != kPre) values<T, V>(ry[k], c[k], y[k]);
-      if constexpr (MODE == kGated) values<T, V>(rg[k], c[k], g[k]);
+      all_values<TX, V>(rd[k], D[k]);
+      all_values<TX, V>(rh[k], hh[k]);
+      all_values<T, V>(rn[k], u[k]);
+      if constexpr (MODE != kPre) all_values<T, V>(ry[k], y[k]);
+      if constexpr (MODE == kGated) all_values<T, V>(rg[k], g[k]);
     }
     if (!has_dh) {
 #pragma unroll
@@ -134,7 +142,7 @@ block_norm_backward_kernel(NormGradArgs a) {
         for (int i = 0; i < V; ++i) D[k][i] = 0.f;
     }
     if (has_dn) {
-      float t[3] = {0.f, 0.f, 0.f};
+      float t[LAYER ? 2 : 1] = {};
 #pragma unroll
       for (int k = 0; k < CH; ++k) {
         float wn[V];
@@ -142,18 +150,18 @@ block_norm_backward_kernel(NormGradArgs a) {
 #pragma unroll
         for (int i = 0; i < V; ++i) {
           hh[k][i] = (hh[k][i] - mean_h) * r_h;
-          if (!c[k].owns(i)) hh[k][i] = 0.f;
           if (live) {
             acc[kSumNext][k][i] = fmaf(u[k][i], hh[k][i], acc[kSumNext][k][i]);
             if constexpr (LAYER) acc[kSumNextBias][k][i] += u[k][i];
           }
           u[k][i] *= wn[i];
-          if constexpr (LAYER) t[0] += u[k][i];
-          t[1] = fmaf(u[k][i], hh[k][i], t[1]);
+          t[0] = fmaf(u[k][i], hh[k][i], t[0]);
+          if constexpr (LAYER) t[1] += u[k][i];
         }
       }
       sum(t);
-      const float m0 = LAYER ? t[0] * inv_d : 0.f, m1 = t[1] * inv_d;
+      float m0 = 0.f, m1 = t[0] * inv_d;
+      if constexpr (LAYER) m0 = t[1] * inv_d;
 #pragma unroll
       for (int k = 0; k < CH; ++k)
 #pragma unroll
@@ -168,7 +176,8 @@ block_norm_backward_kernel(NormGradArgs a) {
       float g_row = 1.f;
       if (MODE == kPost && a.gate != nullptr)
         g_row = elem<T>::load(static_cast<const S*>(a.gate)[live ? row : a.T - 1]);
-      float t[3] = {0.f, 0.f, 0.f};
+      constexpr int kGate = LAYER ? 2 : 1;  // a row's gate: its sum is the last
+      float t[kGate + (MODE == kPost)] = {};
 #pragma unroll
       for (int k = 0; k < CH; ++k) {
         float dg[V], sw[V];
@@ -177,30 +186,34 @@ block_norm_backward_kernel(NormGradArgs a) {
 #pragma unroll
         for (int i = 0; i < V; ++i) {
           const float gi = MODE == kGated ? g[k][i] : g_row;
-          const float Dv = c[k].owns(i) ? D[k][i] : 0.f;
-          y[k][i] = c[k].owns(i) ? (y[k][i] - mean_y) * r_y : 0.f;
+          const float Dv = D[k][i];
+          y[k][i] = (y[k][i] - mean_y) * r_y;
           // s g p's derivative by g, and D g: times s w it is u of dN, summed A and B
           dg[i] = Dv * (LAYER ? fmaf(y[k][i], sw[i], sb[k][i]) : y[k][i] * sw[i]);
-          if constexpr (MODE == kPost) t[2] += dg[i];
+          if constexpr (MODE == kPost) t[kGate] += dg[i];
           const float Dg = Dv * gi;
           if (live) {
             acc[kSumA][k][i] = fmaf(Dg, y[k][i], acc[kSumA][k][i]);
             if constexpr (LAYER) acc[kSumB][k][i] += Dg;
           }
           D[k][i] = Dg * sw[i];
-          if constexpr (LAYER) t[0] += D[k][i];
-          t[1] = fmaf(D[k][i], y[k][i], t[1]);
+          t[0] = fmaf(D[k][i], y[k][i], t[0]);
+          if constexpr (LAYER) t[1] += D[k][i];
         }
         if (MODE == kGated && a.dgate != nullptr && live)
           store_chunk<T, V>(a.dgate, base, c[k], dg);
       }
       sum(t);
-      if (MODE == kPost && a.dgate != nullptr && live && threadIdx.x % TPR == 0)
-        static_cast<S*>(a.dgate)[row] = elem<T>::store(t[2]);
+      if constexpr (MODE == kPost)
+        if (a.dgate != nullptr && live && threadIdx.x % TPR == 0)
+          static_cast<S*>(a.dgate)[row] = elem<T>::store(t[kGate]);
       if (a.dy != nullptr && live) {
         // without a norm's weight p = y: nothing to project out
-        const float m0 = LAYER && a.w != nullptr ? t[0] * inv_d : 0.f;
-        const float m1 = a.w != nullptr ? t[1] * inv_d : 0.f;
+        float m0 = 0.f, m1 = 0.f;
+        if (a.w != nullptr) {
+          m1 = t[0] * inv_d;
+          if constexpr (LAYER) m0 = t[1] * inv_d;
+        }
 #pragma unroll
         for (int k = 0; k < CH; ++k) {
 #pragma unroll
@@ -240,7 +253,7 @@ block_norm_backward_kernel(NormGradArgs a) {
     }
   }
   if (MODE != kPre && a.one) {
-    float t[3] = {0.f, 0.f, 0.f};
+    float t[1] = {0.f};
 #pragma unroll
     for (int k = 0; k < CH; ++k) {
       float w[V], b[V];
