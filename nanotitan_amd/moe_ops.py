@@ -23,6 +23,12 @@ and dispatch block), ``DispatchFN`` (count + offsets + pack, or offsets + pack
 from RouteCountFN's counts) and ``CombineInvFN`` (combine whose backward reads
 each token's grad row once). They compute the same values as pack_tokens_fn /
 combine_tokens_fn on the same inputs.
+
+Beside that path: ``moe_few_tokens`` (the whole layer for a decode step),
+``pre_norm_fn`` / ``post_norm_fn`` (norms, gate and residual of a block) and
+``checkpoint8`` / ``gelu8_fn`` / ``swiglu8_fn`` with the experts' FFNs on them
+(activations kept in 8 bits). The norms' and 8-bit activations' Functions are
+in the extension.
 """
 
 from __future__ import annotations
