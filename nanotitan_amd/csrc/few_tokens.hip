@@ -19,8 +19,8 @@
 // goes through LDS but the waves' partial sums at the end.
 //
 // Measured on MI355X (a read of 2 GiB: 7.1 TB/s): 16 tokens of 4,096, 8 experts
-// of 14,336, bf16: up 282 us (6.7 TB/s), down 139 (6.8), all 430; 64 tokens: up
-// 296, down 172, all 480; 33 tokens of 2,048, 128 experts of 768, top-8, fp16:
+// of 14,336, bf16: up 282 us (6.7 TB/s), down 139 (6.8), all 430; 64 tokens: all
+// 449 (6.3); 33 tokens of 2,048, 128 experts of 768, top-8, fp16:
 // up 60 (6.0), down 59 (6.1), routing 8, gate sum 5, all 131; one token of 512,
 // 16 experts of 2,048: 9 + 8, all 17.5 (its 12.6 MB would take 1.8: launches
 // and a chain of about ten dependent memory latencies).
@@ -47,7 +47,7 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
-struct LiveExpert;
+struct Load;
 
 // Routing in a launch of its own, or in every workgroup of the up projection.
 enum { kRouteApart = 0, kRouteFused = 1, kRouteSmall = 2 };
@@ -60,6 +60,7 @@ struct FewArgs {
   const void* w3;       // [E, f, d]
   int32_t T, E, k, splits;
   int32_t most_live;  // experts that can have tokens, at most
+  int32_t most_loads;  // and the loads (below) that they can make
   int32_t route;      // where the routing is done
   bool arrive;        // gate sum in the down projection
   int64_t d, f;
@@ -68,7 +69,7 @@ struct FewArgs {
   void* out;          // [T, d]
   int32_t* arrived;   // [ceil(d / 64)]: finished parts of the columns' tiles
   int32_t* inv;       // [T, k]: row of an assignment in hidden and partial
-  LiveExpert* live;   // [1 + most_live]: the experts that have tokens
+  Load* loads;        // [1 + most_loads]
   void* hidden;       // [T k, f]
   float* partial;     // [splits][T k][d]
 };
@@ -290,54 +291,62 @@ __device__ __forceinline__ void route_here(const FewArgs& a, const float* s_logi
 // ------------------------------------------------------------- expert tiles
 
 // Which tokens each expert has, the first row of each (rows by expert, then
-// token) and the experts that have any.
+// token) and the loads: an expert's tokens, `most_rows` at a time, so that the
+// workgroups of a load hold all its sums. An expert with more tokens is read
+// once for each of its loads, by different workgroups.
+constexpr int kPartShift = 10;  // a load as 16 bits: expert, part
+constexpr int kMaxLoads = NT_MAX_EXPERTS + kMaxTokens * kMaxTopK / kRowsMma;
+static_assert(NT_MAX_EXPERTS <= 1 << kPartShift, "a load in 16 bits");
 struct Plan {
   uint64_t mask[NT_MAX_EXPERTS];
   uint16_t first[NT_MAX_EXPERTS];
-  uint16_t live[NT_MAX_EXPERTS];
-  int32_t num_live;
+  uint16_t load[kMaxLoads];
+  int32_t num_loads;
 };
 
-// The same for the down projection, in memory: the number of live experts,
-// then each one's {expert, first row, rows, 0}.
-struct LiveExpert {
+// The same for the down projection, in memory: the number of loads, then each
+// one's {expert, first row, rows, 0}.
+struct Load {
   int32_t expert, first, rows, pad;
 };
 
-__device__ __forceinline__ void make_plan(const FewArgs& a, const int32_t* topk, Plan& s) {
+__device__ __forceinline__ void make_plan(const FewArgs& a, const int32_t* topk, int most_rows,
+                                          Plan& s) {
   for (int e = threadIdx.x; e < a.E; e += blockDim.x) s.mask[e] = 0;
   __syncthreads();
   for (int i = threadIdx.x; i < a.T * a.k; i += blockDim.x)
     atomicOr(reinterpret_cast<unsigned long long*>(&s.mask[topk[i]]), 1ull << (i / a.k));
   __syncthreads();
   if (threadIdx.x < kWave) {
-    int row = 0, live = 0;
+    int row = 0, loads = 0;
     for (int e0 = 0; e0 < a.E; e0 += kWave) {
       const int e = e0 + lane_id();
-      const int n = e < a.E ? popc64(s.mask[e]) : 0;
-      const int before = wave_incl_scan(n) - n;
-      const uint64_t on = ballot(n > 0);
+      const int n = e < a.E ? popc64(s.mask[e]) : 0, parts = (n + most_rows - 1) / most_rows;
+      const int before = wave_incl_scan(n) - n, ahead = wave_incl_scan(parts) - parts;
       if (e < a.E) s.first[e] = (uint16_t)(row + before);
-      if (n > 0) s.live[live + popc64(on & lanemask_lt())] = (uint16_t)e;
+      for (int p = 0; p < parts; ++p)
+        s.load[loads + ahead + p] = (uint16_t)(e | p << kPartShift);
       row += __shfl(before + n, kWave - 1, kWave);
-      live += popc64(on);
+      loads += __shfl(ahead + parts, kWave - 1, kWave);
     }
-    if (lane_id() == 0) s.num_live = live;
+    if (lane_id() == 0) s.num_loads = loads;
   }
   __syncthreads();
 }
 
 // What the down projection reads of it, and its counters cleared.
-__device__ __forceinline__ void write_plan(const FewArgs& a, const int32_t* topk, const Plan& s) {
+__device__ __forceinline__ void write_plan(const FewArgs& a, const int32_t* topk, int most_rows,
+                                           const Plan& s) {
   for (int i = threadIdx.x; i < a.T * a.k; i += blockDim.x) {
     const int e = topk[i], t = i / a.k;
     a.inv[i] = s.first[e] + popc64(s.mask[e] & ((1ull << t) - 1));
   }
-  for (int i = threadIdx.x; i < s.num_live; i += blockDim.x) {
-    const int e = s.live[i];
-    a.live[1 + i] = {e, s.first[e], popc64(s.mask[e]), 0};
+  for (int i = threadIdx.x; i < s.num_loads; i += blockDim.x) {
+    const int e = s.load[i] & ((1 << kPartShift) - 1);
+    const int done = (s.load[i] >> kPartShift) * most_rows;
+    a.loads[1 + i] = {e, s.first[e] + done, min(popc64(s.mask[e]) - done, most_rows), 0};
   }
-  if (threadIdx.x == 0) a.live[0] = {s.num_live, 0, 0, 0};
+  if (threadIdx.x == 0) a.loads[0] = {s.num_loads, 0, 0, 0};
   for (int i = threadIdx.x; i < ceil_div(a.d, (int64_t)kCols); i += blockDim.x) a.arrived[i] = 0;
 }
 
@@ -389,8 +398,8 @@ struct SmallPlan {
       a.topk[i] = c;
       a.inv[i] = (int32_t)its_first + __popc(its_mask & ((1u << t) - 1));
     }
-    if (n > 0) a.live[1 + popc64(live & lanemask_lt())] = {e, (int32_t)first, n, 0};
-    if (lane_id() == 0) a.live[0] = {popc64(live), 0, 0, 0};
+    if (n > 0) a.loads[1 + popc64(live & lanemask_lt())] = {e, (int32_t)first, n, 0};
+    if (lane_id() == 0) a.loads[0] = {popc64(live), 0, 0, 0};
     for (int i = lane_id(); i < ceil_div(a.d, (int64_t)kCols); i += kWave) a.arrived[i] = 0;
   }
   // The i-th live expert (uniform).
@@ -726,12 +735,14 @@ __global__ void __launch_bounds__(group_waves(KW) * kWave) few_up_kernel(FewArgs
       s_acc[KW == 1 ? 3 * kFusedLogits : kWaves * MATS * kRowsMma * kCols];
   const int lane = lane_id();
   const bool small = KW == kMaxTileWaves && a.route == kRouteSmall;
+  constexpr int kRows = MT * kRowsMma;
+  static_assert(kSmallTokens <= kRows, "a small plan's experts are one load each");
   SmallPlan here = {};
-  int num_live;
+  int num_loads;
   if (small) {
     logits_here<T>(a, s_acc);
     here.make(a, s_acc, reinterpret_cast<int32_t*>(s_acc + kFusedLogits), s_acc + 2 * kFusedLogits);
-    num_live = popc64(here.live);
+    num_loads = popc64(here.live);
   } else {
     const int32_t* topk = a.topk;
     if (a.route == kRouteFused) {
@@ -740,73 +751,63 @@ __global__ void __launch_bounds__(group_waves(KW) * kWave) few_up_kernel(FewArgs
       route_here(a, s_acc, s_topk, s_acc + 2 * kFusedLogits);
       topk = s_topk;
     }
-    make_plan(a, topk, s_plan);
-    if (blockIdx.x == 0) write_plan(a, topk, s_plan);
-    num_live = s_plan.num_live;
+    make_plan(a, topk, kRows, s_plan);
+    if (blockIdx.x == 0) write_plan(a, topk, kRows, s_plan);
+    num_loads = s_plan.num_loads;
   }
   const int64_t per = ceil_div(a.f, (int64_t)kCols * HALVES), steps = ceil_div(a.d, (int64_t)kStep);
-  const int64_t items = num_live * per;
+  const int64_t items = num_loads * per;
   const int group = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave / KW);
   for (int64_t first = (int64_t)blockIdx.x * kTiles; first < items;
        first += (int64_t)gridDim.x * kTiles) {
     // past the last tile, a group repeats it and stores nothing
     const int64_t item = first + group < items ? first + group : items - 1;
-    const int e = __builtin_amdgcn_readfirstlane(small ? here.expert((int)(item / per))
-                                                      : s_plan.live[item / per]);
+    const int load = __builtin_amdgcn_readfirstlane(small ? here.expert((int)(item / per))
+                                                         : s_plan.load[item / per]);
+    const int e = load & ((1 << kPartShift) - 1), done = (load >> kPartShift) * kRows;
     const int64_t col = item % per * HALVES * kCols;
     TileColumns tc[MATS];
 #pragma unroll
     for (int i = 0; i < MATS; ++i) tc[i] = TileColumns(col + i * (HALVES - 1) * kCols, a.f);
-    const uint64_t mask =
-        small ? (uint32_t)__builtin_amdgcn_readlane(here.mask, e) : s_plan.mask[e];
+    uint64_t mask = small ? (uint32_t)__builtin_amdgcn_readlane(here.mask, e) : s_plan.mask[e];
     const int first_row =
-        small ? __builtin_amdgcn_readlane(here.first, e) : (int)s_plan.first[e];
-    const int rows = __builtin_amdgcn_readfirstlane(popc64(mask));
+        done + (small ? __builtin_amdgcn_readlane(here.first, e) : (int)s_plan.first[e]);
+    for (int i = 0; i < done; ++i) mask &= mask - 1;  // the tokens of its earlier loads
+    const int rows = __builtin_amdgcn_readfirstlane(min(popc64(mask), kRows));
     const S* w[MATS];
     w[0] = static_cast<const S*>(a.w1) + (int64_t)e * a.d * a.f;
     if constexpr (MATS == 2)
       w[1] = static_cast<const S*>(SWIGLU ? a.w2 : a.w1) + (int64_t)e * a.d * a.f;
     S* hidden = static_cast<S*>(a.hidden) + (int64_t)first_row * a.f;
-    // MT x 16 rows at a time. Two groups in a workgroup may have different
-    // numbers of rows: the barriers of the fold are the same for both.
-    int most = rows;
-    if constexpr (kTiles > 1 && KW > 1)
-      for (int g = 0; g < kTiles; ++g) {
-        const int64_t i = first + g < items ? first + g : items - 1;
-        most = max(most, popc64(s_plan.mask[s_plan.live[i / per]]));
-      }
-    most = __builtin_amdgcn_readfirstlane(most);
-    for (int r0 = 0; r0 < most; r0 += MT * kRowsMma) {
-      const int tiles = min((rows - r0 + kRowsMma - 1) / kRowsMma, MT);
-      uint32_t row[MT];
+    const int tiles = (rows + kRowsMma - 1) / kRowsMma;
+    uint32_t row[MT];
 #pragma unroll
-      for (int m = 0; m < MT; ++m) {
-        const int r = r0 + m * kRowsMma + (lane & 15);
-        row[m] = ((uint32_t)nth_token(mask, r < rows ? r : 0) * (uint32_t)a.d + (lane >> 4) * 8) *
-                 (uint32_t)sizeof(S);
-      }
-      f32x4 acc[MATS][MT][4];
-      wave_tiles<KW, NARROW, T>(tiles, w, static_cast<const S*>(a.x), row, tc, a.d, a.f, 0, steps,
-                                acc);
+    for (int m = 0; m < MT; ++m) {
+      const int r = m * kRowsMma + (lane & 15);
+      row[m] = ((uint32_t)nth_token(mask, r < rows ? r : 0) * (uint32_t)a.d + (lane >> 4) * 8) *
+               (uint32_t)sizeof(S);
+    }
+    f32x4 acc[MATS][MT][4];
+    wave_tiles<KW, NARROW, T>(tiles, w, static_cast<const S*>(a.x), row, tc, a.d, a.f, 0, steps,
+                              acc);
 #pragma unroll
-      for (int m = 0; m < MT; ++m) {
-        if ((kTiles == 1 || KW == 1) && m >= tiles) break;
-        float v[MATS][N];
-        fold_waves<KW, MATS, MT>(acc, m, s_acc, v);
-        if (item != first + group) continue;
+    for (int m = 0; m < MT; ++m) {
+      if ((kTiles == 1 || KW == 1) && m >= tiles) break;
+      float v[MATS][N];
+      fold_waves<KW, MATS, MT>(acc, m, s_acc, v);
+      if (item != first + group) continue;
 #pragma unroll
-        for (int h = 0; h < HALVES; ++h)
+      for (int h = 0; h < HALVES; ++h)
 #pragma unroll
-          for (int j = 0; j < N; ++j) {
-            const int r = r0 + fold_row<KW>(m, j);
-            const int64_t c = fold_col<KW, NARROW>(tc[h], a.f, j);
-            float z;
-            if constexpr (SWIGLU) z = v[0][j] / (1.f + __expf(-v[0][j])) * v[1][j];
-            else z = few_gelu(v[h][j]);
-            if (r < rows && c >= col + h * kCols && c < a.f)
-              hidden[(int64_t)r * a.f + c] = to_bits<T>(z);
-          }
-      }
+        for (int j = 0; j < N; ++j) {
+          const int r = fold_row<KW>(m, j);
+          const int64_t c = fold_col<KW, NARROW>(tc[h], a.f, j);
+          float z;
+          if constexpr (SWIGLU) z = v[0][j] / (1.f + __expf(-v[0][j])) * v[1][j];
+          else z = few_gelu(v[h][j]);
+          if (r < rows && c >= col + h * kCols && c < a.f)
+            hidden[(int64_t)r * a.f + c] = to_bits<T>(z);
+        }
     }
   }
 }
@@ -853,78 +854,69 @@ __global__ void __launch_bounds__(group_waves(KW) * kWave) few_down_kernel(FewAr
   __shared__ int32_t s_last;
   const int lane = lane_id();
   const int64_t per = ceil_div(a.d, (int64_t)kCols * HALVES), steps = ceil_div(a.f, (int64_t)kStep);
-  const int64_t most = (int64_t)a.most_live * per * a.splits;
+  const int64_t most = (int64_t)a.most_loads * per * a.splits;
   const int group = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave / KW);
   for (int64_t start = (int64_t)blockIdx.x * kTiles; start < most;
        start += (int64_t)gridDim.x * kTiles) {
     // the entry and the number of entries in one wait: past the number it is
     // arbitrary, but there
     const int64_t at = start + group < most ? start + group : most - 1;
-    const int num_live = __builtin_amdgcn_readfirstlane(a.live[0].expert);
-    LiveExpert le = a.live[1 + at / a.splits / per];
-    const int64_t items = num_live * per * a.splits;
+    const int num_loads = __builtin_amdgcn_readfirstlane(a.loads[0].expert);
+    Load ld = a.loads[1 + at / a.splits / per];
+    const int64_t items = num_loads * per * a.splits;
     if (start >= items) return;
     const bool mine = start + group < items;
     const int64_t item = mine ? start + group : items - 1;
-    if (!mine) le = a.live[num_live];
-    le.expert = __builtin_amdgcn_readfirstlane(le.expert);
-    le.first = __builtin_amdgcn_readfirstlane(le.first);
-    const int rows = __builtin_amdgcn_readfirstlane(le.rows);
+    if (!mine) ld = a.loads[num_loads];
+    ld.expert = __builtin_amdgcn_readfirstlane(ld.expert);
+    ld.first = __builtin_amdgcn_readfirstlane(ld.first);
+    const int rows = __builtin_amdgcn_readfirstlane(ld.rows);
     const int split = (int)(item % a.splits);
     const int64_t tile = item / a.splits % per, col = tile * HALVES * kCols;
     TileColumns tc[HALVES];
 #pragma unroll
     for (int h = 0; h < HALVES; ++h) tc[h] = TileColumns(col + h * kCols, a.d);
-    const S* hidden = static_cast<const S*>(a.hidden) + (int64_t)le.first * a.f;
+    const S* hidden = static_cast<const S*>(a.hidden) + (int64_t)ld.first * a.f;
     const S* w[HALVES];
 #pragma unroll
     for (int h = 0; h < HALVES; ++h)
-      w[h] = static_cast<const S*>(a.w3) + (int64_t)le.expert * a.f * a.d;
-    float* out = a.partial + ((int64_t)split * a.T * a.k + le.first) * a.d;
-    int most_rows = rows;
-    if constexpr (kTiles > 1 && KW > 1)
-      for (int g = 0; g < kTiles; ++g) {
-        const int64_t i = start + g < items ? start + g : items - 1;
-        most_rows = max(most_rows, a.live[1 + i / a.splits / per].rows);
-      }
-    most_rows = __builtin_amdgcn_readfirstlane(most_rows);
-    for (int r0 = 0; r0 < most_rows; r0 += MT * kRowsMma) {
-      const int tiles = min((rows - r0 + kRowsMma - 1) / kRowsMma, MT);
-      uint32_t row[MT];
+      w[h] = static_cast<const S*>(a.w3) + (int64_t)ld.expert * a.f * a.d;
+    float* out = a.partial + ((int64_t)split * a.T * a.k + ld.first) * a.d;
+    const int tiles = (rows + kRowsMma - 1) / kRowsMma;
+    uint32_t row[MT];
 #pragma unroll
-      for (int m = 0; m < MT; ++m) {
-        const int r = r0 + m * kRowsMma + (lane & 15);
-        row[m] = ((uint32_t)(r < rows ? r : 0) * (uint32_t)a.f + (lane >> 4) * 8) *
-                 (uint32_t)sizeof(S);
-      }
-      f32x4 acc[HALVES][MT][4];
-      wave_tiles<KW, NARROW, T>(tiles, w, hidden, row, tc, a.f, a.d, steps * split / a.splits,
-                                steps * (split + 1) / a.splits, acc);
+    for (int m = 0; m < MT; ++m) {
+      const int r = m * kRowsMma + (lane & 15);
+      row[m] = ((uint32_t)(r < rows ? r : 0) * (uint32_t)a.f + (lane >> 4) * 8) *
+               (uint32_t)sizeof(S);
+    }
+    f32x4 acc[HALVES][MT][4];
+    wave_tiles<KW, NARROW, T>(tiles, w, hidden, row, tc, a.f, a.d, steps * split / a.splits,
+                              steps * (split + 1) / a.splits, acc);
 #pragma unroll
-      for (int m = 0; m < MT; ++m) {
-        if ((kTiles == 1 || KW == 1) && m >= tiles) break;
-        float v[HALVES][N];
-        fold_waves<KW, HALVES, MT>(acc, m, s_acc, v);
-        if (!mine) continue;
+    for (int m = 0; m < MT; ++m) {
+      if ((kTiles == 1 || KW == 1) && m >= tiles) break;
+      float v[HALVES][N];
+      fold_waves<KW, HALVES, MT>(acc, m, s_acc, v);
+      if (!mine) continue;
 #pragma unroll
-        for (int h = 0; h < HALVES; ++h)
+      for (int h = 0; h < HALVES; ++h)
 #pragma unroll
-          for (int j = 0; j < N; ++j) {
-            const int r = r0 + fold_row<KW>(m, j);
-            const int64_t c = fold_col<KW, NARROW>(tc[h], a.d, j);
-            if (r >= rows || c < col + h * kCols || c >= a.d) continue;
-            float* p = out + (int64_t)r * a.d + c;
-            if (KW == 8 && HALVES == 1 && a.arrive)
-              __hip_atomic_store(p, v[h][j], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            else
-              *p = v[h][j];
-          }
-      }
+        for (int j = 0; j < N; ++j) {
+          const int r = fold_row<KW>(m, j);
+          const int64_t c = fold_col<KW, NARROW>(tc[h], a.d, j);
+          if (r >= rows || c < col + h * kCols || c >= a.d) continue;
+          float* p = out + (int64_t)r * a.d + c;
+          if (KW == 8 && HALVES == 1 && a.arrive)
+            __hip_atomic_store(p, v[h][j], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+          else
+            *p = v[h][j];
+        }
     }
     if (KW == 8 && HALVES == 1 && a.arrive) {
       wait_batch_loads();
       __syncthreads();
-      if (threadIdx.x == 0) s_last = atomicAdd(&a.arrived[tile], 1) == num_live * a.splits - 1;
+      if (threadIdx.x == 0) s_last = atomicAdd(&a.arrived[tile], 1) == num_loads * a.splits - 1;
       __syncthreads();
       if (s_last && col + lane < a.d)
         for (int t = threadIdx.x / kWave; t < a.T; t += kWaves)
@@ -939,13 +931,21 @@ int64_t few_waves(int row_tiles, int mats) {
   return 256 * (16 - 4 * (mats - 1) - (row_tiles == 1 ? 0 : 4));
 }
 
-// Row tiles taken at once: those of the most tokens that an expert can have; one
-// where experts have few tokens on average (one that has more reads its weights
-// again for every 16), since more take the registers that hold twice the waves
-// (33 tokens, top-8 of 128: 143 -> 131 us).
+// Row tiles of a load: by the tokens that an expert has on average, since more
+// take the registers that hold twice the waves. One up to four tokens (33 tokens,
+// top-8 of 128: 143 -> 131 us), two up to 20 (64 tokens of top-2 of 8, 4,096 x
+// 14,336: SwiGLU 473 -> 447 us, GELU 391 -> 324; with one expert in every
+// token's choice, so twice loaded, 502 -> 520 and 427 -> 397).
 int few_row_tiles(int64_t T, int32_t k, int32_t E) {
   if (T <= kRowsMma || T * k <= 4 * E) return 1;
-  return T <= 2 * kRowsMma ? 2 : 4;
+  return T <= 2 * kRowsMma || T * k <= 20 * E ? 2 : 4;
+}
+
+// Loads that T k assignments make at most: none is empty, and besides each
+// expert's first all follow a full one.
+int32_t few_loads(int64_t T, int32_t k, int32_t E) {
+  const int64_t A = T * k, rows = few_row_tiles(T, k, E) * kRowsMma;
+  return (int32_t)std::min<int64_t>(A, std::min<int64_t>(A, E) + (T > rows ? A / rows : 0));
 }
 
 // Parts of the down projection's reduction: as many as give every CU the
@@ -984,7 +984,7 @@ FewTiles few_tiles(int row_tiles, int64_t experts, int64_t K, int64_t N, int64_t
 }
 
 struct Layout {
-  size_t arrived, inv, live, hidden, partial, bytes;
+  size_t arrived, inv, loads, hidden, partial, bytes;
 };
 Layout few_layout(int dtype, int64_t T, int32_t k, int32_t E, int64_t d, int64_t f) {
   Layout l;
@@ -992,8 +992,8 @@ Layout few_layout(int dtype, int64_t T, int32_t k, int32_t E, int64_t d, int64_t
   auto after = [](size_t at, int64_t bytes) { return at + (size_t)round_up(bytes, 256); };
   l.arrived = 0;
   l.inv = after(l.arrived, ceil_div(d, (int64_t)kCols) * 4);
-  l.live = after(l.inv, A * 4);
-  l.hidden = after(l.live, (1 + std::min<int64_t>(A, E)) * (int64_t)sizeof(LiveExpert));
+  l.loads = after(l.inv, A * 4);
+  l.hidden = after(l.loads, (1 + few_loads(T, k, E)) * (int64_t)sizeof(Load));
   l.partial = after(l.hidden, A * f * dtype_bytes(dtype));
   l.bytes = l.partial + (size_t)few_splits(T, k, E, d, f) * A * d * 4;
   return l;
@@ -1025,10 +1025,11 @@ void by_tiles(const FewTiles& t, F&& f) {
     else f(one, one);
   }
 }
-// A workgroup for every group_waves / KW tiles, up to eight on each CU: past
-// that they take several in turn.
-dim3 few_grid(int64_t tiles, int tile_waves) {
-  const int64_t waves = group_waves(tile_waves);
+// A workgroup for every group_waves / KW tiles of all loads that there can be (a
+// tile in a second round would cost as much as the first; those without one
+// leave), up to eight on each CU: past that they take several in turn.
+dim3 few_grid(const FewArgs& a, const FewTiles& t, int tile_waves) {
+  const int64_t waves = group_waves(tile_waves), tiles = t.count / a.most_live * a.most_loads;
   return dim3((unsigned)std::min<int64_t>(8192 / waves, ceil_div(tiles * tile_waves, waves)));
 }
 
@@ -1051,7 +1052,7 @@ void launch_few(FewArgs a, hipStream_t stream) {
                        a);
   by_tiles<T, NARROW>(up, [&](auto halves, auto waves) {
     constexpr int H = decltype(halves)::value, KW = decltype(waves)::value;
-    const dim3 grid = few_grid(up.count, KW), block(group_waves(KW) * kWave);
+    const dim3 grid = few_grid(a, up, KW), block(group_waves(KW) * kWave);
     if (swiglu && H == 1)
       hipLaunchKernelGGL((few_up_kernel<T, true, 1, MT, KW, NARROW>), grid, block, 0, stream, a);
     if (!swiglu)
@@ -1065,7 +1066,7 @@ void launch_few(FewArgs a, hipStream_t stream) {
              a.most_live * a.splits <= 16 && a.T <= kSmallTokens;
   by_tiles<T, NARROW>(down, [&](auto halves, auto waves) {
     constexpr int H = decltype(halves)::value, KW = decltype(waves)::value;
-    hipLaunchKernelGGL((few_down_kernel<T, H, MT, KW, NARROW>), few_grid(down.count, KW),
+    hipLaunchKernelGGL((few_down_kernel<T, H, MT, KW, NARROW>), few_grid(a, down, KW),
                        dim3(group_waves(KW) * kWave), 0, stream, a);
   });
   if (!a.arrive)
@@ -1115,10 +1116,11 @@ int nt_moe_few_tokens(int dtype, const void* x, const float* router, const float
   a.T = (int32_t)T, a.E = E, a.k = k, a.d = d, a.f = f;
   a.splits = few_splits(T, k, E, d, f);
   a.most_live = (int32_t)std::min<int64_t>(T * k, E);
+  a.most_loads = few_loads(T, k, E);
   a.gates = gates, a.topk = topk, a.out = out;
   a.arrived = reinterpret_cast<int32_t*>(base + l.arrived);
   a.inv = reinterpret_cast<int32_t*>(base + l.inv);
-  a.live = reinterpret_cast<LiveExpert*>(base + l.live);
+  a.loads = reinterpret_cast<Load*>(base + l.loads);
   a.hidden = base + l.hidden;
   a.partial = reinterpret_cast<float*>(base + l.partial);
   if (dtype == NT_F32) launch_few<float>(a, stream);

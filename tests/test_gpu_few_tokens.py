@@ -109,6 +109,25 @@ def test_all_tokens_on_one_expert(ext, dtype, T):
     _check(x, None, logits.cuda(), weights, 2)
 
 
+@pytest.mark.parametrize("dtype,ffn", [("bf16", "swiglu"), ("fp32", "gelu")])
+@pytest.mark.parametrize("sizes", [(16, 1), (17, 16), (32, 17), (33, 32, 1), (48, 33), (49, 48, 2),
+                                   (64, 49), (64, 64), (64, 64, 64)])
+@pytest.mark.parametrize("E", [5, 64])
+def test_an_expert_in_several_loads(ext, dtype, ffn, sizes, E):
+    """Given numbers of tokens on the last experts: at and past every multiple of 16 rows,
+    with few experts (32 rows a load, or 64) and many (16)."""
+    T, k = max(sizes), len(sizes)
+    x, _, weights = _inputs(T, 72, 80, E, TYPES[dtype], ffn, sum(sizes))
+    g = torch.Generator().manual_seed(2)
+    logits = torch.randn(T, E, generator=g)
+    for i, n in enumerate(sizes):
+        # the last n tokens and, for the others, no token of this expert
+        logits[:, E - 1 - i] = torch.where(torch.arange(T) >= T - n, 20.0 + i, -20.0)
+    _, _, ids = _check(x, None, logits.cuda(), weights, k)
+    for i, n in enumerate(sizes):
+        assert int((ids == E - 1 - i).sum()) == n
+
+
 # T, d, f, E, k, skew: by the number of column tiles, 8, 4, 2 and 1 waves take one; long
 # reductions take 128 columns at a time; an expert past 16 tokens among many with few
 # takes its weights more than once.
