@@ -960,7 +960,10 @@ int32_t few_splits(int64_t T, int32_t k, int32_t E, int64_t d, int64_t f) {
 
 // How an expert kernel's tiles lie: as many waves each as leave every tile its
 // place at once. Fewer waves a tile means fewer of the folds and barriers that
-// end one; with more tiles than waves a wave takes several in turn. One matrix
+// end one; with more tiles than waves a wave takes several in turn. Eight waves
+// are for tiles that have a CU each: with more, some CUs have two and the others
+// one, and four waves a tile share them better (4 tokens, top-8 of 64, 2,048 x
+// 768: 80 -> 64 us; 6 tokens, top-2 of 16, 512 x 2,048: 35 -> 25). One matrix
 // over a long reduction is taken 128 columns at a time by eight waves where
 // those tiles fill whole rounds of the CUs: twice as much in flight a wave (16
 // tokens, 14,336 x 4,096: 157 -> 138 us; with three steps a wave instead, 33
@@ -978,6 +981,7 @@ FewTiles few_tiles(int row_tiles, int64_t experts, int64_t K, int64_t N, int64_t
     t.halves = 2;
     t.count = paired;
   } else {
+    if (t.count > 256) t.waves = kMaxTileWaves / 2;
     while (t.waves > 1 && t.count * t.waves > few_waves(row_tiles, mats)) t.waves /= 2;
   }
   return t;
