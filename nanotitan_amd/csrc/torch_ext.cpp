@@ -882,12 +882,24 @@ const float* f32_or_null(const c10::optional<Tensor>& t) {
 const void* ptr_or_null(const c10::optional<Tensor>& t) { return t ? t->data_ptr() : nullptr; }
 void* out_or_null(const c10::optional<Tensor>& t) { return t ? t->data_ptr() : nullptr; }
 
+// Operators without a forward-mode derivative refuse dual tensors, in every grad
+// mode: a kernel's output has no tangent, which torch would read as zero.
+void refuse_tangents(std::initializer_list<const c10::optional<Tensor>*> ts, const char* what) {
+  if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
+  for (const auto* t : ts)
+    TORCH_CHECK_NOT_IMPLEMENTED(
+        !t->has_value() || !(*t)->defined() || !(*t)->_fw_grad(/*level=*/0).defined(), what,
+        " has no forward-mode derivative");
+}
+
 // moe_few_tokens(x, w_up, w_val, w_down, top_k, router, logits) -> (out, gates,
 // topk): a whole MoE layer for at most NT_FEW_TOKENS_MAX tokens.
 std::tuple<Tensor, Tensor, Tensor> moe_few_tokens(Tensor x, Tensor w_up,
                                                   c10::optional<Tensor> w_val, Tensor w_down,
                                                   int64_t top_k, c10::optional<Tensor> router,
                                                   c10::optional<Tensor> logits) {
+  const c10::optional<Tensor> ins[] = {x, w_up, w_down};
+  refuse_tangents({&ins[0], &ins[1], &ins[2], &w_val, &router, &logits}, "moe_few_tokens");
   check_device(x, "x");
   check_same_device(x, {&w_up, &w_down});
   TORCH_CHECK(x.dim() == 2 && w_up.dim() == 3 && w_up.size(1) == x.size(1),
@@ -1250,6 +1262,8 @@ std::tuple<OptTensor, OptTensor> block_norm_fn(Tensor x, OptTensor y, OptTensor 
                                                OptTensor gate, OptTensor scale, OptTensor w_next,
                                                OptTensor b_next, bool layer, double eps,
                                                c10::optional<at::ScalarType> dtype) {
+  const OptTensor x_in = x;
+  refuse_tangents({&x_in, &y, &w, &b, &gate, &scale, &w_next, &b_next}, "block_norm");
   TORCH_CHECK(x.dim() >= 1 && x.size(-1) >= 1, "x must have at least one column");
   TORCH_CHECK(!y || y->sizes() == x.sizes(), "x and y must be of one shape");
   const int64_t d = x.size(-1);
@@ -1266,8 +1280,7 @@ std::tuple<OptTensor, OptTensor> block_norm_fn(Tensor x, OptTensor y, OptTensor 
   if (y) y = rows(*y);
   if (gate) gate = rows(*gate);
   OptTensor h, n;
-  if (tracked({&y, &w, &b, &gate, &scale, &w_next, &b_next}) ||
-      (at::GradMode::is_enabled() && x.requires_grad())) {
+  if (tracked({&x_in, &y, &w, &b, &gate, &scale, &w_next, &b_next})) {
     variable_list out = BlockNormFunction::apply(x2, y, w, b, gate, scale, w_next, b_next, layer,
                                                  eps, dtype);
     if (y) h = out[0];
@@ -1309,11 +1322,15 @@ struct SwiGLU8Function : public torch::autograd::Function<SwiGLU8Function> {
 // gelu8_fn(h), swiglu8_fn(gate, value): the activation, its inputs kept in 8
 // bits where a gradient will be wanted.
 Tensor gelu8_fn(Tensor h) {
+  const OptTensor in = h;
+  refuse_tangents({&in}, "gelu8");
   h = h.contiguous();
   if (at::GradMode::is_enabled() && h.requires_grad()) return Gelu8Function::apply(h);
   return std::get<0>(gelu_checkpoint8(h, false));
 }
 Tensor swiglu8_fn(Tensor gate, Tensor value) {
+  const OptTensor ins[] = {gate, value};
+  refuse_tangents({&ins[0], &ins[1]}, "swiglu8");
   gate = gate.contiguous();
   value = value.contiguous();
   if (at::GradMode::is_enabled() && (gate.requires_grad() || value.requires_grad()))

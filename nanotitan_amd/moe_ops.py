@@ -573,7 +573,7 @@ def moe_few_tokens(x, weights, top_k, router_weight=None, logits=None):
     gates [T,k] float32, ids [T,k] int32): the values of route_fn, dispatch, the experts'
     grouped GEMMs and combine (reference src/model/cuda_backend.py:17-81), with only the
     hidden values rounded to x's dtype on the way. Inference only: it raises where a gradient
-    would be lost.
+    or a forward-mode tangent would be lost.
     """
     if len(weights) not in (2, 3):
         raise RuntimeError("weights are (W_gate, W_val, W_out) or (W_up, W_down)")
