@@ -9,6 +9,7 @@
 // libnanotitan_moe.so on the current HIP stream of the input's device. No
 // function synchronises the host.
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
 #include <torch/extension.h>
 
 #include <c10/hip/HIPGuard.h>
@@ -1201,18 +1202,35 @@ OptTensor optional_of(const Tensor& t) { return t.defined() ? OptTensor(t) : Opt
 OptTensor contiguous_of(const Tensor& t) {
   return t.defined() ? OptTensor(t.contiguous()) : OptTensor();
 }
-// Gradients that are not differentiable again say so when it is tried.
-variable_list once(variable_list grads, const char* what) {
+// Gradients that are not differentiable again say so when it is tried: the
+// kernels' outputs have no graph, so a term made of them (a gradient penalty)
+// would otherwise count as a constant. The error stands between them and all
+// that the first backward leads to, the leaves among them, and what its own
+// inputs came from: any second derivative meets it. Called inside a backward.
+variable_list once(variable_list grads, const variable_list& from, const std::string& what) {
   if (!at::GradMode::is_enabled()) return grads;
-  variable_list given;
+  torch::autograd::edge_list edges;
+  if (const auto node = torch::autograd::get_current_node())
+    for (const auto& e : node->next_edges())
+      if (e.is_valid()) edges.push_back(e);
+  for (const Tensor& t : from)
+    if (t.defined() && t.requires_grad())
+      edges.push_back(torch::autograd::impl::gradient_edge(t));
+  const std::shared_ptr<torch::autograd::Node> error(
+      new torch::autograd::Error(what + " is once differentiable: its backward has none",
+                                 std::move(edges)),
+      torch::autograd::deleteNode);
   for (const Tensor& g : grads)
-    if (g.defined()) given.push_back(g);
-  const int n = (int)given.size();
-  variable_list marked = (*std::make_shared<torch::autograd::DelayedError>(
-      std::string(what) + " is once differentiable: its backward has none", n))(std::move(given));
-  size_t i = 0;
-  for (Tensor& g : grads)
-    if (g.defined()) g = marked[i++];
+    if (g.defined()) torch::autograd::set_history(g, error);
+  return grads;
+}
+// The same for the Functions in Python: (grads, the outputs' gradients, name).
+std::vector<OptTensor> once_differentiable(std::vector<OptTensor> grads,
+                                           std::vector<OptTensor> from, std::string what) {
+  variable_list g, f;
+  for (const OptTensor& t : grads) g.push_back(defined(t));
+  for (const OptTensor& t : from) f.push_back(defined(t));
+  once(g, f, what);
   return grads;
 }
 
@@ -1252,7 +1270,7 @@ struct BlockNormFunction : public torch::autograd::Function<BlockNormFunction> {
                                  dh, dn, ctx->saved_data["layer"].toBool(), need);
     for (int i = 0; i < 8; ++i)
       if (g[i]) out[i] = *g[i];
-    return once(std::move(out), "block_norm");
+    return once(std::move(out), grads, "block_norm");
   }
 };
 
@@ -1304,7 +1322,8 @@ struct Gelu8Function : public torch::autograd::Function<Gelu8Function> {
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const variable_list s = ctx->get_saved_variables();
-    return once({std::get<0>(gelu_backward8(grads[0].contiguous(), s[0], s[1], false))}, "gelu8");
+    return once({std::get<0>(gelu_backward8(grads[0].contiguous(), s[0], s[1], false))}, grads,
+                "gelu8");
   }
 };
 struct SwiGLU8Function : public torch::autograd::Function<SwiGLU8Function> {
@@ -1316,7 +1335,7 @@ struct SwiGLU8Function : public torch::autograd::Function<SwiGLU8Function> {
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const variable_list s = ctx->get_saved_variables();
     auto g = swiglu_backward8(grads[0].contiguous(), s[0], s[1], s[2], s[3], false);
-    return once({std::get<0>(g), std::get<1>(g)}, "swiglu8");
+    return once({std::get<0>(g), std::get<1>(g)}, grads, "swiglu8");
   }
 };
 // gelu8_fn(h), swiglu8_fn(gate, value): the activation, its inputs kept in 8
@@ -1694,6 +1713,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("gelu_backward8", &gelu_backward8, "GELU's backward from an 8-bit checkpoint");
   m.def("swiglu_checkpoint8", &swiglu_checkpoint8, "SwiGLU with its inputs kept in 8 bits");
   m.def("swiglu_backward8", &swiglu_backward8, "SwiGLU's backward from 8-bit checkpoints");
+  m.def("once_differentiable", &once_differentiable,
+        "Marks a backward's gradients: a second derivative through them raises");
   m.def("stream_fill", &stream_fill, "16-byte streaming device fill (write bandwidth reference)",
         pybind11::arg("dst"), pybind11::arg("value") = 0);
   m.def("stream_read", &stream_read, "16-byte streaming device read (read bandwidth reference)",

@@ -33,10 +33,10 @@ in the extension.
 
 from __future__ import annotations
 
+import functools
 from typing import Any
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from nanotitan_amd.extension import get_hip_extension
 
@@ -646,6 +646,23 @@ def swiglu8_fn(gate, value):
     return get_hip_extension().swiglu8_fn(gate, value)
 
 
+def _once_differentiable(backward):
+    """Second derivatives through ``backward`` raise.
+
+    Unlike torch's decorator, also where the output's gradient needs none itself (a
+    gradient penalty on a plain sum), which would count as a constant there.
+    """
+    @functools.wraps(backward)
+    def run(ctx, *dys):
+        with torch.no_grad():
+            grads = backward(ctx, *dys)
+        if not torch.is_grad_enabled():
+            return grads
+        what = backward.__qualname__.split(".")[0]
+        return tuple(get_hip_extension().once_differentiable(list(grads), list(dys), what))
+    return run
+
+
 class GroupedGeluFFN8_FN(torch.autograd.Function):
     """GroupedGeluFFN_FN that keeps X and h = X W_up in 8 bits instead of X, gelu(h), gelu'(h).
 
@@ -663,7 +680,7 @@ class GroupedGeluFFN8_FN(torch.autograd.Function):
         return ext.grouped_gemm_kernel(act, expert_offset, W_down)
 
     @staticmethod
-    @once_differentiable
+    @_once_differentiable
     def backward(ctx, dy):
         ext = get_hip_extension()
         off, W_up, W_down, codes, exps, *kept_X = ctx.saved_tensors
@@ -701,7 +718,7 @@ class SwiGLUFFN8_FN(torch.autograd.Function):
         return ext.grouped_gemm_kernel(hidden, expert_offset, W_out)
 
     @staticmethod
-    @once_differentiable
+    @_once_differentiable
     def backward(ctx, dy):
         ext = get_hip_extension()
         off, W_gate, W_val, W_out, gc, ge, vc, ve, *kept_X = ctx.saved_tensors

@@ -58,3 +58,35 @@ def test_tangents_that_are_switched_off_are_no_reason():
         dual = forward_ad.make_dual(x, torch.ones_like(x))
         with pytest.raises(RuntimeError, match="GPU tensor"):
             moe_ops.gelu8_fn(dual)
+
+
+class _Square(torch.autograd.Function):
+    """x^2 with a backward that, like a kernel's, has no graph of its own."""
+
+    @staticmethod
+    def forward(ctx, x, scale):
+        ctx.save_for_backward(x.detach(), scale.detach())
+        return x * x * scale
+
+    @staticmethod
+    @moe_ops._once_differentiable
+    def backward(ctx, dy):
+        x, scale = ctx.saved_tensors
+        return 2 * x * scale * dy, None
+
+
+def test_a_second_derivative_meets_an_error():
+    """On the way to the leaf and to the output's gradient, not only in backward()."""
+    x, s = torch.tensor([3.0], requires_grad=True), torch.tensor([1.0])
+    (g,) = torch.autograd.grad(_Square.apply(x, s).sum(), x, create_graph=True)
+    assert float(g) == 6.0
+    penalty = (_Square.apply(x, s) + g * g).sum()
+    with pytest.raises(RuntimeError, match="once differentiable"):
+        torch.autograd.grad(penalty, x, retain_graph=True)
+    with pytest.raises(RuntimeError, match="once differentiable"):
+        penalty.backward()
+    with pytest.raises(RuntimeError, match="once differentiable"):
+        torch.autograd.functional.jvp(lambda v: _Square.apply(v, s), x.detach(), torch.ones(1))
+    x.grad = None
+    _Square.apply(x, s).sum().backward()  # the first is as it was
+    assert float(x.grad) == 6.0
