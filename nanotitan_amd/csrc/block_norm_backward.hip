@@ -208,16 +208,16 @@ block_norm_backward_kernel(NormGradArgs a) {
         if (a.dgate != nullptr && live && threadIdx.x % TPR == 0)
           static_cast<S*>(a.dgate)[row] = elem<T>::store(t[kGate]);
       if (a.dy != nullptr && live) {
-        // without a norm's weight p = y: nothing to project out
-        float m0 = 0.f, m1 = 0.f;
-        if (a.w != nullptr) {
-          m1 = t[0] * inv_d;
-          if constexpr (LAYER) m0 = t[1] * inv_d;
-        }
+        // without a norm's weight p = y: nothing to project out, and whatever y
+        // holds (an infinity times zero would be a NaN) dy is D
+        const bool norm = a.w != nullptr;
+        float m0 = 0.f, m1 = t[0] * inv_d;
+        if constexpr (LAYER) m0 = t[1] * inv_d;
 #pragma unroll
         for (int k = 0; k < CH; ++k) {
 #pragma unroll
-          for (int i = 0; i < V; ++i) y[k][i] = r_y * (D[k][i] - m0 - y[k][i] * m1);
+          for (int i = 0; i < V; ++i)
+            y[k][i] = norm ? r_y * (D[k][i] - m0 - y[k][i] * m1) : D[k][i];
           store_chunk<T, V>(a.dy, base, c[k], y[k]);
         }
       }
