@@ -111,11 +111,13 @@ __global__ void __launch_bounds__(block_threads(SH::TPR)) block_norm_kernel(Norm
     for (int k = 0; k < CH; ++k) {
       values<TX, V>(rx[k], c[k], h[k]);
       if constexpr (MODE != kPre) values<T, V>(ry[k], c[k], p[k]);
-      if constexpr (MODE == kGated) all_values<T, V>(rg[k], g[k]);
+      // (a layer norm's row is NaN with any infinity in it, owned or not)
+      if constexpr (MODE == kGated)
+        all_values<T, V>(LAYER ? rg[k] : owned<T, V>(rg[k], c[k]), g[k]);
     }
     if constexpr (kAhead) load(row + step);
     // x, y and the parameters are zero where a chunk does not own a column, and so
-    // is h (unless a value overlapped is an infinity or NaN, as is then the row)
+    // is h, whose gate is cleared for it: an infinity times zero would be a NaN
     float mean_y = 0.f, r_y = 1.f, mean_h = 0.f, r_h = 1.f;
     if constexpr (MODE != kPre) {
       float g_row = 1.f;
