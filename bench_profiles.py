@@ -61,6 +61,7 @@ COPY_BYTES = 1 << 30  # bench.py --copy-probe moves 1 GiB per launch
 # What the profiled kernels are compiled from: the training layer's path. A
 # change to any other source leaves the profiles as they are.
 PROFILED_SOURCES = ("combine.hip", "common.hpp", "dispatch.hip", "gemm_common.hpp",
+                    "gelu.hpp",
                     "gen_gelu_table.py", "grouped_gemm.hip", "library.hip", "router.hip",
                     "router_linear.hip", "staged_gemm.hip")
 

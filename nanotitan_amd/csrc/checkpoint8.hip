@@ -15,11 +15,13 @@
 // the hidden gradient, and write the pre-activations' gradients and, for the
 // down projection's weight gradient, the hidden values again. HBM bounds all
 // of it as long as the arithmetic stays near 30 instructions a value, which is
-// why erf, the division and the conversions are written out below.
+// why the division and the conversions are written out below, and why 16-bit
+// values take the fit of erfc that the plain path's epilogue takes (gelu.hpp).
 #include <algorithm>
 
 #include "bits.hpp"
 #include "common.hpp"
+#include "gelu.hpp"
 
 namespace nt {
 namespace {
@@ -207,21 +209,6 @@ __device__ __forceinline__ float sigmoid(float x) {
   return __builtin_amdgcn_rcpf(1.f + __expf(-x));
 }
 
-// The normal distribution's Phi(x), and e^(-x^2 / 2) on the way, by Abramowitz
-// and Stegun's 7.1.26: erfc(z) = (a1 t + ... + a5 t^5) e^(-z^2), t = 1 / (1 +
-// 0.3275911 z), z = |x| / sqrt(2), within 1.5e-7. The exponential is the one
-// that gelu's slope needs, and small Phi stay relatively exact.
-__device__ __forceinline__ float normal_cdf(float x, float& bell) {
-  bell = __expf(-0.5f * x * x);
-  const float t = __builtin_amdgcn_rcpf(fmaf(0.3275911f * 0.70710678f, fabsf(x), 1.f));
-  float p = fmaf(1.061405429f, t, -1.453152027f);
-  p = fmaf(p, t, 1.421413741f);
-  p = fmaf(p, t, -0.284496736f);
-  p = fmaf(p, t, 0.254829592f);
-  const float tail = 0.5f * p * t * bell;
-  return x < 0.f ? tail : 1.f - tail;
-}
-
 struct Act8Args {
   const void *a, *b;        // pre-activation (gate), value; backward: the hidden gradient in a
   void *out, *da, *db;      // hidden; backward: gradients
@@ -244,7 +231,7 @@ __global__ void __launch_bounds__(kThreads) keep8_kernel(Act8Args g) {
 #pragma unroll
     for (int i = 0; i < kVec; ++i) {
       float bell;
-      o.set(i, ACT == kSwiGLU8 ? a[i] * sigmoid(a[i]) * b[i] : a[i] * normal_cdf(a[i], bell));
+      o.set(i, ACT == kSwiGLU8 ? a[i] * sigmoid(a[i]) * b[i] : a[i] * gelu_cdf<T>(a[i], bell));
     }
     o.store(g.out, p, g.f);
   }
@@ -287,7 +274,7 @@ __global__ void __launch_bounds__(kThreads) held8_kernel(Act8Args g) {
 #pragma unroll
     for (int i = 0; i < kVec; ++i) {
       float bell;
-      const float cdf = normal_cdf(a[i], bell);
+      const float cdf = gelu_cdf<T>(a[i], bell);
       o.set(i, a[i] * cdf);
       da.set(i, d[i] * fmaf(a[i] * 0.39894228f, bell, cdf));
     }

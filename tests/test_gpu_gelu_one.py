@@ -1,5 +1,5 @@
-"""One GELU for the experts: the 8-bit path, the few-token layer and the plain FFN agree,
-and stay relatively exact where the normal distribution's tail is small."""
+"""One GELU for the experts: the 8-bit path and the plain FFN agree, and stay
+relatively exact where the normal distribution's tail is small."""
 
 import math
 from types import SimpleNamespace
@@ -37,7 +37,8 @@ def _tail_tolerance(x, want, dtype):
     if dtype == torch.float32:
         # 0.5 (1 + erf): erf within two units of one at 1, and cancelled there
         return 8 * U * x.abs()
-    sub = 2.0**-25 if dtype == torch.float16 else 0.0  # half a step of its subnormals
+    # half a step of the subnormals: fp16 2^-14 2^-10 / 2, bf16 2^-126 2^-7 / 2
+    sub = 2.0**-25 if dtype == torch.float16 else 2.0**-134
     return (eps / 2 + _fit(x)) * want.abs() * (1 + eps) + sub
 
 
@@ -79,26 +80,9 @@ def test_gelu8_slope_in_the_tail(ext, dtype):
         tol = 16 * U * (1 + k64.abs())
     else:
         tol = torch.finfo(dt).eps / 2 * want.abs() + _fit(k64) * size + (
-            2.0**-25 if dt == torch.float16 else 0.0)
+            2.0**-25 if dt == torch.float16 else 2.0**-134)
     off = (dh.cpu().double() - want).abs() - tol
     assert bool((off <= 0).all()), float(k64.flatten()[off.flatten().argmax()])
-
-
-@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
-@pytest.mark.parametrize("T", [12, 40])
-def test_few_tokens_in_the_tail(ext, dtype, T):
-    """One expert whose projections are diagonal: the output is the rounded hidden row."""
-    dt = TYPES[dtype]
-    n = 256
-    z = torch.linspace(-12, -3, n).to(dt)
-    up, down = torch.diag(z).unsqueeze(0).cuda(), torch.eye(n, dtype=dt).unsqueeze(0).cuda()
-    x = torch.ones(T, n, dtype=dt, device="cuda")
-    with torch.no_grad():
-        got = moe_ops.moe_few_tokens(x, (up, down), 1, logits=torch.zeros(T, 1, device="cuda"))[0]
-    z64 = z.double()
-    want = z64 * _cdf64(z64)
-    off = (got.cpu().double() - want).abs() - _tail_tolerance(z64, want, dt)
-    assert bool((off <= 0).all()), float(z64[off.max(0).values.argmax()])
 
 
 @pytest.mark.parametrize("dtype", TYPES)
