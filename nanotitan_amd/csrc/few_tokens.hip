@@ -29,6 +29,7 @@
 
 #include "bits.hpp"
 #include "common.hpp"
+#include "gelu.hpp"
 
 namespace nt {
 namespace {
@@ -718,10 +719,6 @@ __device__ __forceinline__ int64_t fold_col(const TileColumns& tc, int64_t N, in
   return tc.start + (NARROW || c <= most ? c : most) + (at & 3);
 }
 
-__device__ __forceinline__ float few_gelu(float x) {
-  return 0.5f * x * (1.f + erff(x * 0.70710678f));
-}
-
 // hidden = act(x W1[, x W2]), one tile of 64 hidden columns of one expert (or
 // HALVES = 2 neighbouring ones of a single matrix: as much in flight a wave as
 // with two matrices) for KW waves at a time.
@@ -804,7 +801,10 @@ __global__ void __launch_bounds__(group_waves(KW) * kWave) few_up_kernel(FewArgs
           const int64_t c = fold_col<KW, NARROW>(tc[h], a.f, j);
           float z;
           if constexpr (SWIGLU) z = v[0][j] / (1.f + __expf(-v[0][j])) * v[1][j];
-          else z = few_gelu(v[h][j]);
+          else {
+            float bell;
+            z = v[h][j] * gelu_cdf<T>(v[h][j], bell);
+          }
           if (r < rows && c >= col + h * kCols && c < a.f)
             hidden[(int64_t)r * a.f + c] = to_bits<T>(z);
         }

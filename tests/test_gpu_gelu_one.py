@@ -1,5 +1,5 @@
-"""One GELU for the experts: the 8-bit path and the plain FFN agree, and stay
-relatively exact where the normal distribution's tail is small."""
+"""One GELU for the experts: the 8-bit path, the few-token layer and the plain FFN
+agree, and stay relatively exact where the normal distribution's tail is small."""
 
 import math
 from types import SimpleNamespace
@@ -83,6 +83,23 @@ def test_gelu8_slope_in_the_tail(ext, dtype):
             2.0**-25 if dt == torch.float16 else 2.0**-134)
     off = (dh.cpu().double() - want).abs() - tol
     assert bool((off <= 0).all()), float(k64.flatten()[off.flatten().argmax()])
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("T", [12, 40])
+def test_few_tokens_in_the_tail(ext, dtype, T):
+    """One expert whose projections are diagonal: the output is the rounded hidden row."""
+    dt = TYPES[dtype]
+    n = 256
+    z = torch.linspace(-12, -3, n).to(dt)
+    up, down = torch.diag(z).unsqueeze(0).cuda(), torch.eye(n, dtype=dt).unsqueeze(0).cuda()
+    x = torch.ones(T, n, dtype=dt, device="cuda")
+    with torch.no_grad():
+        got = moe_ops.moe_few_tokens(x, (up, down), 1, logits=torch.zeros(T, 1, device="cuda"))[0]
+    z64 = z.double()
+    want = z64 * _cdf64(z64)
+    off = (got.cpu().double() - want).abs() - _tail_tolerance(z64, want, dt)
+    assert bool((off <= 0).all()), float(z64[off.max(0).values.argmax()])
 
 
 @pytest.mark.parametrize("dtype", TYPES)
