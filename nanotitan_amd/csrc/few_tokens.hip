@@ -914,7 +914,7 @@ __global__ void __launch_bounds__(group_waves(KW) * kWave) few_down_kernel(FewAr
         }
     }
     if (KW == 8 && HALVES == 1 && a.arrive) {
-      wait_batch_loads();
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
       __syncthreads();
       if (threadIdx.x == 0) s_last = atomicAdd(&a.arrived[tile], 1) == num_loads * a.splits - 1;
       __syncthreads();
@@ -1066,8 +1066,8 @@ void launch_few(FewArgs a, hipStream_t stream) {
   // 16 arrivals on a counter and the sum of a few tokens by one workgroup cost
   // less than a launch (one token of 512: 17 against 19 us); 40 arrivals, or 32
   // tokens, do not (25 against 22)
-  a.arrive = down.halves == 1 && down.waves == kMaxTileWaves && down.count <= 512 &&
-             a.most_live * a.splits <= 16 && a.T <= kSmallTokens;
+  a.arrive = down.halves == 1 && down.waves == kMaxTileWaves && a.most_live * a.splits <= 16 &&
+             a.T <= kSmallTokens;
   by_tiles<T, NARROW>(down, [&](auto halves, auto waves) {
     constexpr int H = decltype(halves)::value, KW = decltype(waves)::value;
     hipLaunchKernelGGL((few_down_kernel<T, H, MT, KW, NARROW>), few_grid(a, down, KW),
