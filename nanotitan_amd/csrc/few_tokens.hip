@@ -551,12 +551,15 @@ struct Step {
       __builtin_memcpy(x[m].v, v, sizeof(v));
     }
   }
-  // Matrices of fewer than four columns: element by element.
+  // Layers with a width of less than four: element by element, in both of their
+  // projections.
   __device__ __forceinline__ void load_narrow_weights(const S* const (&base)[MATS], int64_t N,
+                                                      const TileColumns (&tc)[MATS],
                                                       int64_t step, int64_t left) {
-    const int k0 = (lane_id() >> 4) * 8, c0 = (lane_id() & 15) * 4;
+    const int k0 = (lane_id() >> 4) * 8;
 #pragma unroll
-    for (int i = 0; i < MATS; ++i)
+    for (int i = 0; i < MATS; ++i) {
+      const int64_t c0 = tc[i].start + (lane_id() & 15) * 4;
 #pragma unroll
       for (int r = 0; r < 8; ++r) {
         S v[4];
@@ -565,6 +568,7 @@ struct Step {
           v[c] = k0 + r < left && c0 + c < N ? base[i][(step * kStep + k0 + r) * N + c0 + c] : S(0);
         __builtin_memcpy(w[i].r[r], v, sizeof(v));
       }
+    }
   }
   template <int MT>
   __device__ __forceinline__ void multiply(f32x4 (&acc)[MATS][MT][4]) const {
@@ -592,7 +596,7 @@ __device__ __forceinline__ void wave_tile(const typename elem<T>::storage* const
   if constexpr (NARROW) {
     for (; s < s1; s += KW) {
       Held t;
-      t.load_narrow_weights(base, N, s, K - s * kStep);
+      t.load_narrow_weights(base, N, tc, s, K - s * kStep);
       t.load_last_tokens(x0, row, s, K - s * kStep);
       t.multiply(acc);
     }
