@@ -305,7 +305,7 @@ int nt_router_linear_backward_mixed(int x_dtype, int dx_dtype, const void* x, co
  * act = silu(x @ w_up[e]) * (x @ w_val[e]), or the erf GELU where w_val is NULL.
  * x, out [T,d], w_up, w_val [E,d,f], w_down [E,f,d] of dtype (f32, f16, bf16);
  * the hidden values are rounded to dtype, everything else is float32 up to the
- * one rounding of out. k <= 32, E <= NT_MAX_EXPERTS. The workspace (16-byte
+ * one rounding of out. k <= 32, E <= NT_MAX_EXPERTS, d, f <= 2^22. The workspace (16-byte
  * aligned, contents arbitrary) is written before it is read: calls that cannot
  * overlap may share one. Replaces, for few tokens, the dataflow of reference
  * src/model/cuda_backend.py:17-81. */
@@ -325,8 +325,8 @@ int nt_moe_few_tokens(int dtype, const void* x, const float* router, const float
  * (ties to even), exps [rows, nt_checkpoint8_blocks(f)] = x + 127. A block that
  * holds an infinity or a NaN has exponent 255 and decodes to NaN. x is f32, f16
  * or bf16; decoding is exact in the type that was kept, but for a value that
- * rounds past the type's largest: it decodes to that. No counterpart in the
- * reference, which keeps activations as they are. */
+ * rounds past the type's largest: it decodes to that. At most 2^31 - 128 blocks.
+ * No counterpart in the reference, which keeps activations as they are. */
 int64_t nt_checkpoint8_blocks(int64_t f);
 int nt_checkpoint8(int dtype, const void* x, int64_t rows, int64_t f, int8_t* codes,
                    uint8_t* exps, hipStream_t stream);

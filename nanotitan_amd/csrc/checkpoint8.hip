@@ -287,8 +287,8 @@ int check8(int dtype, int64_t rows, int64_t f) {
   if (dtype != NT_F32 && dtype != NT_F16 && dtype != NT_BF16) return NT_ERR_DTYPE;
   if (rows < 0 || f < 1) return NT_ERR_INVALID_ARG;
   if (f > (1 << 30) || rows > INT32_MAX) return NT_ERR_TOO_LARGE;
-  // workgroups of 256 chunks
-  if (rows * (ceil_div(f, kBlock) * kLanes) > (int64_t)INT32_MAX * kThreads)
+  // a thread for every chunk, in whole workgroups: a launch takes fewer than 2^32
+  if (rows * (ceil_div(f, kBlock) * kLanes) > (int64_t)UINT32_MAX + 1 - kThreads)
     return NT_ERR_TOO_LARGE;
   return NT_OK;
 }
