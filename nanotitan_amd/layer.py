@@ -201,6 +201,13 @@ def _plain_router(router, flat) -> bool:
             and flat.shape[0] > 0 and not torch.is_autocast_enabled())
 
 
+def _plain_experts(experts) -> bool:
+    """Whether calling ``experts`` without gradients is its class's ``forward`` and nothing else."""
+    return (not experts._forward_hooks and not experts._forward_pre_hooks
+            and "forward" not in experts.__dict__
+            and not nn.modules.module._has_any_global_hook())
+
+
 class HIPMoEBackend:
     """Reference CUDAMoEBackend dataflow (src/model/cuda_backend.py:11-81) on the HIP path."""
 
@@ -270,14 +277,10 @@ class MoE(nn.Module):
         """The layer's output for the few tokens (at most 64 in all) of a decode step.
 
         x [B,S,d] -> [B,S,d], the values of ``forward`` up to the roundings that the one
-        kernel path does not make; no statistics, no gradients.
+        kernel path does not make; no statistics, no gradients. Hooks on the router run, and
+        hooks on the experts (or a forward put in place of theirs) too, by the full path;
+        those on this module belong to ``forward``.
         """
-        flat = x.reshape(-1, x.shape[-1]).contiguous()
-        if _plain_router(self.router, flat):
-            route = {"router_weight": self.router.weight}
-        else:
-            logits = self.router(flat.to(self.router.weight.dtype))
-            route = {"logits": logits.float().contiguous()}
         e = self.experts
         if type(e) is ExpertFFN:
             weights = (e.W_gate, e.W_val, e.W_out)
@@ -285,6 +288,16 @@ class MoE(nn.Module):
             weights = (e.W_up, e.W_down)
         else:
             raise RuntimeError(f"decode runs this package's experts, not {type(e).__name__}")
+        flat = x.reshape(-1, x.shape[-1]).contiguous()
+        plain = _plain_experts(e)
+        if plain and _plain_router(self.router, flat):
+            route = {"router_weight": self.router.weight}
+        else:
+            logits = self.router(flat.to(self.router.weight.dtype))
+            if not plain:
+                return moe_forward_from_logits(flat, logits, e, self.cfg.num_experts,
+                                               self.cfg.top_k)[0].view(x.shape)
+            route = {"logits": logits.float().contiguous()}
         return moe_few_tokens(flat, weights, self.cfg.top_k, **route)[0].view(x.shape)
 
 
