@@ -15,8 +15,9 @@ fraction to its JSON line from the summaries this script writes:
 
 Every JSON records the commit the measured tree stood on (the parent, where a
 kernel change and its profiles are one commit) and ``source_hash``, a hash of
-their kernels' sources (``kernel_source_hash``); ``bench.py`` recomputes the hash
-and reports whether the profile still matches the code it runs.
+their kernels' sources and all that these include (``kernel_source_hash``);
+``bench.py`` recomputes the hash and reports whether the profile still matches
+the kernels it runs.
 
 Usage, after the profiling runs (``rocprofv3 ... -d <dir>/<pass> -o c<N> --
 python3 bench.py --config N ...``) have written their CSVs under ``<dir>``::
@@ -58,20 +59,40 @@ SIMDS = 1024
 COPY_BYTES = 1 << 30  # bench.py --copy-probe moves 1 GiB per launch
 
 
-# What the profiled kernels are compiled from: the training layer's path. A
-# change to any other source leaves the profiles as they are.
-PROFILED_SOURCES = ("combine.hip", "common.hpp", "dispatch.hip", "gemm_common.hpp",
-                    "gelu.hpp",
-                    "gen_gelu_table.py", "grouped_gemm.hip", "library.hip", "router.hip",
-                    "router_linear.hip", "staged_gemm.hip")
+# The sources that hold the profiled kernels: the training layer's path. What they
+# include counts with them (profiled_files).
+PROFILED_SOURCES = ("combine.hip", "dispatch.hip", "grouped_gemm.hip", "library.hip",
+                    "router.hip", "router_linear.hip", "staged_gemm.hip")
+# Included files that the build generates, and what generates them.
+GENERATED = {"gelu_table_bf16.inc": "gen_gelu_table.py"}
+
+
+def profiled_files(root: Path = ROOT) -> list[Path]:
+    """The profiled kernels' sources with all that their quoted includes lead to, sorted."""
+    csrc = root / "nanotitan_amd" / "csrc"
+    todo, seen = [csrc / name for name in PROFILED_SOURCES], set()
+    while todo:
+        path = todo.pop()
+        if path in seen:
+            continue
+        seen.add(path)
+        if path.suffix == ".py":
+            continue
+        for name in re.findall(r'^\s*#\s*include\s+"([^"]+)"', path.read_text(), re.M):
+            name = GENERATED.get(name, name)
+            hits = [d / name for d in (path.parent, root / "include") if (d / name).is_file()]
+            if not hits:
+                raise FileNotFoundError(f"{path}: #include \"{name}\"")
+            todo.append(hits[0])
+    return sorted(seen)
 
 
 def kernel_source_hash(root: Path = ROOT) -> str:
-    """sha256 over the sources of the profiled kernels (sorted names)."""
+    """sha256 over the profiled kernels' sources and all that they include."""
     h = hashlib.sha256()
-    for name in PROFILED_SOURCES:
-        h.update(name.encode())
-        h.update((root / "nanotitan_amd" / "csrc" / name).read_bytes())
+    for path in profiled_files(root):
+        h.update(path.relative_to(root).as_posix().encode())
+        h.update(path.read_bytes())
     return h.hexdigest()[:16]
 
 

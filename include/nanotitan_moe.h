@@ -366,7 +366,7 @@ int nt_swiglu_backward8(int dtype, const void* dhidden, const int8_t* gate_codes
  * scale [scale_cols] (1 or d) of param_dtype (f32, f16, bf16). gate, scale, b
  * and b_next may be NULL (1, 1, 0, 0); rms norms take no bias. y NULL: h is x
  * and not written, n = N(x). stats [T,4] f32 keeps the rows' means and r for
- * the backward (NULL to skip). d <= 16384. Arithmetic in float32. Outputs must
+ * the backward (NULL to skip). d <= 16384, T < 2^31. Arithmetic in float32. Outputs must
  * not overlap inputs. No counterpart in the reference, whose layer calls torch's
  * LayerNorm before the block (src/model/model.py:205-211). */
 enum nt_norm_kind { NT_NORM_RMS = 0, NT_NORM_LAYER = 1 };
