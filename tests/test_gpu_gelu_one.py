@@ -7,6 +7,7 @@ from types import SimpleNamespace
 import pytest
 import torch
 
+import tests.test_gpu_moe_block as blocks
 from nanotitan_amd import moe_ops
 from nanotitan_amd.layer import MoEBlock
 from tests.test_block_ops_cpu import held64
@@ -126,3 +127,24 @@ def test_checkpoints_leave_gelu_experts_forward_alone(ext, dtype, d, f):
     assert torch.equal(kept(x)[0], out)
     with torch.no_grad():
         assert torch.equal(kept(x)[0], out)
+
+
+def test_checkpoints_change_gelu_experts_gradients_by_their_rounding(ext):
+    """The blocks' test of outputs and weight gradients, with GELU experts."""
+    blocks.test_checkpoints_change_the_weight_gradients_by_their_rounding(ext, blocks.KINDS[2])
+
+
+@pytest.mark.parametrize("fn", ["swiglu", "gelu"])
+def test_ffn8_without_rows(ext, fn):
+    """No row, and experts of which none has one: gradients of zero."""
+    d, f, E = 64, 96, 3
+    up = [torch.randn(E, d, f, device="cuda", requires_grad=True)
+          for _ in range(2 if fn == "swiglu" else 1)]
+    down = torch.randn(E, f, d, device="cuda", requires_grad=True)
+    X = torch.randn(0, d, device="cuda", requires_grad=True)
+    off = torch.zeros(E + 1, dtype=torch.int32, device="cuda")
+    call = moe_ops.swiglu_ffn8_fn if fn == "swiglu" else moe_ops.grouped_gelu_ffn8_fn
+    y = call(X, *up, down, off)
+    assert y.shape == (0, d)
+    dX, *dW = torch.autograd.grad(y, [X, *up, down], torch.zeros_like(y))
+    assert dX.shape == (0, d) and all(float(w.abs().max()) == 0.0 for w in dW)
