@@ -14,8 +14,8 @@
 // Measured on MI355X (a copy: 5.65 TB/s), bf16: 16,384 x 4,096 rms 160 us
 // (5.0 TB/s), layer 172 (4.7); 131,072 x 512 156 and 161 (5.2, 5.0); the sums'
 // launch is 5 to 8 us of each. Above 8,192 columns a thread holds sixteen and
-// the sums no longer fit its registers: 4,096 x 16,384 rms 210 (3.8), layer 454
-// (1.8).
+// the sums no longer fit its registers: 4,096 x 16,384 rms 215 (3.7), layer 424
+// (1.9).
 #include "block_norm.hpp"
 
 namespace nt {

@@ -17,6 +17,12 @@
 // of it as long as the arithmetic stays near 30 instructions a value, which is
 // why the division and the conversions are written out below, and why 16-bit
 // values take the fit of erfc that the plain path's epilogue takes (gelu.hpp).
+//
+// Measured on MI355X (a copy: 5.65 TB/s): SwiGLU of 61,440 x 2,048 bf16 187 us
+// forward, 186 backward (5.45 TB/s); GELU of the same 115 (5.5) and 142 (4.5: with
+// three quarter-rate instructions a value the vector units bound it); GELU of
+// 10,007 x 1,365 fp16 19 and 26, of 1,344 columns, whose rows are aligned, 13 and
+// 23% less.
 #include <algorithm>
 
 #include "bits.hpp"

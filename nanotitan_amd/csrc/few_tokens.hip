@@ -19,10 +19,10 @@
 // goes through LDS but the waves' partial sums at the end.
 //
 // Measured on MI355X (a read of 2 GiB: 7.1 TB/s): 16 tokens of 4,096, 8 experts
-// of 14,336, bf16: up 282 us (6.7 TB/s), down 139 (6.8), all 430; 64 tokens: all
-// 449 (6.3); 33 tokens of 2,048, 128 experts of 768, top-8, fp16:
-// up 60 (6.0), down 59 (6.1), routing 8, gate sum 5, all 131; one token of 512,
-// 16 experts of 2,048: 9 + 8, all 17.5 (its 12.6 MB would take 1.8: launches
+// of 14,336, bf16: up 285 us (6.6 TB/s), down 141 (6.7), all 433; 64 tokens: all
+// 455 (6.2); 33 tokens of 2,048, 128 experts of 768, top-8, fp16:
+// up 59 (6.0), down 58 (6.1), routing 7, gate sum 5, all 129; one token of 512,
+// 16 experts of 2,048: 9 + 8, all 17.2 (its 12.6 MB would take 1.8: launches
 // and a chain of about ten dependent memory latencies).
 #include <algorithm>
 #include <type_traits>
