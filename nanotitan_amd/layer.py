@@ -34,6 +34,7 @@ import torch
 import torch.nn as nn
 from torch.profiler import record_function
 
+from nanotitan_amd.capi import NT_FEW_TOKENS_MAX
 from nanotitan_amd.moe_ops import (
     combine_inv_fn,
     grouped_gelu_ffn8_fn,
@@ -289,6 +290,9 @@ class MoE(nn.Module):
         else:
             raise RuntimeError(f"decode runs this package's experts, not {type(e).__name__}")
         flat = x.reshape(-1, x.shape[-1]).contiguous()
+        if flat.shape[0] > NT_FEW_TOKENS_MAX:  # whatever hangs on the parts
+            raise RuntimeError(f"decode takes at most {NT_FEW_TOKENS_MAX} tokens, "
+                               f"got {flat.shape[0]}")
         plain = _plain_experts(e)
         if plain and _plain_router(self.router, flat):
             route = {"router_weight": self.router.weight}

@@ -59,3 +59,15 @@ def test_what_hangs_on_the_experts_runs(ext, ffn, how):
         else:
             handle.remove()
     assert torch.equal(moe.decode(x), before)
+
+
+@pytest.mark.parametrize("hooked", [False, True])
+def test_sizes_do_not_depend_on_what_hangs(ext, hooked):
+    moe = _moe("swiglu")
+    if hooked:
+        moe.experts.register_forward_hook(lambda module, args, out: out)
+    dt = torch.bfloat16
+    assert moe.decode(torch.zeros(1, 64, 128, device="cuda", dtype=dt)).shape == (1, 64, 128)
+    assert moe.decode(torch.zeros(2, 0, 128, device="cuda", dtype=dt)).shape == (2, 0, 128)
+    with pytest.raises(RuntimeError, match="at most"):
+        moe.decode(torch.zeros(5, 13, 128, device="cuda", dtype=dt))
