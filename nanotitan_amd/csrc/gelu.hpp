@@ -1,7 +1,9 @@
 // GELU, erf form: gelu(x) = x Phi(x) and gelu'(x) = Phi(x) + x phi(x), with Phi
 // the standard normal CDF, Phi(x) = erfc(-x/sqrt2)/2, and phi(x) =
-// exp(-x^2/2)/sqrt(2 pi). One for the grouped GEMMs' epilogues and the kernels
-// beside them, so that an expert's hidden values do not depend on the path.
+// exp(-x^2/2)/sqrt(2 pi). One for the 16-bit grouped GEMMs' epilogues and, in
+// each type, for the kernels beside them, so that an expert's hidden values do not
+// depend on the path. (The register-staged and generic GEMMs, which take 16-bit
+// widths that are no multiple of 8, form 1 + erf: gemm_common.hpp.)
 #pragma once
 
 #include "common.hpp"
