@@ -144,13 +144,15 @@ def _held(v, dim):
     return torch.round(v.double() / s.double()).float(), s
 
 
-def _tiles(q):
-    """The integers of [E,K,N] in the order that the framework keeps: 16 columns by 64 rows a
-    tile, 16 rows of a column together, padded with zeros to 16 columns and 128 rows."""
+def _blocks(q):
+    """The integers of [E,K,N] in the order that the framework keeps: blocks of 64 columns by 64
+    rows, [E, N / 64, K / 64, 4, 4, 16, 16], padded with zeros to 64 columns and 128 rows."""
     E, K, N = q.shape
-    q = torch.nn.functional.pad(q, (0, -N % 16, 0, -K % 128))
+    q = torch.nn.functional.pad(q, (0, -N % 64, 0, -K % 128))
     E, K, N = q.shape
-    return q.view(E, K // 64, 4, 16, N // 16, 16).permute(0, 4, 1, 2, 5, 3).contiguous()
+    # k = 64 kb + 16 g + b, n = 64 nb + 16 i + 4 t + j
+    q = q.view(E, K // 64, 4, 16, N // 64, 4, 4, 4).permute(0, 4, 1, 6, 2, 5, 7, 3)
+    return q.reshape(E, N // 64, K // 64, 4, 4, 16, 16)
 
 
 def _counts(A, E, seed):
@@ -174,7 +176,7 @@ def prepare(case, seed):
         # trained weights' scale: activations of unit order; what a program keeps of them
         q, scale = _held(randn(E, K, N, std=K ** -0.5, dt=torch.float32), 1)
         q = q.to(torch.int8)
-        return SimpleNamespace(q=q, scale=scale.view(E, N), tiles=_tiles(q), shape=(E, K, N))
+        return SimpleNamespace(q=q, scale=scale.view(E, N), blocks=_blocks(q), shape=(E, K, N))
 
     s = SimpleNamespace(case=case, dtype=dtype)
     op = case["op"]
@@ -256,7 +258,7 @@ def _handles(s):
     """The weights as the framework takes them."""
     from nanotitan_amd.moe_ops import Int8Weight
 
-    return [Int8Weight(w.tiles, w.scale, w.shape) for w in s.weights]
+    return [Int8Weight(w.blocks, w.scale, w.shape) for w in s.weights]
 
 
 def _run_grouped(s):
