@@ -1,0 +1,92 @@
+/*
+ * nanotitan_int8.h — C ABI of the 8-bit integer experts and linear layers on the
+ * MI355X (gfx950): part of libnanotitan_moe.so, with the element type and status
+ * codes, the calling rules and nt_strerror() of nanotitan_moe.h.
+ *
+ * Weights are held as integers with a float32 scale for each expert and output
+ * channel, activations as integers with a scale for each row:
+ *   s = max(max|v| / 127, 2^-126),  q = the integer nearest to v / s, ties to even.
+ * A row or channel with an infinity or a NaN has a NaN scale and zero integers.
+ * Products are exact int32 sums, scaled in float32 and rounded once. Sums run over
+ * at most NT_INT8_MAX_K values. Integers given by a caller are -127..127.
+ *
+ * Rows of integers have nt_int8_pitch(f) columns, zeros past f. Weights lie in the
+ * blocks that the matrix instructions read, nt_int8_weight_bytes(E, K, N) in all:
+ *   codes[e][n / 64][k / 64][t][g][i][k % 16],  g = k % 64 / 16,
+ *   n % 64 = 16 (i / 4) + 4 t + i % 4,
+ * n padded with zeros to a multiple of 64, k to one of 128; scales are [E, N].
+ * Integers are 16-byte aligned. Activations are f32, f16 or bf16.
+ * No counterpart in the reference, whose experts keep their training type
+ * (src/model/feed_fwd.py:39-122).
+ */
+#ifndef NANOTITAN_INT8_H
+#define NANOTITAN_INT8_H
+
+#include "nanotitan_moe.h"
+
+#ifdef __cplusplus
+extern "C" {
+#endif
+
+#define NT_INT8_MAX_K (1 << 17)
+
+int64_t nt_int8_pitch(int64_t f);
+size_t nt_int8_weight_bytes(int32_t E, int64_t K, int64_t N);
+
+/* Rows x [rows, f] to codes [rows, nt_int8_pitch(f)] and scales [rows], and the
+ * values q s that they hold in dtype (rounded once; past the type's largest: that). */
+int nt_int8_rows(int dtype, const void* x, int64_t rows, int64_t f, int8_t* codes, float* scales,
+                 hipStream_t stream);
+int nt_int8_rows_decode(int dtype, const int8_t* codes, const float* scales, int64_t rows,
+                        int64_t f, void* x, hipStream_t stream);
+
+/* Weights W [E, K, N] to codes and scales, and back. The workspace (4-byte aligned)
+ * holds the channels' maxima. */
+size_t nt_int8_weight_workspace_bytes(int32_t E, int64_t N);
+int nt_int8_weight(int dtype, const void* W, int32_t E, int64_t K, int64_t N, int8_t* codes,
+                   float* scales, void* ws, size_t ws_bytes, hipStream_t stream);
+int nt_int8_weight_decode(int dtype, const int8_t* codes, const float* scales, int32_t E,
+                          int64_t K, int64_t N, void* W, hipStream_t stream);
+
+/* out[a,:] = x[a] @ W[e] for the rows a of expert e: x as codes and scales of A rows
+ * (nt_int8_rows), offsets as nt_grouped_gemm takes them, or NULL with E = 1 (a linear
+ * layer of all rows). Rows >= offsets[E] are not written. out [A, N] of dtype. */
+int nt_int8_grouped_gemm(int dtype, const int8_t* x, const float* x_scales,
+                         const int32_t* offsets, const int8_t* w, const float* w_scales,
+                         int32_t E, int64_t A, int64_t K, int64_t N, void* out,
+                         hipStream_t stream);
+
+/* Both projections of a gated block, its activation and the product:
+ * hidden = silu(x @ W_gate[e]) * (x @ W_val[e]) in float32, rounded once. gate and
+ * value [A, N] are what a backward needs (both NULL: not written). */
+int nt_int8_grouped_gemm_swiglu(int dtype, const int8_t* x, const float* x_scales,
+                                const int32_t* offsets, const int8_t* w_gate,
+                                const float* gate_scales, const int8_t* w_val,
+                                const float* val_scales, int32_t E, int64_t A, int64_t K,
+                                int64_t N, void* hidden, void* gate, void* value,
+                                hipStream_t stream);
+
+/* act = gelu(x @ W[e]) (erf), and gelu' of the same (NULL: not written). */
+int nt_int8_grouped_gemm_gelu(int dtype, const int8_t* x, const float* x_scales,
+                              const int32_t* offsets, const int8_t* w, const float* w_scales,
+                              int32_t E, int64_t A, int64_t K, int64_t N, void* act,
+                              void* act_grad, hipStream_t stream);
+
+/* nt_moe_few_tokens on 8-bit weights (w_val NULL: GELU): tokens and hidden values go
+ * to 8 bits row by row, the hidden ones from their values in dtype. Everything else,
+ * the limits of sizes and the workspace's rules are nt_moe_few_tokens'; d, f <=
+ * NT_INT8_MAX_K. */
+size_t nt_int8_moe_few_tokens_workspace_bytes(int dtype, int64_t T, int32_t E, int32_t k,
+                                              int64_t d, int64_t f);
+int nt_int8_moe_few_tokens(int dtype, const void* x, const float* router, const float* logits,
+                           const int8_t* w_up, const float* up_scales, const int8_t* w_val,
+                           const float* val_scales, const int8_t* w_down,
+                           const float* down_scales, int64_t T, int32_t E, int32_t k, int64_t d,
+                           int64_t f, float* gates, int32_t* topk, void* out, void* ws,
+                           size_t ws_bytes, hipStream_t stream);
+
+#ifdef __cplusplus
+}
+#endif
+
+#endif /* NANOTITAN_INT8_H */

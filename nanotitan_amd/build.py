@@ -2,8 +2,8 @@
 
 Two artefacts, both next to this file:
 
-* ``libnanotitan_moe.so`` — the C ABI (``include/nanotitan_moe.h``): every HIP
-  kernel, compiled by ``hipcc --offload-arch=gfx950``. No torch dependency.
+* ``libnanotitan_moe.so`` — the C ABI (``include/nanotitan_moe.h``,
+  ``include/nanotitan_int8.h``): every HIP kernel, compiled by ``hipcc --offload-arch=gfx950``. No torch dependency.
 * ``_nanotitan_hip.so`` — the PyTorch-ROCm extension module exposing the
   reference op surface (``csrc/torch_ext.cpp``: the pybind module and the
   ``torch.ops.nanotitan`` op library, whose CPU kernels are
@@ -35,6 +35,8 @@ EXT = PKG / "_nanotitan_hip.so"
 HIP_SOURCES = ["library.hip", "router.hip", "router_linear.hip", "dispatch.hip",
                "combine.hip", "grouped_gemm.hip", "staged_gemm.hip", "block_norm.hip",
                "block_norm_backward.hip", "checkpoint8.hip", "few_tokens.hip"]
+# The 8-bit integer experts and linear layers (include/nanotitan_int8.h), of the same library.
+INT8_SOURCES = ["int8_rows.hip", "int8_gemm.hip", "int8_few.hip"]
 OFFLOAD_ARCH = "gfx950"
 ROCM = Path(os.environ.get("ROCM_PATH", "/opt/rocm"))
 
@@ -79,7 +81,7 @@ def build_library(verbose: bool = False) -> Path:
     hipcc = _hipcc()
     objs = []
     cmds = []
-    for src in HIP_SOURCES:
+    for src in HIP_SOURCES + INT8_SOURCES:
         obj = BUILD_DIR / (Path(src).stem + ".o")
         objs.append(obj)
         cmds.append([hipcc, *HIP_FLAGS, f"-I{INCLUDE}", f"-I{BUILD_DIR}", "-c", str(CSRC / src), "-o", str(obj)])
@@ -107,6 +109,7 @@ def build_extension(verbose: bool = False) -> Path:
         # the add, as the HIP kernels do.
         "-ffp-contract=off",
         str(CSRC / "torch_ext.cpp"),
+        str(CSRC / "torch_int8.cpp"),
         str(CSRC / "cpu_ops.cpp"),
         "-o",
         str(EXT.with_suffix(".so.tmp")),

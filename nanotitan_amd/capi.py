@@ -1,9 +1,10 @@
-"""ctypes binding of the C ABI in ``include/nanotitan_moe.h``.
+"""ctypes binding of the C ABI in ``include/nanotitan_moe.h`` and ``nanotitan_int8.h``.
 
 This is the binding a non-torch host (or a test that wants to exercise the
 boundary itself) uses: raw device pointers, sizes and a ``hipStream_t``.
-``EXPORTS`` lists every symbol the header declares, with its ctypes
-signature; ``load()`` checks that the library exports all of them.
+``EXPORTS`` (and ``INT8_EXPORTS`` for the second header) lists every symbol the
+header declares, with its ctypes signature; ``load()`` checks that the library
+exports all of them.
 """
 
 from __future__ import annotations
@@ -206,6 +207,38 @@ EXPORTS: dict[str, tuple[object, list[object]]] = {
     ),
 }
 
+# include/nanotitan_int8.h
+NT_INT8_MAX_K = 1 << 17
+INT8_EXPORTS: dict[str, tuple[object, list[object]]] = {
+    "nt_int8_pitch": (c_int64, [c_int64]),
+    "nt_int8_weight_bytes": (c_size_t, [c_int32, c_int64, c_int64]),
+    "nt_int8_rows": (c_int, [c_int, _P, c_int64, c_int64, _P, _P, _P]),
+    "nt_int8_rows_decode": (c_int, [c_int, _P, _P, c_int64, c_int64, _P, _P]),
+    "nt_int8_weight_workspace_bytes": (c_size_t, [c_int32, c_int64]),
+    "nt_int8_weight": (
+        c_int, [c_int, _P, c_int32, c_int64, c_int64, _P, _P, _P, c_size_t, _P]),
+    "nt_int8_weight_decode": (c_int, [c_int, _P, _P, c_int32, c_int64, c_int64, _P, _P]),
+    "nt_int8_grouped_gemm": (
+        c_int,
+        [c_int, _P, _P, _P, _P, _P, c_int32, c_int64, c_int64, c_int64, _P, _P],
+    ),
+    "nt_int8_grouped_gemm_swiglu": (
+        c_int,
+        [c_int, _P, _P, _P, _P, _P, _P, _P, c_int32, c_int64, c_int64, c_int64, _P, _P, _P, _P],
+    ),
+    "nt_int8_grouped_gemm_gelu": (
+        c_int,
+        [c_int, _P, _P, _P, _P, _P, c_int32, c_int64, c_int64, c_int64, _P, _P, _P],
+    ),
+    "nt_int8_moe_few_tokens_workspace_bytes": (
+        c_size_t, [c_int, c_int64, c_int32, c_int32, c_int64, c_int64]),
+    "nt_int8_moe_few_tokens": (
+        c_int,
+        [c_int, _P, _P, _P, _P, _P, _P, _P, _P, _P, c_int64, c_int32, c_int32, c_int64, c_int64,
+         _P, _P, _P, _P, c_size_t, _P],
+    ),
+}
+
 
 class NativeError(RuntimeError):
     """A C-ABI call returned a status other than NT_OK."""
@@ -221,10 +254,11 @@ def load() -> ctypes.CDLL:
     if not LIB_PATH.exists():
         raise RuntimeError(f"{LIB_PATH} is not built; run `python -m nanotitan_amd.build`")
     lib = ctypes.CDLL(str(LIB_PATH))
-    missing = [name for name in EXPORTS if not hasattr(lib, name)]
+    exports = EXPORTS | INT8_EXPORTS
+    missing = [name for name in exports if not hasattr(lib, name)]
     if missing:
         raise RuntimeError(f"{LIB_PATH.name} lacks exports: {missing}")
-    for name, (res, args) in EXPORTS.items():
+    for name, (res, args) in exports.items():
         fn = getattr(lib, name)
         fn.restype = res
         fn.argtypes = args

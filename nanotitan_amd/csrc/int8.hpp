@@ -1,0 +1,106 @@
+// Values in 8-bit integers: the scale, the rounding and the layouts that the
+// int8 kernels share.
+//
+// A row of activations (or an output channel of weights) v is held as s q with
+//   s = max(max|v| / 127, 2^-126) in float32,  q = the integer nearest to v / s,
+// ties to even, so |q| <= 127. The division is exact in its decision (int8_code),
+// not a product with a rounded reciprocal: half-way values are common in 16-bit
+// rows (half the row's largest value is one), and which way they go would
+// otherwise depend on the code that computes them. A row that holds an infinity or
+// a NaN has a NaN scale and integers 0: all that is computed from it is NaN.
+#pragma once
+
+#include "common.hpp"
+#include "nanotitan_int8.h"
+
+namespace nt {
+
+constexpr int kInt8Block = 64;   // columns and reduction rows of a weight block
+constexpr int kInt8Pitch = 128;  // rows of integers are padded with zeros to this
+// 127 * 127 * kInt8MaxK < 2^31: an int32 sum cannot overflow
+constexpr int64_t kInt8MaxK = 1 << 17;
+
+// Weights [E, K, N] lie in blocks of 64 columns by 64 reduction rows, 4 KiB each,
+// the blocks of a group of 64 columns one behind the other along K:
+//   codes[e][n / 64][k / 64][t][g][i][k % 16],  g = k % 64 / 16,
+//   n % 64 = 16 (i / 4) + 4 t + i % 4,
+// padded with zeros to whole groups and to 128 reduction rows. [g][i][16] is, lane
+// by lane, the operand of a 16x16x64 matrix instruction: a wave's 16-byte loads
+// read 1 KiB on end, from memory or LDS (where that is free of bank conflicts).
+// Which 16 of the 64 columns make operand t is chosen for the result: lane 16 g +
+// r of the instruction holds 4 values of row r, and over the four t they are 16
+// neighbouring columns.
+__host__ __device__ constexpr int64_t int8_pitch(int64_t k) { return round_up(k, kInt8Pitch); }
+__host__ __device__ constexpr int64_t int8_groups(int64_t n) { return ceil_div(n, kInt8Block); }
+__host__ __device__ constexpr int64_t int8_matrix(int64_t K, int64_t N) {
+  return int8_groups(N) * kInt8Block * int8_pitch(K);
+}
+
+// The scale of values whose largest magnitude has these bits.
+__device__ __forceinline__ float int8_scale(uint32_t most) {
+  if (most >= 0x7f800000u) return __uint_as_float(0x7fc00000u);
+  const float s = __fdiv_rn(__uint_as_float(most), 127.f);
+  return s < 0x1p-126f ? 0x1p-126f : s;
+}
+// 1 / s for int8_code; 0 for a NaN scale, which makes every integer 0.
+__device__ __forceinline__ float int8_inverse(float s) { return s == s ? 1.f / s : 0.f; }
+
+// The integer nearest to x / s, ties to even, for |x| <= 127.5 s. x * inv is off
+// by less than 2^-15, so the first guess is the nearest integer or, next to a
+// border, its neighbour. x - r s is exact where it decides: r s has at most 31
+// bits, and the difference is below 1.01 s and a multiple of both operands'
+// last bits.
+__device__ __forceinline__ int int8_code(float x, float s, float inv) {
+  const float r = rintf(x * inv);
+  const float off = fmaf(-r, s, x), half = 0.5f * s;
+  int q = (int)r;
+  if (fabsf(off) >= half) {
+    const bool odd = q & 1;
+    if (off > half || (off == half && odd)) q += 1;
+    else if (off < -half || (off == -half && odd)) q -= 1;
+  }
+  return inv == 0.f ? 0 : q;
+}
+
+__device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
+__device__ __forceinline__ uint32_t pack_bytes(int a, int b, int c, int d) {
+  return (uint32_t)(a & 255) | (uint32_t)(b & 255) << 8 | (uint32_t)(c & 255) << 16 |
+         (uint32_t)d << 24;
+}
+
+// q s in T: rounded once; a value that rounds past the type's largest is that.
+template <typename T>
+struct int8_most;
+template <>
+struct int8_most<float> {
+  static constexpr float value = 0x1.fffffep127f;
+};
+template <>
+struct int8_most<bf16> {
+  static constexpr float value = 0x1.fep127f;
+};
+template <>
+struct int8_most<f16> {
+  static constexpr float value = 65504.f;
+};
+template <typename T>
+__device__ __forceinline__ typename elem<T>::storage int8_value(int q, float s) {
+  const float v = (float)q * s, most = int8_most<T>::value;
+  return elem<T>::store(v > most ? most : v < -most ? -most : v);  // (a NaN stays one)
+}
+
+inline bool int8_float(int dtype) { return dtype == NT_F32 || dtype == NT_F16 || dtype == NT_BF16; }
+
+// f(type tag) for an activation type.
+template <typename T>
+struct tag {
+  typedef T type;
+};
+template <typename F>
+inline void int8_by_type(int dtype, F&& f) {
+  if (dtype == NT_F32) f(tag<float>());
+  else if (dtype == NT_F16) f(tag<f16>());
+  else f(tag<bf16>());
+}
+
+}  // namespace nt

@@ -1,0 +1,132 @@
+// What the int8 products share: their arguments, the experts' rows and the
+// epilogues. Tiles of many rows: int8_gemm.hip; few rows: int8_few.hip.
+#pragma once
+
+#include "bits.hpp"
+#include "gelu.hpp"
+#include "int8.hpp"
+
+namespace nt {
+
+enum Int8Epilogue { kInt8Plain = 0, kInt8SwiGLU = 1, kInt8Gelu = 2 };
+
+struct Int8Gemm {
+  const int8_t* x;          // [A, pitch]
+  const float* x_scales;    // [A]
+  const int32_t* offsets;   // [E + 1], or null: all rows are one expert's
+  const int8_t *w, *w2;     // blocks of [E, K, N]; w2: the value weights
+  const float *w_scales, *w2_scales;  // [E, N]
+  int32_t E;
+  int64_t A, K, N;
+  void* out;         // [A, N]; hidden, act
+  void *out2, *out3;  // gate, value; gelu' (null: not written)
+  int32_t ntn;
+  bool wide_stores;  // outputs are 16-byte aligned
+};
+
+// int8_few.hip: the product of few rows for each expert.
+void launch_int8_stream(const Int8Gemm& a, int epi, int dtype, hipStream_t s);
+
+namespace {
+
+// Rows of expert e, clamped to [0, A] and non-decreasing whatever offsets holds.
+__device__ __forceinline__ void int8_expert_rows(const Int8Gemm& a, int e, int64_t& r0,
+                                                 int64_t& r1) {
+  r0 = 0;
+  r1 = a.A;
+  if (a.offsets != nullptr) {
+    const int64_t lo = a.offsets[e], hi = a.offsets[e + 1];
+    r0 = lo < 0 ? 0 : lo > a.A ? a.A : lo;
+    r1 = hi < r0 ? r0 : hi > a.A ? a.A : hi;
+  }
+}
+
+// s_pref[e] = tiles of `rows` rows of the experts before e; ends with a barrier.
+__device__ __forceinline__ void int8_row_tiles(const Int8Gemm& a, int rows, int32_t* s_pref) {
+  if (threadIdx.x < kWave) {
+    int carry = 0;
+    for (int s = 0; s < a.E; s += kWave) {
+      const int e = s + lane_id();
+      int v = 0;
+      if (e < a.E) {
+        int64_t r0, r1;
+        int8_expert_rows(a, e, r0, r1);
+        v = (int)ceil_div(r1 - r0, rows);
+      }
+      const int incl = wave_incl_scan(v);
+      if (e < a.E) s_pref[e + 1] = carry + incl;
+      carry += __shfl(incl, kWave - 1, kWave);
+    }
+    if (lane_id() == 0) s_pref[0] = 0;
+  }
+  __syncthreads();
+}
+
+// e^-x and 1 / (1 + e^-x): for 16-bit results by the hardware's exponential and
+// reciprocal (1 ulp each), for float32 ones by the library's.
+template <typename T>
+__device__ __forceinline__ float sigmoid_of(float x) {
+  return __builtin_amdgcn_rcpf(1.f + __expf(-x));
+}
+template <>
+__device__ __forceinline__ float sigmoid_of<float>(float x) {
+  return 1.f / (1.f + expf(-x));
+}
+
+// Phi(x) and exp(-x^2 / 2), relatively exact in both tails: 16-bit results by the
+// fit of erfc, float32 ones by the library's erfc (1 + erf would cancel below 0).
+template <typename T>
+__device__ __forceinline__ float normal_cdf(float x, float& bell) {
+  return norm_cdf(x, bell);
+}
+template <>
+__device__ __forceinline__ float normal_cdf<float>(float x, float& bell) {
+  bell = expf(-0.5f * x * x);
+  return 0.5f * erfcf(x * -0.70710678118654752f);
+}
+
+// The outputs of one column from its scaled sums p (and p2, the value).
+template <typename T, int EPI>
+__device__ __forceinline__ void int8_epilogue(float p, float p2, typename elem<T>::storage& o,
+                                              typename elem<T>::storage& o2,
+                                              typename elem<T>::storage& o3) {
+  if constexpr (EPI == kInt8Plain) {
+    o = to_bits<T>(p);
+  } else if constexpr (EPI == kInt8SwiGLU) {
+    o = to_bits<T>(p * sigmoid_of<T>(p) * p2);
+    o2 = to_bits<T>(p);
+    o3 = to_bits<T>(p2);
+  } else {
+    float bell;
+    const float c = normal_cdf<T>(p, bell);
+    o = to_bits<T>(p * c);
+    o2 = to_bits<T>(fmaf(p, bell * 0.39894228040143268f, c));
+  }
+}
+
+// n (at most 16) neighbouring columns of every output, at element `at`.
+template <typename T, int EPI>
+__device__ __forceinline__ void int8_put(const Int8Gemm& a, int64_t at, int n, bool whole,
+                                         const typename elem<T>::storage (&o)[3][16]) {
+  typedef typename elem<T>::storage S;
+  constexpr int kOuts = EPI == kInt8Plain ? 1 : EPI == kInt8SwiGLU ? 3 : 2;
+#pragma unroll
+  for (int i = 0; i < kOuts; ++i) {
+    S* p = static_cast<S*>(i == 0 ? a.out : i == 1 ? a.out2 : a.out3);
+    if (i > 0 && p == nullptr) continue;
+    p += at;
+    if (whole) {
+      uint4 v[sizeof(S)];
+      __builtin_memcpy(v, o[i], sizeof(v));
+#pragma unroll
+      for (int j = 0; j < (int)sizeof(S); ++j) reinterpret_cast<uint4*>(p)[j] = v[j];
+    } else {
+#pragma unroll
+      for (int j = 0; j < 16; ++j)
+        if (j < n) p[j] = o[i][j];
+    }
+  }
+}
+
+}  // namespace
+}  // namespace nt

@@ -13,8 +13,10 @@
   weights (src/model/feed_fwd.py:39-122), three grouped GEMMs.
 * ``GeluExpertFFN(cfg, spec)`` — the 2-GEMM up -> GELU -> down FFN the
   benchmark configs specify, with the activation fused into the GEMMs.
+* ``Int8ExpertFFN(experts)`` — either of them on frozen 8-bit integer weights.
 * ``MoE(cfg, spec)`` — router + experts + backend (src/model/feed_fwd.py:128-152);
-  ``MoE.decode`` runs the layer on the few tokens of a decode step.
+  ``MoE.decode`` runs the layer on the few tokens of a decode step, and
+  ``MoE.quantize_experts`` puts its experts on 8-bit weights.
 * ``MoEBlock(cfg, spec)`` — the MoE half of a transformer layer: norm, MoE, norm,
   gate, residual scale and sum (src/model/model.py:205-211).
 * ``route(logits, top_k)`` — fp32 softmax, top-k with ties to the lower
@@ -39,6 +41,10 @@ from nanotitan_amd.moe_ops import (
     combine_inv_fn,
     grouped_gelu_ffn8_fn,
     grouped_gelu_ffn_fn,
+    int8_gelu_ffn_fn,
+    int8_swiglu_ffn_fn,
+    int8_weight,
+    Int8Weight,
     moe_few_tokens,
     post_norm_fn,
     pre_norm_fn,
@@ -169,6 +175,44 @@ class GeluExpertFFN(nn.Module):
         return ffn(packed_X, self.W_up, self.W_down, expert_offset)
 
 
+class Int8ExpertFFN(nn.Module):
+    """An ``ExpertFFN``'s or ``GeluExpertFFN``'s weights, frozen, in 8-bit integers.
+
+    Tokens and hidden values go to 8 bits row by row; the tokens get their gradient, the weights
+    none. The weights are buffers: two a projection, ``<name>_codes`` and ``<name>_scale``, the
+    float32 scales as the int32 of their bits, which a cast of the module to another float type
+    leaves alone. ``cfg.ffn_checkpoint8`` does not apply: what the backward keeps is gate and
+    value, or gelu', in the tokens' type.
+    """
+
+    def __init__(self, experts):
+        super().__init__()
+        if type(experts) is ExpertFFN:
+            self.names = ("W_gate", "W_val", "W_out")
+        elif type(experts) is GeluExpertFFN:
+            self.names = ("W_up", "W_down")
+        else:
+            raise RuntimeError(f"8-bit weights of this package's experts, not "
+                               f"{type(experts).__name__}")
+        self.cfg, self.spec = experts.cfg, experts.spec
+        self.shapes = {}
+        for name in self.names:
+            w = int8_weight(getattr(experts, name))
+            self.shapes[name] = w.shape
+            self.register_buffer(f"{name}_codes", w.codes)
+            self.register_buffer(f"{name}_scale", w.scale.view(torch.int32))
+
+    def weights(self):
+        """The projections' Int8Weights, as ``moe_few_tokens`` and the ``int8_*_ffn_fn`` take them."""
+        return tuple(Int8Weight(getattr(self, f"{name}_codes"),
+                                getattr(self, f"{name}_scale").view(torch.float32),
+                                self.shapes[name]) for name in self.names)
+
+    def forward(self, packed_X, expert_offset):
+        ffn = int8_swiglu_ffn_fn if len(self.names) == 3 else int8_gelu_ffn_fn
+        return ffn(packed_X, *self.weights(), expert_offset)
+
+
 def moe_forward_from_logits(x_flat, logits, experts, num_experts, top_k):
     """Hot path from router logits: route, dispatch, experts, combine (output in x's dtype).
 
@@ -274,6 +318,16 @@ class MoE(nn.Module):
         return self.moe_backend.forward(x)
 
     @torch.no_grad()
+    def quantize_experts(self):
+        """Puts the experts' weights into 8-bit integers, in place (``Int8ExpertFFN``): the module
+        then has no expert parameters, and an optimizer made before still holds the old ones.
+        Hooks on the experts do not carry over. Returns self."""
+        if type(self.experts) is not Int8ExpertFFN:
+            self.experts = Int8ExpertFFN(self.experts)
+            self.moe_backend.experts = self.experts
+        return self
+
+    @torch.no_grad()
     def decode(self, x):
         """The layer's output for the few tokens (at most 64 in all) of a decode step.
 
@@ -287,6 +341,8 @@ class MoE(nn.Module):
             weights = (e.W_gate, e.W_val, e.W_out)
         elif type(e) is GeluExpertFFN:
             weights = (e.W_up, e.W_down)
+        elif type(e) is Int8ExpertFFN:
+            weights = e.weights()
         else:
             raise RuntimeError(f"decode runs this package's experts, not {type(e).__name__}")
         flat = x.reshape(-1, x.shape[-1]).contiguous()

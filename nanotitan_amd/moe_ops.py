@@ -29,12 +29,15 @@ Beside that path: ``moe_few_tokens`` (the whole layer for a decode step),
 ``checkpoint8`` / ``gelu8_fn`` / ``swiglu8_fn`` with the experts' FFNs on them
 (activations kept in 8 bits). The norms' and 8-bit activations' Functions are
 in the extension.
+
+``int8_weight`` and the ``int8_*_fn`` run experts and linear layers on 8-bit
+integer weights, with the tokens brought to 8 bits row by row.
 """
 
 from __future__ import annotations
 
 import functools
-from typing import Any
+from typing import Any, NamedTuple
 
 import torch
 
@@ -572,13 +575,23 @@ def moe_few_tokens(x, weights, top_k, router_weight=None, logits=None):
     ones; either the router's weight [E,d] or its logits [T,E], float32. Returns (out [T,d],
     gates [T,k] float32, ids [T,k] int32): the values of route_fn, dispatch, the experts'
     grouped GEMMs and combine (reference src/model/cuda_backend.py:17-81), with only the
-    hidden values rounded to x's dtype on the way. Inference only: it raises where a gradient
-    or a forward-mode tangent would be lost.
+    hidden values rounded to x's dtype on the way. With ``Int8Weight``s tokens and hidden values
+    go to 8 bits row by row. Inference only: it raises where a gradient or a forward-mode tangent
+    would be lost.
     """
     if len(weights) not in (2, 3):
         raise RuntimeError("weights are (W_gate, W_val, W_out) or (W_up, W_down)")
-    if _tracked(x, *weights, router_weight, logits):
+    int8 = [isinstance(w, Int8Weight) for w in weights]
+    if any(int8) and not all(int8):
+        raise RuntimeError("the weights are all in 8 bits or none is")
+    if _tracked(x, *(() if int8[0] else weights), router_weight, logits):
         raise RuntimeError("moe_few_tokens has no backward: call it under torch.no_grad()")
+    if int8[0]:
+        up, val, down = weights[0], weights[1] if len(weights) == 3 else None, weights[-1]
+        _check_chain(x, up, val, down)
+        return get_hip_extension().int8_moe_few_tokens(
+            x, up.codes, up.scale, *((None, None) if val is None else (val.codes, val.scale)),
+            down.codes, down.scale, top_k, router_weight, logits)
     return get_hip_extension().moe_few_tokens(
         x, weights[0], weights[1] if len(weights) == 3 else None, weights[-1], top_k,
         router_weight, logits)
@@ -752,3 +765,196 @@ def swiglu_ffn8_fn(X, W_gate, W_val, W_out, expert_offset):
     if not _tracked(X, W_gate, W_val, W_out):
         return swiglu_ffn_fn(X, W_gate, W_val, W_out, expert_offset)
     return SwiGLUFFN8_FN.apply(X, expert_offset, W_gate, W_val, W_out)
+
+
+# ---------------------------------------------------------- 8-bit integers
+
+
+class Int8Weight(NamedTuple):
+    """Weights [E,K,N] in 8-bit integers with a float32 scale for each expert and column.
+
+    codes int8 [E, N/64, K/64, 4, 4, 16, 16] (N padded with zeros to 64, K to 128): element
+    [e, n//64, k//64, t, g, i, k%16] with g = k%64 // 16 and n%64 = 16 (i//4) + 4 t + i%4;
+    scale [E,N]; shape (E, K, N). ``int8_weight`` makes one.
+    """
+
+    codes: torch.Tensor
+    scale: torch.Tensor
+    shape: tuple[int, int, int]
+
+
+def int8_weight(W):
+    """W [E,K,N] (or [K,N], as one expert) as an Int8Weight: every channel's largest magnitude is 127.
+
+    Each value goes to the nearest multiple of its channel's scale, ties to even. A channel with
+    an infinity or a NaN has a NaN scale.
+    """
+    if W.dim() == 2:
+        W = W.unsqueeze(0)
+    codes, scale = get_hip_extension().int8_weight(W.detach().contiguous())
+    return Int8Weight(codes, scale, tuple(W.shape))
+
+
+def int8_weight_decode(weight, dtype):
+    """The weights [E,K,N] that an Int8Weight holds, in ``dtype``."""
+    _check_int8(weight)
+    return get_hip_extension().int8_weight_decode(weight.codes, weight.scale, weight.shape[1],
+                                                  dtype)
+
+
+def int8_rows(x):
+    """(codes int8 [rows, f padded with zeros to 128], scales float32 [rows]) of x [rows,f].
+
+    codes * scales are x's values, each the nearest multiple of its row's largest magnitude
+    / 127 (ties to even). A row with an infinity or a NaN has a NaN scale.
+    """
+    return get_hip_extension().int8_rows(x.detach().contiguous())
+
+
+def int8_rows_decode(codes, scales, width, dtype):
+    """The rows [rows, width] that codes and scales hold, in ``dtype``."""
+    return get_hip_extension().int8_rows_decode(codes, scales, width, dtype)
+
+
+def _check_int8(*weights):
+    for w in weights:
+        if not isinstance(w, Int8Weight):
+            raise RuntimeError(f"expected an Int8Weight, got {type(w).__name__}")
+        if len(w.shape) != 3 or (w.shape[0], w.shape[2]) != tuple(w.scale.shape):
+            raise RuntimeError(f"an Int8Weight of shape {tuple(w.shape)} with scales "
+                               f"{tuple(w.scale.shape)}")
+
+
+def _check_chain(x, up, val, down):
+    """Whether x, the up (and value) and the down weights of a feed-forward block fit."""
+    _check_int8(up, *(() if val is None else (val,)), down)
+    E, d, f = up.shape
+    if x.dim() != 2 or x.shape[1] != d or tuple(down.shape) != (E, f, d) or (
+            val is not None and tuple(val.shape) != (E, d, f)):
+        raise RuntimeError(f"x {tuple(x.shape)} and weights {tuple(up.shape)}, "
+                           f"{None if val is None else tuple(val.shape)}, {tuple(down.shape)} "
+                           "do not fit")
+
+
+def _all_rows(x, expert_offset):
+    """The offsets of a backward: those given, or one expert's of all rows."""
+    if expert_offset is not None:
+        return expert_offset
+    return torch.arange(2, dtype=torch.int32, device=x.device) * x.shape[0]
+
+
+class Int8GroupedGEMM_FN(torch.autograd.Function):
+    """X by frozen 8-bit weights; the gradient to X is dOut times the weights held, transposed.
+
+    The rounding of X is passed straight through. Weights go to dOut's dtype for the backward's
+    product (a rounding of 16-bit types, as small as the output's own).
+    """
+
+    @staticmethod
+    def forward(ctx, X, expert_offset, weight):
+        ctx.save_for_backward(expert_offset, weight.codes, weight.scale)
+        ctx.shape = weight.shape
+        return get_hip_extension().int8_product(X, expert_offset, weight.codes, weight.scale)
+
+    @staticmethod
+    @_once_differentiable
+    def backward(ctx, dout):
+        ext = get_hip_extension()
+        off, codes, scale = ctx.saved_tensors
+        W = ext.int8_weight_decode(codes, scale, ctx.shape[1], dout.dtype)
+        return ext.bwd_grouped_gemm_dX_kernel(W, _all_rows(dout, off), dout.contiguous()), None, None
+
+
+class Int8SwiGLUFFN_FN(torch.autograd.Function):
+    """SwiGLU FFN on frozen 8-bit weights, with the gradient to X.
+
+    Keeps gate and value in X's dtype; the rounding of X and of the hidden values is passed
+    straight through, and the weights held go to dy's dtype for the backward's products.
+    """
+
+    @staticmethod
+    def forward(ctx, X, expert_offset, W_gate, W_val, W_out):
+        weights = (W_gate, W_val, W_out)
+        held = [t for w in weights for t in (w.codes, w.scale)]
+        y, gate, value = get_hip_extension().int8_swiglu_ffn(X, expert_offset, *held, True)
+        ctx.save_for_backward(expert_offset, gate, value, *held)
+        ctx.shape = W_gate.shape
+        return y
+
+    @staticmethod
+    @_once_differentiable
+    def backward(ctx, dy):
+        ext = get_hip_extension()
+        off, gate, value, gc, gs, vc, vs, oc, os = ctx.saved_tensors
+        _, d, f = ctx.shape
+        off = _all_rows(dy, off)
+        dg, dv = ext.bwd_grouped_gemm_dX_swiglu(ext.int8_weight_decode(oc, os, f, dy.dtype), off,
+                                                dy.contiguous(), gate, value)
+        dX = ext.bwd_grouped_gemm_dX2(ext.int8_weight_decode(gc, gs, d, dy.dtype),
+                                      ext.int8_weight_decode(vc, vs, d, dy.dtype), off, dg, dv)
+        return dX, None, None, None, None
+
+
+class Int8GeluFFN_FN(torch.autograd.Function):
+    """GELU FFN on frozen 8-bit weights, with the gradient to X; keeps gelu' of the up projection."""
+
+    @staticmethod
+    def forward(ctx, X, expert_offset, W_up, W_down):
+        held = [t for w in (W_up, W_down) for t in (w.codes, w.scale)]
+        y, slope = get_hip_extension().int8_gelu_ffn(X, expert_offset, *held, True)
+        ctx.save_for_backward(expert_offset, slope, *held)
+        ctx.shape = W_up.shape
+        return y
+
+    @staticmethod
+    @_once_differentiable
+    def backward(ctx, dy):
+        ext = get_hip_extension()
+        off, slope, uc, us, dc, ds = ctx.saved_tensors
+        _, d, f = ctx.shape
+        off = _all_rows(dy, off)
+        dh = ext.bwd_grouped_gemm_dX_gelu(ext.int8_weight_decode(dc, ds, f, dy.dtype), off,
+                                          dy.contiguous(), slope)
+        dX = ext.bwd_grouped_gemm_dX_kernel(ext.int8_weight_decode(uc, us, d, dy.dtype), off, dh)
+        return dX, None, None, None
+
+
+def int8_grouped_gemm_fn(X, weight, expert_offset=None):
+    """X [A,K] by 8-bit weights [E,K,N], each row by its expert's: [A,N] in X's dtype.
+
+    The rows of X are brought to 8 bits, the products are exact integer sums, scaled in float32
+    and rounded once. Without ``expert_offset`` the weights are one linear layer's (E = 1).
+    Weights are frozen; X gets its gradient.
+    """
+    _check_int8(weight)
+    if X.dim() != 2 or X.shape[1] != weight.shape[1]:
+        raise RuntimeError(f"X {tuple(X.shape)} does not fit weights {tuple(weight.shape)}")
+    X = X.contiguous()
+    if _tracked(X):
+        return Int8GroupedGEMM_FN.apply(X, expert_offset, weight)
+    return get_hip_extension().int8_product(X, expert_offset, weight.codes, weight.scale)
+
+
+def int8_swiglu_ffn_fn(X, W_gate, W_val, W_out, expert_offset=None):
+    """silu(X W_gate) * (X W_val), then W_out, on 8-bit weights: [A,d] in X's dtype.
+
+    X and the hidden values (from their values in X's dtype) are brought to 8 bits row by row;
+    gate and value stay in float32 up to the hidden values. X gets its gradient.
+    """
+    X = X.contiguous()
+    _check_chain(X, W_gate, W_val, W_out)
+    if _tracked(X):
+        return Int8SwiGLUFFN_FN.apply(X, expert_offset, W_gate, W_val, W_out)
+    return get_hip_extension().int8_swiglu_ffn(
+        X, expert_offset, W_gate.codes, W_gate.scale, W_val.codes, W_val.scale, W_out.codes,
+        W_out.scale, False)[0]
+
+
+def int8_gelu_ffn_fn(X, W_up, W_down, expert_offset=None):
+    """gelu(X W_up) W_down (erf) on 8-bit weights, as int8_swiglu_ffn_fn."""
+    X = X.contiguous()
+    _check_chain(X, W_up, None, W_down)
+    if _tracked(X):
+        return Int8GeluFFN_FN.apply(X, expert_offset, W_up, W_down)
+    return get_hip_extension().int8_gelu_ffn(X, expert_offset, W_up.codes, W_up.scale,
+                                             W_down.codes, W_down.scale, False)[0]

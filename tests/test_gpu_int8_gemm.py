@@ -1,0 +1,417 @@
+"""Products with 8-bit integer weights, and the feed-forward blocks on them, against 64 bits."""
+
+import pytest
+import torch
+
+from nanotitan_amd import capi
+from nanotitan_amd.moe_ops import (
+    Int8Weight,
+    int8_gelu_ffn_fn,
+    int8_grouped_gemm_fn,
+    int8_rows,
+    int8_swiglu_ffn_fn,
+    int8_weight,
+    int8_weight_decode,
+)
+from tests import int8_oracle as O
+
+pytestmark = pytest.mark.gpu
+
+TYPES = {"bf16": torch.bfloat16, "fp16": torch.float16, "fp32": torch.float32}
+U = 2.0**-24
+
+
+def _rand(*shape, dtype=torch.float32, std=1.0, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    return (torch.randn(*shape, generator=g) * std).to(dtype).cuda()
+
+
+def _offsets(counts):
+    off = [0]
+    for c in counts:
+        off.append(off[-1] + c)
+    return off, torch.tensor(off, dtype=torch.int32, device="cuda")
+
+
+def _weights(E, K, N, seed):
+    """(Int8Weight, integers, scales [E,1,N]) of normal weights."""
+    W = _rand(E, K, N, std=K**-0.5, seed=seed)
+    q, s = O.held(W.cpu(), 1)
+    return Int8Weight(O.blocks(q).cuda(), s.view(E, N).cuda(), (E, K, N)), q, s
+
+
+def _steps(dtype):
+    """Half a step of dtype's rounding, relative."""
+    return torch.finfo(dtype).eps / 2
+
+
+# Rows an expert: one, a few, the limits of the row tiles of 16, 32 and 64, of 128 and of 256.
+COUNTS = {"one": [1], "few": [3, 0, 16, 1], "sixteen": [17, 9, 0, 22], "streams": [33, 64, 0, 1],
+          "mixed": [200, 0, 3, 50], "tiles": [128, 129, 0, 300], "wide": [256, 1, 700, 513],
+          "dense": None}
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("counts", COUNTS)
+@pytest.mark.parametrize("K,N", [(128, 64), (300, 65), (1024, 272), (77, 1365)])
+def test_product(dtype, counts, K, N):
+    t = TYPES[dtype]
+    if COUNTS[counts] is None:
+        off, gpu_off, E, A = [0, 19], None, 1, 19
+    else:
+        off, gpu_off = _offsets(COUNTS[counts])
+        E, A = len(off) - 1, off[-1]
+    x = _rand(A, K, dtype=t, seed=1)
+    w, qw, sw = _weights(E, K, N, 2)
+    got = int8_grouped_gemm_fn(x, w, gpu_off)
+    assert got.dtype == t and got.shape == (A, N)
+    qx, sx = O.held(x.cpu(), 1)
+    want = O.product(qx, sx, qw, sw, off)
+    # the sum to float32 and two products, each half a step, then the output's rounding
+    tol = (3.1 * U + _steps(t)) * want.abs() + torch.finfo(t).smallest_normal
+    err = (got.cpu().double() - want).abs() - tol
+    assert bool((err <= 0).all()), float(err.max())
+
+
+@pytest.mark.parametrize("rows", [5, 40, 100, 600])
+def test_rows_behind_the_last_stay(rows):
+    """Rows past offsets[E] are not written, by any of the kernels."""
+    E, K, N, A = 3, 200, 130, rows + 37
+    off, gpu_off = _offsets([rows // 2, 0, rows - rows // 2])
+    x = _rand(A, K, dtype=torch.bfloat16, seed=3)
+    codes, scales = int8_rows(x)
+    w, _, _ = _weights(E, K, N, 4)
+    outs = [torch.full((A, N), 7.0, dtype=torch.bfloat16, device="cuda") for _ in range(3)]
+    s = capi.current_stream()
+    args = [capi.NT_BF16, codes.data_ptr(), scales.data_ptr(), gpu_off.data_ptr(),
+            w.codes.data_ptr(), w.scale.data_ptr()]
+    sizes = [E, A, K, N]
+    capi.call("nt_int8_grouped_gemm", *args, *sizes, outs[0].data_ptr(), s)
+    capi.call("nt_int8_grouped_gemm_gelu", *args, *sizes, outs[1].data_ptr(), outs[2].data_ptr(), s)
+    for o in outs:
+        assert bool((o[rows:] == 7.0).all()) and not bool((o[:rows] == 7.0).all())
+    outs = [torch.full((A, N), 7.0, dtype=torch.bfloat16, device="cuda") for _ in range(3)]
+    capi.call("nt_int8_grouped_gemm_swiglu", *args, w.codes.data_ptr(), w.scale.data_ptr(), *sizes,
+              *[o.data_ptr() for o in outs], s)
+    for o in outs:
+        assert bool((o[rows:] == 7.0).all()) and not bool((o[:rows] == 7.0).all())
+
+
+def test_no_rows():
+    w, _, _ = _weights(2, 64, 96, 0)
+    off = torch.zeros(3, dtype=torch.int32, device="cuda")
+    assert int8_grouped_gemm_fn(torch.zeros(0, 64, device="cuda"), w, off).shape == (0, 96)
+    x = torch.zeros(0, 64, device="cuda", requires_grad=True)
+    out = int8_grouped_gemm_fn(x, w, off)
+    out.sum().backward()
+    assert x.grad.shape == (0, 64)
+
+
+def test_malformed_offsets_stay_inside():
+    """Offsets that fall, or lie outside [0, A], move no access out of the tensors."""
+    w, _, _ = _weights(4, 128, 64, 0)
+    for A in (30, 300, 2000):
+        x = _rand(A, 128, dtype=torch.bfloat16)
+        for off in ([-5, A + 9, 3, 2**31 - 1, 10], [A, 0, A, 0, A], [7, 7, 7, 7, 7]):
+            o = torch.tensor(off, dtype=torch.int32, device="cuda")
+            assert int8_grouped_gemm_fn(x, w, o).shape == (A, 64)
+    torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("A", [3, 20, 50, 150, 400])
+def test_infinite_and_nan_rows_stay_their_own(A):
+    """A row with an infinity or a NaN is NaN; the others are as without it. A NaN channel is a
+    NaN column."""
+    w, _, _ = _weights(1, 200, 100, 5)
+    x = _rand(A, 200, dtype=torch.bfloat16, seed=6)
+    want = int8_grouped_gemm_fn(x, w)
+    bad = x.clone()
+    bad[0, 3], bad[2, 199] = float("inf"), float("nan")
+    got = int8_grouped_gemm_fn(bad, w)
+    assert bool(got[0].isnan().all()) and bool(got[2].isnan().all())
+    keep = [i for i in range(A) if i not in (0, 2)]
+    assert torch.equal(got[keep], want[keep])
+    scale = w.scale.clone()
+    scale[0, 37] = float("nan")
+    got = int8_grouped_gemm_fn(x, w._replace(scale=scale))
+    assert bool(got[:, 37].isnan().all())
+    cols = [i for i in range(100) if i != 37]
+    assert torch.equal(got[:, cols], want[:, cols])
+
+
+def test_the_largest_sums():
+    """127 * 127 over the longest reduction is an int32 sum without overflow."""
+    K = capi.NT_INT8_MAX_K
+    W = torch.ones(1, K, 64, device="cuda")
+    w = int8_weight(W)
+    for A in (1, 70, 300):
+        x = torch.ones(A, K, dtype=torch.float32, device="cuda")
+        got = int8_grouped_gemm_fn(x, w)
+        one = (torch.tensor(1.0) / 127.0).double()
+        want = 127.0 * 127.0 * K * one * one
+        assert bool(((got.cpu().double() - want).abs() <= 3.1 * U * want).all())
+
+
+def test_a_row_is_the_same_in_any_batch():
+    w, _, _ = _weights(1, 500, 300, 7)
+    x = _rand(700, 500, dtype=torch.bfloat16, seed=8)
+    whole = int8_grouped_gemm_fn(x, w)
+    for n in (1, 17, 40, 100, 257):
+        assert torch.equal(int8_grouped_gemm_fn(x[:n], w), whole[:n])
+
+
+def test_past_32_bit_offsets():
+    """Outputs past 2^31 values and weights past 2^32 bytes."""
+    A, K, N = 2**18 + 3, 128, 8256
+    w, _, _ = _weights(1, K, N, 9)
+    x = _rand(A, K, dtype=torch.bfloat16, seed=10)
+    out = int8_grouped_gemm_fn(x, w)
+    assert torch.equal(out[-70:], int8_grouped_gemm_fn(x[-70:], w))
+    del out
+    E, K, N = 34, 16384, 8192
+    codes = torch.zeros(E, N // 64, K // 64, 4, 4, 16, 16, dtype=torch.int8, device="cuda")
+    codes[-1].random_(-127, 128)
+    scale = torch.rand(E, N, device="cuda")
+    for rows in (9, 100, 300):
+        off = torch.tensor([0] * E + [rows], dtype=torch.int32, device="cuda")
+        x = _rand(rows, K, dtype=torch.bfloat16, seed=11)
+        got = int8_grouped_gemm_fn(x, Int8Weight(codes, scale, (E, K, N)), off)
+        one = Int8Weight(codes[-1:].contiguous(), scale[-1:].contiguous(), (1, K, N))
+        assert torch.equal(got, int8_grouped_gemm_fn(x, one))
+
+
+# ------------------------------------------------------------- feed-forward
+
+
+def _act64(ffn, pre):
+    if ffn == "swiglu":
+        return torch.nn.functional.silu(pre[0]) * pre[1]
+    return torch.nn.functional.gelu(pre[0])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("ffn", ["swiglu", "gelu"])
+@pytest.mark.parametrize("counts", ["few", "sixteen", "streams", "mixed", "tiles", "wide"])
+def test_hidden_values(dtype, ffn, counts):
+    """Both projections, the activation and the product, elementwise."""
+    t = TYPES[dtype]
+    off, gpu_off = _offsets(COUNTS[counts])
+    E, A, K, N = len(off) - 1, off[-1], 300, 333
+    x = _rand(A, K, dtype=t, seed=1)
+    codes, scales = int8_rows(x)
+    qx, sx = O.held(x.cpu(), 1)
+    ws = [_weights(E, K, N, 2 + i) for i in range(2 if ffn == "swiglu" else 1)]
+    pre = [O.product(qx, sx, q, s, off) for _, q, s in ws]
+    outs = [torch.empty(A, N, dtype=t, device="cuda") for _ in range(3 if ffn == "swiglu" else 2)]
+    handles = [p for w, _, _ in ws for p in (w.codes.data_ptr(), w.scale.data_ptr())]
+    capi.call(f"nt_int8_grouped_gemm_{ffn}", capi.dtype_code(t), codes.data_ptr(),
+              scales.data_ptr(), gpu_off.data_ptr(), *handles, E, A, K, N,
+              *[o.data_ptr() for o in outs], capi.current_stream())
+    got = [o.cpu().double() for o in outs]
+    half, tiny = _steps(t), torch.finfo(t).smallest_normal
+    err = 3.1 * U  # of a pre-activation, relative
+    if ffn == "swiglu":
+        for g, p in zip(got[1:], pre):
+            assert bool(((g - p).abs() <= (err + half) * p.abs() + tiny).all())
+        # silu'(z) z is at most (1 + |z|) |silu(z)|; its exponential and reciprocal add a few
+        # steps of 2^-24 (e^-z from a float32 product: |z| 2^-23 more)
+        slack = err * (2 + pre[0].abs()) + (8 + 2 * pre[0].abs()) * U
+    else:
+        z = pre[0].requires_grad_()
+        cdf = 0.5 * (1 + torch.erf(z.detach() * 0.5**0.5))
+        slope = torch.autograd.grad(torch.nn.functional.gelu(z).sum(), z)[0]
+        z = z.detach()
+        pre = [z]
+        # |gelu''| <= 0.8, the fit of Phi is off by 1.2e-7 of a tail
+        tol = 0.8 * err * z.abs() + 2e-6 * (1 + z.abs()) + half * slope.abs() + tiny
+        assert bool(((got[1] - slope).abs() <= tol).all())
+        # gelu's relative slope z phi / Phi is below 2 + z^2
+        slack = err * (2 + z * z) + 4e-7 + (8 + 2 * z * z) * U + 0 * cdf
+    want = _act64(ffn, pre)
+    tol = (slack + half) * want.abs() + tiny
+    over = (got[0] - want).abs() - tol
+    assert bool((over <= 0).all()), float(over.max())
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("ffn", ["swiglu", "gelu"])
+@pytest.mark.parametrize("counts", ["few", "streams", "tiles", "wide", "dense"])
+def test_block_is_its_stages(dtype, ffn, counts):
+    """The feed-forward block has the bits of its stages, each checked above."""
+    t = TYPES[dtype]
+    off, gpu_off = ([0, 77], None) if counts == "dense" else _offsets(COUNTS[counts])
+    E, A, d, f = len(off) - 1, off[-1], 200, 341
+    x = _rand(A, d, dtype=t, seed=1)
+    up = [_weights(E, d, f, 2 + i)[0] for i in range(2 if ffn == "swiglu" else 1)]
+    down = _weights(E, f, d, 5)[0]
+    block = int8_swiglu_ffn_fn if ffn == "swiglu" else int8_gelu_ffn_fn
+    y = block(x, *up, down, gpu_off)
+    codes, scales = int8_rows(x)
+    hidden = torch.empty(A, f, dtype=t, device="cuda")
+    handles = [p for w in up for p in (w.codes.data_ptr(), w.scale.data_ptr())]
+    capi.call(f"nt_int8_grouped_gemm_{ffn}", capi.dtype_code(t), codes.data_ptr(),
+              scales.data_ptr(), None if gpu_off is None else gpu_off.data_ptr(), *handles, E, A,
+              d, f, hidden.data_ptr(), *([None] * (2 if ffn == "swiglu" else 1)),
+              capi.current_stream())
+    assert torch.equal(y, int8_grouped_gemm_fn(hidden, down, gpu_off))
+
+
+# ----------------------------------------------------------------- gradients
+
+
+def _held_weights(ws):
+    return [int8_weight_decode(w, torch.float32).cpu().double() for w in ws]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("counts", ["few", "mixed", "wide", "dense"])
+def test_product_gradient(dtype, counts):
+    t = TYPES[dtype]
+    off, gpu_off = ([0, 19], None) if counts == "dense" else _offsets(COUNTS[counts])
+    E, A, K, N = len(off) - 1, off[-1], 300, 264
+    x = _rand(A, K, dtype=t, seed=1).requires_grad_()
+    w, _, _ = _weights(E, K, N, 2)
+    dout = _rand(A, N, dtype=t, seed=3)
+    out = int8_grouped_gemm_fn(x, w, gpu_off)
+    assert torch.equal(out, int8_grouped_gemm_fn(x.detach(), w, gpu_off))
+    out.backward(dout)
+    held = _held_weights([w])[0]
+    want, size = torch.zeros(A, K).double(), torch.zeros(A, K).double()
+    d = dout.cpu().double()
+    for e in range(E):
+        a, b = off[e], off[e + 1]
+        want[a:b] = d[a:b] @ held[e].t()
+        size[a:b] = d[a:b].abs() @ held[e].abs().t()
+    # the weights' rounding and the output's, half a step each, and a float32 sum of N terms
+    tol = (_steps(t) + N * U) * size + _steps(t) * want.abs()
+    assert bool(((x.grad.cpu().double() - want).abs() <= tol).all())
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("ffn", ["swiglu", "gelu"])
+@pytest.mark.parametrize("counts", ["few", "mixed", "wide", "dense"])
+def test_block_gradient(dtype, ffn, counts):
+    """dX against the formula in 64 bits, and that against differences."""
+    t = TYPES[dtype]
+    off, gpu_off = ([0, 19], None) if counts == "dense" else _offsets(COUNTS[counts])
+    E, A, d, f = len(off) - 1, off[-1], 128, 264
+    x = _rand(A, d, dtype=t, seed=1).requires_grad_()
+    up = [_weights(E, d, f, 2 + i)[0] for i in range(2 if ffn == "swiglu" else 1)]
+    down = _weights(E, f, d, 5)[0]
+    dy = _rand(A, d, dtype=t, seed=6)
+    block = int8_swiglu_ffn_fn if ffn == "swiglu" else int8_gelu_ffn_fn
+    y = block(x, *up, down, gpu_off)
+    assert torch.equal(y, block(x.detach(), *up, down, gpu_off))
+    y.backward(dy)
+    hu, hd = [_held_weights([w])[0] for w in up], _held_weights([down])[0]
+    q, s = O.held(x.detach().cpu(), 1)
+    at = (q.double() * s.double()).requires_grad_()
+
+    def smooth(v):  # what the gradient is of: the block at the values held
+        return torch.cat([_act64(ffn, [v[a:b] @ h[e] for h in hu]) @ hd[e]
+                          for e, (a, b) in enumerate(zip(off, off[1:]))])
+
+    out = smooth(at)
+    want = torch.autograd.grad(out, at, dy.cpu().double())[0]
+    with torch.no_grad():
+        v = _rand(A, d, seed=7).cpu().double()
+        diff = ((smooth(at + 1e-6 * v) - smooth(at - 1e-6 * v)) * dy.cpu().double()).sum() / 2e-6
+        assert abs(float(diff) - float((want * v).sum())) <= 1e-6 * float(want.norm() * v.norm())
+    # roundings on the way, as a norm: two sets of weights, gate and value (or gelu'), the hidden
+    # gradient, the activation and its product with it, both branches and the output. Independent
+    # errors of at most half a step each (a third of that squared on average) add to below one and
+    # a half steps; float32's sums of up to 264 terms to below 64 of its own.
+    steps = 3 if t != torch.float32 else 64
+    assert float((x.grad.cpu().double() - want).norm()) <= steps * _steps(t) * float(want.norm())
+
+
+def test_gradients_are_once_differentiable_and_have_no_tangents():
+    w, _, _ = _weights(1, 64, 64, 0)
+    x = _rand(5, 64).requires_grad_()
+    for fn in (lambda v: int8_grouped_gemm_fn(v, w), lambda v: int8_gelu_ffn_fn(v, w, w),
+               lambda v: int8_swiglu_ffn_fn(v, w, w, w)):
+        g, = torch.autograd.grad(fn(x).sum(), x, create_graph=True)
+        with pytest.raises(RuntimeError, match="once differentiable"):
+            g.square().sum().backward()
+        with torch.autograd.forward_ad.dual_level(), torch.no_grad():
+            dual = torch.autograd.forward_ad.make_dual(x.detach(), torch.ones_like(x))
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                fn(dual)
+
+
+# ------------------------------------------------- streams, graphs, devices
+
+
+def test_on_another_stream_and_two_at_once():
+    E, d, f = 4, 256, 512
+    off, gpu_off = _offsets([100, 0, 37, 300])
+    x = [_rand(437, d, dtype=torch.bfloat16, seed=i) for i in (1, 2)]
+    up, val, down = (_weights(E, *s, i)[0] for i, s in enumerate([(d, f), (d, f), (f, d)]))
+    want = [int8_swiglu_ffn_fn(v, up, val, down, gpu_off) for v in x]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(5):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(int8_swiglu_ffn_fn(x[i], up, val, down, gpu_off))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(g, want[i]) for g in got[i])
+
+
+@pytest.mark.parametrize("rows", [5, 150, 600])
+def test_captured_and_replayed(rows):
+    E, d, f = 2, 256, 384
+    off, gpu_off = _offsets([rows, rows // 2])
+    A = off[-1]
+    up, val, down = (_weights(E, *s, i)[0] for i, s in enumerate([(d, f), (d, f), (f, d)]))
+    x = _rand(A, d, dtype=torch.bfloat16, seed=1)
+    dy = _rand(A, d, dtype=torch.bfloat16, seed=2)
+    leaf = x.clone().requires_grad_()
+
+    def step():
+        y = int8_swiglu_ffn_fn(leaf, up, val, down, gpu_off)
+        g, = torch.autograd.grad(y, leaf, dy)
+        return y.detach(), g
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for seed in (3, 4, 5):
+        with torch.no_grad():
+            leaf.copy_(_rand(A, d, dtype=torch.bfloat16, seed=seed))
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [o.clone() for o in out]
+        want = step()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+        del want
+
+
+def test_weights_that_would_need_a_gradient_are_refused():
+    w, _, _ = _weights(1, 64, 64, 0)
+    x = _rand(5, 64)
+    with pytest.raises(RuntimeError, match="no gradient"):
+        int8_grouped_gemm_fn(x, w._replace(scale=w.scale.clone().requires_grad_()))
+
+
+def test_refusals():
+    w, _, _ = _weights(2, 64, 96, 0)
+    x, off = _rand(5, 64), torch.tensor([0, 2, 5], dtype=torch.int32, device="cuda")
+    for bad in (lambda: int8_grouped_gemm_fn(x, w), lambda: int8_grouped_gemm_fn(x.double(), w, off),
+                lambda: int8_grouped_gemm_fn(x, w, off[:2]),
+                lambda: int8_grouped_gemm_fn(x, w, off.long()),
+                lambda: int8_grouped_gemm_fn(x, w, off.cpu()),
+                lambda: int8_grouped_gemm_fn(x.cpu(), w, off),
+                lambda: int8_grouped_gemm_fn(x, w._replace(scale=w.scale.double()), off),
+                lambda: int8_grouped_gemm_fn(x, w._replace(codes=w.codes.float()), off),
+                lambda: int8_grouped_gemm_fn(x, w._replace(codes=w.codes[:1]), off)):
+        with pytest.raises(RuntimeError):
+            bad()
