@@ -8,12 +8,14 @@
  *   s = max(max|v| / 127, 2^-126),  q = the integer nearest to v / s, ties to even.
  * A row or channel with an infinity or a NaN has a NaN scale and zero integers.
  * Products are exact int32 sums, scaled in float32 and rounded once. Sums run over
- * at most NT_INT8_MAX_K values. Integers given by a caller are -127..127.
+ * at most NT_INT8_MAX_K values, calls over at most NT_INT8_MAX_ROWS rows. Integers given by a caller are -127..127.
  *
- * Rows of integers have nt_int8_pitch(f) columns, zeros past f. Weights lie in the
- * blocks that the matrix instructions read, nt_int8_weight_bytes(E, K, N) in all:
- *   codes[e][n / 64][k / 64][t][g][i][k % 16],  g = k % 64 / 16,
- *   n % 64 = 16 (i / 4) + 4 t + i % 4,
+ * Integers lie as the operands of the matrix instructions. Rows [A, f], 16 rows of
+ * nt_int8_pitch(f) (a multiple of 128, zeros past f) after another,
+ * nt_int8_rows_bytes(A, f) in all:
+ *   codes[a / 16][k / 64][g][a % 16][k % 16],  g = k % 64 / 16.
+ * Weights, nt_int8_weight_bytes(E, K, N) in all:
+ *   codes[e][n / 64][k / 64][t][g][i][k % 16],  n % 64 = 16 (i / 4) + 4 t + i % 4,
  * n padded with zeros to a multiple of 64, k to one of 128; scales are [E, N].
  * Integers are 16-byte aligned. Activations are f32, f16 or bf16.
  * No counterpart in the reference, whose experts keep their training type
@@ -29,12 +31,14 @@ extern "C" {
 #endif
 
 #define NT_INT8_MAX_K (1 << 17)
+#define NT_INT8_MAX_ROWS ((1 << 24) - 1)
 
 int64_t nt_int8_pitch(int64_t f);
+size_t nt_int8_rows_bytes(int64_t rows, int64_t f);
 size_t nt_int8_weight_bytes(int32_t E, int64_t K, int64_t N);
 
-/* Rows x [rows, f] to codes [rows, nt_int8_pitch(f)] and scales [rows], and the
- * values q s that they hold in dtype (rounded once; past the type's largest: that). */
+/* Rows x [rows, f] to codes and scales [rows], and the values q s that they hold in
+ * dtype (rounded once; past the type's largest: that). */
 int nt_int8_rows(int dtype, const void* x, int64_t rows, int64_t f, int8_t* codes, float* scales,
                  hipStream_t stream);
 int nt_int8_rows_decode(int dtype, const int8_t* codes, const float* scales, int64_t rows,

@@ -211,6 +211,7 @@ EXPORTS: dict[str, tuple[object, list[object]]] = {
 NT_INT8_MAX_K = 1 << 17
 INT8_EXPORTS: dict[str, tuple[object, list[object]]] = {
     "nt_int8_pitch": (c_int64, [c_int64]),
+    "nt_int8_rows_bytes": (c_size_t, [c_int64, c_int64]),
     "nt_int8_weight_bytes": (c_size_t, [c_int32, c_int64, c_int64]),
     "nt_int8_rows": (c_int, [c_int, _P, c_int64, c_int64, _P, _P, _P]),
     "nt_int8_rows_decode": (c_int, [c_int, _P, _P, c_int64, c_int64, _P, _P]),

@@ -16,21 +16,31 @@
 namespace nt {
 
 constexpr int kInt8Block = 64;   // columns and reduction rows of a weight block
-constexpr int kInt8Pitch = 128;  // rows of integers are padded with zeros to this
+constexpr int kInt8Pitch = 128;  // reduction rows are padded with zeros to this: the widest k-step
 // 127 * 127 * kInt8MaxK < 2^31: an int32 sum cannot overflow
-constexpr int64_t kInt8MaxK = 1 << 17;
+constexpr int64_t kInt8MaxK = NT_INT8_MAX_K;
+constexpr int64_t kInt8MaxRows = NT_INT8_MAX_ROWS;  // 256 threads each are a launch's 2^32
 
-// Weights [E, K, N] lie in blocks of 64 columns by 64 reduction rows, 4 KiB each,
-// the blocks of a group of 64 columns one behind the other along K:
-//   codes[e][n / 64][k / 64][t][g][i][k % 16],  g = k % 64 / 16,
-//   n % 64 = 16 (i / 4) + 4 t + i % 4,
-// padded with zeros to whole groups and to 128 reduction rows. [g][i][16] is, lane
-// by lane, the operand of a 16x16x64 matrix instruction: a wave's 16-byte loads
-// read 1 KiB on end, from memory or LDS (where that is free of bank conflicts).
+// Integers lie in operands of a 16x16x64 matrix instruction, 1 KiB each: [g][i][16]
+// holds, lane 16 g + i by lane, values 16 g .. 16 g + 15 of a step's 64 of row (or
+// column) i. A wave's 16-byte loads then read 1 KiB on end, from memory or from LDS
+// (where that is free of bank conflicts), whichever 64 values of a row it takes.
+// Activations [A, K]: 16 rows after another,
+//   codes[a / 16][k / 64][g][a % 16][k % 16],  g = k % 64 / 16.
+// Weights [E, K, N]: the four operands of 64 columns together,
+//   codes[e][n / 64][k / 64][t][g][i][k % 16],  n % 64 = 16 (i / 4) + 4 t + i % 4.
 // Which 16 of the 64 columns make operand t is chosen for the result: lane 16 g +
 // r of the instruction holds 4 values of row r, and over the four t they are 16
-// neighbouring columns.
+// neighbouring columns. K is padded with zeros to a multiple of 128 (the longest
+// k-step), N to one of 64; activations' rows past the last, up to 16, hold anything.
 __host__ __device__ constexpr int64_t int8_pitch(int64_t k) { return round_up(k, kInt8Pitch); }
+// Bytes of A rows, and where row a begins (its 16-byte pieces are 256 bytes apart).
+__host__ __device__ constexpr int64_t int8_rows_bytes(int64_t A, int64_t pitch) {
+  return round_up(A, 16) * pitch;
+}
+__host__ __device__ constexpr int64_t int8_row(int64_t a, int64_t pitch) {
+  return (a >> 4) * 16 * pitch + (a & 15) * 16;
+}
 __host__ __device__ constexpr int64_t int8_groups(int64_t n) { return ceil_div(n, kInt8Block); }
 __host__ __device__ constexpr int64_t int8_matrix(int64_t K, int64_t N) {
   return int8_groups(N) * kInt8Block * int8_pitch(K);

@@ -92,7 +92,7 @@ struct Stage {
     for (int u = 0; u < U; ++u)
 #pragma unroll
       for (int m = 0; m < MT; ++m)
-        x[u][m] = *reinterpret_cast<const i32x4*>(xp[m] + (kb + u) * kInt8Block);
+        x[u][m] = *reinterpret_cast<const i32x4*>(xp[m] + (int64_t)(kb + u) * 1024);
   }
   __device__ __forceinline__ void multiply(i32x4 (&acc)[MATS][CT][MT]) const {
 #pragma unroll
@@ -110,12 +110,11 @@ struct Stage {
 
 // CT of the four operands of a column group, up to 16 MT rows of one expert, for
 // the KW waves of a workgroup at a time.
-template <typename T, int EPI, int MT, int CT, int KW, bool CHOSEN>
+template <typename T, int EPI, int MT, int CT, int KW, int U, bool CHOSEN>
 __global__ void __launch_bounds__(KW* kWave)
     int8_stream_kernel(Int8Gemm a, std::conditional_t<CHOSEN, Chosen, NoChoice> chosen) {
   typedef typename elem<T>::storage S;
   constexpr int MATS = EPI == kInt8SwiGLU ? 2 : 1, kRows = 16 * MT;
-  constexpr int U = MATS * CT >= 4 ? 2 : 4;
   __shared__ std::conditional_t<CHOSEN, ChosenPlan, StreamPlan> s_plan;
   __shared__ __attribute__((aligned(16))) int32_t s_acc[KW * MATS * CT * kWave * 4];
   if constexpr (CHOSEN) make_chosen(chosen, a.E, kRows, s_plan);
@@ -147,8 +146,8 @@ __global__ void __launch_bounds__(KW* kWave)
 #pragma unroll
       for (int m = 0; m < MT; ++m) {
         const int r = m * 16 + (lane & 15);
-        xp[m] = a.x + (int64_t)nth_token(mask, done + (r < rows ? r : 0)) * pitch +
-                (lane >> 4) * 16;
+        xp[m] = a.x + int8_row(nth_token(mask, done + (r < rows ? r : 0)), pitch) +
+                (lane >> 4) * 256;
       }
     } else {
       int64_t r0, r1;
@@ -158,7 +157,7 @@ __global__ void __launch_bounds__(KW* kWave)
 #pragma unroll
       for (int m = 0; m < MT; ++m) {
         const int r = m * 16 + (lane & 15);
-        xp[m] = a.x + (row0 + (r < rows ? r : 0)) * pitch + (lane >> 4) * 16;
+        xp[m] = a.x + int8_row(row0 + (r < rows ? r : 0), pitch) + (lane >> 4) * 256;
       }
     }
     const int8_t* wp[MATS];
@@ -250,24 +249,44 @@ __global__ void __launch_bounds__(KW* kWave)
 template <int V>
 using constant = std::integral_constant<int, V>;
 
+// Row tiles of a load of the weights, by the rows an expert has on average: more
+// take registers and the activations' loads; fewer read the weights of an expert
+// with more rows again (128 rows of 8 experts, 14,336 x 4,096: 77 us with two, 105
+// with one).
+int stream_row_tiles(int64_t rows, int64_t experts) {
+  const int64_t mean = ceil_div(rows, experts);
+  return mean <= 6 ? 1 : mean <= 20 ? 2 : 4;
+}
+
+// A workgroup takes a whole column group (four operands) for four waves where these
+// fill the chip twice; half of one (a row of 4,096 to 14,336: 12.2 us, with a
+// quarter 12.5) or, where there are few, a quarter for eight waves with two blocks
+// each in flight (14,336 to 4,096: 11.9 us; half of one for four waves 13.8). Eight
+// waves or more blocks in flight hold no more bytes in flight than the memory needs
+// and leave fewer workgroups to overlap (940 MB of 8 experts' two matrices: 138 us,
+// 6.8 TB/s; eight waves 153, two blocks 150, four quarters 153).
 template <typename T, int EPI, bool CHOSEN, typename C>
-void launch_stream(const Int8Gemm& a, int64_t mean, int64_t loads, const C& chosen,
-                   hipStream_t s) {
-  auto go = [&](auto mt, auto ct) {
-    constexpr int MT = decltype(mt)::value, CT = decltype(ct)::value, KW = 8;
-    const int64_t parts = int8_groups(a.N) * (4 / CT);
-    const int64_t grid = std::min<int64_t>(loads * parts, 4096);
-    hipLaunchKernelGGL((int8_stream_kernel<T, EPI, MT, CT, KW, CHOSEN>), dim3((unsigned)grid),
+void launch_stream(const Int8Gemm& a, int64_t experts, const C& chosen, hipStream_t s) {
+  const int mt = stream_row_tiles(a.A, a.E);
+  const int64_t groups = int8_groups(a.N);
+  // every load but an expert's last is full
+  const int64_t loads = std::min<int64_t>(a.A, experts + a.A / (16 * mt));
+  auto go = [&](auto mt, auto ct, auto kw, auto u) {
+    constexpr int MT = decltype(mt)::value, CT = decltype(ct)::value, KW = decltype(kw)::value;
+    hipLaunchKernelGGL((int8_stream_kernel<T, EPI, MT, CT, KW, decltype(u)::value, CHOSEN>),
+                       dim3((unsigned)std::min<int64_t>(loads * groups * (4 / CT), 1 << 20)),
                        dim3(KW * kWave), 0, s, a, chosen);
   };
   auto by_columns = [&](auto mt) {
-    const int64_t groups = std::min<int64_t>(a.E, loads) * int8_groups(a.N);
-    if (groups >= 256) go(mt, constant<4>());
-    else if (groups >= 128) go(mt, constant<2>());
-    else go(mt, constant<1>());
+    if (experts * groups >= (decltype(mt)::value == 4 ? 128 : 512))
+      go(mt, constant<4>(), constant<4>(), constant<1>());
+    else if (experts * groups >= 128)
+      go(mt, constant<2>(), constant<4>(), constant<1>());
+    else
+      go(mt, constant<1>(), constant<8>(), constant<2>());
   };
-  if (mean <= 16) by_columns(constant<1>());
-  else if (mean <= 32) by_columns(constant<2>());
+  if (mt == 1) by_columns(constant<1>());
+  else if (mt == 2) by_columns(constant<2>());
   else by_columns(constant<4>());
 }
 
@@ -350,7 +369,8 @@ __global__ void __launch_bounds__(kRouteThreads) int8_route_kernel(FewRoute a) {
     int q[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) q[j] = int8_code(elem<T>::load(v[j]), s, inv);
-    *reinterpret_cast<uint32_t*>(a.codes + t * pitch + c) = pack_bytes(q[0], q[1], q[2], q[3]);
+    *reinterpret_cast<uint32_t*>(a.codes + int8_row(t, pitch) + c / 16 * 256 + c % 16) =
+        pack_bytes(q[0], q[1], q[2], q[3]);
   }
   if (threadIdx.x == 0) a.scales[t] = s;
   const int e = threadIdx.x;
@@ -402,10 +422,10 @@ Layout layout(int dtype, int64_t T, int32_t k, int32_t E, int64_t d, int64_t f) 
   const int64_t A = T * k;
   l.inv = take(A * 4);
   l.offsets = take((E + 1) * 4);
-  l.x = take(T * int8_pitch(d));
+  l.x = take(int8_rows_bytes(T, int8_pitch(d)));
   l.x_scales = take(T * 4);
   l.hidden = take(A * f * dtype_bytes(dtype));
-  l.codes = take(A * int8_pitch(f));
+  l.codes = take(int8_rows_bytes(A, int8_pitch(f)));
   l.scales = take(A * 4);
   l.y = take(A * d * 4);
   l.bytes = at;
@@ -423,13 +443,12 @@ int check_few(int dtype, int64_t T, int32_t E, int32_t k, int64_t d, int64_t f) 
 }  // namespace
 
 void launch_int8_stream(const Int8Gemm& a, int epi, int dtype, hipStream_t s) {
-  const int64_t mean = ceil_div(a.A, (int64_t)a.E), rows = mean <= 16 ? 16 : mean <= 32 ? 32 : 64;
-  const int64_t loads = std::min<int64_t>(a.A, a.E + a.A / rows);
+  const int64_t experts = std::min<int64_t>(a.E, a.A);
   int8_by_type(dtype, [&](auto type) {
     typedef typename decltype(type)::type T;
-    if (epi == kInt8Plain) launch_stream<T, kInt8Plain, false>(a, mean, loads, NoChoice(), s);
-    else if (epi == kInt8SwiGLU) launch_stream<T, kInt8SwiGLU, false>(a, mean, loads, NoChoice(), s);
-    else launch_stream<T, kInt8Gelu, false>(a, mean, loads, NoChoice(), s);
+    if (epi == kInt8Plain) launch_stream<T, kInt8Plain, false>(a, experts, NoChoice(), s);
+    else if (epi == kInt8SwiGLU) launch_stream<T, kInt8SwiGLU, false>(a, experts, NoChoice(), s);
+    else launch_stream<T, kInt8Gelu, false>(a, experts, NoChoice(), s);
   });
 }
 
@@ -471,9 +490,7 @@ int nt_int8_moe_few_tokens(int dtype, const void* x, const float* router, const 
   c.topk = topk, c.T = (int32_t)T, c.k = k;
   c.offsets = reinterpret_cast<int32_t*>(base + l.offsets);
   c.inv = reinterpret_cast<int32_t*>(base + l.inv);
-  const int64_t A = T * k, mean = ceil_div(A, (int64_t)E);
-  const int64_t rows = mean <= 16 ? 16 : mean <= 32 ? 32 : 64;
-  const int64_t loads = std::min<int64_t>(A, std::min<int64_t>(A, E) + A / rows);
+  const int64_t A = T * k, experts = std::min<int64_t>(A, E);
   Int8Gemm up = {};
   up.x = r.codes, up.x_scales = r.scales, up.w = w_up, up.w_scales = up_scales;
   up.w2 = w_val, up.w2_scales = val_scales;
@@ -482,8 +499,8 @@ int nt_int8_moe_few_tokens(int dtype, const void* x, const float* router, const 
     typedef typename decltype(type)::type V;
     hipLaunchKernelGGL((int8_route_kernel<V>), dim3((unsigned)T), dim3(kRouteThreads), 0, stream,
                        r);
-    if (w_val != nullptr) launch_stream<V, kInt8SwiGLU, true>(up, mean, loads, c, stream);
-    else launch_stream<V, kInt8Gelu, true>(up, mean, loads, c, stream);
+    if (w_val != nullptr) launch_stream<V, kInt8SwiGLU, true>(up, experts, c, stream);
+    else launch_stream<V, kInt8Gelu, true>(up, experts, c, stream);
   });
   int8_t* codes = reinterpret_cast<int8_t*>(base + l.codes);
   float* scales = reinterpret_cast<float*>(base + l.scales);
@@ -493,7 +510,7 @@ int nt_int8_moe_few_tokens(int dtype, const void* x, const float* router, const 
   down.x = codes, down.x_scales = scales, down.offsets = c.offsets, down.w = w_down;
   down.w_scales = down_scales;
   down.E = E, down.A = A, down.K = f, down.N = d, down.out = base + l.y;
-  launch_stream<float, kInt8Plain, false>(down, mean, loads, NoChoice(), stream);
+  launch_stream<float, kInt8Plain, false>(down, experts, NoChoice(), stream);
   int8_by_type(dtype, [&](auto type) {
     typedef typename decltype(type)::type V;
     hipLaunchKernelGGL((int8_combine_kernel<V>),

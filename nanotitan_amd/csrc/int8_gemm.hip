@@ -19,42 +19,65 @@ namespace {
 
 // ------------------------------------------------------------ tiled products
 
-// One k-step is 128 integers of each operand row. The activations' tile lies in
-// LDS as the 16-bit GEMMs' K-major tiles do (64 two-byte elements a row: the loads
-// and the bank swizzle do not know what the bytes are); the weights' blocks are
-// copied as they are.
-constexpr int kStepBytes = 128;
-constexpr int kStepBlocks = kStepBytes / kInt8Block;
+// One k-step is SB = 64 or 128 integers of each operand row. Operands are copied to
+// LDS as they are, 1 KiB a load instruction: a lane's offset never changes, and what
+// tells instructions and steps apart is uniform.
+__device__ __forceinline__ void copy_to_lds(i32x4_t rsrc, uint32_t lane_off, uint32_t off,
+                                            uint32_t lds) {
+  asm volatile(
+      "s_mov_b32 m0, %3\n\t"
+      "s_nop 0\n\t"
+      "buffer_load_dwordx4 %0, %1, %2 offen lds"
+      :
+      : "v"(lane_off), "s"(rsrc), "s"(off), "s"(lds)
+      : "memory", "m0");
+}
 
-// Copies of weight blocks to LDS: BN / 64 column groups x 2 blocks of 4 KiB, 1 KiB
-// an instruction.
-template <int BN, int NW>
-struct WeightTile {
-  static constexpr int kBytes = BN * kStepBytes;
+// The step's operands of `ROWS` rows (activations) or columns (weights): UNIT
+// operands (one; a group's four) for each of its SB / 64 blocks, then the next 16
+// rows (or 64 columns).
+template <int ROWS, int UNIT, int SB, int NW>
+struct OperandCopy {
+  static constexpr int kBytes = ROWS * SB;
   static constexpr int kPer = kBytes / 1024 / NW;
   static_assert(kBytes / 1024 % NW == 0, "whole instructions for every wave");
+  static constexpr int kGroup = UNIT * SB / 64;  // instructions of a row block
   i32x4_t rsrc;
-  uint32_t group;  // bytes from one column group to the next
-  // Of expert e's matrix (column groups from g0 on); groups past the last read zeros.
-  __device__ __forceinline__ void init(const int8_t* matrix, int64_t g0, int64_t groups,
-                                       int64_t pitch) {
-    rsrc = make_rsrc(matrix + g0 * pitch * kInt8Block, (groups - g0) * pitch * kInt8Block);
-    group = (uint32_t)(pitch * kInt8Block);
+  uint32_t lane_off;
+  // From `base`, of which `bytes` are readable (what lies past them reads zeros).
+  __device__ __forceinline__ void init(const int8_t* base, int64_t bytes, uint32_t off) {
+    rsrc = make_rsrc(base, bytes);
+    lane_off = off;
   }
-  __device__ __forceinline__ void issue(int64_t kt, char* lds, int wave, int lane) const {
+  __device__ __forceinline__ void issue(int kt, uint32_t group, char* lds, int wave) const {
     const uint32_t l0 = lds_addr(lds);
+    i32x4_t r;  // in scalar registers, wherever the tile loop keeps it
+#pragma unroll
+    for (int j = 0; j < 4; ++j) r[j] = __builtin_amdgcn_readfirstlane(rsrc[j]);
 #pragma unroll
     for (int u = 0; u < kPer; ++u) {
-      const int i = wave + u * NW;  // instruction: group i / 8, KiB i % 8 of the step's two blocks
-      const uint32_t at = (uint32_t)(i / 8) * group + (uint32_t)kt * (kStepBytes * kInt8Block) +
-                          (uint32_t)(i % 8) * 1024u;
-      load16_to_lds(rsrc, (uint32_t)lane * 16u + at,
-                    __builtin_amdgcn_readfirstlane(l0 + (uint32_t)i * 1024u));
+      const uint32_t i = wave + u * NW;
+      copy_to_lds(r, lane_off,
+                  __builtin_amdgcn_readfirstlane(i / kGroup * group + kt * (kGroup * 1024) +
+                                                 i % kGroup * 1024),
+                  __builtin_amdgcn_readfirstlane(l0 + i * 1024u));
     }
   }
 };
 
 typedef int i32x4 __attribute__((ext_vector_type(4)));
+
+// Waits until only the last `younger` stages' loads (at most MOST count) are in
+// flight: the counter's operand is a constant.
+template <int MOST, int LOADS>
+__device__ __forceinline__ void wait_stages(int younger) {
+  if constexpr (MOST <= 0) {
+    wait_vmcnt<0>();
+  } else {
+    if (younger >= MOST) wait_vmcnt<MOST * LOADS>();
+    else wait_stages<MOST - 1, LOADS>(younger);
+  }
+}
 
 // Where a wave's results lie. The weights' operand goes first, so lane l holds
 // rows l % 16 of the row blocks, and of column group c and operand t columns 64 c +
@@ -65,7 +88,6 @@ __device__ __forceinline__ void int8_store(const i32x4 (&acc)[AB][EPI == kInt8Sw
                                            int m0, int64_t n0, int lane) {
   typedef typename elem<T>::storage S;
   constexpr int MATS = EPI == kInt8SwiGLU ? 2 : 1;
-  const bool whole = a.N % 16 == 0 && a.wide_stores;
 #pragma unroll
   for (int c = 0; c < CG; ++c) {
     const int64_t n = n0 + 64 * c + 16 * (lane >> 4);
@@ -90,26 +112,26 @@ __device__ __forceinline__ void int8_store(const i32x4 (&acc)[AB][EPI == kInt8Sw
                                               sw[MATS - 1][j] * sx
                                         : 0.f,
                               o[0][j], o[1][j], o[2][j]);
-      int8_put<T, EPI>(a, row * a.N + n, (int)(a.N - n < 16 ? a.N - n : 16), whole, o);
+      int8_put<T, EPI>(a, row * a.N + n, (int)(a.N - n < 16 ? a.N - n : 16), o);
     }
   }
 }
 
 template <typename T, int EPI, int BM, int BN, int WGM, int WGN, int NS>
-__global__ void __launch_bounds__(WGM* WGN* kWave, 2)
+__global__ void __launch_bounds__(WGM* WGN* kWave, BM* BN / (WGM * WGN) > 128 * 64 ? 1 : 2)
     int8_tile_kernel(Int8Gemm a) {
-  constexpr int NW = WGM * WGN;
+  constexpr int NW = WGM * WGN, SB = kInt8Block;
   constexpr int MATS = EPI == kInt8SwiGLU ? 2 : 1;
   constexpr int WM = BM / WGM, WN = BN / WGN / MATS;  // of each matrix
   constexpr int AB = WM / 16, CG = WN / 64;
   static_assert(WM % 16 == 0 && WN % 64 == 0, "whole operands");
-  typedef OperandTile<BM, true, 64, NW> TA;
-  typedef WeightTile<BN / MATS, NW> TB;
+  typedef OperandCopy<BM, 1, SB, NW> TA;
+  typedef OperandCopy<BN / MATS, 4, SB, NW> TB;
   constexpr int kStage = TA::kBytes + MATS * TB::kBytes;
   __shared__ __attribute__((aligned(1024))) char smem[NS * kStage];
   __shared__ int32_t s_pref[NT_MAX_EXPERTS + 1];
   int8_row_tiles(a, BM, s_pref);
-  const int64_t mtiles = s_pref[a.E];
+  const int64_t mtiles = __builtin_amdgcn_readfirstlane(s_pref[a.E]);
   const int64_t total = mtiles * a.ntn;
   // Tiles are dealt to the XCDs in contiguous ranges, as the 16-bit GEMMs' are.
   constexpr int kXcd = 8;
@@ -118,24 +140,24 @@ __global__ void __launch_bounds__(WGM* WGN* kWave, 2)
   const int64_t q = G / kXcd, r = G % kXcd;
   const int64_t before = xcd * q + (xcd < r ? xcd : r);
   const int64_t nbx = q + (xcd < r ? 1 : 0);
-  const int64_t t_end = xcd_range_start(total, before + nbx, G, s_pref, a.E, a.ntn);
-  const int64_t t_beg = xcd_range_start(total, before, G, s_pref, a.E, a.ntn);
+  // (at most 2^31 tiles)
+  const int64_t t_end = __builtin_amdgcn_readfirstlane(
+      (int)xcd_range_start(total, before + nbx, G, s_pref, a.E, a.ntn));
+  const int64_t t_beg = __builtin_amdgcn_readfirstlane(
+      (int)xcd_range_start(total, before, G, s_pref, a.E, a.ntn));
   int64_t logical = t_beg + wg / kXcd;
   if (logical >= t_end) return;
 
   const int lane = lane_id();
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int wm = wave / WGN, wn = wave % WGN;
-  FragReader<BM, true, AB, 64> fa;
-  fa.init(wm * WM, lane);
   const int64_t pitch = int8_pitch(a.K), groups = int8_groups(a.N);
-  const int nk = (int)(pitch / kStepBytes);
+  const int nk = (int)(pitch / SB);
 
   int e = 0, rows = 0;
   int64_t row0 = 0, col0 = 0;
-  const int8_t* xa = nullptr;
+  const uint32_t row_block = (uint32_t)(16 * pitch), group = (uint32_t)(kInt8Block * pitch);
   TA ta;
-  ta.init(pitch / 2, wave, lane);
   TB tb[MATS];
   auto setup = [&](int64_t t) {
     int64_t r0, r1, mtl;
@@ -148,67 +170,66 @@ __global__ void __launch_bounds__(WGM* WGN* kWave, 2)
     const int64_t left = (int64_t)__builtin_amdgcn_readfirstlane((int)r1) - row0;
     rows = (int)(left < BM ? left : BM);
     col0 = (int64_t)nt * (BN / MATS);
-    xa = a.x + row0 * pitch;
+    // rows from any of 16 on: the lanes past the last of them go to the next 16
+    const int64_t x0 = (row0 >> 4) * row_block;
+    const uint32_t in16 = (uint32_t)(row0 & 15) + (lane & 15);
+    ta.init(a.x + x0, int8_rows_bytes(a.A, pitch) - x0,
+            (in16 >> 4) * row_block + (in16 & 15) * 16 + (lane >> 4) * 256);
 #pragma unroll
-    for (int i = 0; i < MATS; ++i)
-      tb[i].init((i == 0 ? a.w : a.w2) + e * groups * kInt8Block * pitch, col0 / kInt8Block, groups,
-                 pitch);
-  };
-  auto issue = [&](int kt, char* lds) {
-    ta.issue(xa + (int64_t)kt * kStepBytes, (rows - 1) * pitch + kStepBytes, lds, 64, wave);
-#pragma unroll
-    for (int i = 0; i < MATS; ++i) tb[i].issue(kt, lds + TA::kBytes + i * TB::kBytes, wave, lane);
-  };
-  constexpr int kLoads = TA::kPer + MATS * TB::kPer;
-  setup(logical);
-#pragma unroll
-  for (int s0 = 0; s0 < NS - 1; ++s0)
-    if (s0 < nk) issue(s0, smem + s0 * kStage);
-
-  i32x4 acc[AB][MATS][CG][4];
-  constexpr int kB = MATS * CG * 4;  // weight operands of a wave and substep
-  auto compute = [&](const char* sa) {
-    const char* sb = sa + TA::kBytes;
-    auto read_b = [&](int j, int ks) {
-      const int i = j / (CG * 4), c = j / 4 % CG, t = j % 4;
-      return *reinterpret_cast<const i32x4*>(sb + i * TB::kBytes +
-                                             ((wn * CG + c) * 2 + ks) * 4096 + t * 1024 +
-                                             lane * 16);
-    };
-    auto read_a = [&](int b, int ks) { return fa.template read<i32x4>(sa, b, ks); };
-#pragma unroll
-    for (int ks = 0; ks < 2; ++ks) {
-      // the operand with fewer blocks is held, the other streams
-      if constexpr (kB <= AB) {
-        i32x4 held[kB];
-#pragma unroll
-        for (int j = 0; j < kB; ++j) held[j] = read_b(j, ks);
-#pragma unroll
-        for (int b = 0; b < AB; ++b) {
-          const i32x4 x = read_a(b, ks);
-#pragma unroll
-          for (int j = 0; j < kB; ++j) {
-            i32x4& o = acc[b][j / (CG * 4)][j / 4 % CG][j % 4];
-            o = __builtin_amdgcn_mfma_i32_16x16x64_i8(held[j], x, o, 0, 0, 0);
-          }
-        }
-      } else {
-        i32x4 held[AB];
-#pragma unroll
-        for (int b = 0; b < AB; ++b) held[b] = read_a(b, ks);
-#pragma unroll
-        for (int j = 0; j < kB; ++j) {
-          const i32x4 w = read_b(j, ks);
-#pragma unroll
-          for (int b = 0; b < AB; ++b) {
-            i32x4& o = acc[b][j / (CG * 4)][j / 4 % CG][j % 4];
-            o = __builtin_amdgcn_mfma_i32_16x16x64_i8(w, held[b], o, 0, 0, 0);
-          }
-        }
-      }
+    for (int i = 0; i < MATS; ++i) {
+      const int64_t g0 = col0 / kInt8Block;
+      tb[i].init((i == 0 ? a.w : a.w2) + (e * groups + g0) * group, (groups - g0) * group,
+                 lane * 16);
     }
   };
+  auto issue = [&](int kt, char* lds) {
+    ta.issue(kt, row_block, lds, wave);
+#pragma unroll
+    for (int i = 0; i < MATS; ++i) tb[i].issue(kt, group, lds + TA::kBytes + i * TB::kBytes, wave);
+  };
+  constexpr int kLoads = TA::kPer + MATS * TB::kPer;
 
+  // A k-step is multiplied from registers that the step before filled: after the
+  // barrier of step kt every wave holds its operands of kt, so that stage's slot is
+  // free for step kt + NS, and stage kt + 1 has landed and is read behind the
+  // matrix instructions of kt.
+  i32x4 acc[AB][MATS][CG][4];
+  constexpr int kB = MATS * CG * 4;  // weight operands of a wave
+  struct Operands {
+    i32x4 x[AB], w[kB];
+  };
+  auto read = [&](const char* stage, Operands& o) {
+#pragma unroll
+    for (int b = 0; b < AB; ++b)
+      o.x[b] = *reinterpret_cast<const i32x4*>(stage + (wm * AB + b) * 1024 + lane * 16);
+#pragma unroll
+    for (int j = 0; j < kB; ++j)
+      o.w[j] = *reinterpret_cast<const i32x4*>(stage + TA::kBytes + j / (CG * 4) * TB::kBytes +
+                                               (wn * CG + j / 4 % CG) * 4096 + j % 4 * 1024 +
+                                               lane * 16);
+  };
+  auto multiply = [&](const Operands& o) {
+#pragma unroll
+    for (int b = 0; b < AB; ++b)
+#pragma unroll
+      for (int j = 0; j < kB; ++j) {
+        i32x4& c = acc[b][j / (CG * 4)][j / 4 % CG][j % 4];
+        c = __builtin_amdgcn_mfma_i32_16x16x64_i8(o.w[j], o.x[b], c, 0, 0, 0);
+      }
+  };
+  // Every wave's reads are done and all loads but the `younger` last stages' have
+  // landed (vector memory operations retire in order).
+  auto arrive = [&](int younger) {
+    wait_stages<NS - 2, kLoads>(younger);
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+  };
+  auto prefetch = [&]() {
+#pragma unroll
+    for (int s0 = 0; s0 < NS; ++s0)
+      if (s0 < nk) issue(s0, smem + s0 * kStage);
+  };
+  setup(logical);
+  prefetch();
   while (true) {
 #pragma unroll
     for (int b = 0; b < AB; ++b)
@@ -218,30 +239,30 @@ __global__ void __launch_bounds__(WGM* WGN* kWave, 2)
         for (int c = 0; c < CG; ++c)
 #pragma unroll
           for (int t = 0; t < 4; ++t) acc[b][i][c][t] = i32x4{0, 0, 0, 0};
+    Operands o0, o1;
+    if (nk >= NS) wait_vmcnt<(NS - 1) * kLoads>();
+    else wait_vmcnt<0>();
+    asm volatile("s_barrier" ::: "memory");
+    read(smem, o0);
     int slot = 0;
-    for (int kt = 0; kt < nk; ++kt) {
-      // This stage has landed when at most the younger stages' loads are in flight.
-      if (nk - 1 - kt >= NS - 2) wait_vmcnt<(NS - 2) * kLoads>();
-      else wait_vmcnt<0>();
-      __syncthreads();
-      if (kt + NS - 1 < nk) {
-        int fill = slot + NS - 1;
-        if (fill >= NS) fill -= NS;
-        issue(kt + NS - 1, smem + fill * kStage);
-      }
-      compute(smem + slot * kStage);
+    auto step = [&](int kt, const Operands& now, Operands& then) {
+      arrive(nk - 2 - kt);
+      if (kt + NS < nk) issue(kt + NS, smem + slot * kStage);
       slot = slot + 1 == NS ? 0 : slot + 1;
+      if (kt + 1 < nk) read(smem + slot * kStage, then);
+      multiply(now);
+    };
+    for (int kt = 0; kt < nk; kt += 2) {  // (an even number: K is padded to 128)
+      step(kt, o0, o1);
+      step(kt + 1, o1, o0);
     }
-    __syncthreads();  // every wave is done with the stages
     const int64_t next = logical + nbx;
     const int64_t se = e, srow = row0, scol = col0;
     const int srows = rows;
     const bool more = next < t_end;
-    if (more) {
+    if (more) {  // no wave reads the stages any more
       setup(next);
-#pragma unroll
-      for (int s0 = 0; s0 < NS - 1; ++s0)
-        if (s0 < nk) issue(s0, smem + s0 * kStage);
+      prefetch();
     }
     int8_store<T, EPI, AB, CG>(acc, a, se, srow, srows, wm * WM, scol + wn * WN, lane);
     if (!more) break;
@@ -250,37 +271,58 @@ __global__ void __launch_bounds__(WGM* WGN* kWave, 2)
 }
 
 template <typename T, int EPI, int BM, int BN, int WGM, int WGN, int NS>
-void launch_tiles(Int8Gemm a, int per_cu, hipStream_t s) {
+int launch_tiles(Int8Gemm a, int per_cu, hipStream_t s) {
   constexpr int MATS = EPI == kInt8SwiGLU ? 2 : 1;
   a.ntn = (int32_t)ceil_div(a.N, (int64_t)(BN / MATS));
   const int64_t tiles = (ceil_div(a.A, (int64_t)BM) + a.E - 1) * a.ntn;  // at most
+  if (tiles > INT32_MAX) return NT_ERR_TOO_LARGE;
   const int64_t grid = std::min<int64_t>(tiles, (int64_t)device_cus(s) * per_cu);
   hipLaunchKernelGGL((int8_tile_kernel<T, EPI, BM, BN, WGM, WGN, NS>), dim3((unsigned)grid),
                      dim3(WGM * WGN * kWave), 0, s, a);
+  return launch_status();
 }
 
+// Which kernel. With few rows an expert the weights are read straight into registers
+// (int8_few.hip), and where there are fewer 128x128 tiles than CUs and reading the
+// weights once for every 64 rows takes less than a tile's k-steps: a step of 64 lasts
+// 0.32 us whatever the tile holds, that reading runs at 4 TB/s (one expert, 14,336
+// to 4,096: 64 rows 25 us against 72, 128 28 against 73; 4,096 to 14,336: 64 rows 18
+// against 26, 128 29 against 27). Else tiles of 128x256 with two workgroups a CU: one's
+// epilogue runs behind the other's products. Where these are less than about one
+// and a half rounds of the chip's slots, tiles of half the width (E = 8, 4,000 rows
+// of 4,096 to 4,096: 92 -> 79 us; 38,400 rows, E = 128, 2,048 to 768: 94 us against
+// 99). Long reductions of many tiles take 256x256, which reads less from L2 and LDS
+// for a product (32,768 rows, 14,336 to 4,096: 1,793 -> 1,692 us, 8,192: 990 -> 940,
+// but 4,096: 442 -> 486; two matrices, 4,096 to 4,096: 969 -> 942 us, 2,048: 505 ->
+// 512).
 template <typename T, int EPI>
 int launch_by_size(const Int8Gemm& a, hipStream_t s) {
-  const int64_t mean = ceil_div(a.A, (int64_t)a.E);
   constexpr int dtype = std::is_same<T, float>::value ? NT_F32
                         : std::is_same<T, f16>::value ? NT_F16 : NT_BF16;
-  if (mean <= 64) {
+  constexpr bool two = EPI == kInt8SwiGLU;
+  const int64_t cus = device_cus(s), width = two ? 128 : 256;
+  auto tiles = [&](int64_t rows) {  // expected: an expert's last tile is half full
+    return (ceil_div(a.A, rows) + a.E / 2) * ceil_div(a.N, width);
+  };
+  const int64_t loads = ceil_div(a.A, 64) + a.E / 2;
+  if (a.A <= 24 * (int64_t)a.E ||
+      ((ceil_div(a.A, 128) + a.E / 2) * ceil_div(a.N, two ? 64 : 128) <= cus &&
+       loads * a.N * (two ? 2 : 1) < 20000)) {
     launch_int8_stream(a, EPI, dtype, s);
-  } else if constexpr (EPI == kInt8SwiGLU) {
-    if (mean <= 256) launch_tiles<T, EPI, 128, 128, 4, 1, 2>(a, 2, s);
-    else launch_tiles<T, EPI, 256, 256, 4, 2, 2>(a, 1, s);
-  } else {
-    if (mean <= 256) launch_tiles<T, EPI, 128, 128, 2, 2, 2>(a, 2, s);
-    else launch_tiles<T, EPI, 256, 256, 2, 4, 2>(a, 1, s);
+    return launch_status();
   }
-  return launch_status();
+  if (a.K >= (two ? 4096 : 8192) && tiles(256) >= 4 * cus)
+    return launch_tiles<T, EPI, 256, 256, 4, 2, 3>(a, 1, s);
+  if (tiles(128) >= 3 * cus) return launch_tiles<T, EPI, 128, 256, 2, 2, 3>(a, 2, s);
+  if constexpr (two) return launch_tiles<T, EPI, 128, 128, 4, 1, 3>(a, 2, s);
+  else return launch_tiles<T, EPI, 128, 128, 2, 2, 3>(a, 3, s);
 }
 
 int check_int8(int dtype, const Int8Gemm& a) {
   if (!int8_float(dtype)) return NT_ERR_DTYPE;
   if (a.E < 1 || a.A < 0 || a.K < 1 || a.N < 1) return NT_ERR_INVALID_ARG;
   if (a.E > NT_MAX_EXPERTS) return NT_ERR_TOO_MANY_EXPERTS;
-  if (a.K > kInt8MaxK || a.N > (1 << 22) || a.A > INT32_MAX - 512) return NT_ERR_TOO_LARGE;
+  if (a.K > kInt8MaxK || a.N > (1 << 22) || a.A > kInt8MaxRows) return NT_ERR_TOO_LARGE;
   return NT_OK;
 }
 bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
@@ -294,7 +336,6 @@ int run_int8(int dtype, int epi, Int8Gemm a, hipStream_t s) {
       (a.offsets == nullptr && a.E != 1) || (two && (a.out2 == nullptr) != (a.out3 == nullptr)) ||
       !aligned16(a.x) || !aligned16(a.w) || !aligned16(a.w2))
     return NT_ERR_INVALID_ARG;
-  a.wide_stores = aligned16(a.out) && aligned16(a.out2) && aligned16(a.out3);
   int result = NT_OK;
   int8_by_type(dtype, [&](auto type) {
     typedef typename decltype(type)::type T;

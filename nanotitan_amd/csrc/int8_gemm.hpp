@@ -21,7 +21,6 @@ struct Int8Gemm {
   void* out;         // [A, N]; hidden, act
   void *out2, *out3;  // gate, value; gelu' (null: not written)
   int32_t ntn;
-  bool wide_stores;  // outputs are 16-byte aligned
 };
 
 // int8_few.hip: the product of few rows for each expert.
@@ -106,7 +105,7 @@ __device__ __forceinline__ void int8_epilogue(float p, float p2, typename elem<T
 
 // n (at most 16) neighbouring columns of every output, at element `at`.
 template <typename T, int EPI>
-__device__ __forceinline__ void int8_put(const Int8Gemm& a, int64_t at, int n, bool whole,
+__device__ __forceinline__ void int8_put(const Int8Gemm& a, int64_t at, int n,
                                          const typename elem<T>::storage (&o)[3][16]) {
   typedef typename elem<T>::storage S;
   constexpr int kOuts = EPI == kInt8Plain ? 1 : EPI == kInt8SwiGLU ? 3 : 2;
@@ -115,11 +114,13 @@ __device__ __forceinline__ void int8_put(const Int8Gemm& a, int64_t at, int n, b
     S* p = static_cast<S*>(i == 0 ? a.out : i == 1 ? a.out2 : a.out3);
     if (i > 0 && p == nullptr) continue;
     p += at;
-    if (whole) {
-      uint4 v[sizeof(S)];
+    if (n == 16) {
+      typedef S V __attribute__((ext_vector_type(16 / sizeof(S)), aligned(sizeof(S))));
+      V v[sizeof(S)];
       __builtin_memcpy(v, o[i], sizeof(v));
 #pragma unroll
-      for (int j = 0; j < (int)sizeof(S); ++j) reinterpret_cast<uint4*>(p)[j] = v[j];
+      for (int j = 0; j < (int)sizeof(S); ++j)
+        __builtin_nontemporal_store(v[j], reinterpret_cast<V*>(p) + j);
     } else {
 #pragma unroll
       for (int j = 0; j < 16; ++j)

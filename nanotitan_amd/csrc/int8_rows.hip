@@ -1,8 +1,12 @@
 // Rows and weights to 8-bit integers and back.
 //
-// Rows: a wave (or, where there are few rows or wide ones, a workgroup of four)
-// holds a row in registers between finding its largest magnitude and rounding it,
-// so it is read once. HBM bounds all of it.
+// Rows: a team of lanes holds a row in registers between finding its largest
+// magnitude and rounding it, so it is read once. A workgroup takes eight rows (four
+// wide ones), whose integers pass through LDS: in memory the 16-byte pieces of 16
+// rows alternate, and eight of them make a 128-byte line (written piece by piece,
+// 32,768 rows of 14,336 took 534 us for 235 in row order). Rounding one value has to
+// stay near seven instructions for HBM to bound the kernel (Sixteen::codes). Few
+// rows take a workgroup each and write their pieces as they are.
 //
 // Weights: the channels' maxima run down the columns, so a pass over W finds them
 // (an atomic max of magnitudes' bits: the order does not count) and a second one
@@ -41,102 +45,206 @@ struct Sixteen {
     }
   }
   __device__ __forceinline__ uint32_t most() const {
-    uint32_t m = 0;
+    if constexpr (sizeof(S) == 2) {
+      // pairs at once: magnitudes' bits order as the values do
+      typedef unsigned short U2 __attribute__((ext_vector_type(2)));
+      uint32_t w[8];
+      __builtin_memcpy(w, &v, sizeof(w));
+      U2 m = {0, 0};
 #pragma unroll
-    for (int i = 0; i < kVec; ++i) {
-      const uint32_t b = abs_bits(elem<T>::load(v[i]));
-      m = b > m ? b : m;
+      for (int i = 0; i < 8; ++i)
+        m = __builtin_elementwise_max(m, __builtin_bit_cast(U2, w[i] & 0x7fff7fffu));
+      return abs_bits(elem<T>::load(m[0] > m[1] ? m[0] : m[1]));
+    } else {
+      uint32_t m = 0;
+#pragma unroll
+      for (int i = 0; i < kVec; ++i) {
+        const uint32_t b = abs_bits(elem<T>::load(v[i]));
+        m = b > m ? b : m;
+      }
+      return m;
     }
-    return m;
   }
+  // x / s by the inverse, plus 1.5 2^23: the sum's low byte is the nearest integer,
+  // or next to a border its neighbour, which x minus s times it tells. Then
+  // int8_code decides; of normal values in bf16 one group of 1,024 in thirty.
   __device__ __forceinline__ uint4 codes(float s, float inv) const {
+    constexpr float kMagic = 12582912.f;
     uint32_t w[4];
+    float most = 0.f;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      int q[4];
+      uint32_t t[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) q[j] = int8_code(elem<T>::load(v[4 * i + j]), s, inv);
-      w[i] = pack_bytes(q[0], q[1], q[2], q[3]);
+      for (int j = 0; j < 4; ++j) {
+        const float x = elem<T>::load(v[4 * i + j]), sum = fmaf(x, inv, kMagic);
+        most = fmaxf(most, fabsf(fmaf(kMagic - sum, s, x)));
+        t[j] = __float_as_uint(sum);
+      }
+      w[i] = __builtin_amdgcn_perm(__builtin_amdgcn_perm(t[3], t[2], 0x0c0c0400u),
+                                   __builtin_amdgcn_perm(t[1], t[0], 0x0c0c0400u), 0x05040100u);
+    }
+    if (!(most < 0.5f * s) || inv == 0.f) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        int q[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) q[j] = int8_code(elem<T>::load(v[4 * i + j]), s, inv);
+        w[i] = pack_bytes(q[0], q[1], q[2], q[3]);
+      }
     }
     return make_uint4(w[0], w[1], w[2], w[3]);
   }
 };
 
-__device__ __forceinline__ uint32_t wave_most(uint32_t m) {
+constexpr int kThreads = 256;
+
+// ROWS rows a workgroup, TEAM lanes a row, C chunks of 16 columns a lane in
+// registers; HELD false: rows past TEAM * C * 16 columns, read twice. Workgroups b
+// and b + 8 share an XCD and so an L2: the parts of a block of 16 rows go to such.
+template <typename T, int ROWS, int TEAM, int C, bool HELD>
+__global__ void __launch_bounds__(ROWS* TEAM)
+    int8_rows_kernel(const void* x, int64_t rows, int64_t f, int8_t* codes, float* scales) {
+  typedef typename elem<T>::storage S;
+  constexpr int G = C % 2 == 0 ? 2 : 1;  // chunks of a lane that turn at once
+  // a chunk's pieces, padded so that neighbouring lanes' begin in other banks
+  constexpr int kPitch = ROWS * 16 + 16, kParts = 16 / ROWS;
+  __shared__ __attribute__((aligned(16))) char s_turn[2][G * TEAM * kPitch];
+  const int64_t b = blockIdx.x;
+  const int64_t row0 = (b / (8 * kParts) * 8 + b % 8) * 16 + b / 8 % kParts * ROWS;
+  if (row0 >= rows) return;
+  const int r = threadIdx.x / TEAM, lane = threadIdx.x % TEAM;
+  const bool live = row0 + r < rows;
+  const int64_t row = live ? row0 + r : rows - 1;  // past the last: that one again
+  const int64_t pitch = int8_pitch(f);
+  const int chunks = (int)(pitch / kVec);
+  const S* in = static_cast<const S*>(x) + row * f;
+  Sixteen<T> v[C];
+  auto load = [&](int c0) {
+#pragma unroll
+    for (int i = 0; i < C; ++i)
+      if (c0 + i * TEAM < chunks) v[i].load(in, (int64_t)(c0 + i * TEAM + lane) * kVec, f);
+  };
+  uint32_t m = 0;
+  for (int c0 = 0; c0 < (HELD ? 1 : chunks); c0 += TEAM * C) {
+    load(c0);
+#pragma unroll
+    for (int i = 0; i < C; ++i) {
+      const uint32_t most = c0 + i * TEAM < chunks ? v[i].most() : 0u;
+      m = most > m ? most : m;
+    }
+  }
+#pragma unroll
+  for (int o = (TEAM < kWave ? TEAM : kWave) / 2; o >= 1; o >>= 1) {
+    const uint32_t other = __shfl_xor(m, o, kWave);
+    m = other > m ? other : m;
+  }
+  if constexpr (TEAM > kWave) {
+    __shared__ uint32_t s_most[ROWS * TEAM / kWave];
+    if (lane_id() == 0) s_most[threadIdx.x / kWave] = m;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < TEAM / kWave; ++i) {
+      const uint32_t other = s_most[r * (TEAM / kWave) + i];
+      m = other > m ? other : m;
+    }
+  }
+  const float s = int8_scale(m), inv = int8_inverse(s);
+  if (lane == 0 && live) scales[row] = s;
+  // thread: piece threadIdx % ROWS of chunk threadIdx / ROWS
+  int8_t* out = codes + int8_row(row0 + threadIdx.x % ROWS, pitch);
+  int buffer = 0;
+  for (int c0 = 0; c0 < (HELD ? 1 : chunks); c0 += TEAM * C) {
+    if constexpr (!HELD) load(c0);
+#pragma unroll
+    for (int i = 0; i < C; i += G) {
+      if (c0 + i * TEAM >= chunks) break;
+      char* turn = s_turn[buffer];
+      buffer ^= 1;
+#pragma unroll
+      for (int g = 0; g < G; ++g)
+        if (c0 + (i + g) * TEAM < chunks)
+          *reinterpret_cast<uint4*>(turn + (g * TEAM + lane) * kPitch + r * 16) =
+              v[i + g].codes(s, inv);
+      __syncthreads();
+#pragma unroll
+      for (int g = 0; g < G; ++g) {
+        const int at = g * TEAM + threadIdx.x / ROWS, c = c0 + i * TEAM + at;
+        if (c < chunks)
+          *reinterpret_cast<uint4*>(out + (int64_t)c * 256) =
+              *reinterpret_cast<const uint4*>(turn + at * kPitch + threadIdx.x % ROWS * 16);
+      }
+    }
+  }
+}
+
+// A row a workgroup.
+template <typename T, int C, bool HELD>
+__global__ void __launch_bounds__(kThreads)
+    int8_row_kernel(const void* x, int64_t f, int8_t* codes, float* scales) {
+  typedef typename elem<T>::storage S;
+  __shared__ uint32_t s_most[kThreads / kWave];
+  const int64_t row = blockIdx.x, pitch = int8_pitch(f);
+  const int lane = threadIdx.x;
+  const S* in = static_cast<const S*>(x) + row * f;
+  int8_t* out = codes + int8_row(row, pitch);
+  Sixteen<T> v[C];
+  uint32_t m = 0;
+  for (int64_t c0 = 0; c0 < (HELD ? 1 : pitch); c0 += kThreads * C * kVec) {
+#pragma unroll
+    for (int i = 0; i < C; ++i) v[i].load(in, c0 + (i * kThreads + lane) * kVec, f);
+#pragma unroll
+    for (int i = 0; i < C; ++i) {
+      const uint32_t most = v[i].most();
+      m = most > m ? most : m;
+    }
+  }
 #pragma unroll
   for (int o = kWave / 2; o >= 1; o >>= 1) {
     const uint32_t other = __shfl_xor(m, o, kWave);
     m = other > m ? other : m;
   }
-  return m;
-}
-
-constexpr int kThreads = 256;
-
-// TEAM lanes a row (64 or 256), C chunks of 16 columns a lane in registers; HELD
-// false: rows past TEAM * C * 16 columns, read twice.
-template <typename T, int TEAM, int C, bool HELD>
-__global__ void __launch_bounds__(kThreads) int8_rows_kernel(const void* x, int64_t rows, int64_t f,
-                                                             int8_t* codes, float* scales) {
-  typedef typename elem<T>::storage S;
-  __shared__ uint32_t s_most[kThreads / kWave];
-  // (the grid has a second dimension: one holds 2^32 threads at most)
-  const int64_t row =
-      ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * (kThreads / TEAM) + threadIdx.x / TEAM;
-  const int lane = threadIdx.x % TEAM;
-  if (row >= rows) return;  // with a workgroup a row: all its threads
-  const int64_t pitch = int8_pitch(f);
-  const S* in = static_cast<const S*>(x) + row * f;
-  int8_t* out = codes + row * pitch;
-  Sixteen<T> v[C];
-  uint32_t m = 0;
-  for (int64_t c0 = 0; c0 < (HELD ? 1 : pitch); c0 += TEAM * C * kVec) {
+  if (lane_id() == 0) s_most[threadIdx.x / kWave] = m;
+  __syncthreads();
 #pragma unroll
-    for (int i = 0; i < C; ++i) v[i].load(in, c0 + (i * TEAM + lane) * kVec, f);
-#pragma unroll
-    for (int i = 0; i < C; ++i) {
-      const uint32_t b = v[i].most();
-      m = b > m ? b : m;
-    }
-  }
-  m = wave_most(m);
-  if constexpr (TEAM > kWave) {
-    if (lane_id() == 0) s_most[threadIdx.x / kWave] = m;
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < TEAM / kWave; ++i) m = s_most[i] > m ? s_most[i] : m;
-  }
+  for (int i = 0; i < kThreads / kWave; ++i) m = s_most[i] > m ? s_most[i] : m;
   const float s = int8_scale(m), inv = int8_inverse(s);
   if (lane == 0) scales[row] = s;
-  for (int64_t c0 = 0; c0 < (HELD ? 1 : pitch); c0 += TEAM * C * kVec) {
+  for (int64_t c0 = 0; c0 < (HELD ? 1 : pitch); c0 += kThreads * C * kVec) {
 #pragma unroll
     for (int i = 0; i < C; ++i) {
-      const int64_t c = c0 + (i * TEAM + lane) * kVec;
+      const int64_t c = c0 + (i * kThreads + lane) * kVec;
       if constexpr (!HELD) v[i].load(in, c, f);
-      if (c < pitch) *reinterpret_cast<uint4*>(out + c) = v[i].codes(s, inv);
+      if (c < pitch) *reinterpret_cast<uint4*>(out + c * 16) = v[i].codes(s, inv);
     }
   }
 }
 
+// 16 rows by 64 chunks a workgroup, a lane a chunk of four rows: the rows' pieces lie
+// in lines that its waves read one after the other, its writes are whole lines.
 template <typename T>
 __global__ void __launch_bounds__(kThreads) int8_rows_decode_kernel(const int8_t* codes,
                                                                     const float* scales,
                                                                     int64_t rows, int64_t f,
                                                                     void* x) {
   typedef typename elem<T>::storage S;
-  const int64_t chunks = ceil_div(f, (int64_t)kVec), pitch = int8_pitch(f);
-  const int64_t total = rows * chunks;
-  for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < total;
-       i += (int64_t)gridDim.x * kThreads) {
-    const int64_t row = i / chunks, c = (i - row * chunks) * kVec;
+  const int64_t pitch = int8_pitch(f), c = ((int64_t)blockIdx.y * kWave + lane_id()) * kVec;
+  if (c >= f) return;
+  const int64_t row0 = (int64_t)blockIdx.x * 16 + threadIdx.x / kWave * 4;
+  const int8_t* in = codes + int8_row(row0, pitch) + c * 16;
+  uint4 w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) w[i] = reinterpret_cast<const uint4*>(in)[i];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (row0 + i >= rows) break;
     int8_t q[kVec];
-    const uint4 w = *reinterpret_cast<const uint4*>(codes + row * pitch + c);
-    __builtin_memcpy(q, &w, sizeof(q));
-    const float s = scales[row];
+    __builtin_memcpy(q, &w[i], sizeof(q));
+    const float s = scales[row0 + i];
     Sixteen<T> v;
 #pragma unroll
     for (int j = 0; j < kVec; ++j) v.v[j] = int8_value<T>(q[j], s);
-    v.store(static_cast<S*>(x) + row * f, c, f);
+    v.store(static_cast<S*>(x) + (row0 + i) * f, c, f);
   }
 }
 
@@ -277,7 +385,7 @@ __global__ void __launch_bounds__(kThreads) int8_weight_decode_kernel(const int8
 int check_rows(int dtype, int64_t rows, int64_t f) {
   if (!int8_float(dtype)) return NT_ERR_DTYPE;
   if (rows < 0 || f < 1) return NT_ERR_INVALID_ARG;
-  if (rows > INT32_MAX || f > kInt8MaxK) return NT_ERR_TOO_LARGE;
+  if (rows > kInt8MaxRows || f > kInt8MaxK) return NT_ERR_TOO_LARGE;
   return NT_OK;
 }
 int check_weight(int dtype, int32_t E, int64_t K, int64_t N) {
@@ -298,6 +406,10 @@ extern "C" {
 
 int64_t nt_int8_pitch(int64_t f) { return f < 0 ? 0 : int8_pitch(f); }
 
+size_t nt_int8_rows_bytes(int64_t rows, int64_t f) {
+  return check_rows(NT_F32, rows, f) == NT_OK ? (size_t)int8_rows_bytes(rows, int8_pitch(f)) : 0;
+}
+
 size_t nt_int8_weight_bytes(int32_t E, int64_t K, int64_t N) {
   if (check_weight(NT_F32, E, K, N) != NT_OK) return 0;
   return (size_t)E * int8_matrix(K, N);
@@ -311,19 +423,29 @@ int nt_int8_rows(int dtype, const void* x, int64_t rows, int64_t f, int8_t* code
     return NT_ERR_INVALID_ARG;
   int8_by_type(dtype, [&](auto type) {
     typedef typename decltype(type)::type T;
-    auto launch = [&](auto kernel, int team) {
-      const int64_t blocks = ceil_div(rows, (int64_t)(kThreads / team)), wide = 1 << 23;
-      hipLaunchKernelGGL(kernel,
-                         dim3((unsigned)std::min(blocks, wide), (unsigned)ceil_div(blocks, wide)),
-                         dim3(kThreads), 0, stream, x, rows, f, codes, scales);
+    auto launch = [&](auto kernel, int at_once, int team) {
+      const int64_t parts = 16 / at_once, blocks = ceil_div(ceil_div(rows, (int64_t)16), (int64_t)8);
+      hipLaunchKernelGGL(kernel, dim3((unsigned)(blocks * 8 * parts)), dim3(at_once * team), 0,
+                         stream, x, rows, f, codes, scales);
     };
-    const int64_t chunks = ceil_div(f, (int64_t)kVec);
-    if (chunks <= 64) launch(int8_rows_kernel<T, 64, 1, true>, 64);
-    else if (chunks <= 128 && rows >= 1024) launch(int8_rows_kernel<T, 64, 2, true>, 64);
-    else if (chunks <= 256) launch(int8_rows_kernel<T, 256, 1, true>, 256);
-    else if (chunks <= 512) launch(int8_rows_kernel<T, 256, 2, true>, 256);
-    else if (chunks <= 1024) launch(int8_rows_kernel<T, 256, 4, true>, 256);
-    else launch(int8_rows_kernel<T, 256, 4, false>, 256);
+    auto one = [&](auto kernel) {
+      hipLaunchKernelGGL(kernel, dim3((unsigned)rows), dim3(kThreads), 0, stream, x, f, codes,
+                         scales);
+    };
+    const int64_t chunks = int8_pitch(f) / kVec;
+    if (rows <= 512) {
+      if (chunks <= 256) one(int8_row_kernel<T, 1, true>);
+      else if (chunks <= 512) one(int8_row_kernel<T, 2, true>);
+      else if (chunks <= 1024) one(int8_row_kernel<T, 4, true>);
+      else one(int8_row_kernel<T, 4, false>);
+    } else if (chunks <= 16) launch(int8_rows_kernel<T, 8, 16, 1, true>, 8, 16);
+    else if (chunks <= 32) launch(int8_rows_kernel<T, 8, 32, 1, true>, 8, 32);
+    else if (chunks <= 64) launch(int8_rows_kernel<T, 8, 64, 1, true>, 8, 64);
+    else if (chunks <= 128) launch(int8_rows_kernel<T, 8, 64, 2, true>, 8, 64);
+    else if (chunks <= 256) launch(int8_rows_kernel<T, 4, 128, 2, true>, 4, 128);
+    else if (chunks <= 512) launch(int8_rows_kernel<T, 4, 128, 4, true>, 4, 128);
+    else if (chunks <= 1024) launch(int8_rows_kernel<T, 4, 128, 8, true>, 4, 128);
+    else launch(int8_rows_kernel<T, 4, 128, 4, false>, 4, 128);
   });
   return launch_status();
 }
@@ -334,12 +456,12 @@ int nt_int8_rows_decode(int dtype, const int8_t* codes, const float* scales, int
   if (st != NT_OK || rows == 0) return st;
   if (x == nullptr || codes == nullptr || scales == nullptr || !aligned16(codes))
     return NT_ERR_INVALID_ARG;
-  const int64_t blocks = ceil_div(rows * ceil_div(f, (int64_t)kVec), (int64_t)kThreads);
   int8_by_type(dtype, [&](auto type) {
     typedef typename decltype(type)::type T;
     hipLaunchKernelGGL((int8_rows_decode_kernel<T>),
-                       dim3((unsigned)std::min<int64_t>(blocks, 1 << 20)), dim3(kThreads), 0,
-                       stream, codes, scales, rows, f, x);
+                       dim3((unsigned)ceil_div(rows, (int64_t)16),
+                            (unsigned)ceil_div(f, (int64_t)(kWave * kVec))),
+                       dim3(kThreads), 0, stream, codes, scales, rows, f, x);
   });
   return launch_status();
 }

@@ -65,7 +65,8 @@ struct Rows8 {
 };
 Rows8 rows8(const Tensor& x) {
   const int64_t rows = x.size(0), f = x.size(1);
-  Rows8 r = {at::empty({rows, nt_int8_pitch(f)}, x.options().dtype(at::kChar)),
+  Rows8 r = {at::empty({(rows + 15) / 16, nt_int8_pitch(f) / 64, 4, 16, 16},
+                       x.options().dtype(at::kChar)),
              at::empty({rows}, x.options().dtype(at::kFloat))};
   check_status(nt_int8_rows(dtype_code(x), x.data_ptr(), rows, f, r.codes.data_ptr<int8_t>(),
                             r.scales.data_ptr<float>(), stream_of(x)),
@@ -73,7 +74,7 @@ Rows8 rows8(const Tensor& x) {
   return r;
 }
 
-// int8_rows(x) -> (codes, scales), and back.
+// int8_rows(x) -> (codes [rows/16, f/64, 4, 16, 16], scales), and back.
 std::tuple<Tensor, Tensor> int8_rows(Tensor x) {
   const OptTensor in = x;
   refuse_tangents({&in}, "int8_rows");
@@ -87,15 +88,16 @@ Tensor int8_rows_decode(Tensor codes, Tensor scales, int64_t width, at::ScalarTy
   check_f32(scales, "scales");
   check_same_device(codes, {&scales});
   TORCH_CHECK(codes.scalar_type() == at::kChar, "codes must be int8");
-  TORCH_CHECK(width >= 1 && codes.dim() == 2 && codes.is_contiguous() &&
-                  codes.size(1) == nt_int8_pitch(width) && scales.dim() == 1 &&
-                  scales.is_contiguous() && scales.size(0) == codes.size(0),
-              "expected contiguous codes [rows, ", nt_int8_pitch(width < 1 ? 1 : width),
-              "] and scales [rows] for width ", width);
+  TORCH_CHECK(width >= 1 && width <= NT_INT8_MAX_K && scales.dim() == 1 &&
+                  scales.is_contiguous() && codes.is_contiguous() &&
+                  codes.numel() == (scales.size(0) + 15) / 16 * 16 * nt_int8_pitch(width) &&
+                  reinterpret_cast<uintptr_t>(codes.data_ptr()) % 16 == 0,
+              "expected contiguous codes [rows / 16, width / 64, 4, 16, 16], rounded up, and "
+              "scales [rows] for width ", width);
   c10::hip::HIPGuard guard(codes.get_device());
-  Tensor x = at::empty({codes.size(0), width}, codes.options().dtype(dtype));
+  Tensor x = at::empty({scales.size(0), width}, codes.options().dtype(dtype));
   check_status(nt_int8_rows_decode(dtype_code(x), codes.data_ptr<int8_t>(),
-                                   scales.data_ptr<float>(), codes.size(0), width, x.data_ptr(),
+                                   scales.data_ptr<float>(), scales.size(0), width, x.data_ptr(),
                                    stream_of(codes)),
                "int8_rows_decode");
   return x;

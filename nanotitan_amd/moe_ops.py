@@ -803,10 +803,12 @@ def int8_weight_decode(weight, dtype):
 
 
 def int8_rows(x):
-    """(codes int8 [rows, f padded with zeros to 128], scales float32 [rows]) of x [rows,f].
+    """(codes int8 [rows/16, f/64, 4, 16, 16], scales float32 [rows]) of x [rows,f].
 
-    codes * scales are x's values, each the nearest multiple of its row's largest magnitude
-    / 127 (ties to even). A row with an infinity or a NaN has a NaN scale.
+    Row r's integer for column c is codes[r//16, c//64, c%64 // 16, r%16, c%16]; f is padded with
+    zeros to 128, rows past the last hold anything. Times its row's scale it is the value's
+    nearest multiple of the row's largest magnitude / 127 (ties to even). A row with an infinity
+    or a NaN has a NaN scale.
     """
     return get_hip_extension().int8_rows(x.detach().contiguous())
 

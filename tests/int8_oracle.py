@@ -32,6 +32,12 @@ def blocks(q):
     return out
 
 
+def plain_rows(codes):
+    """Rows [16 A', pitch] of codes [A', pitch / 64, 4, 16, 16]."""
+    a, kb = codes.shape[:2]
+    return codes.permute(0, 3, 1, 2, 4).reshape(16 * a, 64 * kb)
+
+
 def product(qx, sx, qw, sw, offsets):
     """Rows by their experts' weights in float64: integers [A,K], scales [A,1], integers [E,K,N],
     scales [E,1,N]; rows past the last offset are zero."""

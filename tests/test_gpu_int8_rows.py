@@ -31,9 +31,11 @@ def _check_rows(x):
     codes, scales = int8_rows(x)
     f = x.shape[1]
     q, s = O.held(x.cpu(), 1)
-    assert codes.shape == (x.shape[0], O.pitch(f)) and codes.dtype == torch.int8
-    assert torch.equal(codes[:, :f].cpu().long(), q)
-    assert not bool(codes[:, f:].any())
+    assert codes.shape == (-(-x.shape[0] // 16), O.pitch(f) // 64, 4, 16, 16)
+    assert codes.dtype == torch.int8
+    plain = O.plain_rows(codes)[:x.shape[0]]
+    assert torch.equal(plain[:, :f].cpu().long(), q)
+    assert not bool(plain[:, f:].any())
     assert torch.equal(scales.cpu().nan_to_num(-1.0), s.view(-1).nan_to_num(-1.0))
     for dtype in {x.dtype, torch.float32}:
         got = int8_rows_decode(codes, scales, f, dtype)
@@ -95,7 +97,7 @@ def test_extremes(dtype):
 
 def test_no_rows():
     codes, scales = int8_rows(torch.zeros(0, 300, device="cuda"))
-    assert codes.shape == (0, 384) and scales.shape == (0,)
+    assert codes.shape == (0, 6, 4, 16, 16) and scales.shape == (0,)
     assert int8_rows_decode(codes, scales, 300, torch.float16).shape == (0, 300)
 
 
@@ -143,8 +145,9 @@ def test_past_32_bit_offsets():
     x[-7:] = tail
     codes, scales = int8_rows(x)
     c, s = int8_rows(tail)
-    assert torch.equal(codes[-7:], c) and torch.equal(scales[-7:], s)
-    assert not bool(codes[-9:-7].any())
+    last = O.plain_rows(codes[-2:])[:16 + A % 16]
+    assert torch.equal(last[-7:], O.plain_rows(c)[:7]) and torch.equal(scales[-7:], s)
+    assert not bool(last[:-7].any())
     back = int8_rows_decode(codes, scales, f, torch.float16)
     assert torch.equal(back[-7:], int8_rows_decode(c, s, f, torch.float16))
     del x, codes, back
@@ -163,7 +166,7 @@ def test_refusals():
     codes, scales = int8_rows(x)
     for bad in (lambda: int8_rows(x.double()), lambda: int8_rows(x.view(-1)),
                 lambda: int8_rows_decode(codes, scales, 200, torch.float32),
-                lambda: int8_rows_decode(codes, scales[:3], 64, torch.float32),
+                lambda: int8_rows_decode(codes, scales.repeat(5), 64, torch.float32),
                 lambda: int8_rows_decode(codes.float(), scales, 64, torch.float32),
                 lambda: int8_rows_decode(codes, scales, 64, torch.float64),
                 lambda: int8_weight(x.double()), lambda: int8_weight(x.view(-1)),

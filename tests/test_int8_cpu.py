@@ -53,6 +53,8 @@ def test_oracle():
 def test_sizes():
     lib = capi.load()
     assert [lib.nt_int8_pitch(f) for f in (1, 127, 128, 129, 14336)] == [128, 128, 128, 256, 14336]
+    assert lib.nt_int8_rows_bytes(17, 129) == 32 * 256 and lib.nt_int8_rows_bytes(0, 5) == 0
+    assert lib.nt_int8_rows_bytes(-1, 5) == 0
     assert lib.nt_int8_weight_bytes(3, 129, 65) == 3 * 256 * 128
     assert lib.nt_int8_weight_bytes(0, 128, 64) == 0
     assert lib.nt_int8_weight_bytes(1025, 128, 64) == 0
@@ -71,7 +73,7 @@ MAX_K = capi.NT_INT8_MAX_K
     ("nt_int8_rows", (BF, P, 4, 8, P + 8, P, None), capi.NT_ERR_INVALID_ARG),
     ("nt_int8_rows", (BF, P, 4, 8, P, None, None), capi.NT_ERR_INVALID_ARG),
     ("nt_int8_rows", (BF, P, 4, MAX_K + 1, P, P, None), capi.NT_ERR_TOO_LARGE),
-    ("nt_int8_rows", (BF, P, 2**31, 8, P, P, None), capi.NT_ERR_TOO_LARGE),
+    ("nt_int8_rows", (BF, P, 2**24, 8, P, P, None), capi.NT_ERR_TOO_LARGE),
     ("nt_int8_rows", (BF, None, 0, 8, None, None, None), capi.NT_OK),
     ("nt_int8_rows_decode", (9, P, P, 4, 8, P, None), capi.NT_ERR_DTYPE),
     ("nt_int8_rows_decode", (BF, P, P, 4, 8, None, None), capi.NT_ERR_INVALID_ARG),
@@ -103,7 +105,7 @@ def _gemm(**over):
     (dict(A=-1), capi.NT_ERR_INVALID_ARG), (dict(K=0), capi.NT_ERR_INVALID_ARG),
     (dict(N=0), capi.NT_ERR_INVALID_ARG), (dict(E=1025), capi.NT_ERR_TOO_MANY_EXPERTS),
     (dict(K=MAX_K + 1), capi.NT_ERR_TOO_LARGE), (dict(N=2**22 + 1), capi.NT_ERR_TOO_LARGE),
-    (dict(A=2**31), capi.NT_ERR_TOO_LARGE), (dict(offsets=None), capi.NT_ERR_INVALID_ARG),
+    (dict(A=2**24), capi.NT_ERR_TOO_LARGE), (dict(offsets=None), capi.NT_ERR_INVALID_ARG),
     (dict(x=None), capi.NT_ERR_INVALID_ARG), (dict(x=P + 8), capi.NT_ERR_INVALID_ARG),
     (dict(xs=None), capi.NT_ERR_INVALID_ARG), (dict(w=None), capi.NT_ERR_INVALID_ARG),
     (dict(w=P + 1), capi.NT_ERR_INVALID_ARG), (dict(ws=None), capi.NT_ERR_INVALID_ARG),
