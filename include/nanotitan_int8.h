@@ -76,6 +76,29 @@ int nt_int8_grouped_gemm_gelu(int dtype, const int8_t* x, const float* x_scales,
                               int32_t E, int64_t A, int64_t K, int64_t N, void* act,
                               void* act_grad, hipStream_t stream);
 
+/* Gradients through frozen 8-bit weights, for f16 and bf16 rows and N a multiple of 8
+ * (otherwise: nt_int8_weight_decode and nt_grouped_gemm_dx); dout 16-byte aligned. The
+ * rounding of x to 8 bits is passed straight through; weights are the values held,
+ * rounded to dtype. dx = dout @ W[e]^T [A, K]; dx2: the sum of two such products;
+ * dx_gelu: dh = that times act_grad; dx_swiglu: dgate and dvalue of dhidden = that,
+ * with gate and value as the forward kept them, all [A, K]. Sums and epilogues in
+ * float32, one rounding. */
+int nt_int8_grouped_gemm_dx(int dtype, const int8_t* w, const float* w_scales,
+                            const int32_t* offsets, const void* dout, int32_t E, int64_t A,
+                            int64_t K, int64_t N, void* dx, hipStream_t stream);
+int nt_int8_grouped_gemm_dx2(int dtype, const int8_t* w1, const float* scales1, const int8_t* w2,
+                             const float* scales2, const int32_t* offsets, const void* dout1,
+                             const void* dout2, int32_t E, int64_t A, int64_t K, int64_t N,
+                             void* dx, hipStream_t stream);
+int nt_int8_grouped_gemm_dx_gelu(int dtype, const int8_t* w, const float* w_scales,
+                                 const int32_t* offsets, const void* dout, const void* act_grad,
+                                 int32_t E, int64_t A, int64_t K, int64_t N, void* dh,
+                                 hipStream_t stream);
+int nt_int8_grouped_gemm_dx_swiglu(int dtype, const int8_t* w, const float* w_scales,
+                                   const int32_t* offsets, const void* dout, const void* gate,
+                                   const void* value, int32_t E, int64_t A, int64_t K, int64_t N,
+                                   void* dgate, void* dvalue, hipStream_t stream);
+
 /* nt_moe_few_tokens on 8-bit weights (w_val NULL: GELU): tokens and hidden values go
  * to 8 bits row by row, the hidden ones from their values in dtype. Everything else,
  * the limits of sizes and the workspace's rules are nt_moe_few_tokens'; d, f <=

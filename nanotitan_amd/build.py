@@ -36,7 +36,7 @@ HIP_SOURCES = ["library.hip", "router.hip", "router_linear.hip", "dispatch.hip",
                "combine.hip", "grouped_gemm.hip", "staged_gemm.hip", "block_norm.hip",
                "block_norm_backward.hip", "checkpoint8.hip", "few_tokens.hip"]
 # The 8-bit integer experts and linear layers (include/nanotitan_int8.h), of the same library.
-INT8_SOURCES = ["int8_rows.hip", "int8_gemm.hip", "int8_few.hip"]
+INT8_SOURCES = ["int8_rows.hip", "int8_gemm.hip", "int8_few.hip", "int8_grad.hip"]
 OFFLOAD_ARCH = "gfx950"
 ROCM = Path(os.environ.get("ROCM_PATH", "/opt/rocm"))
 

@@ -208,7 +208,7 @@ EXPORTS: dict[str, tuple[object, list[object]]] = {
 }
 
 # include/nanotitan_int8.h
-NT_INT8_MAX_K = 1 << 17
+NT_INT8_MAX_K, NT_INT8_MAX_ROWS = 1 << 17, (1 << 24) - 1
 INT8_EXPORTS: dict[str, tuple[object, list[object]]] = {
     "nt_int8_pitch": (c_int64, [c_int64]),
     "nt_int8_rows_bytes": (c_size_t, [c_int64, c_int64]),
@@ -230,6 +230,18 @@ INT8_EXPORTS: dict[str, tuple[object, list[object]]] = {
     "nt_int8_grouped_gemm_gelu": (
         c_int,
         [c_int, _P, _P, _P, _P, _P, c_int32, c_int64, c_int64, c_int64, _P, _P, _P],
+    ),
+    "nt_int8_grouped_gemm_dx": (
+        c_int, [c_int, _P, _P, _P, _P, c_int32, c_int64, c_int64, c_int64, _P, _P]),
+    "nt_int8_grouped_gemm_dx2": (
+        c_int,
+        [c_int, _P, _P, _P, _P, _P, _P, _P, c_int32, c_int64, c_int64, c_int64, _P, _P],
+    ),
+    "nt_int8_grouped_gemm_dx_gelu": (
+        c_int, [c_int, _P, _P, _P, _P, _P, c_int32, c_int64, c_int64, c_int64, _P, _P]),
+    "nt_int8_grouped_gemm_dx_swiglu": (
+        c_int,
+        [c_int, _P, _P, _P, _P, _P, _P, c_int32, c_int64, c_int64, c_int64, _P, _P, _P],
     ),
     "nt_int8_moe_few_tokens_workspace_bytes": (
         c_size_t, [c_int, c_int64, c_int32, c_int32, c_int64, c_int64]),

@@ -112,7 +112,8 @@ __device__ __forceinline__ void int8_store(const i32x4 (&acc)[AB][EPI == kInt8Sw
                                               sw[MATS - 1][j] * sx
                                         : 0.f,
                               o[0][j], o[1][j], o[2][j]);
-      int8_put<T, EPI>(a, row * a.N + n, (int)(a.N - n < 16 ? a.N - n : 16), o);
+      int8_put<T, EPI == kInt8Plain ? 1 : EPI == kInt8SwiGLU ? 3 : 2>(
+          a, row * a.N + n, (int)(a.N - n < 16 ? a.N - n : 16), o);
     }
   }
 }

@@ -104,13 +104,12 @@ __device__ __forceinline__ void int8_epilogue(float p, float p2, typename elem<T
 }
 
 // n (at most 16) neighbouring columns of every output, at element `at`.
-template <typename T, int EPI>
+template <typename T, int OUTS>
 __device__ __forceinline__ void int8_put(const Int8Gemm& a, int64_t at, int n,
                                          const typename elem<T>::storage (&o)[3][16]) {
   typedef typename elem<T>::storage S;
-  constexpr int kOuts = EPI == kInt8Plain ? 1 : EPI == kInt8SwiGLU ? 3 : 2;
 #pragma unroll
-  for (int i = 0; i < kOuts; ++i) {
+  for (int i = 0; i < OUTS; ++i) {
     S* p = static_cast<S*>(i == 0 ? a.out : i == 1 ? a.out2 : a.out3);
     if (i > 0 && p == nullptr) continue;
     p += at;
@@ -126,6 +125,22 @@ __device__ __forceinline__ void int8_put(const Int8Gemm& a, int64_t at, int n,
       for (int j = 0; j < 16; ++j)
         if (j < n) p[j] = o[i][j];
     }
+  }
+}
+
+// n (at most 16) neighbouring values from element `at` on, zeros behind them.
+template <typename T>
+__device__ __forceinline__ void int8_get(const void* p, int64_t at, int n,
+                                         typename elem<T>::storage (&v)[16]) {
+  typedef typename elem<T>::storage S;
+  typedef S V __attribute__((ext_vector_type(16), aligned(sizeof(S))));
+  const S* s = static_cast<const S*>(p) + at;
+  if (n == 16) {
+    const V u = *reinterpret_cast<const V*>(s);
+    __builtin_memcpy(v, &u, sizeof(v));
+  } else {
+#pragma unroll
+    for (int j = 0; j < 16; ++j) v[j] = j < n ? s[j] : S(0);
   }
 }
 

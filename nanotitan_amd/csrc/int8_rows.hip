@@ -255,57 +255,87 @@ __global__ void __launch_bounds__(kThreads) int8_zero_kernel(uint32_t* p, int64_
   if (i < n) p[i] = 0;
 }
 
-// Maxima of 256 columns over `span` reduction rows: a thread has four columns, its
-// wave 64 rows apart. Grid: column blocks, row spans, experts.
-constexpr int kMostCols = 256;
+// Maxima of `span` reduction rows: a lane has 16 bytes of columns (kMostBytes a
+// wave), its workgroup's waves are rows apart. Grid: column blocks, row spans,
+// experts.
+constexpr int kMostBytes = kWave * 16;
 template <typename T>
 __global__ void __launch_bounds__(kThreads) int8_most_kernel(const void* W, int64_t K, int64_t N,
-                                                             int64_t span, uint32_t* most) {
+                                                             int64_t span,
+                                                             uint32_t* most) {
   typedef typename elem<T>::storage S;
-  typedef S V4 __attribute__((ext_vector_type(4), aligned(sizeof(S))));
-  const int64_t e = blockIdx.z, n = (int64_t)blockIdx.x * kMostCols + lane_id() * 4;
+  constexpr int kCols = 16 / sizeof(S);
+  typedef S V __attribute__((ext_vector_type(kCols), aligned(sizeof(S))));
+  const int64_t e = blockIdx.z;
+  const int64_t n = ((int64_t)blockIdx.x * kWave + lane_id()) * kCols;
   const int64_t k0 = (int64_t)blockIdx.y * span, k1 = k0 + span < K ? k0 + span : K;
-  if (n >= N) return;
+  __shared__ uint32_t s_most[kThreads / kWave][kCols * kWave];
   const S* w = static_cast<const S*>(W) + e * K * N + n;
-  uint32_t m[4] = {0, 0, 0, 0};
+  uint32_t m[kCols];
+#pragma unroll
+  for (int j = 0; j < kCols; ++j) m[j] = 0;
   auto take = [&](int j, S v) {
     const uint32_t b = abs_bits(elem<T>::load(v));
     m[j] = b > m[j] ? b : m[j];
   };
-  if (n + 4 <= N) {
-#pragma unroll 8
+  if (n + kCols <= N) {
+#pragma unroll 16
     for (int64_t k = k0 + threadIdx.x / kWave; k < k1; k += kThreads / kWave) {
-      const V4 v = *reinterpret_cast<const V4*>(w + k * N);
+      const V v = *reinterpret_cast<const V*>(w + k * N);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) take(j, v[j]);
+      for (int j = 0; j < kCols; ++j) take(j, v[j]);
     }
-  } else {
+  } else if (n < N) {
     for (int64_t k = k0 + threadIdx.x / kWave; k < k1; k += kThreads / kWave)
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
+      for (int j = 0; j < kCols; ++j)
         if (n + j < N) take(j, w[k * N + j]);
   }
+  // the waves' maxima: one atomic a column of the workgroup
 #pragma unroll
-  for (int j = 0; j < 4; ++j)
-    if (n + j < N) atomicMax(&most[e * N + n + j], m[j]);
+  for (int j = 0; j < kCols; ++j) s_most[threadIdx.x / kWave][j * kWave + lane_id()] = m[j];
+  __syncthreads();
+  for (int i = threadIdx.x; i < kCols * kWave; i += kThreads) {
+    const int64_t col = ((int64_t)blockIdx.x * kWave + i % kWave) * kCols + i / kWave;
+    uint32_t top = s_most[0][i];
+#pragma unroll
+    for (int u = 1; u < kThreads / kWave; ++u) top = s_most[u][i] > top ? s_most[u][i] : top;
+    if (col < N) atomicMax(&most[e * N + col], top);
+  }
 }
 
 // Bytes of a block in LDS: [64 columns][64 reduction rows], a column's 64 bytes
 // padded to 80, so that 16-byte reads stay aligned and columns spread over banks.
 constexpr int kTurnPitch = 80;
+constexpr int kRun = 4;  // blocks of a workgroup along the reduction, loaded at once
 
-// A 64x64 block to integers. Grid: column groups, reduction blocks, experts.
+// 64 columns by 256 reduction rows to integers. Grid: column groups, runs of blocks,
+// experts.
 template <typename T>
 __global__ void __launch_bounds__(kThreads) int8_weight_kernel(const void* W, int64_t K, int64_t N,
                                                                const uint32_t* most, int8_t* codes,
                                                                float* scales) {
   typedef typename elem<T>::storage S;
   typedef S V4 __attribute__((ext_vector_type(4), aligned(sizeof(S))));
-  __shared__ __attribute__((aligned(16))) int8_t s_turn[kInt8Block * kTurnPitch];
+  constexpr float kMagic = 12582912.f;  // see Sixteen::codes
+  __shared__ __attribute__((aligned(16))) int8_t s_turn[2][kInt8Block * kTurnPitch];
   const int64_t e = blockIdx.z, n0 = (int64_t)blockIdx.x * kInt8Block;
-  const int64_t k0 = (int64_t)blockIdx.y * kInt8Block;
+  const int64_t blocks = int8_pitch(K) / kInt8Block, b0 = (int64_t)blockIdx.y * kRun;
   const int c = threadIdx.x % 16 * 4, r = threadIdx.x / 16 * 4;
   const S* w = static_cast<const S*>(W) + e * K * N + n0 + c;
+  V4 v[kRun][4];
+#pragma unroll
+  for (int u = 0; u < kRun; ++u)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int64_t k = (b0 + u) * kInt8Block + r + i;
+      if (k < K && n0 + c + 4 <= N) {
+        v[u][i] = *reinterpret_cast<const V4*>(w + k * N);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[u][i][j] = k < K && n0 + c + j < N ? w[k * N + j] : S(0);
+      }
+    }
   float s[4], inv[4];
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
@@ -313,32 +343,39 @@ __global__ void __launch_bounds__(kThreads) int8_weight_kernel(const void* W, in
     inv[j] = int8_inverse(s[j]);
     if (blockIdx.y == 0 && r == 0 && n0 + c + j < N) scales[e * N + n0 + c + j] = s[j];
   }
-  int q[4][4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    V4 v;
-    const int64_t k = k0 + r + i;
-    if (k < K && n0 + c + 4 <= N) {
-      v = *reinterpret_cast<const V4*>(w + k * N);
-    } else {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) v[j] = k < K && n0 + c + j < N ? w[k * N + j] : S(0);
-    }
-#pragma unroll
-    for (int j = 0; j < 4; ++j) q[i][j] = int8_code(elem<T>::load(v[j]), s[j], inv[j]);
-  }
-#pragma unroll
-  for (int j = 0; j < 4; ++j)
-    *reinterpret_cast<uint32_t*>(s_turn + (c + j) * kTurnPitch + r) =
-        pack_bytes(q[0][j], q[1][j], q[2][j], q[3][j]);
-  __syncthreads();
   // thread: operand t, lane (g, i)
-  const int t = threadIdx.x / kWave, g = threadIdx.x % kWave / 16, i = threadIdx.x % 16;
-  const int col = 16 * (i / 4) + 4 * t + i % 4;
-  const int64_t block = (e * int8_groups(N) + blockIdx.x) * (int8_pitch(K) / kInt8Block) +
-                        blockIdx.y;
-  *reinterpret_cast<uint4*>(codes + block * kInt8Block * kInt8Block + threadIdx.x * 16) =
-      *reinterpret_cast<const uint4*>(s_turn + col * kTurnPitch + g * 16);
+  const int t = threadIdx.x / kWave, g = threadIdx.x % kWave / 16, i16 = threadIdx.x % 16;
+  const int col = 16 * (i16 / 4) + 4 * t + i16 % 4;
+  int8_t* out = codes + ((e * int8_groups(N) + blockIdx.x) * blocks + b0) * 4096 + threadIdx.x * 16;
+#pragma unroll
+  for (int u = 0; u < kRun; ++u) {
+    if (b0 + u >= blocks) break;
+    int8_t* turn = s_turn[u & 1];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      uint32_t sum[4];
+      float off = 0.f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float x = elem<T>::load(v[u][i][j]), near = fmaf(x, inv[j], kMagic);
+        off = fmaxf(off, fabsf(fmaf(kMagic - near, s[j], x)));
+        sum[i] = __float_as_uint(near);
+      }
+      uint32_t word = __builtin_amdgcn_perm(__builtin_amdgcn_perm(sum[3], sum[2], 0x0c0c0400u),
+                                            __builtin_amdgcn_perm(sum[1], sum[0], 0x0c0c0400u),
+                                            0x05040100u);
+      if (!(off < 0.5f * s[j]) || inv[j] == 0.f) {
+        int q[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) q[i] = int8_code(elem<T>::load(v[u][i][j]), s[j], inv[j]);
+        word = pack_bytes(q[0], q[1], q[2], q[3]);
+      }
+      *reinterpret_cast<uint32_t*>(turn + (c + j) * kTurnPitch + r) = word;
+    }
+    __syncthreads();
+    *reinterpret_cast<uint4*>(out + u * 4096) =
+        *reinterpret_cast<const uint4*>(turn + col * kTurnPitch + g * 16);
+  }
 }
 
 template <typename T>
@@ -484,13 +521,18 @@ int nt_int8_weight(int dtype, const void* W, int32_t E, int64_t K, int64_t N, in
                      dim3(kThreads), 0, stream, most, (int64_t)E * N);
   int8_by_type(dtype, [&](auto type) {
     typedef typename decltype(type)::type T;
-    const int64_t span = 256;
+    // Long spans for few atomics (they run at memory, not in an XCD's L2), but four
+    // workgroups a CU (both passes, 8 x 4,096 x 14,336 bf16: spans of 64 rows 551 us,
+    // 512 469, 2,048 580; 16 x 512 x 2,048: 31 and 63).
+    const int64_t cols = ceil_div(N * dtype_bytes(dtype), (int64_t)kMostBytes);
+    int64_t span = 1024;
+    while (span > 64 && E * cols * ceil_div(K, span) < 1024) span /= 2;
     hipLaunchKernelGGL((int8_most_kernel<T>),
-                       dim3((unsigned)ceil_div(N, (int64_t)kMostCols),
-                            (unsigned)ceil_div(K, span), (unsigned)E),
+                       dim3((unsigned)cols, (unsigned)ceil_div(K, span), (unsigned)E),
                        dim3(kThreads), 0, stream, W, K, N, span, most);
     hipLaunchKernelGGL((int8_weight_kernel<T>),
-                       dim3((unsigned)int8_groups(N), (unsigned)(int8_pitch(K) / kInt8Block),
+                       dim3((unsigned)int8_groups(N),
+                            (unsigned)ceil_div(int8_pitch(K), (int64_t)(kRun * kInt8Block)),
                             (unsigned)E),
                        dim3(kThreads), 0, stream, W, K, N, most, codes, scales);
   });

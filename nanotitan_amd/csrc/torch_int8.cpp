@@ -221,6 +221,88 @@ std::tuple<Tensor, OptTensor> int8_gelu_ffn(Tensor x, OptTensor offsets, Tensor 
   return {y, slope};
 }
 
+// Rows [A, N] of a gradient, or [A, K] of what the forward kept, for the 16-bit
+// products with the weights held.
+void check_grad(const Tensor& t, int64_t rows, int64_t cols, const Tensor& like,
+                const char* name) {
+  check_device(t, name);
+  check_same_device(like, {&t});
+  TORCH_CHECK(t.dim() == 2 && t.size(0) == rows && t.size(1) == cols && t.is_contiguous() &&
+                  t.scalar_type() == like.scalar_type(),
+              name, " must be a contiguous [", rows, ", ", cols, "] of ", like.scalar_type());
+}
+struct GradIn {
+  Weight w;
+  const int32_t* off;
+  int64_t A;
+};
+GradIn check_dx(const Tensor& dout, const OptTensor& offsets, const Tensor& codes,
+                const Tensor& scales, int64_t K) {
+  check_device(dout, "dOut");
+  TORCH_CHECK(dout.dim() == 2 && (dout.scalar_type() == at::kHalf ||
+                                  dout.scalar_type() == at::kBFloat16),
+              "dOut must be [rows, columns] of float16 or bfloat16");
+  const Weight w = check_weight(codes, scales, K, dout, "weight");
+  TORCH_CHECK(w.N % 8 == 0, "dOut must have a multiple of 8 columns");
+  check_grad(dout, dout.size(0), w.N, dout, "dOut");
+  TORCH_CHECK(reinterpret_cast<uintptr_t>(dout.data_ptr()) % 16 == 0,
+              "dOut must be 16-byte aligned");
+  return {w, check_offsets(offsets, dout, w.E), dout.size(0)};
+}
+
+// int8_dx(dOut, offsets, codes, scales, K) -> dOut @ W^T; int8_dx2: the sum of two.
+Tensor int8_dx(Tensor dout, OptTensor offsets, Tensor codes, Tensor scales, int64_t K) {
+  const GradIn g = check_dx(dout, offsets, codes, scales, K);
+  c10::hip::HIPGuard guard(dout.get_device());
+  Tensor dx = at::empty({g.A, K}, dout.options());
+  check_status(nt_int8_grouped_gemm_dx(dtype_code(dout), g.w.codes, g.w.scales, g.off,
+                                       dout.data_ptr(), g.w.E, g.A, K, g.w.N, dx.data_ptr(),
+                                       stream_of(dout)),
+               "int8_dx");
+  return dx;
+}
+Tensor int8_dx2(Tensor dout1, Tensor dout2, OptTensor offsets, Tensor c1, Tensor s1, Tensor c2,
+                Tensor s2, int64_t K) {
+  const GradIn g = check_dx(dout1, offsets, c1, s1, K), h = check_dx(dout2, offsets, c2, s2, K);
+  check_grad(dout2, g.A, g.w.N, dout1, "dOut2");
+  TORCH_CHECK(h.w.E == g.w.E && h.w.N == g.w.N, "the two weights must be alike");
+  c10::hip::HIPGuard guard(dout1.get_device());
+  Tensor dx = at::empty({g.A, K}, dout1.options());
+  check_status(nt_int8_grouped_gemm_dx2(dtype_code(dout1), g.w.codes, g.w.scales, h.w.codes,
+                                        h.w.scales, g.off, dout1.data_ptr(), dout2.data_ptr(),
+                                        g.w.E, g.A, K, g.w.N, dx.data_ptr(), stream_of(dout1)),
+               "int8_dx2");
+  return dx;
+}
+// The same before an activation's gradient: dh, or (dgate, dvalue).
+Tensor int8_dx_gelu(Tensor dout, Tensor slope, OptTensor offsets, Tensor codes, Tensor scales,
+                    int64_t K) {
+  const GradIn g = check_dx(dout, offsets, codes, scales, K);
+  check_grad(slope, g.A, K, dout, "gelu'");
+  c10::hip::HIPGuard guard(dout.get_device());
+  Tensor dh = at::empty_like(slope);
+  check_status(nt_int8_grouped_gemm_dx_gelu(dtype_code(dout), g.w.codes, g.w.scales, g.off,
+                                            dout.data_ptr(), slope.data_ptr(), g.w.E, g.A, K,
+                                            g.w.N, dh.data_ptr(), stream_of(dout)),
+               "int8_dx_gelu");
+  return dh;
+}
+std::tuple<Tensor, Tensor> int8_dx_swiglu(Tensor dout, Tensor gate, Tensor value,
+                                          OptTensor offsets, Tensor codes, Tensor scales,
+                                          int64_t K) {
+  const GradIn g = check_dx(dout, offsets, codes, scales, K);
+  check_grad(gate, g.A, K, dout, "gate");
+  check_grad(value, g.A, K, dout, "value");
+  c10::hip::HIPGuard guard(dout.get_device());
+  Tensor dgate = at::empty_like(gate), dvalue = at::empty_like(gate);
+  check_status(nt_int8_grouped_gemm_dx_swiglu(dtype_code(dout), g.w.codes, g.w.scales, g.off,
+                                              dout.data_ptr(), gate.data_ptr(), value.data_ptr(),
+                                              g.w.E, g.A, K, g.w.N, dgate.data_ptr(),
+                                              dvalue.data_ptr(), stream_of(dout)),
+               "int8_dx_swiglu");
+  return {dgate, dvalue};
+}
+
 // int8_moe_few_tokens(x, up, value and down weights, top_k, router, logits) -> (out,
 // gates, topk): moe_few_tokens on 8-bit weights.
 std::tuple<Tensor, Tensor, Tensor> int8_moe_few_tokens(Tensor x, Tensor wu, Tensor su,
@@ -276,6 +358,10 @@ void bind_int8(py::module& m) {
   m.def("int8_product", &int8_product, "Rows by 8-bit weights, grouped by expert");
   m.def("int8_swiglu_ffn", &int8_swiglu_ffn, "SwiGLU FFN on 8-bit weights -> (y, gate, value)");
   m.def("int8_gelu_ffn", &int8_gelu_ffn, "GELU FFN on 8-bit weights -> (y, gelu')");
+  m.def("int8_dx", &int8_dx, "Gradient rows by 8-bit weights, transposed");
+  m.def("int8_dx2", &int8_dx2, "The sum of two such products");
+  m.def("int8_dx_gelu", &int8_dx_gelu, "Such a product times gelu'");
+  m.def("int8_dx_swiglu", &int8_dx_swiglu, "Such a product by SwiGLU's gradient -> (dgate, dvalue)");
   m.def("int8_moe_few_tokens", &int8_moe_few_tokens,
         "A whole MoE layer for few tokens on 8-bit weights -> (out, gates, topk)");
 }

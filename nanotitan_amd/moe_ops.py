@@ -845,11 +845,32 @@ def _all_rows(x, expert_offset):
     return torch.arange(2, dtype=torch.int32, device=x.device) * x.shape[0]
 
 
+def _int8_direct(dout):
+    """Whether the kernels that read 8-bit weights take this gradient; else the weights go to
+    its dtype first."""
+    return dout.dtype != torch.float32 and dout.shape[1] % 8 == 0
+
+
+def _aligned(t):
+    """A contiguous t that starts at a multiple of 16 bytes."""
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def _int8_dx(dout, off, codes, scale, K):
+    """dout @ W^T for the weights [E,K,N] that codes and scale hold."""
+    ext = get_hip_extension()
+    if _int8_direct(dout):
+        return ext.int8_dx(_aligned(dout), off, codes, scale, K)
+    W = ext.int8_weight_decode(codes, scale, K, dout.dtype)
+    return ext.bwd_grouped_gemm_dX_kernel(W, _all_rows(dout, off), dout.contiguous())
+
+
 class Int8GroupedGEMM_FN(torch.autograd.Function):
     """X by frozen 8-bit weights; the gradient to X is dOut times the weights held, transposed.
 
-    The rounding of X is passed straight through. Weights go to dOut's dtype for the backward's
-    product (a rounding of 16-bit types, as small as the output's own).
+    The rounding of X is passed straight through. The backward's product takes the weights in
+    dOut's dtype (a rounding of 16-bit types, as small as the output's own).
     """
 
     @staticmethod
@@ -861,17 +882,15 @@ class Int8GroupedGEMM_FN(torch.autograd.Function):
     @staticmethod
     @_once_differentiable
     def backward(ctx, dout):
-        ext = get_hip_extension()
         off, codes, scale = ctx.saved_tensors
-        W = ext.int8_weight_decode(codes, scale, ctx.shape[1], dout.dtype)
-        return ext.bwd_grouped_gemm_dX_kernel(W, _all_rows(dout, off), dout.contiguous()), None, None
+        return _int8_dx(dout, off, codes, scale, ctx.shape[1]), None, None
 
 
 class Int8SwiGLUFFN_FN(torch.autograd.Function):
     """SwiGLU FFN on frozen 8-bit weights, with the gradient to X.
 
     Keeps gate and value in X's dtype; the rounding of X and of the hidden values is passed
-    straight through, and the weights held go to dy's dtype for the backward's products.
+    straight through, and the backward's products take the weights held in dy's dtype.
     """
 
     @staticmethod
@@ -889,11 +908,18 @@ class Int8SwiGLUFFN_FN(torch.autograd.Function):
         ext = get_hip_extension()
         off, gate, value, gc, gs, vc, vs, oc, os = ctx.saved_tensors
         _, d, f = ctx.shape
-        off = _all_rows(dy, off)
-        dg, dv = ext.bwd_grouped_gemm_dX_swiglu(ext.int8_weight_decode(oc, os, f, dy.dtype), off,
-                                                dy.contiguous(), gate, value)
-        dX = ext.bwd_grouped_gemm_dX2(ext.int8_weight_decode(gc, gs, d, dy.dtype),
-                                      ext.int8_weight_decode(vc, vs, d, dy.dtype), off, dg, dv)
+        if _int8_direct(dy):
+            dg, dv = ext.int8_dx_swiglu(_aligned(dy), gate, value, off, oc, os, f)
+        else:
+            dg, dv = ext.bwd_grouped_gemm_dX_swiglu(
+                ext.int8_weight_decode(oc, os, f, dy.dtype), _all_rows(dy, off), dy.contiguous(),
+                gate, value)
+        if _int8_direct(dg):
+            dX = ext.int8_dx2(dg, dv, off, gc, gs, vc, vs, d)
+        else:
+            dX = ext.bwd_grouped_gemm_dX2(
+                ext.int8_weight_decode(gc, gs, d, dy.dtype),
+                ext.int8_weight_decode(vc, vs, d, dy.dtype), _all_rows(dy, off), dg, dv)
         return dX, None, None, None, None
 
 
@@ -914,10 +940,12 @@ class Int8GeluFFN_FN(torch.autograd.Function):
         ext = get_hip_extension()
         off, slope, uc, us, dc, ds = ctx.saved_tensors
         _, d, f = ctx.shape
-        off = _all_rows(dy, off)
-        dh = ext.bwd_grouped_gemm_dX_gelu(ext.int8_weight_decode(dc, ds, f, dy.dtype), off,
-                                          dy.contiguous(), slope)
-        dX = ext.bwd_grouped_gemm_dX_kernel(ext.int8_weight_decode(uc, us, d, dy.dtype), off, dh)
+        if _int8_direct(dy):
+            dh = ext.int8_dx_gelu(_aligned(dy), slope, off, dc, ds, f)
+        else:
+            dh = ext.bwd_grouped_gemm_dX_gelu(ext.int8_weight_decode(dc, ds, f, dy.dtype),
+                                              _all_rows(dy, off), dy.contiguous(), slope)
+        dX = _int8_dx(dh, off, uc, us, d)
         return dX, None, None, None
 
 

@@ -265,10 +265,11 @@ def _held_weights(ws):
 
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("counts", ["few", "mixed", "wide", "dense"])
-def test_product_gradient(dtype, counts):
+@pytest.mark.parametrize("K,N", [(300, 264), (65, 8), (1030, 72), (130, 77), (256, 640)])
+def test_product_gradient(dtype, counts, K, N):
     t = TYPES[dtype]
     off, gpu_off = ([0, 19], None) if counts == "dense" else _offsets(COUNTS[counts])
-    E, A, K, N = len(off) - 1, off[-1], 300, 264
+    E, A = len(off) - 1, off[-1]
     x = _rand(A, K, dtype=t, seed=1).requires_grad_()
     w, _, _ = _weights(E, K, N, 2)
     dout = _rand(A, N, dtype=t, seed=3)
@@ -290,11 +291,12 @@ def test_product_gradient(dtype, counts):
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("ffn", ["swiglu", "gelu"])
 @pytest.mark.parametrize("counts", ["few", "mixed", "wide", "dense"])
-def test_block_gradient(dtype, ffn, counts):
+@pytest.mark.parametrize("d,f", [(128, 264), (72, 333), (77, 256), (300, 520)])
+def test_block_gradient(dtype, ffn, counts, d, f):
     """dX against the formula in 64 bits, and that against differences."""
     t = TYPES[dtype]
     off, gpu_off = ([0, 19], None) if counts == "dense" else _offsets(COUNTS[counts])
-    E, A, d, f = len(off) - 1, off[-1], 128, 264
+    E, A = len(off) - 1, off[-1]
     x = _rand(A, d, dtype=t, seed=1).requires_grad_()
     up = [_weights(E, d, f, 2 + i)[0] for i in range(2 if ffn == "swiglu" else 1)]
     down = _weights(E, f, d, 5)[0]
@@ -323,6 +325,54 @@ def test_block_gradient(dtype, ffn, counts):
     # a half steps; float32's sums of up to 264 terms to below 64 of its own.
     steps = 3 if t != torch.float32 else 64
     assert float((x.grad.cpu().double() - want).norm()) <= steps * _steps(t) * float(want.norm())
+
+
+def test_gradient_rows_behind_the_last_stay():
+    E, K, N, rows, A = 3, 200, 136, 150, 180
+    _, off = _offsets([100, 0, 50])
+    w, _, _ = _weights(E, K, N, 4)
+    dout = _rand(A, N, dtype=torch.bfloat16, seed=1)
+    kept = [_rand(A, K, dtype=torch.bfloat16, seed=i) for i in (2, 3)]
+    outs = [torch.full((A, K), 7.0, dtype=torch.bfloat16, device="cuda") for _ in range(5)]
+    head = [capi.NT_BF16, w.codes.data_ptr(), w.scale.data_ptr()]
+    tail, s = [E, A, K, N], capi.current_stream()
+    o, d, k = off.data_ptr(), dout.data_ptr(), [t.data_ptr() for t in kept]
+    p = [t.data_ptr() for t in outs]
+    capi.call("nt_int8_grouped_gemm_dx", *head, o, d, *tail, p[0], s)
+    capi.call("nt_int8_grouped_gemm_dx2", *head, *head[1:], o, d, d, *tail, p[1], s)
+    capi.call("nt_int8_grouped_gemm_dx_gelu", *head, o, d, k[0], *tail, p[2], s)
+    capi.call("nt_int8_grouped_gemm_dx_swiglu", *head, o, d, *k, *tail, p[3], p[4], s)
+    for t in outs:
+        assert bool((t[rows:] == 7.0).all()) and not bool((t[:rows] == 7.0).all())
+
+
+def test_gradient_of_any_alignment_and_layout():
+    w, _, _ = _weights(1, 100, 64, 0)
+    x = _rand(33, 100, dtype=torch.bfloat16).requires_grad_()
+    dout = _rand(33, 64, dtype=torch.bfloat16, seed=1)
+    want, = torch.autograd.grad(int8_grouped_gemm_fn(x, w), x, dout)
+    buf = torch.empty(33 * 64 + 3, dtype=torch.bfloat16, device="cuda")
+    shifted = buf[3:].view(33, 64).copy_(dout)
+    turned = dout.t().contiguous().t()
+    for g in (shifted, turned):
+        got, = torch.autograd.grad(int8_grouped_gemm_fn(x, w), x, g)
+        assert torch.equal(got, want)
+
+
+def test_gradient_at_the_last_of_many_weights():
+    """The last expert's weights, past 2^32 bytes."""
+    E, K, N = 34, 16384, 8192
+    codes = torch.zeros(E, N // 64, K // 64, 4, 4, 16, 16, dtype=torch.int8, device="cuda")
+    codes[-1].random_(-127, 128)
+    scale = torch.rand(E, N, device="cuda")
+    off = torch.tensor([0] * E + [90], dtype=torch.int32, device="cuda")
+    x = _rand(90, K, dtype=torch.bfloat16).requires_grad_()
+    dout = _rand(90, N, dtype=torch.bfloat16, seed=1)
+    got, = torch.autograd.grad(int8_grouped_gemm_fn(x, Int8Weight(codes, scale, (E, K, N)), off),
+                               x, dout)
+    one = Int8Weight(codes[-1:].contiguous(), scale[-1:].contiguous(), (1, K, N))
+    want, = torch.autograd.grad(int8_grouped_gemm_fn(x, one), x, dout)
+    assert torch.equal(got, want)
 
 
 def test_gradients_are_once_differentiable_and_have_no_tangents():

@@ -128,6 +128,48 @@ def test_swiglu_refuses_half_of_a_pair():
         assert fn(*ins, w2, s2, 2, 4, 8, 8, P, gate, value, None) == capi.NT_ERR_INVALID_ARG
 
 
+def _grad(**over):
+    a = dict(dtype=BF, w=P, s=P, offsets=P, dout=P, E=2, A=4, K=9, N=16, out=P)
+    a.update(over)
+    return a
+
+
+@pytest.mark.parametrize("over,code", [
+    (dict(dtype=F32), capi.NT_ERR_DTYPE), (dict(E=0), capi.NT_ERR_INVALID_ARG),
+    (dict(A=-1), capi.NT_ERR_INVALID_ARG), (dict(K=0), capi.NT_ERR_INVALID_ARG),
+    (dict(N=12), capi.NT_ERR_INVALID_ARG), (dict(E=1025), capi.NT_ERR_TOO_MANY_EXPERTS),
+    (dict(K=MAX_K + 1), capi.NT_ERR_TOO_LARGE), (dict(N=2**20 + 8), capi.NT_ERR_TOO_LARGE),
+    (dict(A=2**24), capi.NT_ERR_TOO_LARGE), (dict(offsets=None), capi.NT_ERR_INVALID_ARG),
+    (dict(w=None), capi.NT_ERR_INVALID_ARG), (dict(w=P + 8), capi.NT_ERR_INVALID_ARG),
+    (dict(s=None), capi.NT_ERR_INVALID_ARG), (dict(dout=None), capi.NT_ERR_INVALID_ARG),
+    (dict(dout=P + 2), capi.NT_ERR_INVALID_ARG), (dict(out=None), capi.NT_ERR_INVALID_ARG),
+    (dict(A=0, dout=None, out=None), capi.NT_OK)])
+def test_gradients_refuse(over, code):
+    lib, a = capi.load(), _grad(**over)
+    head = [a[n] for n in ("dtype", "w", "s")]
+    sizes = [a[n] for n in ("E", "A", "K", "N")]
+    assert lib.nt_int8_grouped_gemm_dx(*head, a["offsets"], a["dout"], *sizes, a["out"],
+                                       None) == code
+    assert lib.nt_int8_grouped_gemm_dx2(*head, P, P, a["offsets"], a["dout"], P, *sizes, a["out"],
+                                        None) == code
+    assert lib.nt_int8_grouped_gemm_dx_gelu(*head, a["offsets"], a["dout"], P, *sizes, a["out"],
+                                            None) == code
+    assert lib.nt_int8_grouped_gemm_dx_swiglu(*head, a["offsets"], a["dout"], P, P, *sizes,
+                                              a["out"], P, None) == code
+
+
+def test_gradients_refuse_missing_inputs():
+    lib, a = capi.load(), _grad()
+    head, sizes = [BF, P, P], [2, 4, 9, 16]
+    bad = capi.NT_ERR_INVALID_ARG
+    assert lib.nt_int8_grouped_gemm_dx2(*head, None, P, P, P, P, *sizes, P, None) == bad
+    assert lib.nt_int8_grouped_gemm_dx2(*head, P, None, P, P, P, *sizes, P, None) == bad
+    assert lib.nt_int8_grouped_gemm_dx2(*head, P, P, P, P, P + 4, *sizes, P, None) == bad
+    assert lib.nt_int8_grouped_gemm_dx_gelu(*head, P, P, None, *sizes, P, None) == bad
+    assert lib.nt_int8_grouped_gemm_dx_swiglu(*head, P, P, P, None, *sizes, P, P, None) == bad
+    assert lib.nt_int8_grouped_gemm_dx_swiglu(*head, P, P, P, P, *sizes, P, None, None) == bad
+
+
 def _few(**over):
     a = dict(dtype=BF, x=P, router=P, logits=None, wu=P, su=P, wv=P, sv=P, wd=P, sd=P, T=4, E=8,
              k=2, d=64, f=128, gates=P, topk=P, out=P, ws=P, ws_bytes=2**30, stream=None)
