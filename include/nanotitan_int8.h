@@ -76,6 +76,22 @@ int nt_int8_grouped_gemm_gelu(int dtype, const int8_t* x, const float* x_scales,
                               int32_t E, int64_t A, int64_t K, int64_t N, void* act,
                               void* act_grad, hipStream_t stream);
 
+/* The same three from rows x [A, K] of dtype, which they bring to 8 bits themselves:
+ * the bits of nt_int8_rows and the product. The workspace (16-byte aligned, contents
+ * arbitrary) is written before it is read: calls that cannot overlap may share one. */
+size_t nt_int8_linear_workspace_bytes(int64_t A, int64_t K);
+int nt_int8_linear(int dtype, const void* x, const int32_t* offsets, const int8_t* w,
+                   const float* w_scales, int32_t E, int64_t A, int64_t K, int64_t N, void* out,
+                   void* ws, size_t ws_bytes, hipStream_t stream);
+int nt_int8_linear_swiglu(int dtype, const void* x, const int32_t* offsets, const int8_t* w_gate,
+                          const float* gate_scales, const int8_t* w_val, const float* val_scales,
+                          int32_t E, int64_t A, int64_t K, int64_t N, void* hidden, void* gate,
+                          void* value, void* ws, size_t ws_bytes, hipStream_t stream);
+int nt_int8_linear_gelu(int dtype, const void* x, const int32_t* offsets, const int8_t* w,
+                        const float* w_scales, int32_t E, int64_t A, int64_t K, int64_t N,
+                        void* act, void* act_grad, void* ws, size_t ws_bytes,
+                        hipStream_t stream);
+
 /* Gradients through frozen 8-bit weights, for f16 and bf16 rows and N a multiple of 8
  * (otherwise: nt_int8_weight_decode and nt_grouped_gemm_dx); dout 16-byte aligned. The
  * rounding of x to 8 bits is passed straight through; weights are the values held,

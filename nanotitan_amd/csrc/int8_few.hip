@@ -7,9 +7,13 @@
 // a column group's reduction and add their integer sums in LDS. Sums of integers are
 // exact, so neither the split nor the batch shows in a result.
 //
+// A few short rows are brought to integers by every workgroup for itself, in LDS: a
+// launch that did it would take longer than all of the product.
+//
 // The layer: routing and the tokens' integers (a workgroup a token); the up
 // projections with the activation; the hidden rows' integers; the down projection;
-// the gate-weighted sum.
+// the gate-weighted sum. For a few tokens both roundings are the products' own, and
+// who finishes the last expert's part of a column sums it.
 #include <algorithm>
 #include <type_traits>
 
@@ -30,6 +34,16 @@ struct Chosen {
   int32_t* inv;      // [T, k]: row of an assignment
 };
 struct NoChoice {};
+// The gate-weighted sum in the down projection: what its last workgroup for a part of
+// the columns needs. Of `arrived` a counter a part, zero at the start.
+struct Arrive {
+  const float* gates;
+  const int32_t* inv;
+  void* out;  // [T, N] of the hidden rows' type
+  int32_t* arrived;
+  int32_t T, k;
+};
+struct NoArrive {};
 
 struct StreamPlan {
   int32_t pref[NT_MAX_EXPERTS + 1];  // loads of the experts before e
@@ -78,8 +92,7 @@ __device__ __forceinline__ int nth_token(uint64_t mask, int r) {
 template <int MATS, int CT, int MT, int U>
 struct Stage {
   i32x4 w[U][MATS][CT], x[U][MT];
-  __device__ __forceinline__ void load(const int8_t* const (&wp)[MATS],
-                                       const int8_t* const (&xp)[MT], int kb) {
+  __device__ __forceinline__ void load_weights(const int8_t* const (&wp)[MATS], int kb) {
 #pragma unroll
     for (int u = 0; u < U; ++u)
 #pragma unroll
@@ -88,11 +101,21 @@ struct Stage {
         for (int t = 0; t < CT; ++t)
           w[u][i][t] = __builtin_nontemporal_load(reinterpret_cast<const i32x4*>(
               wp[i] + (int64_t)(kb + u) * (kInt8Block * kInt8Block) + t * 1024));
+  }
+  // xp: this lane's pieces, `step` bytes a block apart; in LDS or memory.
+  template <typename P>
+  __device__ __forceinline__ void load_rows(const P (&xp)[MT], int step, int kb) {
 #pragma unroll
     for (int u = 0; u < U; ++u)
 #pragma unroll
       for (int m = 0; m < MT; ++m)
-        x[u][m] = *reinterpret_cast<const i32x4*>(xp[m] + (int64_t)(kb + u) * 1024);
+        x[u][m] = *reinterpret_cast<const i32x4*>(xp[m] + (int64_t)(kb + u) * step);
+  }
+  template <typename P>
+  __device__ __forceinline__ void load(const int8_t* const (&wp)[MATS], const P (&xp)[MT],
+                                       int step, int kb) {
+    load_weights(wp, kb);
+    load_rows(xp, step, kb);
   }
   __device__ __forceinline__ void multiply(i32x4 (&acc)[MATS][CT][MT]) const {
 #pragma unroll
@@ -108,13 +131,61 @@ struct Stage {
   }
 };
 
+constexpr int kOwnRows = 8;  // rows that a workgroup brings to integers itself, at most
+
+// `rows` rows of f values to integers and scales in LDS, by the WAVES waves of a
+// workgroup, as many a row as there are: codes[k / 64][g][held][k % 16]. row(r):
+// where row r begins. Ends with a barrier.
+template <typename X, int WAVES, typename F>
+__device__ __forceinline__ void own_integers(F&& row, int rows, int64_t f, int held, char* codes,
+                                             uint32_t* s_most, float* s_scale) {
+  const int chunks = (int)(int8_pitch(f) / kVec), wave = threadIdx.x / kWave;
+  const int share = rows < WAVES ? WAVES / rows : 1;  // waves of a row
+  for (int r0 = 0; r0 < rows; r0 += WAVES) {
+    const int r = r0 + wave / share, c0 = wave % share * kWave + lane_id();
+    const bool live = r < rows;
+    Sixteen<X> v;
+    uint32_t m = 0;
+    if (live)
+      for (int c = c0; c < chunks; c += share * kWave) {
+        v.load(row(r), (int64_t)c * kVec, f);
+        const uint32_t most = v.most();
+        m = most > m ? most : m;
+      }
+#pragma unroll
+    for (int o = kWave / 2; o >= 1; o >>= 1) m = max(m, (uint32_t)__shfl_xor(m, o, kWave));
+    __syncthreads();  // the rows before, or the item before, are read no more
+    if (lane_id() == 0) s_most[wave] = m;
+    __syncthreads();
+    if (!live) continue;
+    for (int i = 0; i < share; ++i) m = max(m, s_most[wave / share * share + i]);
+    const float s = int8_scale(m), inv = int8_inverse(s);
+    if (c0 == 0) s_scale[r] = s;
+    const bool once = chunks <= share * kWave;  // then v still holds it
+    for (int c = c0; c < chunks; c += share * kWave) {
+      if (!once) v.load(row(r), (int64_t)c * kVec, f);
+      *reinterpret_cast<uint4*>(codes + (c * held + r) * 16) = v.codes(s, inv);
+    }
+  }
+  __syncthreads();
+}
+
 // CT of the four operands of a column group, up to 16 MT rows of one expert, for
-// the KW waves of a workgroup at a time.
-template <typename T, int EPI, int MT, int CT, int KW, int U, bool CHOSEN>
+// the KW waves of a workgroup at a time. X: the rows' values, of which `held` (at
+// most kOwnRows) rows an item come to integers here; or int8_t, integers.
+template <typename T, typename X, int EPI, int MT, int CT, int KW, int U, bool CHOSEN,
+          bool ARRIVE>
 __global__ void __launch_bounds__(KW* kWave)
-    int8_stream_kernel(Int8Gemm a, std::conditional_t<CHOSEN, Chosen, NoChoice> chosen) {
+    int8_stream_kernel(Int8Gemm a, std::conditional_t<CHOSEN, Chosen, NoChoice> chosen,
+                       std::conditional_t<ARRIVE, Arrive, NoArrive> arrive, int held) {
   typedef typename elem<T>::storage S;
   constexpr int MATS = EPI == kInt8SwiGLU ? 2 : 1, kRows = 16 * MT;
+  constexpr bool kOwn = !std::is_same<X, int8_t>::value;
+  static_assert(!kOwn || MT == 1, "a row tile's integers in LDS");
+  extern __shared__ __attribute__((aligned(16))) char s_codes[];
+  __shared__ uint32_t s_most[KW];
+  __shared__ float s_scale[kOwnRows];
+  __shared__ int32_t s_last;
   __shared__ std::conditional_t<CHOSEN, ChosenPlan, StreamPlan> s_plan;
   __shared__ __attribute__((aligned(16))) int32_t s_acc[KW * MATS * CT * kWave * 4];
   if constexpr (CHOSEN) make_chosen(chosen, a.E, kRows, s_plan);
@@ -138,33 +209,55 @@ __global__ void __launch_bounds__(KW* kWave)
     const int done = (load - s_plan.pref[e]) * kRows;
     int64_t row0;
     int rows;
-    const int8_t* xp[MT];
     if constexpr (CHOSEN) {
-      uint64_t mask = s_plan.mask[e];
       row0 = s_plan.first[e] + done;
-      rows = min(popc64(mask) - done, kRows);
-#pragma unroll
-      for (int m = 0; m < MT; ++m) {
-        const int r = m * 16 + (lane & 15);
-        xp[m] = a.x + int8_row(nth_token(mask, done + (r < rows ? r : 0)), pitch) +
-                (lane >> 4) * 256;
-      }
+      rows = min(popc64(s_plan.mask[e]) - done, kRows);
     } else {
       int64_t r0, r1;
       int8_expert_rows(a, e, r0, r1);
       row0 = r0 + done;
       rows = (int)(r1 - row0 < kRows ? r1 - row0 : kRows);
-#pragma unroll
-      for (int m = 0; m < MT; ++m) {
-        const int r = m * 16 + (lane & 15);
-        xp[m] = a.x + int8_row(row0 + (r < rows ? r : 0), pitch) + (lane >> 4) * 256;
-      }
     }
+    auto x_row = [&](int r) -> int64_t {  // of the item's row r
+      if constexpr (CHOSEN) return nth_token(s_plan.mask[e], done + r);
+      else return row0 + r;
+    };
     const int8_t* wp[MATS];
 #pragma unroll
     for (int i = 0; i < MATS; ++i)
       wp[i] = (i == 0 ? a.w : a.w2) + (e * groups + group) * kInt8Block * pitch + t0 * 1024 +
               lane * 16;
+    // this wave's blocks, a stage ahead in flight; the first and the columns' scales
+    // before anything is waited for
+    int kb = blocks * wave / KW;
+    const int kb1 = blocks * (wave + 1) / KW;
+    Stage<MATS, CT, MT, U> s0, s1;
+    if (kOwn && kb + U <= kb1) s0.load_weights(wp, kb);
+    float sw[MATS][4];
+    static_assert(CT <= KW, "a wave for each operand's columns at the end");
+    const int64_t n_mine =
+        group * kInt8Block + 16 * (lane >> 4) + 4 * (t0 + (wave < CT ? wave : 0));
+#pragma unroll
+    for (int i = 0; i < MATS; ++i)
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        sw[i][q] = n_mine + q < a.N ? (i == 0 ? a.w_scales : a.w2_scales)[e * a.N + n_mine + q] : 0.f;
+    if constexpr (kOwn) {
+      rows = min(rows, held);  // (what the caller promised)
+      own_integers<X, KW>(
+          [&](int r) {
+            return static_cast<const typename elem<X>::storage*>(a.values) + x_row(r) * a.K;
+          },
+          rows, a.K, held, s_codes, s_most, s_scale);
+    }
+    std::conditional_t<kOwn, const char*, const int8_t*> xp[MT];
+    const int step = kOwn ? 64 * held : 1024;
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+      const int r = m * 16 + (lane & 15), in = r < rows ? r : 0;
+      if constexpr (kOwn) xp[m] = s_codes + ((lane >> 4) * held + in) * 16;
+      else xp[m] = a.x + int8_row(x_row(in), pitch) + (lane >> 4) * 256;
+    }
     i32x4 acc[MATS][CT][MT];
 #pragma unroll
     for (int i = 0; i < MATS; ++i)
@@ -172,21 +265,18 @@ __global__ void __launch_bounds__(KW* kWave)
       for (int t = 0; t < CT; ++t)
 #pragma unroll
         for (int m = 0; m < MT; ++m) acc[i][t][m] = i32x4{0, 0, 0, 0};
-    // this wave's blocks, a stage ahead in flight
-    int kb = blocks * wave / KW;
-    const int kb1 = blocks * (wave + 1) / KW;
     if (kb + U <= kb1) {
-      Stage<MATS, CT, MT, U> s0, s1;
-      s0.load(wp, xp, kb);
+      if (!kOwn) s0.load_weights(wp, kb);
+      s0.load_rows(xp, step, kb);
       kb += U;
       for (; kb + 2 * U <= kb1; kb += 2 * U) {
-        s1.load(wp, xp, kb);
+        s1.load(wp, xp, step, kb);
         s0.multiply(acc);
-        s0.load(wp, xp, kb + U);
+        s0.load(wp, xp, step, kb + U);
         s1.multiply(acc);
       }
       const bool more = kb + U <= kb1;
-      if (more) s1.load(wp, xp, kb);
+      if (more) s1.load(wp, xp, step, kb);
       s0.multiply(acc);
       if (more) {
         s1.multiply(acc);
@@ -195,7 +285,7 @@ __global__ void __launch_bounds__(KW* kWave)
     }
     for (; kb < kb1; ++kb) {
       Stage<MATS, CT, MT, 1> s;
-      s.load(wp, xp, kb);
+      s.load(wp, xp, step, kb);
       s.multiply(acc);
     }
     // the waves' sums, a row tile at a time; then a wave an operand's columns
@@ -211,8 +301,8 @@ __global__ void __launch_bounds__(KW* kWave)
               acc[i][t][m];
       __syncthreads();
       const int r = m * 16 + (lane & 15);
-      for (int t = wave; t < CT; t += KW) {
-        const int64_t n = group * kInt8Block + 16 * (lane >> 4) + 4 * (t0 + t);
+      if (const int t = wave; t < CT) {
+        const int64_t n = n_mine;
         i32x4 sum[MATS];
 #pragma unroll
         for (int i = 0; i < MATS; ++i) {
@@ -223,24 +313,49 @@ __global__ void __launch_bounds__(KW* kWave)
                 s_acc + (((w * MATS + i) * CT + t) * kWave + lane) * 4);
         }
         if (r >= rows) continue;
-        float sx;
-        if constexpr (CHOSEN) sx = a.x_scales[nth_token(s_plan.mask[e], done + r)];
-        else sx = a.x_scales[row0 + r];
+        const float sx = kOwn ? s_scale[r & (kOwnRows - 1)] : a.x_scales[x_row(r)];
         const int64_t at = (row0 + r) * a.N;
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
           if (n + q >= a.N) break;
           S o[3];
-          const float p = (float)sum[0][q] * a.w_scales[e * a.N + n + q] * sx;
-          const float p2 =
-              MATS == 2 ? (float)sum[MATS - 1][q] * a.w2_scales[e * a.N + n + q] * sx : 0.f;
+          const float p = (float)sum[0][q] * sw[0][q] * sx;
+          const float p2 = MATS == 2 ? (float)sum[MATS - 1][q] * sw[MATS - 1][q] * sx : 0.f;
           int8_epilogue<T, EPI>(p, p2, o[0], o[1], o[2]);
-          static_cast<S*>(a.out)[at + n + q] = o[0];
+          if constexpr (ARRIVE)  // through the L2s: the workgroups run on any XCD
+            __hip_atomic_store(static_cast<float*>(a.out) + at + n + q, p, __ATOMIC_RELAXED,
+                               __HIP_MEMORY_SCOPE_AGENT);
+          else
+            static_cast<S*>(a.out)[at + n + q] = o[0];
           if (EPI != kInt8Plain && a.out2 != nullptr) {
             static_cast<S*>(a.out2)[at + n + q] = o[1];
             if (EPI == kInt8SwiGLU) static_cast<S*>(a.out3)[at + n + q] = o[2];
           }
         }
+      }
+    }
+    if constexpr (ARRIVE) {
+      // a wave's stores are complete when its vmcnt is zero; the counter behind that
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      __syncthreads();
+      const int loads = s_plan.pref[a.E];
+      if (threadIdx.x == 0) s_last = atomicAdd(&arrive.arrived[part], 1) == loads - 1;
+      __syncthreads();
+      if (s_last == 0) continue;
+      const int cols = 16 * CT;
+      for (int i = threadIdx.x; i < arrive.T * cols; i += blockDim.x) {
+        const int t = i / cols, c = i - t * cols, j4 = c / 4 % CT;
+        const int64_t n = group * kInt8Block + 16 * (c / (4 * CT)) + 4 * (t0 + j4) + c % 4;
+        if (n >= a.N) continue;
+        float sum = 0.f;
+        for (int j = 0; j < arrive.k; ++j) {
+          const float* y = static_cast<const float*>(a.out) +
+                           (int64_t)arrive.inv[t * arrive.k + j] * a.N + n;
+          sum = fmaf(arrive.gates[t * arrive.k + j],
+                     __hip_atomic_load(y, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT), sum);
+        }
+        if constexpr (kOwn)
+          static_cast<typename elem<X>::storage*>(arrive.out)[t * a.N + n] = to_bits<X>(sum);
       }
     }
   }
@@ -265,29 +380,53 @@ int stream_row_tiles(int64_t rows, int64_t experts) {
 // waves or more blocks in flight hold no more bytes in flight than the memory needs
 // and leave fewer workgroups to overlap (940 MB of 8 experts' two matrices: 138 us,
 // 6.8 TB/s; eight waves 153, two blocks 150, four quarters 153).
+// What a launch's workgroups are, by the column groups that all experts have.
+template <typename F>
+void by_columns(int64_t groups, int row_tiles, F&& f) {
+  if (groups >= (row_tiles == 4 ? 128 : 512)) f(constant<4>(), constant<4>(), constant<1>());
+  else if (groups >= 128) f(constant<2>(), constant<4>(), constant<1>());
+  else f(constant<1>(), constant<8>(), constant<2>());
+}
+
 template <typename T, int EPI, bool CHOSEN, typename C>
 void launch_stream(const Int8Gemm& a, int64_t experts, const C& chosen, hipStream_t s) {
   const int mt = stream_row_tiles(a.A, a.E);
   const int64_t groups = int8_groups(a.N);
   // every load but an expert's last is full
   const int64_t loads = std::min<int64_t>(a.A, experts + a.A / (16 * mt));
-  auto go = [&](auto mt, auto ct, auto kw, auto u) {
-    constexpr int MT = decltype(mt)::value, CT = decltype(ct)::value, KW = decltype(kw)::value;
-    hipLaunchKernelGGL((int8_stream_kernel<T, EPI, MT, CT, KW, decltype(u)::value, CHOSEN>),
-                       dim3((unsigned)std::min<int64_t>(loads * groups * (4 / CT), 1 << 20)),
-                       dim3(KW * kWave), 0, s, a, chosen);
+  auto by_rows = [&](auto mt) {
+    constexpr int MT = decltype(mt)::value;
+    by_columns(experts * groups, MT, [&](auto ct, auto kw, auto u) {
+      constexpr int CT = decltype(ct)::value, KW = decltype(kw)::value;
+      hipLaunchKernelGGL(
+          (int8_stream_kernel<T, int8_t, EPI, MT, CT, KW, decltype(u)::value, CHOSEN, false>),
+          dim3((unsigned)std::min<int64_t>(loads * groups * (4 / CT), 1 << 20)), dim3(KW * kWave),
+          0, s, a, chosen, NoArrive(), 0);
+    });
   };
-  auto by_columns = [&](auto mt) {
-    if (experts * groups >= (decltype(mt)::value == 4 ? 128 : 512))
-      go(mt, constant<4>(), constant<4>(), constant<1>());
-    else if (experts * groups >= 128)
-      go(mt, constant<2>(), constant<4>(), constant<1>());
-    else
-      go(mt, constant<1>(), constant<8>(), constant<2>());
-  };
-  if (mt == 1) by_columns(constant<1>());
-  else if (mt == 2) by_columns(constant<2>());
-  else by_columns(constant<4>());
+  if (mt == 1) by_rows(constant<1>());
+  else if (mt == 2) by_rows(constant<2>());
+  else by_rows(constant<4>());
+}
+
+// Rows of `width` values that workgroups bring to integers themselves: up to eight,
+// and 16,384 values in all (four a thread and pass; see the measurements at the end).
+bool own_rows(int64_t rows, int64_t width) {
+  return rows <= kOwnRows && rows * int8_pitch(width) <= 16384;
+}
+
+// The product of at most kOwnRows rows from their values (a.values, of type X).
+template <typename T, typename X, int EPI, bool CHOSEN, bool ARRIVE, typename C, typename R>
+void launch_own(const Int8Gemm& a, int64_t experts, int64_t loads, int held, const C& chosen,
+                const R& arrive, hipStream_t s) {
+  const int64_t groups = int8_groups(a.N);
+  by_columns(experts * groups, 1, [&](auto ct, auto kw, auto u) {
+    constexpr int CT = decltype(ct)::value, KW = decltype(kw)::value;
+    hipLaunchKernelGGL(
+        (int8_stream_kernel<T, X, EPI, 1, CT, KW, decltype(u)::value, CHOSEN, ARRIVE>),
+        dim3((unsigned)(loads * groups * (4 / CT))), dim3(KW * kWave), held * int8_pitch(a.K), s,
+        a, chosen, arrive, held);
+  });
 }
 
 // ------------------------------------------------------------------ routing
@@ -300,8 +439,10 @@ struct FewRoute {
   int64_t d;
   float* gates;
   int32_t* topk;
-  int8_t* codes;  // [T, pitch]
+  int8_t* codes;  // of the tokens; null: not written
   float* scales;
+  int32_t* arrived;  // counters to clear, `parts` of them (or null)
+  int32_t parts;
 };
 
 constexpr int kRouteThreads = 1024;
@@ -332,7 +473,9 @@ __global__ void __launch_bounds__(kRouteThreads) int8_route_kernel(FewRoute a) {
     return v;
   };
   uint32_t m = 0;
-  for (int64_t c = threadIdx.x * 4; c < a.d; c += kRouteThreads * 4) {
+  if (a.arrived != nullptr && t == 0)
+    for (int i = threadIdx.x; i < a.parts; i += kRouteThreads) a.arrived[i] = 0;
+  for (int64_t c = threadIdx.x * 4; c < (a.codes == nullptr ? 0 : a.d); c += kRouteThreads * 4) {
     const X4 v = four(c);
 #pragma unroll
     for (int j = 0; j < 4; ++j) m = max(m, abs_bits(elem<T>::load(v[j])));
@@ -364,7 +507,8 @@ __global__ void __launch_bounds__(kRouteThreads) int8_route_kernel(FewRoute a) {
   for (int i = 0; i < kRouteWaves; ++i) m = max(m, s_most[i]);
   const float s = int8_scale(m), inv = int8_inverse(s);
   const int64_t pitch = int8_pitch(a.d);
-  for (int64_t c = threadIdx.x * 4; c < pitch; c += kRouteThreads * 4) {
+  for (int64_t c = threadIdx.x * 4; c < (a.codes == nullptr ? 0 : pitch);
+       c += kRouteThreads * 4) {
     const X4 v = four(c);
     int q[4];
 #pragma unroll
@@ -372,7 +516,7 @@ __global__ void __launch_bounds__(kRouteThreads) int8_route_kernel(FewRoute a) {
     *reinterpret_cast<uint32_t*>(a.codes + int8_row(t, pitch) + c / 16 * 256 + c % 16) =
         pack_bytes(q[0], q[1], q[2], q[3]);
   }
-  if (threadIdx.x == 0) a.scales[t] = s;
+  if (threadIdx.x == 0 && a.codes != nullptr) a.scales[t] = s;
   const int e = threadIdx.x;
   const uint64_t key = e < a.E ? choice_key(s_logit[e], e) : 0;
   if (e < a.E) s_key[e] = key;
@@ -409,7 +553,7 @@ __global__ void __launch_bounds__(256) int8_combine_kernel(const float* y, const
 }
 
 struct Layout {
-  size_t inv, offsets, x, x_scales, hidden, codes, scales, y, bytes;
+  size_t inv, offsets, arrived, x, x_scales, hidden, codes, scales, y, bytes;
 };
 Layout layout(int dtype, int64_t T, int32_t k, int32_t E, int64_t d, int64_t f) {
   Layout l;
@@ -422,6 +566,7 @@ Layout layout(int dtype, int64_t T, int32_t k, int32_t E, int64_t d, int64_t f) 
   const int64_t A = T * k;
   l.inv = take(A * 4);
   l.offsets = take((E + 1) * 4);
+  l.arrived = take(4 * int8_groups(d) * 4);
   l.x = take(int8_rows_bytes(T, int8_pitch(d)));
   l.x_scales = take(T * 4);
   l.hidden = take(A * f * dtype_bytes(dtype));
@@ -441,6 +586,22 @@ int check_few(int dtype, int64_t T, int32_t E, int32_t k, int64_t d, int64_t f) 
 }
 
 }  // namespace
+
+bool launch_int8_own(const Int8Gemm& a, int epi, int dtype, hipStream_t s) {
+  if (!own_rows(a.A, a.K)) return false;
+  const int64_t experts = std::min<int64_t>(a.E, a.A);
+  int8_by_type(dtype, [&](auto type) {
+    typedef typename decltype(type)::type T;
+    auto go = [&](auto epilogue) {
+      launch_own<T, T, decltype(epilogue)::value, false, false>(a, experts, experts, (int)a.A,
+                                                                NoChoice(), NoArrive(), s);
+    };
+    if (epi == kInt8Plain) go(constant<kInt8Plain>());
+    else if (epi == kInt8SwiGLU) go(constant<kInt8SwiGLU>());
+    else go(constant<kInt8Gelu>());
+  });
+  return true;
+}
 
 void launch_int8_stream(const Int8Gemm& a, int epi, int dtype, hipStream_t s) {
   const int64_t experts = std::min<int64_t>(a.E, a.A);
@@ -495,6 +656,43 @@ int nt_int8_moe_few_tokens(int dtype, const void* x, const float* router, const 
   up.x = r.codes, up.x_scales = r.scales, up.w = w_up, up.w_scales = up_scales;
   up.w2 = w_val, up.w2_scales = val_scales;
   up.E = E, up.A = A, up.K = d, up.N = f, up.out = base + l.hidden;
+  Int8Gemm down = {};
+  down.offsets = c.offsets, down.w = w_down, down.w_scales = down_scales;
+  down.E = E, down.A = A, down.K = f, down.N = d, down.out = base + l.y;
+  float* y = reinterpret_cast<float*>(base + l.y);
+  if (own_rows(T, d) && own_rows(T, f)) {
+    // 16 arrivals on a counter cost less than a launch, many do not
+    const bool sum_here = experts <= 16;
+    r.codes = nullptr;
+    if (sum_here) {
+      r.arrived = reinterpret_cast<int32_t*>(base + l.arrived);
+      r.parts = (int32_t)(4 * int8_groups(d));
+    }
+    up.values = x, down.values = up.out;
+    int8_by_type(dtype, [&](auto type) {
+      typedef typename decltype(type)::type V;
+      hipLaunchKernelGGL((int8_route_kernel<V>), dim3((unsigned)T), dim3(kRouteThreads), 0,
+                         stream, r);
+      if (w_val != nullptr)
+        launch_own<V, V, kInt8SwiGLU, true, false>(up, experts, experts, (int)T, c, NoArrive(),
+                                                   stream);
+      else
+        launch_own<V, V, kInt8Gelu, true, false>(up, experts, experts, (int)T, c, NoArrive(),
+                                                 stream);
+      if (sum_here) {
+        Arrive sum = {gates, c.inv, out, r.arrived, (int32_t)T, k};
+        launch_own<float, V, kInt8Plain, false, true>(down, experts, experts, (int)T, NoChoice(),
+                                                      sum, stream);
+      } else {
+        launch_own<float, V, kInt8Plain, false, false>(down, experts, experts, (int)T,
+                                                       NoChoice(), NoArrive(), stream);
+        hipLaunchKernelGGL((int8_combine_kernel<V>),
+                           dim3((unsigned)ceil_div(d, (int64_t)256), (unsigned)T), dim3(256), 0,
+                           stream, y, c.inv, gates, k, d, out);
+      }
+    });
+    return launch_status();
+  }
   int8_by_type(dtype, [&](auto type) {
     typedef typename decltype(type)::type V;
     hipLaunchKernelGGL((int8_route_kernel<V>), dim3((unsigned)T), dim3(kRouteThreads), 0, stream,
@@ -506,16 +704,13 @@ int nt_int8_moe_few_tokens(int dtype, const void* x, const float* router, const 
   float* scales = reinterpret_cast<float*>(base + l.scales);
   st = nt_int8_rows(dtype, up.out, A, f, codes, scales, stream);
   if (st != NT_OK) return st;
-  Int8Gemm down = {};
-  down.x = codes, down.x_scales = scales, down.offsets = c.offsets, down.w = w_down;
-  down.w_scales = down_scales;
-  down.E = E, down.A = A, down.K = f, down.N = d, down.out = base + l.y;
+  down.x = codes, down.x_scales = scales;
   launch_stream<float, kInt8Plain, false>(down, experts, NoChoice(), stream);
   int8_by_type(dtype, [&](auto type) {
     typedef typename decltype(type)::type V;
     hipLaunchKernelGGL((int8_combine_kernel<V>),
                        dim3((unsigned)ceil_div(d, (int64_t)256), (unsigned)T), dim3(256), 0,
-                       stream, reinterpret_cast<const float*>(base + l.y), c.inv, gates, k, d, out);
+                       stream, y, c.inv, gates, k, d, out);
   });
   return launch_status();
 }

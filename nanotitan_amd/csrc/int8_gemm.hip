@@ -328,15 +328,26 @@ int check_int8(int dtype, const Int8Gemm& a) {
 }
 bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
-int run_int8(int dtype, int epi, Int8Gemm a, hipStream_t s) {
+int run_int8(int dtype, int epi, Int8Gemm a, hipStream_t s, void* ws = nullptr,
+             size_t ws_bytes = 0) {
   const int st = check_int8(dtype, a);
   if (st != NT_OK || a.A == 0) return st;
   const bool two = epi == kInt8SwiGLU;
-  if (a.x == nullptr || a.x_scales == nullptr || a.w == nullptr || a.w_scales == nullptr ||
+  if ((a.values == nullptr && (a.x == nullptr || a.x_scales == nullptr)) || a.w == nullptr || a.w_scales == nullptr ||
       a.out == nullptr || (two && (a.w2 == nullptr || a.w2_scales == nullptr)) ||
       (a.offsets == nullptr && a.E != 1) || (two && (a.out2 == nullptr) != (a.out3 == nullptr)) ||
       !aligned16(a.x) || !aligned16(a.w) || !aligned16(a.w2))
     return NT_ERR_INVALID_ARG;
+  if (a.values != nullptr) {
+    if (ws == nullptr || ws_bytes < nt_int8_linear_workspace_bytes(a.A, a.K) || !aligned16(ws))
+      return NT_ERR_WORKSPACE;
+    if (launch_int8_own(a, epi, dtype, s)) return launch_status();
+    int8_t* codes = static_cast<int8_t*>(ws);
+    float* scales = reinterpret_cast<float*>(codes + int8_rows_bytes(a.A, int8_pitch(a.K)));
+    const int made = nt_int8_rows(dtype, a.values, a.A, a.K, codes, scales, s);
+    if (made != NT_OK) return made;
+    a.x = codes, a.x_scales = scales;
+  }
   int result = NT_OK;
   int8_by_type(dtype, [&](auto type) {
     typedef typename decltype(type)::type T;
@@ -353,6 +364,44 @@ int run_int8(int dtype, int epi, Int8Gemm a, hipStream_t s) {
 using namespace nt;
 
 extern "C" {
+
+size_t nt_int8_linear_workspace_bytes(int64_t A, int64_t K) {
+  if (A < 0 || A > kInt8MaxRows || K < 1 || K > kInt8MaxK) return 0;
+  return (size_t)(int8_rows_bytes(A, int8_pitch(K)) + round_up(A * 4, 16));
+}
+
+int nt_int8_linear(int dtype, const void* x, const int32_t* offsets, const int8_t* w,
+                   const float* w_scales, int32_t E, int64_t A, int64_t K, int64_t N, void* out,
+                   void* ws, size_t ws_bytes, hipStream_t stream) {
+  Int8Gemm a = {};
+  a.values = x, a.offsets = offsets, a.w = w, a.w_scales = w_scales;
+  a.E = E, a.A = A, a.K = K, a.N = N, a.out = out;
+  if (x == nullptr && A > 0) return NT_ERR_INVALID_ARG;
+  return run_int8(dtype, kInt8Plain, a, stream, ws, ws_bytes);
+}
+
+int nt_int8_linear_swiglu(int dtype, const void* x, const int32_t* offsets, const int8_t* w_gate,
+                          const float* gate_scales, const int8_t* w_val, const float* val_scales,
+                          int32_t E, int64_t A, int64_t K, int64_t N, void* hidden, void* gate,
+                          void* value, void* ws, size_t ws_bytes, hipStream_t stream) {
+  Int8Gemm a = {};
+  a.values = x, a.offsets = offsets, a.w = w_gate, a.w_scales = gate_scales;
+  a.w2 = w_val, a.w2_scales = val_scales;
+  a.E = E, a.A = A, a.K = K, a.N = N, a.out = hidden, a.out2 = gate, a.out3 = value;
+  if (x == nullptr && A > 0) return NT_ERR_INVALID_ARG;
+  return run_int8(dtype, kInt8SwiGLU, a, stream, ws, ws_bytes);
+}
+
+int nt_int8_linear_gelu(int dtype, const void* x, const int32_t* offsets, const int8_t* w,
+                        const float* w_scales, int32_t E, int64_t A, int64_t K, int64_t N,
+                        void* act, void* act_grad, void* ws, size_t ws_bytes,
+                        hipStream_t stream) {
+  Int8Gemm a = {};
+  a.values = x, a.offsets = offsets, a.w = w, a.w_scales = w_scales;
+  a.E = E, a.A = A, a.K = K, a.N = N, a.out = act, a.out2 = act_grad;
+  if (x == nullptr && A > 0) return NT_ERR_INVALID_ARG;
+  return run_int8(dtype, kInt8Gelu, a, stream, ws, ws_bytes);
+}
 
 int nt_int8_grouped_gemm(int dtype, const int8_t* x, const float* x_scales,
                          const int32_t* offsets, const int8_t* w, const float* w_scales,

@@ -11,8 +11,9 @@ namespace nt {
 enum Int8Epilogue { kInt8Plain = 0, kInt8SwiGLU = 1, kInt8Gelu = 2 };
 
 struct Int8Gemm {
-  const int8_t* x;          // [A, pitch]
-  const float* x_scales;    // [A]
+  const int8_t* x;          // rows of integers, and their scales [A]
+  const float* x_scales;
+  const void* values;       // or few rows' values [A, K], of the outputs' type
   const int32_t* offsets;   // [E + 1], or null: all rows are one expert's
   const int8_t *w, *w2;     // blocks of [E, K, N]; w2: the value weights
   const float *w_scales, *w2_scales;  // [E, N]
@@ -23,8 +24,10 @@ struct Int8Gemm {
   int32_t ntn;
 };
 
-// int8_few.hip: the product of few rows for each expert.
+// int8_few.hip: the product of few rows for each expert; and that of a few rows from
+// their values (false where it does not take them).
 void launch_int8_stream(const Int8Gemm& a, int epi, int dtype, hipStream_t s);
+bool launch_int8_own(const Int8Gemm& a, int epi, int dtype, hipStream_t s);
 
 namespace {
 

@@ -58,30 +58,20 @@ const int32_t* check_offsets(const OptTensor& offsets, const Tensor& x, int32_t 
   return offsets->data_ptr<int32_t>();
 }
 
-struct Rows8 {
-  Tensor codes, scales;
-  const int8_t* q() const { return codes.data_ptr<int8_t>(); }
-  const float* s() const { return scales.data_ptr<float>(); }
-};
-Rows8 rows8(const Tensor& x) {
-  const int64_t rows = x.size(0), f = x.size(1);
-  Rows8 r = {at::empty({(rows + 15) / 16, nt_int8_pitch(f) / 64, 4, 16, 16},
-                       x.options().dtype(at::kChar)),
-             at::empty({rows}, x.options().dtype(at::kFloat))};
-  check_status(nt_int8_rows(dtype_code(x), x.data_ptr(), rows, f, r.codes.data_ptr<int8_t>(),
-                            r.scales.data_ptr<float>(), stream_of(x)),
-               "int8_rows");
-  return r;
-}
-
 // int8_rows(x) -> (codes [rows/16, f/64, 4, 16, 16], scales), and back.
 std::tuple<Tensor, Tensor> int8_rows(Tensor x) {
   const OptTensor in = x;
   refuse_tangents({&in}, "int8_rows");
   check_rows(x, "x");
   c10::hip::HIPGuard guard(x.get_device());
-  Rows8 r = rows8(x);
-  return {r.codes, r.scales};
+  const int64_t rows = x.size(0), f = x.size(1);
+  Tensor codes = at::empty({(rows + 15) / 16, nt_int8_pitch(f) / 64, 4, 16, 16},
+                           x.options().dtype(at::kChar));
+  Tensor scales = at::empty({rows}, x.options().dtype(at::kFloat));
+  check_status(nt_int8_rows(dtype_code(x), x.data_ptr(), rows, f, codes.data_ptr<int8_t>(),
+                            scales.data_ptr<float>(), stream_of(x)),
+               "int8_rows");
+  return {codes, scales};
 }
 Tensor int8_rows_decode(Tensor codes, Tensor scales, int64_t width, at::ScalarType dtype) {
   check_device(codes, "codes");
@@ -137,7 +127,18 @@ Tensor int8_weight_decode(Tensor codes, Tensor scales, int64_t K, at::ScalarType
   return W;
 }
 
-// int8_product(x, offsets, codes, scales) -> x @ W, x's rows brought to 8 bits.
+// x @ W, x's rows brought to 8 bits.
+Tensor linear(const Tensor& x, const int32_t* off, const Weight& w) {
+  const int64_t A = x.size(0);
+  Tensor out = at::empty({A, w.N}, x.options());
+  Tensor ws = workspace(x, nt_int8_linear_workspace_bytes(A, w.K));
+  check_status(nt_int8_linear(dtype_code(x), x.data_ptr(), off, w.codes, w.scales, w.E, A, w.K,
+                              w.N, out.data_ptr(), ws.data_ptr(), ws.numel(), stream_of(x)),
+               "int8_linear");
+  return out;
+}
+
+// int8_product(x, offsets, codes, scales) -> x @ W.
 Tensor int8_product(Tensor x, OptTensor offsets, Tensor codes, Tensor scales) {
   const OptTensor in = x;
   refuse_tangents({&in}, "int8_grouped_gemm");
@@ -145,12 +146,7 @@ Tensor int8_product(Tensor x, OptTensor offsets, Tensor codes, Tensor scales) {
   const Weight w = check_weight(codes, scales, x.size(1), x, "weight");
   const int32_t* off = check_offsets(offsets, x, w.E);
   c10::hip::HIPGuard guard(x.get_device());
-  const Rows8 q = rows8(x);
-  Tensor out = at::empty({x.size(0), w.N}, x.options());
-  check_status(nt_int8_grouped_gemm(dtype_code(x), q.q(), q.s(), off, w.codes, w.scales, w.E,
-                                    x.size(0), w.K, w.N, out.data_ptr(), stream_of(x)),
-               "int8_grouped_gemm");
-  return out;
+  return linear(x, off, w);
 }
 
 void check_down(const Weight& up, const Weight& down, int64_t d) {
@@ -177,17 +173,14 @@ std::tuple<Tensor, OptTensor, OptTensor> int8_swiglu_ffn(Tensor x, OptTensor off
   OptTensor gate, value;
   if (keep) gate = at::empty_like(hidden), value = at::empty_like(hidden);
   {
-    const Rows8 q = rows8(x);
-    check_status(nt_int8_grouped_gemm_swiglu(dtype_code(x), q.q(), q.s(), off, g.codes, g.scales,
-                                             v.codes, v.scales, g.E, A, d, g.N, hidden.data_ptr(),
-                                             out_or_null(gate), out_or_null(value), stream_of(x)),
-                 "int8_grouped_gemm_swiglu");
+    Tensor ws = workspace(x, nt_int8_linear_workspace_bytes(A, d));
+    check_status(nt_int8_linear_swiglu(dtype_code(x), x.data_ptr(), off, g.codes, g.scales,
+                                       v.codes, v.scales, g.E, A, d, g.N, hidden.data_ptr(),
+                                       out_or_null(gate), out_or_null(value), ws.data_ptr(),
+                                       ws.numel(), stream_of(x)),
+                 "int8_linear_swiglu");
   }
-  const Rows8 q = rows8(hidden);
-  Tensor y = at::empty({A, d}, x.options());
-  check_status(nt_int8_grouped_gemm(dtype_code(x), q.q(), q.s(), off, o.codes, o.scales, o.E, A,
-                                    o.K, d, y.data_ptr(), stream_of(x)),
-               "int8_grouped_gemm");
+  Tensor y = linear(hidden, off, o);
   return {y, gate, value};
 }
 
@@ -207,17 +200,13 @@ std::tuple<Tensor, OptTensor> int8_gelu_ffn(Tensor x, OptTensor offsets, Tensor 
   OptTensor slope;
   if (keep) slope = at::empty_like(act);
   {
-    const Rows8 q = rows8(x);
-    check_status(nt_int8_grouped_gemm_gelu(dtype_code(x), q.q(), q.s(), off, u.codes, u.scales,
-                                           u.E, A, d, u.N, act.data_ptr(), out_or_null(slope),
-                                           stream_of(x)),
-                 "int8_grouped_gemm_gelu");
+    Tensor ws = workspace(x, nt_int8_linear_workspace_bytes(A, d));
+    check_status(nt_int8_linear_gelu(dtype_code(x), x.data_ptr(), off, u.codes, u.scales, u.E, A,
+                                     d, u.N, act.data_ptr(), out_or_null(slope), ws.data_ptr(),
+                                     ws.numel(), stream_of(x)),
+                 "int8_linear_gelu");
   }
-  const Rows8 q = rows8(act);
-  Tensor y = at::empty({A, d}, x.options());
-  check_status(nt_int8_grouped_gemm(dtype_code(x), q.q(), q.s(), off, o.codes, o.scales, o.E, A,
-                                    o.K, d, y.data_ptr(), stream_of(x)),
-               "int8_grouped_gemm");
+  Tensor y = linear(act, off, o);
   return {y, slope};
 }
 

@@ -46,7 +46,7 @@ def _steps(dtype):
 
 
 # Rows an expert: one, a few, the limits of the row tiles of 16, 32 and 64, of 128 and of 256.
-COUNTS = {"one": [1], "few": [3, 0, 16, 1], "sixteen": [17, 9, 0, 22], "streams": [33, 64, 0, 1],
+COUNTS = {"one": [1], "eight": [3, 0, 5], "few": [3, 0, 16, 1], "sixteen": [17, 9, 0, 22], "streams": [33, 64, 0, 1],
           "mixed": [200, 0, 3, 50], "tiles": [128, 129, 0, 300], "wide": [256, 1, 700, 513],
           "dense": None}
 
@@ -156,7 +156,7 @@ def test_a_row_is_the_same_in_any_batch():
     w, _, _ = _weights(1, 500, 300, 7)
     x = _rand(700, 500, dtype=torch.bfloat16, seed=8)
     whole = int8_grouped_gemm_fn(x, w)
-    for n in (1, 17, 40, 100, 257):
+    for n in (1, 5, 8, 9, 17, 40, 100, 257):
         assert torch.equal(int8_grouped_gemm_fn(x[:n], w), whole[:n])
 
 
@@ -235,11 +235,14 @@ def test_hidden_values(dtype, ffn, counts):
 
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("ffn", ["swiglu", "gelu"])
-@pytest.mark.parametrize("counts", ["few", "streams", "tiles", "wide", "dense"])
+@pytest.mark.parametrize("counts", ["few", "streams", "tiles", "wide", "dense", "one", "three",
+                                    "eight"])
 def test_block_is_its_stages(dtype, ffn, counts):
-    """The feed-forward block has the bits of its stages, each checked above."""
+    """The feed-forward block has the bits of its stages, each checked above; up to eight rows
+    come to 8 bits within the products."""
     t = TYPES[dtype]
-    off, gpu_off = ([0, 77], None) if counts == "dense" else _offsets(COUNTS[counts])
+    off, gpu_off = ([0, 77], None) if counts == "dense" else _offsets(
+        {"three": [1, 0, 2], "eight": [0, 7, 1]}.get(counts) or COUNTS[counts])
     E, A, d, f = len(off) - 1, off[-1], 200, 341
     x = _rand(A, d, dtype=t, seed=1)
     up = [_weights(E, d, f, 2 + i)[0] for i in range(2 if ffn == "swiglu" else 1)]

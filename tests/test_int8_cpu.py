@@ -119,6 +119,26 @@ def test_products_refuse(over, code):
     assert lib.nt_int8_grouped_gemm_swiglu(*ins, P, P, *sizes, a["out"], None, None, None) == code
 
 
+@pytest.mark.parametrize("over,code", [
+    (dict(dtype=F64), capi.NT_ERR_DTYPE), (dict(E=0), capi.NT_ERR_INVALID_ARG),
+    (dict(K=0), capi.NT_ERR_INVALID_ARG), (dict(offsets=None), capi.NT_ERR_INVALID_ARG),
+    (dict(x=None), capi.NT_ERR_INVALID_ARG), (dict(w=None), capi.NT_ERR_INVALID_ARG),
+    (dict(out=None), capi.NT_ERR_INVALID_ARG), (dict(A=2**24), capi.NT_ERR_TOO_LARGE),
+    (dict(ws_bytes=100), capi.NT_ERR_WORKSPACE), (dict(ws=None), capi.NT_ERR_WORKSPACE),
+    (dict(ws=P + 8), capi.NT_ERR_WORKSPACE), (dict(A=0, x=None, out=None, ws=None), capi.NT_OK)])
+def test_linear_refuses(over, code):
+    lib, a = capi.load(), dict(dtype=BF, x=P, offsets=P, w=P, s=P, E=2, A=4, K=8, N=8, out=P, ws=P,
+                               ws_bytes=2**20)
+    a.update(over)
+    head = [a[n] for n in ("dtype", "x", "offsets", "w", "s")]
+    sizes = [a[n] for n in ("E", "A", "K", "N")]
+    tail = [a["ws"], a["ws_bytes"], None]
+    assert lib.nt_int8_linear(*head, *sizes, a["out"], *tail) == code
+    assert lib.nt_int8_linear_gelu(*head, *sizes, a["out"], None, *tail) == code
+    assert lib.nt_int8_linear_swiglu(*head, P, P, *sizes, a["out"], None, None, *tail) == code
+    assert lib.nt_int8_linear_workspace_bytes(17, 129) == 32 * 256 + 80
+
+
 def test_swiglu_refuses_half_of_a_pair():
     a = _gemm()
     ins = [a[n] for n in ("dtype", "x", "xs", "offsets", "w", "ws")]
