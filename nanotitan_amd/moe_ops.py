@@ -845,10 +845,21 @@ def _all_rows(x, expert_offset):
     return torch.arange(2, dtype=torch.int32, device=x.device) * x.shape[0]
 
 
-def _int8_direct(dout):
-    """Whether the kernels that read 8-bit weights take this gradient; else the weights go to
-    its dtype first."""
+def _int8_takes(dout):
+    """Whether the kernels that read 8-bit weights take this gradient."""
     return dout.dtype != torch.float32 and dout.shape[1] % 8 == 0
+
+
+def _int8_direct(dout, experts, K):
+    """Whether they are the faster ones; else the weights go to dout's dtype first.
+
+    They pay where reading and writing the weights costs more than the products gain from weights
+    in 16 bits: at most 512 rows an expert and 2^25 weights or more (128 experts of 2,048 x 768,
+    14,312 rows: 88 us against 111 + 104; 8 of 4,096 x 14,336, 1,000 rows: 338 against 300 + 262,
+    8,192 rows: 1,331 against 301 + 1,022; 8 of 512 x 2,048, 4,096 rows: 54 against 9 + 28).
+    """
+    A, N = dout.shape
+    return _int8_takes(dout) and A <= 512 * experts and experts * K * N >= 1 << 25
 
 
 def _aligned(t):
@@ -860,7 +871,7 @@ def _aligned(t):
 def _int8_dx(dout, off, codes, scale, K):
     """dout @ W^T for the weights [E,K,N] that codes and scale hold."""
     ext = get_hip_extension()
-    if _int8_direct(dout):
+    if _int8_direct(dout, scale.shape[0], K):
         return ext.int8_dx(_aligned(dout), off, codes, scale, K)
     W = ext.int8_weight_decode(codes, scale, K, dout.dtype)
     return ext.bwd_grouped_gemm_dX_kernel(W, _all_rows(dout, off), dout.contiguous())
@@ -907,14 +918,14 @@ class Int8SwiGLUFFN_FN(torch.autograd.Function):
     def backward(ctx, dy):
         ext = get_hip_extension()
         off, gate, value, gc, gs, vc, vs, oc, os = ctx.saved_tensors
-        _, d, f = ctx.shape
-        if _int8_direct(dy):
+        E, d, f = ctx.shape
+        if _int8_direct(dy, E, f):
             dg, dv = ext.int8_dx_swiglu(_aligned(dy), gate, value, off, oc, os, f)
         else:
             dg, dv = ext.bwd_grouped_gemm_dX_swiglu(
                 ext.int8_weight_decode(oc, os, f, dy.dtype), _all_rows(dy, off), dy.contiguous(),
                 gate, value)
-        if _int8_direct(dg):
+        if _int8_direct(dg, E, d):
             dX = ext.int8_dx2(dg, dv, off, gc, gs, vc, vs, d)
         else:
             dX = ext.bwd_grouped_gemm_dX2(
@@ -939,8 +950,8 @@ class Int8GeluFFN_FN(torch.autograd.Function):
     def backward(ctx, dy):
         ext = get_hip_extension()
         off, slope, uc, us, dc, ds = ctx.saved_tensors
-        _, d, f = ctx.shape
-        if _int8_direct(dy):
+        E, d, f = ctx.shape
+        if _int8_direct(dy, E, f):
             dh = ext.int8_dx_gelu(_aligned(dy), slope, off, dc, ds, f)
         else:
             dh = ext.bwd_grouped_gemm_dX_gelu(ext.int8_weight_decode(dc, ds, f, dy.dtype),

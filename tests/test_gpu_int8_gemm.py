@@ -3,7 +3,7 @@
 import pytest
 import torch
 
-from nanotitan_amd import capi
+from nanotitan_amd import capi, moe_ops
 from nanotitan_amd.moe_ops import (
     Int8Weight,
     int8_gelu_ffn_fn,
@@ -262,6 +262,23 @@ def test_block_is_its_stages(dtype, ffn, counts):
 # ----------------------------------------------------------------- gradients
 
 
+@pytest.fixture(params=["by_size", "direct"])
+def direct(request, monkeypatch):
+    """Gradients as the sizes choose them (at these, by weights in the tokens' type), and by the
+    kernels that read 8-bit weights wherever those take them."""
+    if request.param == "direct":
+        monkeypatch.setattr(moe_ops, "_int8_direct", lambda d, E, K: moe_ops._int8_takes(d))
+
+
+def test_which_gradient():
+    """Few rows of many weights read them as they are."""
+    dout = torch.empty(2000, 4096, dtype=torch.bfloat16, device="meta")
+    assert moe_ops._int8_direct(dout, 4, 2048) and not moe_ops._int8_direct(dout, 3, 4096)
+    assert not moe_ops._int8_direct(dout, 4, 2047)
+    assert not moe_ops._int8_direct(dout.float(), 4, 4096)
+    assert not moe_ops._int8_direct(dout[:, :4095], 64, 4096)
+
+
 def _held_weights(ws):
     return [int8_weight_decode(w, torch.float32).cpu().double() for w in ws]
 
@@ -269,7 +286,7 @@ def _held_weights(ws):
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("counts", ["few", "mixed", "wide", "dense"])
 @pytest.mark.parametrize("K,N", [(300, 264), (65, 8), (1030, 72), (130, 77), (256, 640)])
-def test_product_gradient(dtype, counts, K, N):
+def test_product_gradient(dtype, counts, K, N, direct):
     t = TYPES[dtype]
     off, gpu_off = ([0, 19], None) if counts == "dense" else _offsets(COUNTS[counts])
     E, A = len(off) - 1, off[-1]
@@ -295,7 +312,7 @@ def test_product_gradient(dtype, counts, K, N):
 @pytest.mark.parametrize("ffn", ["swiglu", "gelu"])
 @pytest.mark.parametrize("counts", ["few", "mixed", "wide", "dense"])
 @pytest.mark.parametrize("d,f", [(128, 264), (72, 333), (77, 256), (300, 520)])
-def test_block_gradient(dtype, ffn, counts, d, f):
+def test_block_gradient(dtype, ffn, counts, d, f, direct):
     """dX against the formula in 64 bits, and that against differences."""
     t = TYPES[dtype]
     off, gpu_off = ([0, 19], None) if counts == "dense" else _offsets(COUNTS[counts])
@@ -349,7 +366,7 @@ def test_gradient_rows_behind_the_last_stay():
         assert bool((t[rows:] == 7.0).all()) and not bool((t[:rows] == 7.0).all())
 
 
-def test_gradient_of_any_alignment_and_layout():
+def test_gradient_of_any_alignment_and_layout(direct):
     w, _, _ = _weights(1, 100, 64, 0)
     x = _rand(33, 100, dtype=torch.bfloat16).requires_grad_()
     dout = _rand(33, 64, dtype=torch.bfloat16, seed=1)
@@ -378,7 +395,7 @@ def test_gradient_at_the_last_of_many_weights():
     assert torch.equal(got, want)
 
 
-def test_gradients_are_once_differentiable_and_have_no_tangents():
+def test_gradients_are_once_differentiable_and_have_no_tangents(direct):
     w, _, _ = _weights(1, 64, 64, 0)
     x = _rand(5, 64).requires_grad_()
     for fn in (lambda v: int8_grouped_gemm_fn(v, w), lambda v: int8_gelu_ffn_fn(v, w, w),
@@ -414,7 +431,7 @@ def test_on_another_stream_and_two_at_once():
 
 
 @pytest.mark.parametrize("rows", [5, 150, 600])
-def test_captured_and_replayed(rows):
+def test_captured_and_replayed(rows, direct):
     E, d, f = 2, 256, 384
     off, gpu_off = _offsets([rows, rows // 2])
     A = off[-1]
