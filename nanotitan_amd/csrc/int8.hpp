@@ -99,29 +99,29 @@ __device__ __forceinline__ typename elem<T>::storage int8_value(int q, float s) 
   return elem<T>::store(v > most ? most : v < -most ? -most : v);  // (a NaN stays one)
 }
 
-// Sixteen neighbouring values of a row.
-constexpr int kVec = 16;  // values of a lane at a time: 16 bytes of integers
+constexpr int kVec = 16;  // values of a 16-byte piece of integers
 
-template <typename T>
-struct Sixteen {
+// N (8 or 16) neighbouring values of a row.
+template <typename T, int N = kVec>
+struct Some {
   typedef typename elem<T>::storage S;
-  typedef S V __attribute__((ext_vector_type(kVec), aligned(sizeof(S))));
+  typedef S V __attribute__((ext_vector_type(N), aligned(sizeof(S))));
   V v;
-  // Columns c .. c + 15 of a row of f, zeros past its end.
+  // Columns c .. c + N - 1 of a row of f, zeros past its end.
   __device__ __forceinline__ void load(const S* row, int64_t c, int64_t f) {
-    if (c + kVec <= f) {
+    if (c + N <= f) {
       v = *reinterpret_cast<const V*>(row + c);
     } else {
 #pragma unroll
-      for (int i = 0; i < kVec; ++i) v[i] = c + i < f ? row[c + i] : S(0);
+      for (int i = 0; i < N; ++i) v[i] = c + i < f ? row[c + i] : S(0);
     }
   }
   __device__ __forceinline__ void store(S* row, int64_t c, int64_t f) const {
-    if (c + kVec <= f) {
+    if (c + N <= f) {
       *reinterpret_cast<V*>(row + c) = v;
     } else {
 #pragma unroll
-      for (int i = 0; i < kVec; ++i)
+      for (int i = 0; i < N; ++i)
         if (c + i < f) row[c + i] = v[i];
     }
   }
@@ -129,17 +129,17 @@ struct Sixteen {
     if constexpr (sizeof(S) == 2) {
       // pairs at once: magnitudes' bits order as the values do
       typedef unsigned short U2 __attribute__((ext_vector_type(2)));
-      uint32_t w[8];
+      uint32_t w[N / 2];
       __builtin_memcpy(w, &v, sizeof(w));
       U2 m = {0, 0};
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
+      for (int i = 0; i < N / 2; ++i)
         m = __builtin_elementwise_max(m, __builtin_bit_cast(U2, w[i] & 0x7fff7fffu));
       return abs_bits(elem<T>::load(m[0] > m[1] ? m[0] : m[1]));
     } else {
       uint32_t m = 0;
 #pragma unroll
-      for (int i = 0; i < kVec; ++i) {
+      for (int i = 0; i < N; ++i) {
         const uint32_t b = abs_bits(elem<T>::load(v[i]));
         m = b > m ? b : m;
       }
@@ -149,12 +149,13 @@ struct Sixteen {
   // x / s by the inverse, plus 1.5 2^23: the sum's low byte is the nearest integer,
   // or next to a border its neighbour, which x minus s times it tells. Then
   // int8_code decides; of normal values in bf16 one group of 1,024 in thirty.
-  __device__ __forceinline__ uint4 codes(float s, float inv) const {
+  typedef uint32_t Codes __attribute__((ext_vector_type(N / 4)));
+  __device__ __forceinline__ Codes codes(float s, float inv) const {
     constexpr float kMagic = 12582912.f;
-    uint32_t w[4];
+    Codes w;
     float most = 0.f;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < N / 4; ++i) {
       uint32_t t[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
@@ -167,14 +168,14 @@ struct Sixteen {
     }
     if (!(most < 0.5f * s) || inv == 0.f) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
+      for (int i = 0; i < N / 4; ++i) {
         int q[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) q[j] = int8_code(elem<T>::load(v[4 * i + j]), s, inv);
         w[i] = pack_bytes(q[0], q[1], q[2], q[3]);
       }
     }
-    return make_uint4(w[0], w[1], w[2], w[3]);
+    return w;
   }
 };
 

@@ -144,7 +144,7 @@ __device__ __forceinline__ void own_integers(F&& row, int rows, int64_t f, int h
   for (int r0 = 0; r0 < rows; r0 += WAVES) {
     const int r = r0 + wave / share, c0 = wave % share * kWave + lane_id();
     const bool live = r < rows;
-    Sixteen<X> v;
+    Some<X> v;
     uint32_t m = 0;
     if (live)
       for (int c = c0; c < chunks; c += share * kWave) {
@@ -164,7 +164,7 @@ __device__ __forceinline__ void own_integers(F&& row, int rows, int64_t f, int h
     const bool once = chunks <= share * kWave;  // then v still holds it
     for (int c = c0; c < chunks; c += share * kWave) {
       if (!once) v.load(row(r), (int64_t)c * kVec, f);
-      *reinterpret_cast<uint4*>(codes + (c * held + r) * 16) = v.codes(s, inv);
+      *reinterpret_cast<typename Some<X>::Codes*>(codes + (c * held + r) * 16) = v.codes(s, inv);
     }
   }
   __syncthreads();

@@ -5,7 +5,7 @@
 // wide ones), whose integers pass through LDS: in memory the 16-byte pieces of 16
 // rows alternate, and eight of them make a 128-byte line (written piece by piece,
 // 32,768 rows of 14,336 took 534 us for 235 in row order). Rounding one value has to
-// stay near seven instructions for HBM to bound the kernel (Sixteen::codes). Few
+// stay near seven instructions for HBM to bound the kernel (Some::codes). Few
 // rows take a workgroup each and write their pieces as they are.
 //
 // Weights: the channels' maxima run down the columns, so a pass over W finds them
@@ -21,17 +21,18 @@ namespace {
 
 constexpr int kThreads = 256;
 
-// ROWS rows a workgroup, TEAM lanes a row, C chunks of 16 columns a lane in
-// registers; HELD false: rows past TEAM * C * 16 columns, read twice. Workgroups b
+// ROWS rows a workgroup, TEAM lanes a row, C chunks of 8 columns a lane in
+// registers (a wave's loads of 16-bit values are then 1 KiB on end); HELD false: rows
+// past TEAM * C * 8 columns, read twice. Workgroups b
 // and b + 8 share an XCD and so an L2: the parts of a block of 16 rows go to such.
 template <typename T, int ROWS, int TEAM, int C, bool HELD>
 __global__ void __launch_bounds__(ROWS* TEAM)
     int8_rows_kernel(const void* x, int64_t rows, int64_t f, int8_t* codes, float* scales) {
   typedef typename elem<T>::storage S;
-  constexpr int G = C % 2 == 0 ? 2 : 1;  // chunks of a lane that turn at once
-  // a chunk's pieces, padded so that neighbouring lanes' begin in other banks
-  constexpr int kPitch = ROWS * 16 + 16, kParts = 16 / ROWS;
-  __shared__ __attribute__((aligned(16))) char s_turn[2][G * TEAM * kPitch];
+  constexpr int G = C % 4 == 0 ? 4 : C % 2 == 0 ? 2 : 1;  // chunks of a lane that turn at once
+  // the rows' pieces of 16 columns, padded so that neighbours begin in other banks
+  constexpr int kPitch = ROWS * 16 + 16, kParts = 16 / ROWS, kPieces = G * TEAM / 2;
+  __shared__ __attribute__((aligned(16))) char s_turn[2][kPieces * kPitch];
   const int64_t b = blockIdx.x;
   const int64_t row0 = (b / (8 * kParts) * 8 + b % 8) * 16 + b / 8 % kParts * ROWS;
   if (row0 >= rows) return;
@@ -39,13 +40,14 @@ __global__ void __launch_bounds__(ROWS* TEAM)
   const bool live = row0 + r < rows;
   const int64_t row = live ? row0 + r : rows - 1;  // past the last: that one again
   const int64_t pitch = int8_pitch(f);
-  const int chunks = (int)(pitch / kVec);
+  const int chunks = (int)(pitch / 8);
   const S* in = static_cast<const S*>(x) + row * f;
-  Sixteen<T> v[C];
+  typedef Some<T, 8> Chunk;
+  Chunk v[C];
   auto load = [&](int c0) {
 #pragma unroll
     for (int i = 0; i < C; ++i)
-      if (c0 + i * TEAM < chunks) v[i].load(in, (int64_t)(c0 + i * TEAM + lane) * kVec, f);
+      if (c0 + i * TEAM < chunks) v[i].load(in, (int64_t)(c0 + i * TEAM + lane) * 8, f);
   };
   uint32_t m = 0;
   for (int c0 = 0; c0 < (HELD ? 1 : chunks); c0 += TEAM * C) {
@@ -73,7 +75,7 @@ __global__ void __launch_bounds__(ROWS* TEAM)
   }
   const float s = int8_scale(m), inv = int8_inverse(s);
   if (lane == 0 && live) scales[row] = s;
-  // thread: piece threadIdx % ROWS of chunk threadIdx / ROWS
+  // thread: row threadIdx % ROWS of piece threadIdx / ROWS
   int8_t* out = codes + int8_row(row0 + threadIdx.x % ROWS, pitch);
   int buffer = 0;
   for (int c0 = 0; c0 < (HELD ? 1 : chunks); c0 += TEAM * C) {
@@ -86,13 +88,13 @@ __global__ void __launch_bounds__(ROWS* TEAM)
 #pragma unroll
       for (int g = 0; g < G; ++g)
         if (c0 + (i + g) * TEAM < chunks)
-          *reinterpret_cast<uint4*>(turn + (g * TEAM + lane) * kPitch + r * 16) =
-              v[i + g].codes(s, inv);
+          *reinterpret_cast<typename Chunk::Codes*>(turn + (g * TEAM + lane) / 2 * kPitch + r * 16 +
+                                                    lane % 2 * 8) = v[i + g].codes(s, inv);
       __syncthreads();
 #pragma unroll
-      for (int g = 0; g < G; ++g) {
-        const int at = g * TEAM + threadIdx.x / ROWS, c = c0 + i * TEAM + at;
-        if (c < chunks)
+      for (int at = threadIdx.x / ROWS; at < kPieces; at += TEAM) {
+        const int c = (c0 + i * TEAM) / 2 + at;
+        if (c < chunks / 2)
           *reinterpret_cast<uint4*>(out + (int64_t)c * 256) =
               *reinterpret_cast<const uint4*>(turn + at * kPitch + threadIdx.x % ROWS * 16);
       }
@@ -110,7 +112,7 @@ __global__ void __launch_bounds__(kThreads)
   const int lane = threadIdx.x;
   const S* in = static_cast<const S*>(x) + row * f;
   int8_t* out = codes + int8_row(row, pitch);
-  Sixteen<T> v[C];
+  Some<T> v[C];
   uint32_t m = 0;
   for (int64_t c0 = 0; c0 < (HELD ? 1 : pitch); c0 += kThreads * C * kVec) {
 #pragma unroll
@@ -137,7 +139,8 @@ __global__ void __launch_bounds__(kThreads)
     for (int i = 0; i < C; ++i) {
       const int64_t c = c0 + (i * kThreads + lane) * kVec;
       if constexpr (!HELD) v[i].load(in, c, f);
-      if (c < pitch) *reinterpret_cast<uint4*>(out + c * 16) = v[i].codes(s, inv);
+      if (c < pitch)
+        *reinterpret_cast<typename Some<T>::Codes*>(out + c * 16) = v[i].codes(s, inv);
     }
   }
 }
@@ -163,7 +166,7 @@ __global__ void __launch_bounds__(kThreads) int8_rows_decode_kernel(const int8_t
     int8_t q[kVec];
     __builtin_memcpy(q, &w[i], sizeof(q));
     const float s = scales[row0 + i];
-    Sixteen<T> v;
+    Some<T> v;
 #pragma unroll
     for (int j = 0; j < kVec; ++j) v.v[j] = int8_value<T>(q[j], s);
     v.store(static_cast<S*>(x) + (row0 + i) * f, c, f);
@@ -239,7 +242,7 @@ __global__ void __launch_bounds__(kThreads) int8_weight_kernel(const void* W, in
                                                                float* scales) {
   typedef typename elem<T>::storage S;
   typedef S V4 __attribute__((ext_vector_type(4), aligned(sizeof(S))));
-  constexpr float kMagic = 12582912.f;  // see Sixteen::codes
+  constexpr float kMagic = 12582912.f;  // see Some::codes
   __shared__ __attribute__((aligned(16))) int8_t s_turn[2][kInt8Block * kTurnPitch];
   const int64_t e = blockIdx.z, n0 = (int64_t)blockIdx.x * kInt8Block;
   const int64_t blocks = int8_pitch(K) / kInt8Block, b0 = (int64_t)blockIdx.y * kRun;
@@ -397,14 +400,14 @@ int nt_int8_rows(int dtype, const void* x, int64_t rows, int64_t f, int8_t* code
       else if (chunks <= 512) one(int8_row_kernel<T, 2, true>);
       else if (chunks <= 1024) one(int8_row_kernel<T, 4, true>);
       else one(int8_row_kernel<T, 4, false>);
-    } else if (chunks <= 16) launch(int8_rows_kernel<T, 8, 16, 1, true>, 8, 16);
-    else if (chunks <= 32) launch(int8_rows_kernel<T, 8, 32, 1, true>, 8, 32);
-    else if (chunks <= 64) launch(int8_rows_kernel<T, 8, 64, 1, true>, 8, 64);
-    else if (chunks <= 128) launch(int8_rows_kernel<T, 8, 64, 2, true>, 8, 64);
-    else if (chunks <= 256) launch(int8_rows_kernel<T, 4, 128, 2, true>, 4, 128);
-    else if (chunks <= 512) launch(int8_rows_kernel<T, 4, 128, 4, true>, 4, 128);
-    else if (chunks <= 1024) launch(int8_rows_kernel<T, 4, 128, 8, true>, 4, 128);
-    else launch(int8_rows_kernel<T, 4, 128, 4, false>, 4, 128);
+    } else if (chunks <= 16) launch(int8_rows_kernel<T, 8, 32, 1, true>, 8, 32);
+    else if (chunks <= 32) launch(int8_rows_kernel<T, 8, 32, 2, true>, 8, 32);
+    else if (chunks <= 64) launch(int8_rows_kernel<T, 8, 64, 2, true>, 8, 64);
+    else if (chunks <= 128) launch(int8_rows_kernel<T, 8, 64, 4, true>, 8, 64);
+    else if (chunks <= 256) launch(int8_rows_kernel<T, 4, 128, 4, true>, 4, 128);
+    else if (chunks <= 512) launch(int8_rows_kernel<T, 4, 128, 8, true>, 4, 128);
+    else if (chunks <= 1024) launch(int8_rows_kernel<T, 4, 256, 8, true>, 4, 256);
+    else launch(int8_rows_kernel<T, 4, 256, 8, false>, 4, 256);
   });
   return launch_status();
 }

@@ -110,7 +110,7 @@ def test_no_rows():
 def test_malformed_offsets_stay_inside():
     """Offsets that fall, or lie outside [0, A], move no access out of the tensors."""
     w, _, _ = _weights(4, 128, 64, 0)
-    for A in (30, 300, 2000):
+    for A in (5, 30, 300, 2000):
         x = _rand(A, 128, dtype=torch.bfloat16)
         for off in ([-5, A + 9, 3, 2**31 - 1, 10], [A, 0, A, 0, A], [7, 7, 7, 7, 7]):
             o = torch.tensor(off, dtype=torch.int32, device="cuda")
@@ -150,6 +150,22 @@ def test_the_largest_sums():
         one = (torch.tensor(1.0) / 127.0).double()
         want = 127.0 * 127.0 * K * one * one
         assert bool(((got.cpu().double() - want).abs() <= 3.1 * U * want).all())
+
+
+@pytest.mark.parametrize("A,K", [(8, 2048), (8, 2049), (9, 1700), (4, 4096), (4, 4097), (1, 16384),
+                                 (1, 16385), (7, 2300)])
+def test_few_rows_are_rounded_as_many(A, K):
+    """Rows that the product brings to integers itself, in LDS, and just past those."""
+    w, _, _ = _weights(2, K, 130, 12)
+    x = _rand(80, K, dtype=torch.bfloat16, seed=13)
+    off = torch.tensor([0, A, A], dtype=torch.int32, device="cuda")
+    codes, scales = int8_rows(x)
+    want = torch.empty(80, 130, dtype=torch.bfloat16, device="cuda")
+    many = torch.tensor([0, 80, 80], dtype=torch.int32, device="cuda")
+    capi.call("nt_int8_grouped_gemm", capi.NT_BF16, codes.data_ptr(), scales.data_ptr(),
+              many.data_ptr(), w.codes.data_ptr(), w.scale.data_ptr(), 2, 80, K, 130,
+              want.data_ptr(), capi.current_stream())
+    assert torch.equal(int8_grouped_gemm_fn(x[:A], w, off), want[:A])
 
 
 def test_a_row_is_the_same_in_any_batch():

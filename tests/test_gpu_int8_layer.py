@@ -81,6 +81,19 @@ def test_few_tokens(dtype, ffn, T, d, f, E, k):
     _check_few(x, router, None, w, k)
 
 
+@pytest.mark.parametrize("ffn", ["swiglu", "gelu"])
+@pytest.mark.parametrize("T,d,f,E,k", [(8, 512, 256, 64, 8), (8, 2048, 2048, 16, 2),
+                                       (8, 256, 2049, 8, 2), (9, 256, 2048, 8, 1),
+                                       (4, 4096, 4096, 8, 2), (4, 4096, 4096, 16, 4),
+                                       (1, 16384, 200, 17, 17), (1, 128, 16385, 4, 1),
+                                       (2, 16, 16, 1024, 32)])
+def test_where_the_rows_are_rounded(ffn, T, d, f, E, k):
+    """Around the limits of the rows that the products round for themselves, of the experts whose
+    sum is made by the last of them, and of the memory that a workgroup then holds."""
+    x, router, w = _case(T, d, f, E, torch.bfloat16, ffn, seed=T)
+    _check_few(x, router, None, w, k)
+
+
 def test_logits_of_the_program():
     x, _, w = _case(9, 128, 256, 8, torch.bfloat16, "swiglu")
     logits = torch.randn(9, 8, generator=torch.Generator().manual_seed(1)).cuda()
@@ -122,8 +135,9 @@ def test_no_tokens_and_limits():
             moe_few_tokens(x, w, 2)
 
 
-def test_a_nan_token_stays_its_own():
-    x, router, w = _case(20, 128, 256, 4, torch.bfloat16, "swiglu")
+@pytest.mark.parametrize("T", [6, 20])
+def test_a_nan_token_stays_its_own(T):
+    x, router, w = _case(T, 128, 256, 4, torch.bfloat16, "swiglu")
     logits = (x.float() @ router.t()).contiguous()
     with torch.no_grad():
         want = moe_few_tokens(x, w, 2, logits=logits)[0]
@@ -131,7 +145,7 @@ def test_a_nan_token_stays_its_own():
         bad[4, 9] = float("inf")
         got = moe_few_tokens(bad, w, 2, logits=logits)[0]
     assert bool(got[4].isnan().all())
-    keep = [i for i in range(20) if i != 4]
+    keep = [i for i in range(T) if i != 4]
     assert torch.equal(got[keep], want[keep])
 
 
