@@ -62,19 +62,19 @@ int nt_int8_grouped_gemm(int dtype, const int8_t* x, const float* x_scales,
 
 /* Both projections of a gated block, its activation and the product:
  * hidden = silu(x @ W_gate[e]) * (x @ W_val[e]) in float32, rounded once. gate and
- * value [A, N] are what a backward needs (both NULL: not written). */
+ * value [A, N] in float32 are what a backward needs (both NULL: not written). */
 int nt_int8_grouped_gemm_swiglu(int dtype, const int8_t* x, const float* x_scales,
                                 const int32_t* offsets, const int8_t* w_gate,
                                 const float* gate_scales, const int8_t* w_val,
                                 const float* val_scales, int32_t E, int64_t A, int64_t K,
-                                int64_t N, void* hidden, void* gate, void* value,
+                                int64_t N, void* hidden, float* gate, float* value,
                                 hipStream_t stream);
 
-/* act = gelu(x @ W[e]) (erf), and gelu' of the same (NULL: not written). */
+/* act = gelu(x @ W[e]) (erf), and gelu' of the same in float32 (NULL: not written). */
 int nt_int8_grouped_gemm_gelu(int dtype, const int8_t* x, const float* x_scales,
                               const int32_t* offsets, const int8_t* w, const float* w_scales,
                               int32_t E, int64_t A, int64_t K, int64_t N, void* act,
-                              void* act_grad, hipStream_t stream);
+                              float* act_grad, hipStream_t stream);
 
 /* The same three from rows x [A, K] of dtype, which they bring to 8 bits themselves:
  * the bits of nt_int8_rows and the product. The workspace (16-byte aligned, contents
@@ -85,35 +85,49 @@ int nt_int8_linear(int dtype, const void* x, const int32_t* offsets, const int8_
                    void* ws, size_t ws_bytes, hipStream_t stream);
 int nt_int8_linear_swiglu(int dtype, const void* x, const int32_t* offsets, const int8_t* w_gate,
                           const float* gate_scales, const int8_t* w_val, const float* val_scales,
-                          int32_t E, int64_t A, int64_t K, int64_t N, void* hidden, void* gate,
-                          void* value, void* ws, size_t ws_bytes, hipStream_t stream);
+                          int32_t E, int64_t A, int64_t K, int64_t N, void* hidden, float* gate,
+                          float* value, void* ws, size_t ws_bytes, hipStream_t stream);
 int nt_int8_linear_gelu(int dtype, const void* x, const int32_t* offsets, const int8_t* w,
                         const float* w_scales, int32_t E, int64_t A, int64_t K, int64_t N,
-                        void* act, void* act_grad, void* ws, size_t ws_bytes,
+                        void* act, float* act_grad, void* ws, size_t ws_bytes,
                         hipStream_t stream);
 
-/* Gradients through frozen 8-bit weights, for f16 and bf16 rows and N a multiple of 8
- * (otherwise: nt_int8_weight_decode and nt_grouped_gemm_dx); dout 16-byte aligned. The
- * rounding of x to 8 bits is passed straight through; weights are the values held,
- * rounded to dtype. dx = dout @ W[e]^T [A, K]; dx2: the sum of two such products;
- * dx_gelu: dh = that times act_grad; dx_swiglu: dgate and dvalue of dhidden = that,
- * with gate and value as the forward kept them, all [A, K]. Sums and epilogues in
- * float32, one rounding. */
+/* dx = dout @ W[e]^T [A, K] for f16 and bf16 (f32: nt_int8_weight_decode and
+ * nt_grouped_gemm_dx). The rounding of x to 8 bits is passed straight through; the
+ * weights are the values held, rounded to dtype; sums in float32, one rounding. Row r
+ * of dout is at r * dout_pitch, a multiple of 8 from N on; columns from N to the next
+ * multiple of 8 are read and must be finite. dout is 16-byte aligned. N <= 2^20. */
 int nt_int8_grouped_gemm_dx(int dtype, const int8_t* w, const float* w_scales,
-                            const int32_t* offsets, const void* dout, int32_t E, int64_t A,
-                            int64_t K, int64_t N, void* dx, hipStream_t stream);
-int nt_int8_grouped_gemm_dx2(int dtype, const int8_t* w1, const float* scales1, const int8_t* w2,
-                             const float* scales2, const int32_t* offsets, const void* dout1,
-                             const void* dout2, int32_t E, int64_t A, int64_t K, int64_t N,
-                             void* dx, hipStream_t stream);
+                            const int32_t* offsets, const void* dout, int64_t dout_pitch,
+                            int32_t E, int64_t A, int64_t K, int64_t N, void* dx,
+                            hipStream_t stream);
+
+/* The gradient through a feed-forward block, in two products. The first takes dout to
+ * the gradient dz of the up projections, that times the float32 act_grad (dx_gelu), or
+ * by SwiGLU's from gate and value as the forward kept them (dx_swiglu), where w is the
+ * down projection [E, K, N]. dz is not rounded to dtype: what is written are the terms
+ * of dz times the up projection's scales [E, K], as two bfloat16 numbers whose sum it
+ * is to 2^-17. nt_int8_terms_bytes(A, K) is their size, 16-byte aligned, laid out
+ * [2][A][nt_int8_pitch(K)], columns from K on zero to the next multiple of 16 (the
+ * rest is not written, nor read). The second takes them times the up projections'
+ * integers (w2 and terms2 NULL: of one) to dx [A, K], rounded once to dtype; N is the
+ * terms' width. Of dtype f16 or bf16, as above. */
+size_t nt_int8_terms_bytes(int64_t A, int64_t K);
 int nt_int8_grouped_gemm_dx_gelu(int dtype, const int8_t* w, const float* w_scales,
-                                 const int32_t* offsets, const void* dout, const void* act_grad,
-                                 int32_t E, int64_t A, int64_t K, int64_t N, void* dh,
+                                 const int32_t* offsets, const void* dout, int64_t dout_pitch,
+                                 const float* act_grad, const float* up_scales, int32_t E,
+                                 int64_t A, int64_t K, int64_t N, void* terms,
                                  hipStream_t stream);
 int nt_int8_grouped_gemm_dx_swiglu(int dtype, const int8_t* w, const float* w_scales,
-                                   const int32_t* offsets, const void* dout, const void* gate,
-                                   const void* value, int32_t E, int64_t A, int64_t K, int64_t N,
-                                   void* dgate, void* dvalue, hipStream_t stream);
+                                   const int32_t* offsets, const void* dout, int64_t dout_pitch,
+                                   const float* gate, const float* value,
+                                   const float* gate_scales, const float* val_scales, int32_t E,
+                                   int64_t A, int64_t K, int64_t N, void* gate_terms,
+                                   void* val_terms, hipStream_t stream);
+int nt_int8_grouped_gemm_dx_terms(int dtype, const int8_t* w, const int8_t* w2,
+                                  const int32_t* offsets, const void* terms, const void* terms2,
+                                  int32_t E, int64_t A, int64_t K, int64_t N, void* dx,
+                                  hipStream_t stream);
 
 /* nt_moe_few_tokens on 8-bit weights (w_val NULL: GELU): tokens and hidden values go
  * to 8 bits row by row, the hidden ones from their values in dtype. Everything else,

@@ -318,18 +318,19 @@ __global__ void __launch_bounds__(KW* kWave)
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
           if (n + q >= a.N) break;
-          S o[3];
+          S o;
+          float o2, o3;
           const float p = (float)sum[0][q] * sw[0][q] * sx;
           const float p2 = MATS == 2 ? (float)sum[MATS - 1][q] * sw[MATS - 1][q] * sx : 0.f;
-          int8_epilogue<T, EPI>(p, p2, o[0], o[1], o[2]);
+          int8_epilogue<T, EPI>(p, p2, o, o2, o3);
           if constexpr (ARRIVE)  // through the L2s: the workgroups run on any XCD
             __hip_atomic_store(static_cast<float*>(a.out) + at + n + q, p, __ATOMIC_RELAXED,
                                __HIP_MEMORY_SCOPE_AGENT);
           else
-            static_cast<S*>(a.out)[at + n + q] = o[0];
+            static_cast<S*>(a.out)[at + n + q] = o;
           if (EPI != kInt8Plain && a.out2 != nullptr) {
-            static_cast<S*>(a.out2)[at + n + q] = o[1];
-            if (EPI == kInt8SwiGLU) static_cast<S*>(a.out3)[at + n + q] = o[2];
+            a.out2[at + n + q] = o2;
+            if (EPI == kInt8SwiGLU) a.out3[at + n + q] = o3;
           }
         }
       }
@@ -410,7 +411,7 @@ void launch_stream(const Int8Gemm& a, int64_t experts, const C& chosen, hipStrea
 }
 
 // Rows of `width` values that workgroups bring to integers themselves: up to eight,
-// and 16,384 values in all (four a thread and pass; see the measurements at the end).
+// and 16,384 values in all.
 bool own_rows(int64_t rows, int64_t width) {
   return rows <= kOwnRows && rows * int8_pitch(width) <= 16384;
 }

@@ -104,16 +104,20 @@ __device__ __forceinline__ void int8_store(const i32x4 (&acc)[AB][EPI == kInt8Sw
       if (m >= rows || n >= a.N) continue;
       const int64_t row = row0 + m;
       const float sx = a.x_scales[row];
-      S o[3][16];
+      S o[16];
+      float o2[16], o3[16];
 #pragma unroll
       for (int j = 0; j < 16; ++j)
         int8_epilogue<T, EPI>((float)acc[b][0][c][j / 4][j % 4] * sw[0][j] * sx,
                               MATS == 2 ? (float)acc[b][MATS - 1][c][j / 4][j % 4] *
                                               sw[MATS - 1][j] * sx
                                         : 0.f,
-                              o[0][j], o[1][j], o[2][j]);
-      int8_put<T, EPI == kInt8Plain ? 1 : EPI == kInt8SwiGLU ? 3 : 2>(
-          a, row * a.N + n, (int)(a.N - n < 16 ? a.N - n : 16), o);
+                              o[j], o2[j], o3[j]);
+      const int64_t at = row * a.N + n;
+      const int width = (int)(a.N - n < 16 ? a.N - n : 16);
+      int8_put(static_cast<S*>(a.out) + at, width, o);
+      if (EPI != kInt8Plain && a.out2 != nullptr) int8_put(a.out2 + at, width, o2);
+      if (EPI == kInt8SwiGLU && a.out3 != nullptr) int8_put(a.out3 + at, width, o3);
     }
   }
 }
@@ -382,8 +386,8 @@ int nt_int8_linear(int dtype, const void* x, const int32_t* offsets, const int8_
 
 int nt_int8_linear_swiglu(int dtype, const void* x, const int32_t* offsets, const int8_t* w_gate,
                           const float* gate_scales, const int8_t* w_val, const float* val_scales,
-                          int32_t E, int64_t A, int64_t K, int64_t N, void* hidden, void* gate,
-                          void* value, void* ws, size_t ws_bytes, hipStream_t stream) {
+                          int32_t E, int64_t A, int64_t K, int64_t N, void* hidden, float* gate,
+                          float* value, void* ws, size_t ws_bytes, hipStream_t stream) {
   Int8Gemm a = {};
   a.values = x, a.offsets = offsets, a.w = w_gate, a.w_scales = gate_scales;
   a.w2 = w_val, a.w2_scales = val_scales;
@@ -394,7 +398,7 @@ int nt_int8_linear_swiglu(int dtype, const void* x, const int32_t* offsets, cons
 
 int nt_int8_linear_gelu(int dtype, const void* x, const int32_t* offsets, const int8_t* w,
                         const float* w_scales, int32_t E, int64_t A, int64_t K, int64_t N,
-                        void* act, void* act_grad, void* ws, size_t ws_bytes,
+                        void* act, float* act_grad, void* ws, size_t ws_bytes,
                         hipStream_t stream) {
   Int8Gemm a = {};
   a.values = x, a.offsets = offsets, a.w = w, a.w_scales = w_scales;
@@ -417,7 +421,7 @@ int nt_int8_grouped_gemm_swiglu(int dtype, const int8_t* x, const float* x_scale
                                 const int32_t* offsets, const int8_t* w_gate,
                                 const float* gate_scales, const int8_t* w_val,
                                 const float* val_scales, int32_t E, int64_t A, int64_t K,
-                                int64_t N, void* hidden, void* gate, void* value,
+                                int64_t N, void* hidden, float* gate, float* value,
                                 hipStream_t stream) {
   Int8Gemm a = {};
   a.x = x, a.x_scales = x_scales, a.offsets = offsets, a.w = w_gate, a.w_scales = gate_scales;
@@ -429,7 +433,7 @@ int nt_int8_grouped_gemm_swiglu(int dtype, const int8_t* x, const float* x_scale
 int nt_int8_grouped_gemm_gelu(int dtype, const int8_t* x, const float* x_scales,
                               const int32_t* offsets, const int8_t* w, const float* w_scales,
                               int32_t E, int64_t A, int64_t K, int64_t N, void* act,
-                              void* act_grad, hipStream_t stream) {
+                              float* act_grad, hipStream_t stream) {
   Int8Gemm a = {};
   a.x = x, a.x_scales = x_scales, a.offsets = offsets, a.w = w, a.w_scales = w_scales;
   a.E = E, a.A = A, a.K = K, a.N = N, a.out = act, a.out2 = act_grad;

@@ -19,8 +19,8 @@ struct Int8Gemm {
   const float *w_scales, *w2_scales;  // [E, N]
   int32_t E;
   int64_t A, K, N;
-  void* out;         // [A, N]; hidden, act
-  void *out2, *out3;  // gate, value; gelu' (null: not written)
+  void* out;          // [A, N]; hidden, act
+  float *out2, *out3;  // gate, value; gelu' (null: not written)
   int32_t ntn;
 };
 
@@ -87,63 +87,51 @@ __device__ __forceinline__ float normal_cdf<float>(float x, float& bell) {
   return 0.5f * erfcf(x * -0.70710678118654752f);
 }
 
-// The outputs of one column from its scaled sums p (and p2, the value).
+// The outputs of one column from its scaled sums p (and p2, the value). What a backward
+// needs stays in float32: rounded to 16 bits it would be half of the gradient's error.
 template <typename T, int EPI>
 __device__ __forceinline__ void int8_epilogue(float p, float p2, typename elem<T>::storage& o,
-                                              typename elem<T>::storage& o2,
-                                              typename elem<T>::storage& o3) {
+                                              float& o2, float& o3) {
   if constexpr (EPI == kInt8Plain) {
     o = to_bits<T>(p);
   } else if constexpr (EPI == kInt8SwiGLU) {
     o = to_bits<T>(p * sigmoid_of<T>(p) * p2);
-    o2 = to_bits<T>(p);
-    o3 = to_bits<T>(p2);
+    o2 = p;
+    o3 = p2;
   } else {
     float bell;
     const float c = normal_cdf<T>(p, bell);
     o = to_bits<T>(p * c);
-    o2 = to_bits<T>(fmaf(p, bell * 0.39894228040143268f, c));
+    o2 = fmaf(p, bell * 0.39894228040143268f, c);
   }
 }
 
-// n (at most 16) neighbouring columns of every output, at element `at`.
-template <typename T, int OUTS>
-__device__ __forceinline__ void int8_put(const Int8Gemm& a, int64_t at, int n,
-                                         const typename elem<T>::storage (&o)[3][16]) {
-  typedef typename elem<T>::storage S;
-#pragma unroll
-  for (int i = 0; i < OUTS; ++i) {
-    S* p = static_cast<S*>(i == 0 ? a.out : i == 1 ? a.out2 : a.out3);
-    if (i > 0 && p == nullptr) continue;
-    p += at;
-    if (n == 16) {
-      typedef S V __attribute__((ext_vector_type(16 / sizeof(S)), aligned(sizeof(S))));
-      V v[sizeof(S)];
-      __builtin_memcpy(v, o[i], sizeof(v));
-#pragma unroll
-      for (int j = 0; j < (int)sizeof(S); ++j)
-        __builtin_nontemporal_store(v[j], reinterpret_cast<V*>(p) + j);
-    } else {
-#pragma unroll
-      for (int j = 0; j < 16; ++j)
-        if (j < n) p[j] = o[i][j];
-    }
-  }
-}
-
-// n (at most 16) neighbouring values from element `at` on, zeros behind them.
-template <typename T>
-__device__ __forceinline__ void int8_get(const void* p, int64_t at, int n,
-                                         typename elem<T>::storage (&v)[16]) {
-  typedef typename elem<T>::storage S;
-  typedef S V __attribute__((ext_vector_type(16), aligned(sizeof(S))));
-  const S* s = static_cast<const S*>(p) + at;
+// n (at most 16) neighbouring columns of an output.
+template <typename S>
+__device__ __forceinline__ void int8_put(S* p, int n, const S (&o)[16]) {
   if (n == 16) {
-    const V u = *reinterpret_cast<const V*>(s);
+    typedef S V __attribute__((ext_vector_type(16 / sizeof(S)), aligned(sizeof(S))));
+    V v[sizeof(S)];
+    __builtin_memcpy(v, o, sizeof(v));
+#pragma unroll
+    for (int j = 0; j < (int)sizeof(S); ++j)
+      __builtin_nontemporal_store(v[j], reinterpret_cast<V*>(p) + j);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 16; ++j)
+      if (j < n) p[j] = o[j];
+  }
+}
+
+// n (at most 16) neighbouring values, zeros behind them.
+__device__ __forceinline__ void int8_get(const float* p, int n, float (&v)[16]) {
+  typedef float V __attribute__((ext_vector_type(16), aligned(4)));
+  if (n == 16) {
+    const V u = *reinterpret_cast<const V*>(p);
     __builtin_memcpy(v, &u, sizeof(v));
   } else {
 #pragma unroll
-    for (int j = 0; j < 16; ++j) v[j] = j < n ? s[j] : S(0);
+    for (int j = 0; j < 16; ++j) v[j] = j < n ? p[j] : 0.f;
   }
 }
 

@@ -1,14 +1,20 @@
 // Gradients through frozen 8-bit weights, for 16-bit activations:
 //
-//   dX[a, k] = sum_n dOut[a, n] w[e, n, k],   w = q s[e, n] rounded to the type
+//   dX[a, k] = sum_n dOut[a, n] w[e, n, k],   w = q s[e, n]
 //
 // on the 16-bit matrix cores. The weights are read as integers, a quarter of what
 // bringing them to 16 bits first would read and write, and turned on the way to LDS:
 // a thread's 64 bytes are 16 values of k for four neighbouring n, and it writes for
 // each k its four n. (v + 128) s - 128 s as one fused multiply-add rounds q s once.
 //
-// The epilogues keep float32 up to their one rounding: the gradient of the hidden
-// values is not rounded before the activation's gradient is taken of it.
+// Through a feed-forward block a gradient would round five times on the way: weights,
+// activation's gradient and product with it, weights, output; in float16 4.7e-4 of
+// the gradient, 2.1e-4 of that its output's. Three of these are taken out: what the
+// forward keeps and the epilogue are float32, the gradient of the hidden values goes
+// on as two bfloat16 terms, times the next weights' scales, and these weights are
+// their integers, exact in bfloat16. Both terms meet the same operands in LDS, a step
+// each, so the second costs matrix instructions but no weights (14,312 rows of 768 by
+// 128 experts' 2,048: 116 us with one rounded term, 150 with two).
 #include <algorithm>
 #include <type_traits>
 
@@ -18,12 +24,17 @@
 namespace nt {
 namespace {
 
-enum Int8GradEpilogue { kGradPlain = 0, kGradDual = 1, kGradGelu = 2, kGradSwiGLU = 3 };
+// Terms, TermsDual: from two terms a value and the weights' integers, out for one or
+// two matrices; Gelu, SwiGLU: to such terms.
+enum Int8GradEpilogue { kGradPlain, kGradGelu, kGradSwiGLU, kGradTerms, kGradTermsDual };
 
 struct Int8Grad {
-  Int8Gemm rows;           // offsets, E, A; K: output columns, N: the reduction
-  const void *dout, *dout2;  // [A, N]; of the second matrix
-  const void *aux, *aux2;    // gelu' or gate, value [A, K]
+  Int8Gemm rows;             // offsets, E, A; K: output columns, N: the reduction
+  const void *dout, *dout2;  // [A, N] or terms; of the second matrix
+  int64_t pitch;             // of dout's rows
+  const float *aux, *aux2;   // gelu' or gate, value [A, K]
+  const float *next, *next2;  // scales of the weights that the terms meet [E, K]
+  void* terms2;
 };
 
 constexpr int kGradBM = 128, kGradBN = 256, kGradWaves = 4;
@@ -34,10 +45,33 @@ constexpr int kGradThreads = kGradWaves * kWave;
 // < 4), whose swizzles are all eight values twice: its reads touch every bank once.
 __device__ __forceinline__ int turned_swizzle(int k) { return (k >> 1 & 1) | (k >> 4 & 3) << 1; }
 
+// 16 values of row `row` from column n on as two terms, the second one what the first
+// leaves: a value of 2^-100 or more to 2^-17. (Of an infinity the second is NaN; a
+// gradient with one is no more finite as their sum.)
+__device__ __forceinline__ void put_terms(uint16_t* terms, int64_t row, int64_t rows,
+                                          int64_t pitch, int64_t n, const float (&z)[16]) {
+  uint32_t w[2][8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    w[0][j] = pack2<bf16>(z[2 * j], z[2 * j + 1]);
+    const float first[2] = {__uint_as_float(w[0][j] << 16),
+                            __uint_as_float(w[0][j] & 0xffff0000u)};
+    w[1][j] = pack2<bf16>(z[2 * j] - first[0], z[2 * j + 1] - first[1]);
+  }
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    uint4* p = reinterpret_cast<uint4*>(terms + (i * rows + row) * pitch + n);
+    p[0] = make_uint4(w[i][0], w[i][1], w[i][2], w[i][3]);
+    p[1] = make_uint4(w[i][4], w[i][5], w[i][6], w[i][7]);
+  }
+}
+
 template <typename T, int EPI>
 __global__ void __launch_bounds__(kGradThreads, 2) int8_grad_kernel(Int8Grad g) {
   typedef typename elem<T>::storage S;
-  typedef typename mfma_op<T>::vec vec;
+  constexpr bool TERMS = EPI == kGradTerms || EPI == kGradTermsDual;
+  typedef std::conditional_t<TERMS, bf16, T> M;
+  typedef typename mfma_op<M>::vec vec;
   const Int8Gemm& a = g.rows;
   constexpr int BM = kGradBM, BN = kGradBN, WGN = 2;
   constexpr int AB = BM / 2 / 16, CG = BN / 2 / 64;  // of a wave: 64 rows by 128 columns
@@ -64,9 +98,10 @@ __global__ void __launch_bounds__(kGradThreads, 2) int8_grad_kernel(Int8Grad g) 
   const int wm = wave / WGN, wn = wave % WGN;
   const int64_t kpitch = int8_pitch(a.K), kblocks = kpitch / kInt8Block;
   const int64_t groups = int8_groups(a.N);
-  const int nk1 = (int)ceil_div(a.N, (int64_t)64), nk = EPI == kGradDual ? 2 * nk1 : nk1;
+  const int nk1 = (int)ceil_div(a.N, (int64_t)64), nw = EPI == kGradTermsDual ? 2 * nk1 : nk1;
+  const int nk = TERMS ? 2 * nw : nw;  // a step a term
   TA ta;
-  ta.init(a.N, wave, lane);
+  ta.init(g.pitch, wave, lane);
   FragReader<BM, true, AB, 64> fa;
   fa.init(wm * 64, lane);
   // thread: 16 values of k, four n from n0 on
@@ -89,25 +124,36 @@ __global__ void __launch_bounds__(kGradThreads, 2) int8_grad_kernel(Int8Grad g) 
 
     uint4 w[4];
     float4 s;
-    auto fetch = [&](int kt, char* lds) {
-      const bool second = EPI == kGradDual && kt >= nk1;
-      const int64_t nb = second ? kt - nk1 : kt;
-      const int8_t* m = second ? a.w2 : a.w;
-      const float* sc = second ? a.w2_scales : a.w_scales;
-      const int8_t* at = m + ((e * groups + nb) * kblocks + (has ? kb : kblocks - 1)) * 4096 +
+    auto fetch_weights = [&](int step) {
+      const bool second = EPI == kGradTermsDual && step >= nk1;
+      const int64_t nb = second ? step - nk1 : step;
+      const int8_t* at = (second ? a.w2 : a.w) +
+                         ((e * groups + nb) * kblocks + (has ? kb : kblocks - 1)) * 4096 +
                          lane * 64;
 #pragma unroll
       for (int i = 0; i < 4; ++i) w[i] = reinterpret_cast<const uint4*>(at)[i];
-      const int64_t n = nb * 64 + n0;
-      s = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (n < a.N) {  // (N is a multiple of 8)
-        typedef float V4 __attribute__((ext_vector_type(4), aligned(4)));
-        const V4 v = *reinterpret_cast<const V4*>(sc + e * a.N + n);
-        s = make_float4(v[0], v[1], v[2], v[3]);
+      if constexpr (!TERMS) {
+        const int64_t n = nb * 64 + n0;
+        const float* sc = a.w_scales + e * a.N + n;
+        if (n + 4 <= a.N) {
+          typedef float V4 __attribute__((ext_vector_type(4), aligned(4)));
+          const V4 v = *reinterpret_cast<const V4*>(sc);
+          s = make_float4(v[0], v[1], v[2], v[3]);
+        } else {
+          s = make_float4(n < a.N ? sc[0] : 0.f, n + 1 < a.N ? sc[1] : 0.f,
+                          n + 2 < a.N ? sc[2] : 0.f, 0.f);
+        }
       }
-      const int64_t kv = a.N - nb * 64 < 64 ? a.N - nb * 64 : 64;
-      const S* d = static_cast<const S*>(second ? g.dout2 : g.dout) + row0 * a.N + nb * 64;
-      ta.issue(d, ((rows - 1) * a.N + kv) * 2, lds, kv, wave);
+    };
+    auto fetch_rows = [&](int kt, char* lds) {
+      const int step = TERMS ? kt / 2 : kt;
+      const bool second = EPI == kGradTermsDual && step >= nk1;
+      const int64_t nb = second ? step - nk1 : step;
+      const int64_t left = round_up(a.N, (int64_t)(TERMS ? 16 : 8)) - nb * 64;
+      const int64_t kv = left < 64 ? left : 64;
+      const uint16_t* d = static_cast<const uint16_t*>(second ? g.dout2 : g.dout) +
+                          ((TERMS ? kt % 2 * a.A : 0) + row0) * g.pitch + nb * 64;
+      ta.issue(d, ((rows - 1) * g.pitch + kv) * 2, lds, kv, wave);
     };
     auto turn = [&]() {
       const float sc[4] = {s.x, s.y, s.z, s.w};
@@ -123,12 +169,14 @@ __global__ void __launch_bounds__(kGradThreads, 2) int8_grad_kernel(Int8Grad g) 
         float v[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-          v[i] = fmaf((float)(u[i][j / 4] >> (8 * (j % 4)) & 255u), sc[i], -128.f * sc[i]);
+          v[i] = TERMS ? (float)(u[i][j / 4] >> (8 * (j % 4)) & 255u) - 128.f
+                       : fmaf((float)(u[i][j / 4] >> (8 * (j % 4)) & 255u), sc[i],
+                              -128.f * sc[i]);
         const int k = wave * 64 + 16 * g4 + j;
         *reinterpret_cast<uint2*>(turned + k * 128 +
                                   ((2 * i4 + (t4 >> 1)) ^ turned_swizzle(k)) * 16 +
                                   (t4 & 1) * 8) =
-            make_uint2(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]));
+            make_uint2(pack2<M>(v[0], v[1]), pack2<M>(v[2], v[3]));
       }
     };
 
@@ -140,12 +188,17 @@ __global__ void __launch_bounds__(kGradThreads, 2) int8_grad_kernel(Int8Grad g) 
 #pragma unroll
         for (int t = 0; t < 4; ++t) acc[b][c][t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
     __syncthreads();  // the tile before is read no more
-    fetch(0, smem);
+    fetch_weights(0);
+    fetch_rows(0, smem);
     for (int kt = 0; kt < nk; ++kt) {
       wait_vmcnt<0>();  // this step's rows are in LDS, its weights in registers
-      turn();
+      if (!TERMS || kt % 2 == 0) turn();
       __syncthreads();
-      if (kt + 1 < nk) fetch(kt + 1, smem + (kt + 1 & 1) * kA);
+      if (kt + 1 < nk) {
+        if (!TERMS) fetch_weights(kt + 1);
+        else if (kt % 2 == 1) fetch_weights(kt / 2 + 1);
+        fetch_rows(kt + 1, smem + (kt + 1 & 1) * kA);
+      }
       const char* sa = smem + (kt & 1) * kA;
 #pragma unroll
       for (int ks = 0; ks < 2; ++ks) {
@@ -160,7 +213,7 @@ __global__ void __launch_bounds__(kGradThreads, 2) int8_grad_kernel(Int8Grad g) 
             const vec y = *reinterpret_cast<const vec*>(
                 turned + k * 128 + ((4 * ks + (lane >> 4)) ^ turned_swizzle(k)) * 16);
 #pragma unroll
-            for (int b = 0; b < AB; ++b) acc[b][c][t] = mfma_op<T>::run(y, x[b], acc[b][c][t]);
+            for (int b = 0; b < AB; ++b) acc[b][c][t] = mfma_op<M>::run(y, x[b], acc[b][c][t]);
           }
       }
       __syncthreads();
@@ -175,23 +228,34 @@ __global__ void __launch_bounds__(kGradThreads, 2) int8_grad_kernel(Int8Grad g) 
         const int m = wm * 64 + 16 * b + (lane & 15);
         if (m >= rows || n >= a.K) continue;
         const int64_t at = (row0 + m) * a.K + n;
-        S o[3][16], x1[16], x2[16];
-        if constexpr (EPI == kGradGelu || EPI == kGradSwiGLU) int8_get<T>(g.aux, at, width, x1);
-        if constexpr (EPI == kGradSwiGLU) int8_get<T>(g.aux2, at, width, x2);
-#pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          const float d = acc[b][c][j / 4][j % 4];
-          if constexpr (EPI == kGradGelu) {
-            o[0][j] = to_bits<T>(d * elem<T>::load(x1[j]));
-          } else if constexpr (EPI == kGradSwiGLU) {
-            const float z = elem<T>::load(x1[j]), sg = sigmoid_of<T>(z);
-            o[0][j] = to_bits<T>(d * elem<T>::load(x2[j]) * sg * (1.f + z * (1.f - sg)));
-            o[1][j] = to_bits<T>(d * z * sg);
-          } else {
-            o[0][j] = to_bits<T>(d);
+        if constexpr (EPI == kGradGelu || EPI == kGradSwiGLU) {
+          float x1[16], x2[16], s1[16], s2[16], z1[16], z2[16];
+          int8_get(g.aux + at, width, x1);
+          int8_get(g.next + e * a.K + n, width, s1);
+          if constexpr (EPI == kGradSwiGLU) {
+            int8_get(g.aux2 + at, width, x2);
+            int8_get(g.next2 + e * a.K + n, width, s2);
           }
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            const float d = acc[b][c][j / 4][j % 4];
+            if constexpr (EPI == kGradGelu) {
+              z1[j] = j < width ? d * x1[j] * s1[j] : 0.f;
+            } else {
+              const float z = x1[j], sg = sigmoid_of<T>(z);
+              z1[j] = j < width ? d * x2[j] * sg * (1.f + z * (1.f - sg)) * s1[j] : 0.f;
+              z2[j] = j < width ? d * z * sg * s2[j] : 0.f;
+            }
+          }
+          put_terms(static_cast<uint16_t*>(a.out), row0 + m, a.A, kpitch, n, z1);
+          if constexpr (EPI == kGradSwiGLU)
+            put_terms(static_cast<uint16_t*>(g.terms2), row0 + m, a.A, kpitch, n, z2);
+        } else {
+          S o[16];
+#pragma unroll
+          for (int j = 0; j < 16; ++j) o[j] = to_bits<T>(acc[b][c][j / 4][j % 4]);
+          int8_put(static_cast<S*>(a.out) + at, width, o);
         }
-        int8_put<T, EPI == kGradSwiGLU ? 2 : 1>(a, at, width, o);
       }
     }
   }
@@ -199,18 +263,21 @@ __global__ void __launch_bounds__(kGradThreads, 2) int8_grad_kernel(Int8Grad g) 
 
 int run_grad(int dtype, int epi, Int8Grad g, hipStream_t s) {
   Int8Gemm& a = g.rows;
+  const bool terms = epi >= kGradTerms, to_terms = epi == kGradGelu || epi == kGradSwiGLU;
   if (dtype != NT_F16 && dtype != NT_BF16) return NT_ERR_DTYPE;
-  if (a.E < 1 || a.A < 0 || a.K < 1 || a.N < 1 || a.N % 8 != 0) return NT_ERR_INVALID_ARG;
+  if (a.E < 1 || a.A < 0 || a.K < 1 || a.N < 1) return NT_ERR_INVALID_ARG;
   if (a.E > NT_MAX_EXPERTS) return NT_ERR_TOO_MANY_EXPERTS;
   if (a.K > kInt8MaxK || a.N > 1 << 20 || a.A > kInt8MaxRows) return NT_ERR_TOO_LARGE;
+  if (terms) g.pitch = int8_pitch(a.N);
+  if (g.pitch > 1 << 20) return NT_ERR_TOO_LARGE;  // a tile's rows within 32 bits
   if (a.A == 0) return NT_OK;
-  auto bad = [](const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 != 0; };
-  if (g.dout == nullptr || a.w == nullptr || a.w_scales == nullptr || a.out == nullptr ||
-      (a.offsets == nullptr && a.E != 1) || bad(g.dout) || bad(a.w) ||
-      (epi == kGradDual && (g.dout2 == nullptr || a.w2 == nullptr || a.w2_scales == nullptr ||
-                            bad(g.dout2) || bad(a.w2))) ||
-      (epi >= kGradGelu && g.aux == nullptr) ||
-      (epi == kGradSwiGLU && (g.aux2 == nullptr || a.out2 == nullptr)))
+  auto bad = [](const void* p) { return p == nullptr || reinterpret_cast<uintptr_t>(p) % 16 != 0; };
+  const bool two = epi == kGradTermsDual;
+  if (g.pitch < a.N || g.pitch % 8 != 0 || bad(g.dout) || bad(a.w) || a.out == nullptr ||
+      (a.offsets == nullptr && a.E != 1) || (!terms && a.w_scales == nullptr) ||
+      (two && (bad(g.dout2) || bad(a.w2))) ||
+      (to_terms && (g.aux == nullptr || g.next == nullptr || bad(a.out))) ||
+      (epi == kGradSwiGLU && (g.aux2 == nullptr || g.next2 == nullptr || bad(g.terms2))))
     return NT_ERR_INVALID_ARG;
   a.ntn = (int32_t)ceil_div(a.K, (int64_t)kGradBN);
   const int64_t tiles = (ceil_div(a.A, (int64_t)kGradBM) + a.E - 1) * a.ntn;
@@ -222,9 +289,10 @@ int run_grad(int dtype, int epi, Int8Grad g, hipStream_t s) {
       hipLaunchKernelGGL(kernel, dim3(grid), dim3(kGradThreads), 0, s, g);
     };
     if (epi == kGradPlain) launch(int8_grad_kernel<T, kGradPlain>);
-    else if (epi == kGradDual) launch(int8_grad_kernel<T, kGradDual>);
     else if (epi == kGradGelu) launch(int8_grad_kernel<T, kGradGelu>);
-    else launch(int8_grad_kernel<T, kGradSwiGLU>);
+    else if (epi == kGradSwiGLU) launch(int8_grad_kernel<T, kGradSwiGLU>);
+    else if (epi == kGradTerms) launch(int8_grad_kernel<T, kGradTerms>);
+    else launch(int8_grad_kernel<T, kGradTermsDual>);
   };
   if (dtype == NT_F16) go(tag<f16>());
   else go(tag<bf16>());
@@ -232,11 +300,12 @@ int run_grad(int dtype, int epi, Int8Grad g, hipStream_t s) {
 }
 
 Int8Grad make_grad(const int8_t* w, const float* w_scales, const int32_t* offsets,
-                   const void* dout, int32_t E, int64_t A, int64_t K, int64_t N, void* out) {
+                   const void* dout, int64_t dout_pitch, int32_t E, int64_t A, int64_t K,
+                   int64_t N, void* out) {
   Int8Grad g = {};
   g.rows.w = w, g.rows.w_scales = w_scales, g.rows.offsets = offsets;
   g.rows.E = E, g.rows.A = A, g.rows.K = K, g.rows.N = N, g.rows.out = out;
-  g.dout = dout;
+  g.dout = dout, g.pitch = dout_pitch;
   return g;
 }
 
@@ -247,38 +316,49 @@ using namespace nt;
 
 extern "C" {
 
-int nt_int8_grouped_gemm_dx(int dtype, const int8_t* w, const float* w_scales,
-                            const int32_t* offsets, const void* dout, int32_t E, int64_t A,
-                            int64_t K, int64_t N, void* dx, hipStream_t stream) {
-  return run_grad(dtype, kGradPlain, make_grad(w, w_scales, offsets, dout, E, A, K, N, dx),
-                  stream);
+size_t nt_int8_terms_bytes(int64_t A, int64_t K) {
+  if (A < 0 || A > kInt8MaxRows || K < 1 || K > kInt8MaxK) return 0;
+  return (size_t)(2 * A * int8_pitch(K) * 2);
 }
 
-int nt_int8_grouped_gemm_dx2(int dtype, const int8_t* w1, const float* scales1, const int8_t* w2,
-                             const float* scales2, const int32_t* offsets, const void* dout1,
-                             const void* dout2, int32_t E, int64_t A, int64_t K, int64_t N,
-                             void* dx, hipStream_t stream) {
-  Int8Grad g = make_grad(w1, scales1, offsets, dout1, E, A, K, N, dx);
-  g.rows.w2 = w2, g.rows.w2_scales = scales2, g.dout2 = dout2;
-  return run_grad(dtype, kGradDual, g, stream);
+int nt_int8_grouped_gemm_dx(int dtype, const int8_t* w, const float* w_scales,
+                            const int32_t* offsets, const void* dout, int64_t dout_pitch,
+                            int32_t E, int64_t A, int64_t K, int64_t N, void* dx,
+                            hipStream_t stream) {
+  return run_grad(dtype, kGradPlain,
+                  make_grad(w, w_scales, offsets, dout, dout_pitch, E, A, K, N, dx), stream);
 }
 
 int nt_int8_grouped_gemm_dx_gelu(int dtype, const int8_t* w, const float* w_scales,
-                                 const int32_t* offsets, const void* dout, const void* act_grad,
-                                 int32_t E, int64_t A, int64_t K, int64_t N, void* dh,
+                                 const int32_t* offsets, const void* dout, int64_t dout_pitch,
+                                 const float* act_grad, const float* up_scales, int32_t E,
+                                 int64_t A, int64_t K, int64_t N, void* terms,
                                  hipStream_t stream) {
-  Int8Grad g = make_grad(w, w_scales, offsets, dout, E, A, K, N, dh);
-  g.aux = act_grad;
+  Int8Grad g = make_grad(w, w_scales, offsets, dout, dout_pitch, E, A, K, N, terms);
+  g.aux = act_grad, g.next = up_scales;
   return run_grad(dtype, kGradGelu, g, stream);
 }
 
 int nt_int8_grouped_gemm_dx_swiglu(int dtype, const int8_t* w, const float* w_scales,
-                                   const int32_t* offsets, const void* dout, const void* gate,
-                                   const void* value, int32_t E, int64_t A, int64_t K, int64_t N,
-                                   void* dgate, void* dvalue, hipStream_t stream) {
-  Int8Grad g = make_grad(w, w_scales, offsets, dout, E, A, K, N, dgate);
-  g.aux = gate, g.aux2 = value, g.rows.out2 = dvalue;
+                                   const int32_t* offsets, const void* dout, int64_t dout_pitch,
+                                   const float* gate, const float* value,
+                                   const float* gate_scales, const float* val_scales, int32_t E,
+                                   int64_t A, int64_t K, int64_t N, void* gate_terms,
+                                   void* val_terms, hipStream_t stream) {
+  Int8Grad g = make_grad(w, w_scales, offsets, dout, dout_pitch, E, A, K, N, gate_terms);
+  g.aux = gate, g.aux2 = value, g.next = gate_scales, g.next2 = val_scales;
+  g.terms2 = val_terms;
   return run_grad(dtype, kGradSwiGLU, g, stream);
+}
+
+int nt_int8_grouped_gemm_dx_terms(int dtype, const int8_t* w, const int8_t* w2,
+                                  const int32_t* offsets, const void* terms, const void* terms2,
+                                  int32_t E, int64_t A, int64_t K, int64_t N, void* dx,
+                                  hipStream_t stream) {
+  Int8Grad g = make_grad(w, nullptr, offsets, terms, 0, E, A, K, N, dx);
+  g.rows.w2 = w2, g.dout2 = terms2;
+  if ((w2 == nullptr) != (terms2 == nullptr)) return NT_ERR_INVALID_ARG;
+  return run_grad(dtype, w2 == nullptr ? kGradTerms : kGradTermsDual, g, stream);
 }
 
 }  // extern "C"

@@ -127,6 +127,8 @@ Tensor int8_weight_decode(Tensor codes, Tensor scales, int64_t K, at::ScalarType
   return W;
 }
 
+float* kept_or_null(const OptTensor& t) { return t ? t->data_ptr<float>() : nullptr; }
+
 // x @ W, x's rows brought to 8 bits.
 Tensor linear(const Tensor& x, const int32_t* off, const Weight& w) {
   const int64_t A = x.size(0);
@@ -171,12 +173,15 @@ std::tuple<Tensor, OptTensor, OptTensor> int8_swiglu_ffn(Tensor x, OptTensor off
   c10::hip::HIPGuard guard(x.get_device());
   Tensor hidden = at::empty({A, g.N}, x.options());
   OptTensor gate, value;
-  if (keep) gate = at::empty_like(hidden), value = at::empty_like(hidden);
+  if (keep) {
+    gate = at::empty({A, g.N}, x.options().dtype(at::kFloat));
+    value = at::empty_like(*gate);
+  }
   {
     Tensor ws = workspace(x, nt_int8_linear_workspace_bytes(A, d));
     check_status(nt_int8_linear_swiglu(dtype_code(x), x.data_ptr(), off, g.codes, g.scales,
                                        v.codes, v.scales, g.E, A, d, g.N, hidden.data_ptr(),
-                                       out_or_null(gate), out_or_null(value), ws.data_ptr(),
+                                       kept_or_null(gate), kept_or_null(value), ws.data_ptr(),
                                        ws.numel(), stream_of(x)),
                  "int8_linear_swiglu");
   }
@@ -198,11 +203,11 @@ std::tuple<Tensor, OptTensor> int8_gelu_ffn(Tensor x, OptTensor offsets, Tensor 
   c10::hip::HIPGuard guard(x.get_device());
   Tensor act = at::empty({A, u.N}, x.options());
   OptTensor slope;
-  if (keep) slope = at::empty_like(act);
+  if (keep) slope = at::empty({A, u.N}, x.options().dtype(at::kFloat));
   {
     Tensor ws = workspace(x, nt_int8_linear_workspace_bytes(A, d));
     check_status(nt_int8_linear_gelu(dtype_code(x), x.data_ptr(), off, u.codes, u.scales, u.E, A,
-                                     d, u.N, act.data_ptr(), out_or_null(slope), ws.data_ptr(),
+                                     d, u.N, act.data_ptr(), kept_or_null(slope), ws.data_ptr(),
                                      ws.numel(), stream_of(x)),
                  "int8_linear_gelu");
   }
@@ -210,20 +215,12 @@ std::tuple<Tensor, OptTensor> int8_gelu_ffn(Tensor x, OptTensor offsets, Tensor 
   return {y, slope};
 }
 
-// Rows [A, N] of a gradient, or [A, K] of what the forward kept, for the 16-bit
-// products with the weights held.
-void check_grad(const Tensor& t, int64_t rows, int64_t cols, const Tensor& like,
-                const char* name) {
-  check_device(t, name);
-  check_same_device(like, {&t});
-  TORCH_CHECK(t.dim() == 2 && t.size(0) == rows && t.size(1) == cols && t.is_contiguous() &&
-                  t.scalar_type() == like.scalar_type(),
-              name, " must be a contiguous [", rows, ", ", cols, "] of ", like.scalar_type());
-}
+// Rows [A, N] of a 16-bit gradient, of any multiple of 8 values a row, aligned, for
+// the products with the weights held.
 struct GradIn {
   Weight w;
   const int32_t* off;
-  int64_t A;
+  int64_t A, pitch;
 };
 GradIn check_dx(const Tensor& dout, const OptTensor& offsets, const Tensor& codes,
                 const Tensor& scales, int64_t K) {
@@ -232,64 +229,95 @@ GradIn check_dx(const Tensor& dout, const OptTensor& offsets, const Tensor& code
                                   dout.scalar_type() == at::kBFloat16),
               "dOut must be [rows, columns] of float16 or bfloat16");
   const Weight w = check_weight(codes, scales, K, dout, "weight");
-  TORCH_CHECK(w.N % 8 == 0, "dOut must have a multiple of 8 columns");
-  check_grad(dout, dout.size(0), w.N, dout, "dOut");
-  TORCH_CHECK(reinterpret_cast<uintptr_t>(dout.data_ptr()) % 16 == 0,
-              "dOut must be 16-byte aligned");
-  return {w, check_offsets(offsets, dout, w.E), dout.size(0)};
+  const int64_t pitch = dout.size(1);
+  TORCH_CHECK(pitch == (w.N + 7) / 8 * 8 && dout.is_contiguous() &&
+                  reinterpret_cast<uintptr_t>(dout.data_ptr()) % 16 == 0,
+              "dOut must be contiguous rows of ", w.N, " values, rounded up to a multiple of 8, "
+              "16-byte aligned");
+  return {w, check_offsets(offsets, dout, w.E), dout.size(0), pitch};
+}
+// What the forward kept [A, K], and the scales of the weights before [E, K].
+void check_kept(const Tensor& t, int64_t rows, int64_t cols, const Tensor& like,
+                const char* name) {
+  check_f32(t, name);
+  check_same_device(like, {&t});
+  TORCH_CHECK(t.dim() == 2 && t.size(0) == rows && t.size(1) == cols && t.is_contiguous(), name,
+              " must be a contiguous [", rows, ", ", cols, "]");
+}
+Tensor new_terms(const Tensor& like, int64_t A, int64_t K) {
+  return at::empty({2, A, nt_int8_pitch(K)}, like.options().dtype(at::kBFloat16));
 }
 
-// int8_dx(dOut, offsets, codes, scales, K) -> dOut @ W^T; int8_dx2: the sum of two.
+// int8_dx(dOut, offsets, codes, scales, K) -> dOut @ W^T.
 Tensor int8_dx(Tensor dout, OptTensor offsets, Tensor codes, Tensor scales, int64_t K) {
   const GradIn g = check_dx(dout, offsets, codes, scales, K);
   c10::hip::HIPGuard guard(dout.get_device());
   Tensor dx = at::empty({g.A, K}, dout.options());
   check_status(nt_int8_grouped_gemm_dx(dtype_code(dout), g.w.codes, g.w.scales, g.off,
-                                       dout.data_ptr(), g.w.E, g.A, K, g.w.N, dx.data_ptr(),
-                                       stream_of(dout)),
+                                       dout.data_ptr(), g.pitch, g.w.E, g.A, K, g.w.N,
+                                       dx.data_ptr(), stream_of(dout)),
                "int8_dx");
   return dx;
 }
-Tensor int8_dx2(Tensor dout1, Tensor dout2, OptTensor offsets, Tensor c1, Tensor s1, Tensor c2,
-                Tensor s2, int64_t K) {
-  const GradIn g = check_dx(dout1, offsets, c1, s1, K), h = check_dx(dout2, offsets, c2, s2, K);
-  check_grad(dout2, g.A, g.w.N, dout1, "dOut2");
-  TORCH_CHECK(h.w.E == g.w.E && h.w.N == g.w.N, "the two weights must be alike");
-  c10::hip::HIPGuard guard(dout1.get_device());
-  Tensor dx = at::empty({g.A, K}, dout1.options());
-  check_status(nt_int8_grouped_gemm_dx2(dtype_code(dout1), g.w.codes, g.w.scales, h.w.codes,
-                                        h.w.scales, g.off, dout1.data_ptr(), dout2.data_ptr(),
-                                        g.w.E, g.A, K, g.w.N, dx.data_ptr(), stream_of(dout1)),
-               "int8_dx2");
-  return dx;
-}
-// The same before an activation's gradient: dh, or (dgate, dvalue).
+// The same and an activation's gradient, in terms for the up projections: (terms of
+// up or gate, of value).
 Tensor int8_dx_gelu(Tensor dout, Tensor slope, OptTensor offsets, Tensor codes, Tensor scales,
-                    int64_t K) {
+                    Tensor up_scales, int64_t K) {
   const GradIn g = check_dx(dout, offsets, codes, scales, K);
-  check_grad(slope, g.A, K, dout, "gelu'");
+  check_kept(slope, g.A, K, dout, "gelu'");
+  check_kept(up_scales, g.w.E, K, dout, "up scales");
   c10::hip::HIPGuard guard(dout.get_device());
-  Tensor dh = at::empty_like(slope);
+  Tensor terms = new_terms(dout, g.A, K);
   check_status(nt_int8_grouped_gemm_dx_gelu(dtype_code(dout), g.w.codes, g.w.scales, g.off,
-                                            dout.data_ptr(), slope.data_ptr(), g.w.E, g.A, K,
-                                            g.w.N, dh.data_ptr(), stream_of(dout)),
+                                            dout.data_ptr(), g.pitch, slope.data_ptr<float>(),
+                                            up_scales.data_ptr<float>(), g.w.E, g.A, K, g.w.N,
+                                            terms.data_ptr(), stream_of(dout)),
                "int8_dx_gelu");
-  return dh;
+  return terms;
 }
 std::tuple<Tensor, Tensor> int8_dx_swiglu(Tensor dout, Tensor gate, Tensor value,
                                           OptTensor offsets, Tensor codes, Tensor scales,
-                                          int64_t K) {
+                                          Tensor gate_scales, Tensor val_scales, int64_t K) {
   const GradIn g = check_dx(dout, offsets, codes, scales, K);
-  check_grad(gate, g.A, K, dout, "gate");
-  check_grad(value, g.A, K, dout, "value");
+  check_kept(gate, g.A, K, dout, "gate");
+  check_kept(value, g.A, K, dout, "value");
+  check_kept(gate_scales, g.w.E, K, dout, "gate scales");
+  check_kept(val_scales, g.w.E, K, dout, "value scales");
   c10::hip::HIPGuard guard(dout.get_device());
-  Tensor dgate = at::empty_like(gate), dvalue = at::empty_like(gate);
-  check_status(nt_int8_grouped_gemm_dx_swiglu(dtype_code(dout), g.w.codes, g.w.scales, g.off,
-                                              dout.data_ptr(), gate.data_ptr(), value.data_ptr(),
-                                              g.w.E, g.A, K, g.w.N, dgate.data_ptr(),
-                                              dvalue.data_ptr(), stream_of(dout)),
+  Tensor tg = new_terms(dout, g.A, K), tv = new_terms(dout, g.A, K);
+  check_status(nt_int8_grouped_gemm_dx_swiglu(
+                   dtype_code(dout), g.w.codes, g.w.scales, g.off, dout.data_ptr(), g.pitch,
+                   gate.data_ptr<float>(), value.data_ptr<float>(),
+                   gate_scales.data_ptr<float>(), val_scales.data_ptr<float>(), g.w.E, g.A, K,
+                   g.w.N, tg.data_ptr(), tv.data_ptr(), stream_of(dout)),
                "int8_dx_swiglu");
-  return {dgate, dvalue};
+  return {tg, tv};
+}
+// int8_dx_terms(terms, second terms, offsets, codes, scales, second codes, K, dtype):
+// their products with the weights that they hold the scales of.
+Tensor int8_dx_terms(Tensor terms, OptTensor terms2, OptTensor offsets, Tensor codes,
+                     Tensor scales, OptTensor codes2, int64_t K, at::ScalarType dtype) {
+  check_device(terms, "terms");
+  const Weight w = check_weight(codes, scales, K, terms, "weight");
+  TORCH_CHECK(terms2.has_value() == codes2.has_value(), "each weight needs its terms");
+  for (const Tensor* t : {&terms, terms2 ? &*terms2 : &terms}) {
+    check_same_device(terms, {t});
+    TORCH_CHECK(t->scalar_type() == at::kBFloat16 && t->is_contiguous() &&
+                    t->sizes() == at::IntArrayRef({2, terms.size(1), nt_int8_pitch(w.N)}) &&
+                    reinterpret_cast<uintptr_t>(t->data_ptr()) % 16 == 0,
+                "terms must be contiguous, aligned [2, rows, columns] of bfloat16");
+  }
+  if (codes2) check_weight(*codes2, scales, K, terms, "second weight");
+  TORCH_CHECK(dtype == at::kHalf || dtype == at::kBFloat16, "float16 or bfloat16 gradients");
+  const int32_t* off = check_offsets(offsets, terms, w.E);
+  c10::hip::HIPGuard guard(terms.get_device());
+  Tensor dx = at::empty({terms.size(1), K}, terms.options().dtype(dtype));
+  check_status(nt_int8_grouped_gemm_dx_terms(
+                   dtype_code(dx), w.codes, codes2 ? codes2->data_ptr<int8_t>() : nullptr, off,
+                   terms.data_ptr(), terms2 ? terms2->data_ptr() : nullptr, w.E, terms.size(1), K,
+                   w.N, dx.data_ptr(), stream_of(terms)),
+               "int8_dx_terms");
+  return dx;
 }
 
 // int8_moe_few_tokens(x, up, value and down weights, top_k, router, logits) -> (out,
@@ -348,9 +376,9 @@ void bind_int8(py::module& m) {
   m.def("int8_swiglu_ffn", &int8_swiglu_ffn, "SwiGLU FFN on 8-bit weights -> (y, gate, value)");
   m.def("int8_gelu_ffn", &int8_gelu_ffn, "GELU FFN on 8-bit weights -> (y, gelu')");
   m.def("int8_dx", &int8_dx, "Gradient rows by 8-bit weights, transposed");
-  m.def("int8_dx2", &int8_dx2, "The sum of two such products");
-  m.def("int8_dx_gelu", &int8_dx_gelu, "Such a product times gelu'");
-  m.def("int8_dx_swiglu", &int8_dx_swiglu, "Such a product by SwiGLU's gradient -> (dgate, dvalue)");
+  m.def("int8_dx_gelu", &int8_dx_gelu, "Such a product times gelu' -> terms");
+  m.def("int8_dx_swiglu", &int8_dx_swiglu, "Such a product by SwiGLU's gradient -> (terms, terms)");
+  m.def("int8_dx_terms", &int8_dx_terms, "Terms by the integers of 8-bit weights, transposed");
   m.def("int8_moe_few_tokens", &int8_moe_few_tokens,
         "A whole MoE layer for few tokens on 8-bit weights -> (out, gates, topk)");
 }

@@ -863,7 +863,9 @@ def _int8_direct(dout, experts, K):
 
 
 def _aligned(t):
-    """A contiguous t that starts at a multiple of 16 bytes."""
+    """t's rows, of a multiple of 8 values (zeros are added), from a multiple of 16 bytes on."""
+    if t.shape[1] % 8:
+        return torch.nn.functional.pad(t, (0, -t.shape[1] % 8)).contiguous()
     t = t.contiguous()
     return t if t.data_ptr() % 16 == 0 else t.clone()
 
@@ -900,8 +902,9 @@ class Int8GroupedGEMM_FN(torch.autograd.Function):
 class Int8SwiGLUFFN_FN(torch.autograd.Function):
     """SwiGLU FFN on frozen 8-bit weights, with the gradient to X.
 
-    Keeps gate and value in X's dtype; the rounding of X and of the hidden values is passed
-    straight through, and the backward's products take the weights held in dy's dtype.
+    Keeps gate and value in float32; the rounding of X and of the hidden values is passed
+    straight through. Of 16-bit gradients the down projection's weights and the result are
+    rounded to their dtype, and nothing between.
     """
 
     @staticmethod
@@ -919,23 +922,21 @@ class Int8SwiGLUFFN_FN(torch.autograd.Function):
         ext = get_hip_extension()
         off, gate, value, gc, gs, vc, vs, oc, os = ctx.saved_tensors
         E, d, f = ctx.shape
-        if _int8_direct(dy, E, f):
-            dg, dv = ext.int8_dx_swiglu(_aligned(dy), gate, value, off, oc, os, f)
+        if dy.dtype != torch.float32:
+            tg, tv = ext.int8_dx_swiglu(_aligned(dy), gate, value, off, oc, os, gs, vs, f)
+            dX = ext.int8_dx_terms(tg, tv, off, gc, gs, vc, d, dy.dtype)
         else:
+            off = _all_rows(dy, off)
             dg, dv = ext.bwd_grouped_gemm_dX_swiglu(
-                ext.int8_weight_decode(oc, os, f, dy.dtype), _all_rows(dy, off), dy.contiguous(),
-                gate, value)
-        if _int8_direct(dg, E, d):
-            dX = ext.int8_dx2(dg, dv, off, gc, gs, vc, vs, d)
-        else:
+                ext.int8_weight_decode(oc, os, f, dy.dtype), off, dy.contiguous(), gate, value)
             dX = ext.bwd_grouped_gemm_dX2(
                 ext.int8_weight_decode(gc, gs, d, dy.dtype),
-                ext.int8_weight_decode(vc, vs, d, dy.dtype), _all_rows(dy, off), dg, dv)
+                ext.int8_weight_decode(vc, vs, d, dy.dtype), off, dg, dv)
         return dX, None, None, None, None
 
 
 class Int8GeluFFN_FN(torch.autograd.Function):
-    """GELU FFN on frozen 8-bit weights, with the gradient to X; keeps gelu' of the up projection."""
+    """GELU FFN on frozen 8-bit weights, with the gradient to X; keeps gelu' in float32."""
 
     @staticmethod
     def forward(ctx, X, expert_offset, W_up, W_down):
@@ -951,12 +952,13 @@ class Int8GeluFFN_FN(torch.autograd.Function):
         ext = get_hip_extension()
         off, slope, uc, us, dc, ds = ctx.saved_tensors
         E, d, f = ctx.shape
-        if _int8_direct(dy, E, f):
-            dh = ext.int8_dx_gelu(_aligned(dy), slope, off, dc, ds, f)
+        if dy.dtype != torch.float32:
+            terms = ext.int8_dx_gelu(_aligned(dy), slope, off, dc, ds, us, f)
+            dX = ext.int8_dx_terms(terms, None, off, uc, us, None, d, dy.dtype)
         else:
             dh = ext.bwd_grouped_gemm_dX_gelu(ext.int8_weight_decode(dc, ds, f, dy.dtype),
                                               _all_rows(dy, off), dy.contiguous(), slope)
-        dX = _int8_dx(dh, off, uc, us, d)
+            dX = _int8_dx(dh, off, uc, us, d)
         return dX, None, None, None
 
 

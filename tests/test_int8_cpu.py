@@ -149,7 +149,7 @@ def test_swiglu_refuses_half_of_a_pair():
 
 
 def _grad(**over):
-    a = dict(dtype=BF, w=P, s=P, offsets=P, dout=P, E=2, A=4, K=9, N=16, out=P)
+    a = dict(dtype=BF, w=P, s=P, offsets=P, dout=P, pitch=16, E=2, A=4, K=9, N=16, out=P)
     a.update(over)
     return a
 
@@ -157,37 +157,52 @@ def _grad(**over):
 @pytest.mark.parametrize("over,code", [
     (dict(dtype=F32), capi.NT_ERR_DTYPE), (dict(E=0), capi.NT_ERR_INVALID_ARG),
     (dict(A=-1), capi.NT_ERR_INVALID_ARG), (dict(K=0), capi.NT_ERR_INVALID_ARG),
-    (dict(N=12), capi.NT_ERR_INVALID_ARG), (dict(E=1025), capi.NT_ERR_TOO_MANY_EXPERTS),
+    (dict(E=1025), capi.NT_ERR_TOO_MANY_EXPERTS),
     (dict(K=MAX_K + 1), capi.NT_ERR_TOO_LARGE), (dict(N=2**20 + 8), capi.NT_ERR_TOO_LARGE),
     (dict(A=2**24), capi.NT_ERR_TOO_LARGE), (dict(offsets=None), capi.NT_ERR_INVALID_ARG),
     (dict(w=None), capi.NT_ERR_INVALID_ARG), (dict(w=P + 8), capi.NT_ERR_INVALID_ARG),
-    (dict(s=None), capi.NT_ERR_INVALID_ARG), (dict(dout=None), capi.NT_ERR_INVALID_ARG),
+    (dict(dout=None), capi.NT_ERR_INVALID_ARG),
     (dict(dout=P + 2), capi.NT_ERR_INVALID_ARG), (dict(out=None), capi.NT_ERR_INVALID_ARG),
     (dict(A=0, dout=None, out=None), capi.NT_OK)])
 def test_gradients_refuse(over, code):
     lib, a = capi.load(), _grad(**over)
-    head = [a[n] for n in ("dtype", "w", "s")]
+    head = [a[n] for n in ("dtype", "w", "s", "offsets", "dout", "pitch")]
     sizes = [a[n] for n in ("E", "A", "K", "N")]
-    assert lib.nt_int8_grouped_gemm_dx(*head, a["offsets"], a["dout"], *sizes, a["out"],
-                                       None) == code
-    assert lib.nt_int8_grouped_gemm_dx2(*head, P, P, a["offsets"], a["dout"], P, *sizes, a["out"],
-                                        None) == code
-    assert lib.nt_int8_grouped_gemm_dx_gelu(*head, a["offsets"], a["dout"], P, *sizes, a["out"],
-                                            None) == code
-    assert lib.nt_int8_grouped_gemm_dx_swiglu(*head, a["offsets"], a["dout"], P, P, *sizes,
-                                              a["out"], P, None) == code
+    assert lib.nt_int8_grouped_gemm_dx(*head, *sizes, a["out"], None) == code
+    assert lib.nt_int8_grouped_gemm_dx_gelu(*head, P, P, *sizes, a["out"], None) == code
+    assert lib.nt_int8_grouped_gemm_dx_swiglu(*head, P, P, P, P, *sizes, a["out"], P, None) == code
+    assert lib.nt_int8_grouped_gemm_dx_terms(a["dtype"], a["w"], None, a["offsets"], a["dout"],
+                                             None, *sizes, a["out"], None) == code
 
 
 def test_gradients_refuse_missing_inputs():
-    lib, a = capi.load(), _grad()
-    head, sizes = [BF, P, P], [2, 4, 9, 16]
-    bad = capi.NT_ERR_INVALID_ARG
-    assert lib.nt_int8_grouped_gemm_dx2(*head, None, P, P, P, P, *sizes, P, None) == bad
-    assert lib.nt_int8_grouped_gemm_dx2(*head, P, None, P, P, P, *sizes, P, None) == bad
-    assert lib.nt_int8_grouped_gemm_dx2(*head, P, P, P, P, P + 4, *sizes, P, None) == bad
-    assert lib.nt_int8_grouped_gemm_dx_gelu(*head, P, P, None, *sizes, P, None) == bad
-    assert lib.nt_int8_grouped_gemm_dx_swiglu(*head, P, P, P, None, *sizes, P, P, None) == bad
+    lib = capi.load()
+    sizes, bad = [2, 4, 9, 16], capi.NT_ERR_INVALID_ARG
+    head = [BF, P, P, P, P, 16]
+    for pitch in (8, 20):  # below N, and no multiple of 8
+        assert lib.nt_int8_grouped_gemm_dx(*head[:5], pitch, *sizes, P, None) == bad
+    assert lib.nt_int8_grouped_gemm_dx(*head[:5], 2**20 + 8, *sizes, P,
+                                       None) == capi.NT_ERR_TOO_LARGE
+    assert lib.nt_int8_grouped_gemm_dx(BF, P, None, *head[3:], *sizes, P, None) == bad
+    for i in range(2):
+        args = [None if i == j else P for j in range(2)]
+        assert lib.nt_int8_grouped_gemm_dx_gelu(*head, *args, *sizes, P, None) == bad
+    assert lib.nt_int8_grouped_gemm_dx_gelu(*head, P, P, *sizes, P + 8, None) == bad
+    for i in range(4):
+        args = [None if i == j else P for j in range(4)]
+        assert lib.nt_int8_grouped_gemm_dx_swiglu(*head, *args, *sizes, P, P, None) == bad
     assert lib.nt_int8_grouped_gemm_dx_swiglu(*head, P, P, P, P, *sizes, P, None, None) == bad
+    assert lib.nt_int8_grouped_gemm_dx_swiglu(*head, P, P, P, P, *sizes, P, P + 8, None) == bad
+    for two in ((P, None), (None, P), (P, P + 8), (P + 8, P)):
+        assert lib.nt_int8_grouped_gemm_dx_terms(BF, P, two[0], P, P, two[1], *sizes, P,
+                                                 None) == bad
+
+
+def test_sizes_of_terms():
+    lib = capi.load()
+    assert lib.nt_int8_terms_bytes(5, 129) == 2 * 5 * 256 * 2
+    assert lib.nt_int8_terms_bytes(0, 4) == lib.nt_int8_terms_bytes(4, 0) == 0
+    assert lib.nt_int8_terms_bytes(4, MAX_K + 1) == lib.nt_int8_terms_bytes(2**24, 4) == 0
 
 
 def _few(**over):
