@@ -92,27 +92,35 @@ int nt_int8_linear_gelu(int dtype, const void* x, const int32_t* offsets, const 
                         void* act, float* act_grad, void* ws, size_t ws_bytes,
                         hipStream_t stream);
 
-/* dx = dout @ W[e]^T [A, K] for f16 and bf16 (f32: nt_int8_weight_decode and
- * nt_grouped_gemm_dx). The rounding of x to 8 bits is passed straight through; the
- * weights are the values held, rounded to dtype; sums in float32, one rounding. Row r
- * of dout is at r * dout_pitch, a multiple of 8 from N on; columns from N to the next
- * multiple of 8 are read and must be finite. dout is 16-byte aligned. N <= 2^20. */
+/* Gradients through frozen 8-bit weights; the rounding of x to 8 bits is passed
+ * straight through. dx = dout @ W[e]^T [A, K]: sums in float32, one rounding.
+ * f16 and bf16: the weights are the values held, rounded to dtype. Row r of dout is at
+ * r * dout_pitch, a multiple of 8 from N on; columns from N to the next multiple of 8
+ * are read and must be finite. dout is 16-byte aligned.
+ * f32: dout stands for its terms (below) from nt_int8_terms with the weights' scales;
+ * dout_pitch and w_scales are not read. */
 int nt_int8_grouped_gemm_dx(int dtype, const int8_t* w, const float* w_scales,
                             const int32_t* offsets, const void* dout, int64_t dout_pitch,
                             int32_t E, int64_t A, int64_t K, int64_t N, void* dx,
                             hipStream_t stream);
 
-/* The gradient through a feed-forward block, in two products. The first takes dout to
- * the gradient dz of the up projections, that times the float32 act_grad (dx_gelu), or
- * by SwiGLU's from gate and value as the forward kept them (dx_swiglu), where w is the
- * down projection [E, K, N]. dz is not rounded to dtype: what is written are the terms
- * of dz times the up projection's scales [E, K], as two bfloat16 numbers whose sum it
- * is to 2^-17. nt_int8_terms_bytes(A, K) is their size, 16-byte aligned, laid out
- * [2][A][nt_int8_pitch(K)], columns from K on zero to the next multiple of 16 (the
- * rest is not written, nor read). The second takes them times the up projections'
- * integers (w2 and terms2 NULL: of one) to dx [A, K], rounded once to dtype; N is the
- * terms' width. Of dtype f16 or bf16, as above. */
-size_t nt_int8_terms_bytes(int64_t A, int64_t K);
+/* Terms: a gradient [A, N] times the scales [E, N] of the weights that it will meet, as
+ * sums of bfloat16 numbers: two, to 2^-17, where gradients are f16 or bf16, three, to
+ * 2^-25, where they are f32. [terms][A][nt_int8_pitch(N)], 16-byte aligned, columns
+ * from N on zero to the next multiple of 16 (the rest is not written, nor read).
+ * nt_int8_terms_bytes is their size (0: too large). nt_int8_terms makes them of float32
+ * rows dout [A, N]. */
+size_t nt_int8_terms_bytes(int dtype, int64_t A, int64_t N);
+int nt_int8_terms(const float* dout, const int32_t* offsets, const float* w_scales, int32_t E,
+                  int64_t A, int64_t N, void* terms, hipStream_t stream);
+
+/* The gradient through a feed-forward block, in two products. The first takes dout, as
+ * above, to the gradient of the up projections, that times the float32 act_grad
+ * (dx_gelu), or by SwiGLU's from gate and value as the forward kept them (dx_swiglu),
+ * where w is the down projection [E, K, N]. It is not rounded to dtype: what is written
+ * are its terms for up projections of the scales given [E, K]. The second takes terms
+ * times the up projections' integers (w2 and terms2 NULL: of one) to dx [A, K], rounded
+ * once to dtype; N is the terms' width. */
 int nt_int8_grouped_gemm_dx_gelu(int dtype, const int8_t* w, const float* w_scales,
                                  const int32_t* offsets, const void* dout, int64_t dout_pitch,
                                  const float* act_grad, const float* up_scales, int32_t E,

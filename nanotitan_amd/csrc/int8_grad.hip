@@ -1,4 +1,4 @@
-// Gradients through frozen 8-bit weights, for 16-bit activations:
+// Gradients through frozen 8-bit weights:
 //
 //   dX[a, k] = sum_n dOut[a, n] w[e, n, k],   w = q s[e, n]
 //
@@ -15,6 +15,10 @@
 // their integers, exact in bfloat16. Both terms meet the same operands in LDS, a step
 // each, so the second costs matrix instructions but no weights (14,312 rows of 768 by
 // 128 experts' 2,048: 116 us with one rounded term, 150 with two).
+//
+// Gradients in float32 are three such terms everywhere: 24 bits, and no weight is
+// rounded. That is three 16-bit products where one in float32 has a 16th of their
+// rate (8 experts of 4,096 x 14,336, 8,192 rows: 2.7 ms, with float32 weights 5.4).
 #include <algorithm>
 #include <type_traits>
 
@@ -24,8 +28,8 @@
 namespace nt {
 namespace {
 
-// Terms, TermsDual: from two terms a value and the weights' integers, out for one or
-// two matrices; Gelu, SwiGLU: to such terms.
+// Terms, TermsDual: from terms and the weights' integers, out for one or two matrices;
+// Gelu, SwiGLU: to such terms (and in float32 from them).
 enum Int8GradEpilogue { kGradPlain, kGradGelu, kGradSwiGLU, kGradTerms, kGradTermsDual };
 
 struct Int8Grad {
@@ -37,6 +41,7 @@ struct Int8Grad {
   void* terms2;
 };
 
+constexpr int64_t kGradMaxN = 1 << 22;
 constexpr int kGradBM = 128, kGradBN = 256, kGradWaves = 4;
 constexpr int kGradThreads = kGradWaves * kWave;
 
@@ -45,32 +50,67 @@ constexpr int kGradThreads = kGradWaves * kWave;
 // < 4), whose swizzles are all eight values twice: its reads touch every bank once.
 __device__ __forceinline__ int turned_swizzle(int k) { return (k >> 1 & 1) | (k >> 4 & 3) << 1; }
 
-// 16 values of row `row` from column n on as two terms, the second one what the first
-// leaves: a value of 2^-100 or more to 2^-17. (Of an infinity the second is NaN; a
-// gradient with one is no more finite as their sum.)
-__device__ __forceinline__ void put_terms(uint16_t* terms, int64_t row, int64_t rows,
-                                          int64_t pitch, int64_t n, const float (&z)[16]) {
-  uint32_t w[2][8];
+template <typename T>
+constexpr int terms_of = std::is_same<T, float>::value ? 3 : 2;
+
+// Eight values of row `row` from column n on as TERMS planes of terms, each what those
+// before leave: a value of 2^-100 or more to 2^-17 by two, 2^-25 by three. (Of an
+// infinity the others are NaN: a gradient with one is no more finite as their sum.)
+template <int TERMS>
+__device__ __forceinline__ void put_terms(void* terms, int64_t row, int64_t rows, int64_t pitch,
+                                          int64_t n, const float* values) {
+  float z[8];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    w[0][j] = pack2<bf16>(z[2 * j], z[2 * j + 1]);
-    const float first[2] = {__uint_as_float(w[0][j] << 16),
-                            __uint_as_float(w[0][j] & 0xffff0000u)};
-    w[1][j] = pack2<bf16>(z[2 * j] - first[0], z[2 * j + 1] - first[1]);
+  for (int j = 0; j < 8; ++j) z[j] = values[j];
+#pragma unroll
+  for (int i = 0; i < TERMS; ++i) {
+    uint32_t w[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      w[j] = pack2<bf16>(z[2 * j], z[2 * j + 1]);
+      z[2 * j] -= __uint_as_float(w[j] << 16);
+      z[2 * j + 1] -= __uint_as_float(w[j] & 0xffff0000u);
+    }
+    *reinterpret_cast<uint4*>(static_cast<uint16_t*>(terms) + (i * rows + row) * pitch + n) =
+        make_uint4(w[0], w[1], w[2], w[3]);
   }
+}
+
+// Terms of a float32 gradient times its experts' scales, a wave a row.
+constexpr int kTermRows = 4;
+__global__ void __launch_bounds__(kTermRows* kWave)
+    int8_terms_kernel(const float* dout, const int32_t* offsets, const float* w_scales, int32_t E,
+                      int64_t A, int64_t N, void* terms) {
+  const int64_t row = (int64_t)blockIdx.x * kTermRows +
+                      __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  if (row >= A) return;
+  int lo = 0, hi = E - 1;  // the last expert that begins at or before the row
+  while (offsets != nullptr && lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (offsets[mid] <= row) lo = mid;
+    else hi = mid - 1;
+  }
+  const float *in = dout + row * N, *sc = w_scales + lo * N;
+  const int64_t pitch = int8_pitch(N), end = round_up(N, (int64_t)16);
+  for (int64_t n = lane_id() * 8; n < end; n += kWave * 8) {
+    Some<float, 8> v, s;
+    v.load(in, n, N);
+    s.load(sc, n, N);
+    float z[8];
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    uint4* p = reinterpret_cast<uint4*>(terms + (i * rows + row) * pitch + n);
-    p[0] = make_uint4(w[i][0], w[i][1], w[i][2], w[i][3]);
-    p[1] = make_uint4(w[i][4], w[i][5], w[i][6], w[i][7]);
+    for (int j = 0; j < 8; ++j) z[j] = v.v[j] * s.v[j];
+    put_terms<3>(terms, row, A, pitch, n, z);
   }
 }
 
 template <typename T, int EPI>
 __global__ void __launch_bounds__(kGradThreads, 2) int8_grad_kernel(Int8Grad g) {
   typedef typename elem<T>::storage S;
-  constexpr bool TERMS = EPI == kGradTerms || EPI == kGradTermsDual;
-  typedef std::conditional_t<TERMS, bf16, T> M;
+  // terms of a value of dOut; none: rounded weights
+  constexpr int TERMS = std::is_same<T, float>::value                      ? 3
+                        : EPI == kGradTerms || EPI == kGradTermsDual ? 2 : 0;
+  constexpr int TURNS = TERMS > 0 ? TERMS : 1;  // steps of the same weights
+  typedef std::conditional_t<(TERMS > 0), bf16, T> M;
   typedef typename mfma_op<M>::vec vec;
   const Int8Gemm& a = g.rows;
   constexpr int BM = kGradBM, BN = kGradBN, WGN = 2;
@@ -99,7 +139,7 @@ __global__ void __launch_bounds__(kGradThreads, 2) int8_grad_kernel(Int8Grad g) 
   const int64_t kpitch = int8_pitch(a.K), kblocks = kpitch / kInt8Block;
   const int64_t groups = int8_groups(a.N);
   const int nk1 = (int)ceil_div(a.N, (int64_t)64), nw = EPI == kGradTermsDual ? 2 * nk1 : nk1;
-  const int nk = TERMS ? 2 * nw : nw;  // a step a term
+  const int nk = nw * TURNS;
   TA ta;
   ta.init(g.pitch, wave, lane);
   FragReader<BM, true, AB, 64> fa;
@@ -132,7 +172,7 @@ __global__ void __launch_bounds__(kGradThreads, 2) int8_grad_kernel(Int8Grad g) 
                          lane * 64;
 #pragma unroll
       for (int i = 0; i < 4; ++i) w[i] = reinterpret_cast<const uint4*>(at)[i];
-      if constexpr (!TERMS) {
+      if constexpr (TERMS == 0) {
         const int64_t n = nb * 64 + n0;
         const float* sc = a.w_scales + e * a.N + n;
         if (n + 4 <= a.N) {
@@ -146,13 +186,13 @@ __global__ void __launch_bounds__(kGradThreads, 2) int8_grad_kernel(Int8Grad g) 
       }
     };
     auto fetch_rows = [&](int kt, char* lds) {
-      const int step = TERMS ? kt / 2 : kt;
+      const int step = kt / TURNS;
       const bool second = EPI == kGradTermsDual && step >= nk1;
       const int64_t nb = second ? step - nk1 : step;
-      const int64_t left = round_up(a.N, (int64_t)(TERMS ? 16 : 8)) - nb * 64;
+      const int64_t left = round_up(a.N, (int64_t)(TERMS > 0 ? 16 : 8)) - nb * 64;
       const int64_t kv = left < 64 ? left : 64;
       const uint16_t* d = static_cast<const uint16_t*>(second ? g.dout2 : g.dout) +
-                          ((TERMS ? kt % 2 * a.A : 0) + row0) * g.pitch + nb * 64;
+                          (kt % TURNS * a.A + row0) * g.pitch + nb * 64;
       ta.issue(d, ((rows - 1) * g.pitch + kv) * 2, lds, kv, wave);
     };
     auto turn = [&]() {
@@ -169,7 +209,7 @@ __global__ void __launch_bounds__(kGradThreads, 2) int8_grad_kernel(Int8Grad g) 
         float v[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-          v[i] = TERMS ? (float)(u[i][j / 4] >> (8 * (j % 4)) & 255u) - 128.f
+          v[i] = TERMS > 0 ? (float)(u[i][j / 4] >> (8 * (j % 4)) & 255u) - 128.f
                        : fmaf((float)(u[i][j / 4] >> (8 * (j % 4)) & 255u), sc[i],
                               -128.f * sc[i]);
         const int k = wave * 64 + 16 * g4 + j;
@@ -192,11 +232,10 @@ __global__ void __launch_bounds__(kGradThreads, 2) int8_grad_kernel(Int8Grad g) 
     fetch_rows(0, smem);
     for (int kt = 0; kt < nk; ++kt) {
       wait_vmcnt<0>();  // this step's rows are in LDS, its weights in registers
-      if (!TERMS || kt % 2 == 0) turn();
+      if (kt % TURNS == 0) turn();
       __syncthreads();
       if (kt + 1 < nk) {
-        if (!TERMS) fetch_weights(kt + 1);
-        else if (kt % 2 == 1) fetch_weights(kt / 2 + 1);
+        if ((kt + 1) % TURNS == 0) fetch_weights((kt + 1) / TURNS);
         fetch_rows(kt + 1, smem + (kt + 1 & 1) * kA);
       }
       const char* sa = smem + (kt & 1) * kA;
@@ -247,9 +286,12 @@ __global__ void __launch_bounds__(kGradThreads, 2) int8_grad_kernel(Int8Grad g) 
               z2[j] = j < width ? d * z * sg * s2[j] : 0.f;
             }
           }
-          put_terms(static_cast<uint16_t*>(a.out), row0 + m, a.A, kpitch, n, z1);
-          if constexpr (EPI == kGradSwiGLU)
-            put_terms(static_cast<uint16_t*>(g.terms2), row0 + m, a.A, kpitch, n, z2);
+#pragma unroll
+          for (int h = 0; h < 16; h += 8) {
+            put_terms<terms_of<T>>(a.out, row0 + m, a.A, kpitch, n + h, z1 + h);
+            if constexpr (EPI == kGradSwiGLU)
+              put_terms<terms_of<T>>(g.terms2, row0 + m, a.A, kpitch, n + h, z2 + h);
+          }
         } else {
           S o[16];
 #pragma unroll
@@ -264,17 +306,17 @@ __global__ void __launch_bounds__(kGradThreads, 2) int8_grad_kernel(Int8Grad g) 
 int run_grad(int dtype, int epi, Int8Grad g, hipStream_t s) {
   Int8Gemm& a = g.rows;
   const bool terms = epi >= kGradTerms, to_terms = epi == kGradGelu || epi == kGradSwiGLU;
-  if (dtype != NT_F16 && dtype != NT_BF16) return NT_ERR_DTYPE;
+  if (!int8_float(dtype)) return NT_ERR_DTYPE;
   if (a.E < 1 || a.A < 0 || a.K < 1 || a.N < 1) return NT_ERR_INVALID_ARG;
   if (a.E > NT_MAX_EXPERTS) return NT_ERR_TOO_MANY_EXPERTS;
-  if (a.K > kInt8MaxK || a.N > 1 << 20 || a.A > kInt8MaxRows) return NT_ERR_TOO_LARGE;
-  if (terms) g.pitch = int8_pitch(a.N);
-  if (g.pitch > 1 << 20) return NT_ERR_TOO_LARGE;  // a tile's rows within 32 bits
+  if (a.K > kInt8MaxK || a.N > kGradMaxN || a.A > kInt8MaxRows) return NT_ERR_TOO_LARGE;
+  if (terms || dtype == NT_F32) g.pitch = int8_pitch(a.N);
+  if (g.pitch > kGradMaxN) return NT_ERR_TOO_LARGE;  // a tile's rows within 31 bits
   if (a.A == 0) return NT_OK;
   auto bad = [](const void* p) { return p == nullptr || reinterpret_cast<uintptr_t>(p) % 16 != 0; };
   const bool two = epi == kGradTermsDual;
   if (g.pitch < a.N || g.pitch % 8 != 0 || bad(g.dout) || bad(a.w) || a.out == nullptr ||
-      (a.offsets == nullptr && a.E != 1) || (!terms && a.w_scales == nullptr) ||
+      (a.offsets == nullptr && a.E != 1) || (!terms && dtype != NT_F32 && a.w_scales == nullptr) ||
       (two && (bad(g.dout2) || bad(a.w2))) ||
       (to_terms && (g.aux == nullptr || g.next == nullptr || bad(a.out))) ||
       (epi == kGradSwiGLU && (g.aux2 == nullptr || g.next2 == nullptr || bad(g.terms2))))
@@ -288,14 +330,16 @@ int run_grad(int dtype, int epi, Int8Grad g, hipStream_t s) {
     auto launch = [&](auto kernel) {
       hipLaunchKernelGGL(kernel, dim3(grid), dim3(kGradThreads), 0, s, g);
     };
-    if (epi == kGradPlain) launch(int8_grad_kernel<T, kGradPlain>);
-    else if (epi == kGradGelu) launch(int8_grad_kernel<T, kGradGelu>);
+    if constexpr (!std::is_same<T, float>::value) {
+      if (epi == kGradPlain) return launch(int8_grad_kernel<T, kGradPlain>);
+    }
+    if (epi == kGradGelu) launch(int8_grad_kernel<T, kGradGelu>);
     else if (epi == kGradSwiGLU) launch(int8_grad_kernel<T, kGradSwiGLU>);
     else if (epi == kGradTerms) launch(int8_grad_kernel<T, kGradTerms>);
     else launch(int8_grad_kernel<T, kGradTermsDual>);
   };
-  if (dtype == NT_F16) go(tag<f16>());
-  else go(tag<bf16>());
+  if (dtype == NT_F32 && epi == kGradPlain) epi = kGradTerms;
+  int8_by_type(dtype, go);
   return launch_status();
 }
 
@@ -316,9 +360,23 @@ using namespace nt;
 
 extern "C" {
 
-size_t nt_int8_terms_bytes(int64_t A, int64_t K) {
-  if (A < 0 || A > kInt8MaxRows || K < 1 || K > kInt8MaxK) return 0;
-  return (size_t)(2 * A * int8_pitch(K) * 2);
+size_t nt_int8_terms_bytes(int dtype, int64_t A, int64_t N) {
+  if (!int8_float(dtype) || A < 0 || A > kInt8MaxRows || N < 1 || N > kGradMaxN) return 0;
+  return (size_t)((dtype == NT_F32 ? 3 : 2) * A * int8_pitch(N) * 2);
+}
+
+int nt_int8_terms(const float* dout, const int32_t* offsets, const float* w_scales, int32_t E,
+                  int64_t A, int64_t N, void* terms, hipStream_t stream) {
+  if (E < 1 || A < 0 || N < 1) return NT_ERR_INVALID_ARG;
+  if (E > NT_MAX_EXPERTS) return NT_ERR_TOO_MANY_EXPERTS;
+  if (N > kGradMaxN || A > kInt8MaxRows) return NT_ERR_TOO_LARGE;
+  if (A == 0) return NT_OK;
+  if (dout == nullptr || w_scales == nullptr || terms == nullptr ||
+      reinterpret_cast<uintptr_t>(terms) % 16 != 0 || (offsets == nullptr && E != 1))
+    return NT_ERR_INVALID_ARG;
+  hipLaunchKernelGGL(int8_terms_kernel, dim3((unsigned)ceil_div(A, (int64_t)kTermRows)),
+                     dim3(kTermRows * kWave), 0, stream, dout, offsets, w_scales, E, A, N, terms);
+  return launch_status();
 }
 
 int nt_int8_grouped_gemm_dx(int dtype, const int8_t* w, const float* w_scales,

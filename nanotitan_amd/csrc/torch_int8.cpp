@@ -215,26 +215,39 @@ std::tuple<Tensor, OptTensor> int8_gelu_ffn(Tensor x, OptTensor offsets, Tensor 
   return {y, slope};
 }
 
-// Rows [A, N] of a 16-bit gradient, of any multiple of 8 values a row, aligned, for
-// the products with the weights held.
+Tensor new_terms(const Tensor& like, int64_t A, int64_t N) {
+  return at::empty({like.scalar_type() == at::kFloat ? 3 : 2, A, nt_int8_pitch(N)},
+                   like.options().dtype(at::kBFloat16));
+}
+
+// A gradient's rows for the products with the weights held: of 16-bit types of a
+// multiple of 8 values, aligned; of float32 their terms.
 struct GradIn {
   Weight w;
   const int32_t* off;
   int64_t A, pitch;
+  Tensor rows;
 };
 GradIn check_dx(const Tensor& dout, const OptTensor& offsets, const Tensor& codes,
                 const Tensor& scales, int64_t K) {
-  check_device(dout, "dOut");
-  TORCH_CHECK(dout.dim() == 2 && (dout.scalar_type() == at::kHalf ||
-                                  dout.scalar_type() == at::kBFloat16),
-              "dOut must be [rows, columns] of float16 or bfloat16");
+  check_rows(dout, "dOut");
   const Weight w = check_weight(codes, scales, K, dout, "weight");
-  const int64_t pitch = dout.size(1);
-  TORCH_CHECK(pitch == (w.N + 7) / 8 * 8 && dout.is_contiguous() &&
+  const int32_t* off = check_offsets(offsets, dout, w.E);
+  const int64_t A = dout.size(0), pitch = dout.size(1);
+  if (dout.scalar_type() == at::kFloat) {
+    TORCH_CHECK(pitch == w.N, "dOut must have ", w.N, " columns, has ", pitch);
+    c10::hip::HIPGuard guard(dout.get_device());
+    Tensor terms = new_terms(dout, A, w.N);
+    check_status(nt_int8_terms(dout.data_ptr<float>(), off, w.scales, w.E, A, w.N,
+                               terms.data_ptr(), stream_of(dout)),
+                 "int8_terms");
+    return {w, off, A, pitch, terms};
+  }
+  TORCH_CHECK(pitch == (w.N + 7) / 8 * 8 &&
                   reinterpret_cast<uintptr_t>(dout.data_ptr()) % 16 == 0,
-              "dOut must be contiguous rows of ", w.N, " values, rounded up to a multiple of 8, "
-              "16-byte aligned");
-  return {w, check_offsets(offsets, dout, w.E), dout.size(0), pitch};
+              "dOut must be rows of ", w.N, " values, rounded up to a multiple of 8, 16-byte "
+              "aligned");
+  return {w, off, A, pitch, dout};
 }
 // What the forward kept [A, K], and the scales of the weights before [E, K].
 void check_kept(const Tensor& t, int64_t rows, int64_t cols, const Tensor& like,
@@ -244,9 +257,6 @@ void check_kept(const Tensor& t, int64_t rows, int64_t cols, const Tensor& like,
   TORCH_CHECK(t.dim() == 2 && t.size(0) == rows && t.size(1) == cols && t.is_contiguous(), name,
               " must be a contiguous [", rows, ", ", cols, "]");
 }
-Tensor new_terms(const Tensor& like, int64_t A, int64_t K) {
-  return at::empty({2, A, nt_int8_pitch(K)}, like.options().dtype(at::kBFloat16));
-}
 
 // int8_dx(dOut, offsets, codes, scales, K) -> dOut @ W^T.
 Tensor int8_dx(Tensor dout, OptTensor offsets, Tensor codes, Tensor scales, int64_t K) {
@@ -254,7 +264,7 @@ Tensor int8_dx(Tensor dout, OptTensor offsets, Tensor codes, Tensor scales, int6
   c10::hip::HIPGuard guard(dout.get_device());
   Tensor dx = at::empty({g.A, K}, dout.options());
   check_status(nt_int8_grouped_gemm_dx(dtype_code(dout), g.w.codes, g.w.scales, g.off,
-                                       dout.data_ptr(), g.pitch, g.w.E, g.A, K, g.w.N,
+                                       g.rows.data_ptr(), g.pitch, g.w.E, g.A, K, g.w.N,
                                        dx.data_ptr(), stream_of(dout)),
                "int8_dx");
   return dx;
@@ -269,7 +279,7 @@ Tensor int8_dx_gelu(Tensor dout, Tensor slope, OptTensor offsets, Tensor codes, 
   c10::hip::HIPGuard guard(dout.get_device());
   Tensor terms = new_terms(dout, g.A, K);
   check_status(nt_int8_grouped_gemm_dx_gelu(dtype_code(dout), g.w.codes, g.w.scales, g.off,
-                                            dout.data_ptr(), g.pitch, slope.data_ptr<float>(),
+                                            g.rows.data_ptr(), g.pitch, slope.data_ptr<float>(),
                                             up_scales.data_ptr<float>(), g.w.E, g.A, K, g.w.N,
                                             terms.data_ptr(), stream_of(dout)),
                "int8_dx_gelu");
@@ -286,7 +296,7 @@ std::tuple<Tensor, Tensor> int8_dx_swiglu(Tensor dout, Tensor gate, Tensor value
   c10::hip::HIPGuard guard(dout.get_device());
   Tensor tg = new_terms(dout, g.A, K), tv = new_terms(dout, g.A, K);
   check_status(nt_int8_grouped_gemm_dx_swiglu(
-                   dtype_code(dout), g.w.codes, g.w.scales, g.off, dout.data_ptr(), g.pitch,
+                   dtype_code(dout), g.w.codes, g.w.scales, g.off, g.rows.data_ptr(), g.pitch,
                    gate.data_ptr<float>(), value.data_ptr<float>(),
                    gate_scales.data_ptr<float>(), val_scales.data_ptr<float>(), g.w.E, g.A, K,
                    g.w.N, tg.data_ptr(), tv.data_ptr(), stream_of(dout)),
@@ -303,12 +313,12 @@ Tensor int8_dx_terms(Tensor terms, OptTensor terms2, OptTensor offsets, Tensor c
   for (const Tensor* t : {&terms, terms2 ? &*terms2 : &terms}) {
     check_same_device(terms, {t});
     TORCH_CHECK(t->scalar_type() == at::kBFloat16 && t->is_contiguous() &&
-                    t->sizes() == at::IntArrayRef({2, terms.size(1), nt_int8_pitch(w.N)}) &&
+                    t->dim() == 3 && t->size(0) == (dtype == at::kFloat ? 3 : 2) &&
+                    t->size(1) == terms.size(1) && t->size(2) == nt_int8_pitch(w.N) &&
                     reinterpret_cast<uintptr_t>(t->data_ptr()) % 16 == 0,
-                "terms must be contiguous, aligned [2, rows, columns] of bfloat16");
+                "terms must be contiguous, aligned [2 or 3, rows, columns] of bfloat16");
   }
   if (codes2) check_weight(*codes2, scales, K, terms, "second weight");
-  TORCH_CHECK(dtype == at::kHalf || dtype == at::kBFloat16, "float16 or bfloat16 gradients");
   const int32_t* off = check_offsets(offsets, terms, w.E);
   c10::hip::HIPGuard guard(terms.get_device());
   Tensor dx = at::empty({terms.size(1), K}, terms.options().dtype(dtype));

@@ -845,26 +845,27 @@ def _all_rows(x, expert_offset):
     return torch.arange(2, dtype=torch.int32, device=x.device) * x.shape[0]
 
 
-def _int8_takes(dout):
-    """Whether the kernels that read 8-bit weights take this gradient."""
-    return dout.dtype != torch.float32 and dout.shape[1] % 8 == 0
-
-
 def _int8_direct(dout, experts, K):
-    """Whether they are the faster ones; else the weights go to dout's dtype first.
+    """Whether the kernels that read 8-bit weights give dout @ W^T; else the weights go to
+    dout's dtype first and to the product of that.
 
-    They pay where reading and writing the weights costs more than the products gain from weights
-    in 16 bits: at most 512 rows an expert and 2^25 weights or more (128 experts of 2,048 x 768,
-    14,312 rows: 88 us against 111 + 104; 8 of 4,096 x 14,336, 1,000 rows: 338 against 300 + 262,
-    8,192 rows: 1,331 against 301 + 1,022; 8 of 512 x 2,048, 4,096 rows: 54 against 9 + 28).
+    16-bit gradients: where reading and writing the weights costs more than the products gain from
+    weights in 16 bits, at most 512 rows an expert and 2^25 weights or more (128 experts of 2,048 x
+    768, 14,312 rows: 88 us against 111 + 104; 8 of 4,096 x 14,336, 1,000 rows: 338 against 300 +
+    262, 8,192 rows: 1,331 against 301 + 1,022; 8 of 512 x 2,048, 4,096 rows: 54 against 9 + 28).
+    float32: where their tiles of 128 rows by 256 columns fill the chip (8 of 1,024 x 2,730, 8,192
+    rows: 228 us against 286; 8 of 4,096 x 14,336: 2,698 against 5,446; 8 of 512 x 2,048, 4,096
+    rows, a quarter of it: 131 against 91).
     """
     A, N = dout.shape
-    return _int8_takes(dout) and A <= 512 * experts and experts * K * N >= 1 << 25
+    if dout.dtype == torch.float32:
+        return (A + 128 * experts) * K >= 1 << 23
+    return A <= 512 * experts and experts * K * N >= 1 << 25
 
 
 def _aligned(t):
-    """t's rows, of a multiple of 8 values (zeros are added), from a multiple of 16 bytes on."""
-    if t.shape[1] % 8:
+    """t's rows, those of 16 bits of a multiple of 8 values (zeros are added) and aligned."""
+    if t.shape[1] % 8 and t.dtype != torch.float32:
         return torch.nn.functional.pad(t, (0, -t.shape[1] % 8)).contiguous()
     t = t.contiguous()
     return t if t.data_ptr() % 16 == 0 else t.clone()
@@ -922,16 +923,8 @@ class Int8SwiGLUFFN_FN(torch.autograd.Function):
         ext = get_hip_extension()
         off, gate, value, gc, gs, vc, vs, oc, os = ctx.saved_tensors
         E, d, f = ctx.shape
-        if dy.dtype != torch.float32:
-            tg, tv = ext.int8_dx_swiglu(_aligned(dy), gate, value, off, oc, os, gs, vs, f)
-            dX = ext.int8_dx_terms(tg, tv, off, gc, gs, vc, d, dy.dtype)
-        else:
-            off = _all_rows(dy, off)
-            dg, dv = ext.bwd_grouped_gemm_dX_swiglu(
-                ext.int8_weight_decode(oc, os, f, dy.dtype), off, dy.contiguous(), gate, value)
-            dX = ext.bwd_grouped_gemm_dX2(
-                ext.int8_weight_decode(gc, gs, d, dy.dtype),
-                ext.int8_weight_decode(vc, vs, d, dy.dtype), off, dg, dv)
+        tg, tv = ext.int8_dx_swiglu(_aligned(dy), gate, value, off, oc, os, gs, vs, f)
+        dX = ext.int8_dx_terms(tg, tv, off, gc, gs, vc, d, dy.dtype)
         return dX, None, None, None, None
 
 
@@ -952,13 +945,8 @@ class Int8GeluFFN_FN(torch.autograd.Function):
         ext = get_hip_extension()
         off, slope, uc, us, dc, ds = ctx.saved_tensors
         E, d, f = ctx.shape
-        if dy.dtype != torch.float32:
-            terms = ext.int8_dx_gelu(_aligned(dy), slope, off, dc, ds, us, f)
-            dX = ext.int8_dx_terms(terms, None, off, uc, us, None, d, dy.dtype)
-        else:
-            dh = ext.bwd_grouped_gemm_dX_gelu(ext.int8_weight_decode(dc, ds, f, dy.dtype),
-                                              _all_rows(dy, off), dy.contiguous(), slope)
-            dX = _int8_dx(dh, off, uc, us, d)
+        terms = ext.int8_dx_gelu(_aligned(dy), slope, off, dc, ds, us, f)
+        dX = ext.int8_dx_terms(terms, None, off, uc, us, None, d, dy.dtype)
         return dX, None, None, None
 
 

@@ -284,9 +284,9 @@ def test_block_is_its_stages(dtype, ffn, counts):
 @pytest.fixture(params=["by_size", "direct"])
 def direct(request, monkeypatch):
     """Gradients as the sizes choose them (at these, by weights in the tokens' type), and by the
-    kernels that read 8-bit weights wherever those take them."""
+    kernels that read 8-bit weights."""
     if request.param == "direct":
-        monkeypatch.setattr(moe_ops, "_int8_direct", lambda d, E, K: moe_ops._int8_takes(d))
+        monkeypatch.setattr(moe_ops, "_int8_direct", lambda d, E, K: True)
 
 
 def test_which_gradient():
@@ -294,8 +294,8 @@ def test_which_gradient():
     dout = torch.empty(2000, 4096, dtype=torch.bfloat16, device="meta")
     assert moe_ops._int8_direct(dout, 4, 2048) and not moe_ops._int8_direct(dout, 3, 4096)
     assert not moe_ops._int8_direct(dout, 4, 2047)
-    assert not moe_ops._int8_direct(dout.float(), 4, 4096)
-    assert not moe_ops._int8_direct(dout[:, :4095], 64, 4096)
+    assert moe_ops._int8_direct(dout.float(), 4, 4096)
+    assert not moe_ops._int8_direct(dout.float(), 4, 2048)
 
 
 def _held_weights(ws):
@@ -365,19 +365,20 @@ def test_block_gradient(dtype, ffn, counts, d, f):
     assert float((x.grad.cpu().double() - want).norm()) <= steps * _steps(t) * float(want.norm())
 
 
-def _terms(A, K):
-    assert capi.load().nt_int8_terms_bytes(A, K) == 4 * A * _pitch(K)
-    return torch.full((2, A, _pitch(K)), 7.0, dtype=torch.bfloat16, device="cuda")
+def _terms(t, A, K):
+    terms = 3 if t == torch.float32 else 2
+    assert capi.load().nt_int8_terms_bytes(capi.dtype_code(t), A, K) == 2 * terms * A * _pitch(K)
+    return torch.full((terms, A, _pitch(K)), 7.0, dtype=torch.bfloat16, device="cuda")
 
 
 def _pitch(K):
     return (K + 127) // 128 * 128
 
 
-@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("K,N", [(200, 136), (77, 43), (300, 64)])
 def test_terms_of_the_hidden_gradient(dtype, K, N):
-    """To 2^-17 of the value, zeros to a multiple of 16, nothing behind the last row."""
+    """To 2^-17 or 2^-25 of the value, zeros to a multiple of 16, nothing behind the last row."""
     t, E, rows, A = TYPES[dtype], 3, 150, 180
     off, gpu_off = [0, 100, 100, 150], _offsets([100, 0, 50])[1]
     w, _, _ = _weights(E, K, N, 4)
@@ -385,10 +386,20 @@ def test_terms_of_the_hidden_gradient(dtype, K, N):
     dout[:, :N] = _rand(A, N, dtype=t, seed=1)
     kept = [_rand(A, K, seed=i) for i in (2, 3)]
     scales = [_rand(E, K, seed=i).abs() + 1e-5 for i in (5, 6)]
-    terms = [_terms(A, K) for _ in range(3)]
-    head = [capi.dtype_code(t), w.codes.data_ptr(), w.scale.data_ptr(), gpu_off.data_ptr(),
-            dout.data_ptr(), dout.shape[1]]
+    terms = [_terms(t, A, K) for _ in range(3)]
     tail, s = [E, A, K, N], capi.current_stream()
+    rows_in = dout
+    if t == torch.float32:
+        rows_in = _terms(t, A, N)
+        dense = dout[:, :N].contiguous()
+        capi.call("nt_int8_terms", dense.data_ptr(), gpu_off.data_ptr(), w.scale.data_ptr(), E, A,
+                  N, rows_in.data_ptr(), s)
+        assert bool((rows_in[:, :, N:(N + 15) // 16 * 16] == 0.0).all())
+        want = dense.cpu().double() * w.scale.cpu().double()[[0] * 100 + [2] * 80]
+        err = (rows_in[:, :, :N].cpu().double().sum(0) - want).abs() - (2.0**-25 + U) * want.abs()
+        assert float(err.max()) <= 2.0**-120
+    head = [capi.dtype_code(t), w.codes.data_ptr(), w.scale.data_ptr(), gpu_off.data_ptr(),
+            rows_in.data_ptr(), dout.shape[1]]
     capi.call("nt_int8_grouped_gemm_dx_gelu", *head, kept[0].data_ptr(), scales[0].data_ptr(),
               *tail, terms[0].data_ptr(), s)
     capi.call("nt_int8_grouped_gemm_dx_swiglu", *head, *[v.data_ptr() for v in kept + scales],
@@ -411,7 +422,8 @@ def test_terms_of_the_hidden_gradient(dtype, K, N):
         # the terms, the float32 sum, the operations after it with the hardware's exponential and
         # reciprocal; of SwiGLU's slope 1 + z (1 - sg) also where it cancels
         f = factor[:rows]
-        tol = (2.0**-17 + (N + 24) * U) * size[:rows] * f.abs()
+        tol = (2.0**-17 + (N + 24) * U if t != torch.float32 else (3 * N + 26) * U) \
+            * size[:rows] * f.abs()
         tol += 24 * U * (size * (v * sc[0]).abs() * (1 + z.abs()))[:rows]
         want = d[:rows] * f
         err = (sums - want).abs() - tol
@@ -424,7 +436,7 @@ def test_gradient_rows_behind_the_last_stay():
     w, _, _ = _weights(E, K, N, 4)
     dout = _rand(A, N, dtype=torch.bfloat16, seed=1)
     outs = [torch.full((A, K), 7.0, dtype=torch.bfloat16, device="cuda") for _ in range(3)]
-    terms = _terms(A, N)
+    terms = _terms(torch.bfloat16, A, N)
     terms[:, :rows] = 0.5
     tail, s = [E, A, K, N], capi.current_stream()
     o, p, c = off.data_ptr(), [t.data_ptr() for t in outs], w.codes.data_ptr()

@@ -155,10 +155,10 @@ def _grad(**over):
 
 
 @pytest.mark.parametrize("over,code", [
-    (dict(dtype=F32), capi.NT_ERR_DTYPE), (dict(E=0), capi.NT_ERR_INVALID_ARG),
+    (dict(dtype=9), capi.NT_ERR_DTYPE), (dict(E=0), capi.NT_ERR_INVALID_ARG),
     (dict(A=-1), capi.NT_ERR_INVALID_ARG), (dict(K=0), capi.NT_ERR_INVALID_ARG),
     (dict(E=1025), capi.NT_ERR_TOO_MANY_EXPERTS),
-    (dict(K=MAX_K + 1), capi.NT_ERR_TOO_LARGE), (dict(N=2**20 + 8), capi.NT_ERR_TOO_LARGE),
+    (dict(K=MAX_K + 1), capi.NT_ERR_TOO_LARGE), (dict(N=2**22 + 8), capi.NT_ERR_TOO_LARGE),
     (dict(A=2**24), capi.NT_ERR_TOO_LARGE), (dict(offsets=None), capi.NT_ERR_INVALID_ARG),
     (dict(w=None), capi.NT_ERR_INVALID_ARG), (dict(w=P + 8), capi.NT_ERR_INVALID_ARG),
     (dict(dout=None), capi.NT_ERR_INVALID_ARG),
@@ -181,7 +181,7 @@ def test_gradients_refuse_missing_inputs():
     head = [BF, P, P, P, P, 16]
     for pitch in (8, 20):  # below N, and no multiple of 8
         assert lib.nt_int8_grouped_gemm_dx(*head[:5], pitch, *sizes, P, None) == bad
-    assert lib.nt_int8_grouped_gemm_dx(*head[:5], 2**20 + 8, *sizes, P,
+    assert lib.nt_int8_grouped_gemm_dx(*head[:5], 2**22 + 8, *sizes, P,
                                        None) == capi.NT_ERR_TOO_LARGE
     assert lib.nt_int8_grouped_gemm_dx(BF, P, None, *head[3:], *sizes, P, None) == bad
     for i in range(2):
@@ -198,11 +198,19 @@ def test_gradients_refuse_missing_inputs():
                                                  None) == bad
 
 
-def test_sizes_of_terms():
+def test_terms():
     lib = capi.load()
-    assert lib.nt_int8_terms_bytes(5, 129) == 2 * 5 * 256 * 2
-    assert lib.nt_int8_terms_bytes(0, 4) == lib.nt_int8_terms_bytes(4, 0) == 0
-    assert lib.nt_int8_terms_bytes(4, MAX_K + 1) == lib.nt_int8_terms_bytes(2**24, 4) == 0
+    size = lib.nt_int8_terms_bytes
+    assert size(BF, 5, 129) == 2 * 5 * 256 * 2 and size(F32, 5, 129) == 3 * 5 * 256 * 2
+    assert size(BF, 0, 4) == size(BF, 4, 0) == size(9, 4, 4) == 0
+    assert size(BF, 4, 2**22 + 1) == size(BF, 2**24, 4) == 0
+    good = [P, P, P, 2, 4, 9, P]
+    for i, (v, code) in enumerate([(None, capi.NT_ERR_INVALID_ARG)] * 3 + [
+            (0, capi.NT_ERR_INVALID_ARG), (2**24, capi.NT_ERR_TOO_LARGE),
+            (0, capi.NT_ERR_INVALID_ARG), (P + 8, capi.NT_ERR_INVALID_ARG)]):
+        assert lib.nt_int8_terms(*good[:i], v, *good[i + 1:], None) == code
+    assert lib.nt_int8_terms(*good[:3], 1025, *good[4:], None) == capi.NT_ERR_TOO_MANY_EXPERTS
+    assert lib.nt_int8_terms(None, None, None, 1, 0, 9, None, None) == capi.NT_OK
 
 
 def _few(**over):
