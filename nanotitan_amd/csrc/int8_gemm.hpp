@@ -115,7 +115,7 @@ __device__ __forceinline__ void int8_put(S* p, int n, const S (&o)[16]) {
     __builtin_memcpy(v, o, sizeof(v));
 #pragma unroll
     for (int j = 0; j < (int)sizeof(S); ++j)
-      __builtin_nontemporal_store(v[j], reinterpret_cast<V*>(p) + j);
+      reinterpret_cast<V*>(p)[j] = v[j];
   } else {
 #pragma unroll
     for (int j = 0; j < 16; ++j)
