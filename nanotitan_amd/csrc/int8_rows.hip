@@ -10,8 +10,8 @@
 //
 // Weights: the channels' maxima run down the columns, so a pass over W finds them
 // (an atomic max of magnitudes' bits: the order does not count) and a second one
-// rounds. That one reads 64x64 blocks; a thread turns 4x4 values into four words
-// of four reduction rows each, and the block's bytes turn in LDS.
+// rounds. A thread turns 4x4 values into four words of four reduction rows each, and
+// a block's bytes turn in LDS.
 #include <algorithm>
 
 #include "int8.hpp"
@@ -229,60 +229,73 @@ __global__ void __launch_bounds__(kThreads) int8_most_kernel(const void* W, int6
   }
 }
 
-// Bytes of a block in LDS: [64 columns][64 reduction rows], a column's 64 bytes
-// padded to 80, so that 16-byte reads stay aligned and columns spread over banks.
-constexpr int kTurnPitch = 80;
+// A thread turns 4 reduction rows of C columns, a workgroup 64 rows of 16 threads'
+// columns. In LDS a column's 64 bytes are padded to 68: words of neighbouring columns
+// lie in different banks.
+constexpr int kTurnPitch = kInt8Block + 4;
+template <int C>
+struct Turn {
+  static constexpr int kColumns = C, kCols = 16 * C, kGroups = kCols / kInt8Block, kBytes = kCols * kTurnPitch;
+  // thread: columns col .. + C - 1 and rows row .. + 3 of values; piece (operand t, lane
+  // (g, i)) of integers
+  const int col = threadIdx.x % 16 * C, row = threadIdx.x / 16 * 4;
+  const int t = threadIdx.x / kWave, g = threadIdx.x % kWave / 16, i = threadIdx.x % 16;
+  __device__ __forceinline__ uint32_t* word(int8_t* turn, int j) const {
+    return reinterpret_cast<uint32_t*>(turn + (col + j) * kTurnPitch + row);
+  }
+  __device__ __forceinline__ uint32_t* piece(int8_t* turn, int group) const {
+    return reinterpret_cast<uint32_t*>(
+        turn + (group * kInt8Block + 16 * (i / 4) + 4 * t + i % 4) * kTurnPitch + g * 16);
+  }
+};
+
 constexpr int kRun = 4;  // blocks of a workgroup along the reduction, loaded at once
 
-// 64 columns by 256 reduction rows to integers. Grid: column groups, runs of blocks,
-// experts.
+// 64 columns by 256 reduction rows to integers (8 x 4,096 x 14,336 in bf16: 280 us, 128
+// by 128 300). Grid: column groups, runs of blocks, experts.
 template <typename T>
 __global__ void __launch_bounds__(kThreads) int8_weight_kernel(const void* W, int64_t K, int64_t N,
                                                                const uint32_t* most, int8_t* codes,
                                                                float* scales) {
   typedef typename elem<T>::storage S;
-  typedef S V4 __attribute__((ext_vector_type(4), aligned(sizeof(S))));
+  constexpr int C = 4;
+  typedef Turn<C> U;
   constexpr float kMagic = 12582912.f;  // see Some::codes
-  __shared__ __attribute__((aligned(16))) int8_t s_turn[2][kInt8Block * kTurnPitch];
-  const int64_t e = blockIdx.z, n0 = (int64_t)blockIdx.x * kInt8Block;
+  __shared__ __attribute__((aligned(16))) int8_t s_turn[2][U::kBytes];
+  const int64_t e = blockIdx.z, n0 = (int64_t)blockIdx.x * U::kCols;
   const int64_t blocks = int8_pitch(K) / kInt8Block, b0 = (int64_t)blockIdx.y * kRun;
-  const int c = threadIdx.x % 16 * 4, r = threadIdx.x / 16 * 4;
-  const S* w = static_cast<const S*>(W) + e * K * N + n0 + c;
-  V4 v[kRun][4];
+  const U at;
+  const S* w = static_cast<const S*>(W) + e * K * N;
+  Some<T, C> v[kRun][4];
 #pragma unroll
   for (int u = 0; u < kRun; ++u)
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int64_t k = (b0 + u) * kInt8Block + r + i;
-      if (k < K && n0 + c + 4 <= N) {
-        v[u][i] = *reinterpret_cast<const V4*>(w + k * N);
-      } else {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) v[u][i][j] = k < K && n0 + c + j < N ? w[k * N + j] : S(0);
-      }
+      const int64_t k = (b0 + u) * kInt8Block + at.row + i;
+      v[u][i].load(w + k * N, k < K ? n0 + at.col : N, N);  // zeros past the last row
     }
-  float s[4], inv[4];
+  float s[C], inv[C];
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    s[j] = int8_scale(n0 + c + j < N ? most[e * N + n0 + c + j] : 0u);
+  for (int j = 0; j < C; ++j) {
+    const int64_t n = n0 + at.col + j;
+    s[j] = int8_scale(n < N ? most[e * N + n] : 0u);
     inv[j] = int8_inverse(s[j]);
-    if (blockIdx.y == 0 && r == 0 && n0 + c + j < N) scales[e * N + n0 + c + j] = s[j];
+    if (blockIdx.y == 0 && at.row == 0 && n < N) scales[e * N + n] = s[j];
   }
-  // thread: operand t, lane (g, i)
-  const int t = threadIdx.x / kWave, g = threadIdx.x % kWave / 16, i16 = threadIdx.x % 16;
-  const int col = 16 * (i16 / 4) + 4 * t + i16 % 4;
-  int8_t* out = codes + ((e * int8_groups(N) + blockIdx.x) * blocks + b0) * 4096 + threadIdx.x * 16;
+  uint4* out = reinterpret_cast<uint4*>(
+                   codes + ((e * int8_groups(N) + blockIdx.x) * blocks + b0) * 4096) +
+               threadIdx.x;
 #pragma unroll
   for (int u = 0; u < kRun; ++u) {
     if (b0 + u >= blocks) break;
     int8_t* turn = s_turn[u & 1];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
+    for (int j = 0; j < C; ++j) {
       uint32_t sum[4];
       float off = 0.f;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const float x = elem<T>::load(v[u][i][j]), near = fmaf(x, inv[j], kMagic);
+        const float x = elem<T>::load(v[u][i].v[j]), near = fmaf(x, inv[j], kMagic);
         off = fmaxf(off, fabsf(fmaf(kMagic - near, s[j], x)));
         sum[i] = __float_as_uint(near);
       }
@@ -292,55 +305,59 @@ __global__ void __launch_bounds__(kThreads) int8_weight_kernel(const void* W, in
       if (!(off < 0.5f * s[j]) || inv[j] == 0.f) {
         int q[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) q[i] = int8_code(elem<T>::load(v[u][i][j]), s[j], inv[j]);
+        for (int i = 0; i < 4; ++i)
+          q[i] = int8_code(elem<T>::load(v[u][i].v[j]), s[j], inv[j]);
         word = pack_bytes(q[0], q[1], q[2], q[3]);
       }
-      *reinterpret_cast<uint32_t*>(turn + (c + j) * kTurnPitch + r) = word;
+      *at.word(turn, j) = word;
     }
     __syncthreads();
-    *reinterpret_cast<uint4*>(out + u * 4096) =
-        *reinterpret_cast<const uint4*>(turn + col * kTurnPitch + g * 16);
+    const uint32_t* p = at.piece(turn, 0);
+    out[(int64_t)u * (4096 / 16)] = make_uint4(p[0], p[1], p[2], p[3]);
   }
 }
 
+// And back, 256 bytes of a row in columns (283 us, by 128 bytes 310) and a block of
+// reduction rows a workgroup (four on end, loaded at once: 410).
 template <typename T>
 __global__ void __launch_bounds__(kThreads) int8_weight_decode_kernel(const int8_t* codes,
                                                                       const float* scales,
                                                                       int64_t K, int64_t N,
                                                                       void* W) {
   typedef typename elem<T>::storage S;
-  typedef S V4 __attribute__((ext_vector_type(4), aligned(sizeof(S))));
-  __shared__ __attribute__((aligned(16))) int8_t s_turn[kInt8Block * kTurnPitch];
-  const int64_t e = blockIdx.z, n0 = (int64_t)blockIdx.x * kInt8Block;
-  const int64_t k0 = (int64_t)blockIdx.y * kInt8Block;
-  const int t = threadIdx.x / kWave, g = threadIdx.x % kWave / 16, i = threadIdx.x % 16;
-  const int col = 16 * (i / 4) + 4 * t + i % 4;
-  const int64_t block = (e * int8_groups(N) + blockIdx.x) * (int8_pitch(K) / kInt8Block) +
-                        blockIdx.y;
-  *reinterpret_cast<uint4*>(s_turn + col * kTurnPitch + g * 16) =
-      *reinterpret_cast<const uint4*>(codes + block * kInt8Block * kInt8Block + threadIdx.x * 16);
-  __syncthreads();
-  const int c = threadIdx.x % 16 * 4, r = threadIdx.x / 16 * 4;
-  S* w = static_cast<S*>(W) + e * K * N + n0 + c;
-  V4 v[4];
+  typedef Turn<16 / (int)sizeof(S)> U;
+  __shared__ __attribute__((aligned(16))) int8_t s_turn[U::kBytes];
+  const int64_t e = blockIdx.z, groups = int8_groups(N), n0 = (int64_t)blockIdx.x * U::kCols;
+  const int64_t k0 = (int64_t)blockIdx.y * kInt8Block, blocks = int8_pitch(K) / kInt8Block;
+  const U at;
+  uint4 q[U::kGroups];
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const float s = n0 + c + j < N ? scales[e * N + n0 + c + j] : 0.f;
-    const uint32_t word = *reinterpret_cast<const uint32_t*>(s_turn + (c + j) * kTurnPitch + r);
-#pragma unroll
-    for (int b = 0; b < 4; ++b) v[b][j] = int8_value<T>((int8_t)(word >> (8 * b)), s);
+  for (int h = 0; h < U::kGroups; ++h) {
+    const int64_t group = (int64_t)blockIdx.x * U::kGroups + h;
+    q[h] = reinterpret_cast<const uint4*>(
+        codes + ((e * groups + (group < groups ? group : groups - 1)) * blocks + blockIdx.y) *
+                    4096)[threadIdx.x];
   }
 #pragma unroll
-  for (int b = 0; b < 4; ++b) {
-    const int64_t k = k0 + r + b;
-    if (k >= K) break;
-    if (n0 + c + 4 <= N) {
-      *reinterpret_cast<V4*>(w + k * N) = v[b];
-    } else {
+  for (int h = 0; h < U::kGroups; ++h) {
+    uint32_t* p = at.piece(s_turn, h);
+    p[0] = q[h].x, p[1] = q[h].y, p[2] = q[h].z, p[3] = q[h].w;
+  }
+  Some<float, U::kColumns> s;
+  s.load(scales + e * N, n0 + at.col, N);
+  __syncthreads();
+  if (n0 + at.col >= N) return;
+  Some<T, U::kColumns> v[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (n0 + c + j < N) w[k * N + j] = v[b][j];
-    }
+  for (int j = 0; j < U::kColumns; ++j) {
+    const uint32_t word = *at.word(s_turn, j);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i].v[j] = int8_value<T>((int8_t)(word >> (8 * i)), s.v[j]);
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int64_t k = k0 + at.row + i;
+    if (k < K) v[i].store(static_cast<S*>(W) + (e * K + k) * N, n0 + at.col, N);
   }
 }
 
@@ -473,7 +490,7 @@ int nt_int8_weight_decode(int dtype, const int8_t* codes, const float* scales, i
   int8_by_type(dtype, [&](auto type) {
     typedef typename decltype(type)::type T;
     hipLaunchKernelGGL((int8_weight_decode_kernel<T>),
-                       dim3((unsigned)int8_groups(N),
+                       dim3((unsigned)ceil_div(N, (int64_t)(256 / dtype_bytes(dtype))),
                             (unsigned)ceil_div(K, (int64_t)kInt8Block), (unsigned)E),
                        dim3(kThreads), 0, stream, codes, scales, K, N, W);
   });
