@@ -7,6 +7,14 @@
 // int32 holds them up to 2^17 reduction rows. Two scalings and one rounding
 // follow, or in float32 an activation: silu(gate) * value of two weight matrices
 // side by side, or GELU.
+//
+// Many rows are bound by the matrix instructions (32,768 rows, 8 experts of 14,336 to
+// 4,096: 1.70 to 1.82 ms, 2.1 to 2.3 Pop/s; the library's plain product of 16,384^3 reaches
+// 2.35) and by what feeds them: a ring of three stages in LDS, filled directly, with
+// operands that lie in memory as the instructions take them, and the next step's
+// fragments read behind this one's instructions. Few rows are one read of the weights
+// (int8_few.hip). In between an expert's last tile is part empty and its weights are
+// read for few products (128 experts with 112 rows each, 2,048 to 768: 0.5 Pop/s).
 #include <algorithm>
 
 #include "gelu.hpp"
@@ -137,7 +145,8 @@ __global__ void __launch_bounds__(WGM* WGN* kWave, BM* BN / (WGM * WGN) > 128 * 
   __shared__ int32_t s_pref[NT_MAX_EXPERTS + 1];
   int8_row_tiles(a, BM, s_pref);
   const int64_t mtiles = __builtin_amdgcn_readfirstlane(s_pref[a.E]);
-  const int64_t total = mtiles * a.ntn;
+  // (more than that many only where offsets are malformed)
+  const int64_t total = mtiles * a.ntn < INT32_MAX ? mtiles * a.ntn : INT32_MAX;
   // Tiles are dealt to the XCDs in contiguous ranges, as the 16-bit GEMMs' are.
   constexpr int kXcd = 8;
   const int64_t G = gridDim.x, wg = blockIdx.x;
@@ -145,7 +154,6 @@ __global__ void __launch_bounds__(WGM* WGN* kWave, BM* BN / (WGM * WGN) > 128 * 
   const int64_t q = G / kXcd, r = G % kXcd;
   const int64_t before = xcd * q + (xcd < r ? xcd : r);
   const int64_t nbx = q + (xcd < r ? 1 : 0);
-  // (at most 2^31 tiles)
   const int64_t t_end = __builtin_amdgcn_readfirstlane(
       (int)xcd_range_start(total, before + nbx, G, s_pref, a.E, a.ntn));
   const int64_t t_beg = __builtin_amdgcn_readfirstlane(
@@ -337,8 +345,8 @@ int run_int8(int dtype, int epi, Int8Gemm a, hipStream_t s, void* ws = nullptr,
   const int st = check_int8(dtype, a);
   if (st != NT_OK || a.A == 0) return st;
   const bool two = epi == kInt8SwiGLU;
-  if ((a.values == nullptr && (a.x == nullptr || a.x_scales == nullptr)) || a.w == nullptr || a.w_scales == nullptr ||
-      a.out == nullptr || (two && (a.w2 == nullptr || a.w2_scales == nullptr)) ||
+  if ((a.values == nullptr && (a.x == nullptr || a.x_scales == nullptr)) || a.w == nullptr ||
+      a.w_scales == nullptr || a.out == nullptr || (two && (a.w2 == nullptr || a.w2_scales == nullptr)) ||
       (a.offsets == nullptr && a.E != 1) || (two && (a.out2 == nullptr) != (a.out3 == nullptr)) ||
       !aligned16(a.x) || !aligned16(a.w) || !aligned16(a.w2))
     return NT_ERR_INVALID_ARG;

@@ -121,7 +121,8 @@ __global__ void __launch_bounds__(kGradThreads, 2) int8_grad_kernel(Int8Grad g) 
   __shared__ int32_t s_pref[NT_MAX_EXPERTS + 1];
   char* turned = smem + 2 * kA;
   int8_row_tiles(a, BM, s_pref);
-  const int64_t total = (int64_t)__builtin_amdgcn_readfirstlane(s_pref[a.E]) * a.ntn;
+  const int64_t all = (int64_t)__builtin_amdgcn_readfirstlane(s_pref[a.E]) * a.ntn;
+  const int64_t total = all < INT32_MAX ? all : INT32_MAX;  // (more: malformed offsets)
   constexpr int kXcd = 8;
   const int64_t G = gridDim.x, wg = blockIdx.x;
   const int xcd = (int)(wg % kXcd);

@@ -182,7 +182,7 @@ class Int8ExpertFFN(nn.Module):
     none. The weights are buffers: two a projection, ``<name>_codes`` and ``<name>_scale``, the
     float32 scales as the int32 of their bits, which a cast of the module to another float type
     leaves alone. ``cfg.ffn_checkpoint8`` does not apply: what the backward keeps is gate and
-    value, or gelu', in the tokens' type.
+    value, or gelu', in float32.
     """
 
     def __init__(self, experts):
