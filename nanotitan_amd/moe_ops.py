@@ -853,13 +853,13 @@ def _int8_direct(dout, experts, K):
     weights in 16 bits, at most 512 rows an expert and 2^25 weights or more (128 experts of 2,048 x
     768, 14,312 rows: 88 us against 111 + 104; 8 of 4,096 x 14,336, 1,000 rows: 338 against 300 +
     262, 8,192 rows: 1,331 against 301 + 1,022; 8 of 512 x 2,048, 4,096 rows: 54 against 9 + 28).
-    float32: where their tiles of 128 rows by 256 columns fill the chip (8 of 1,024 x 2,730, 8,192
-    rows: 228 us against 286; 8 of 4,096 x 14,336: 2,698 against 5,446; 8 of 512 x 2,048, 4,096
-    rows, a quarter of it: 131 against 91).
+    float32: where their tiles of 128 rows by 256 columns fill half of the chip (8 of 1,024 x
+    2,730, 8,192 rows: 228 us against 286; 1 of 4,096 x 4,096, 1,323 rows: 246 against 337; 8 of
+    1,024 x 4,096, 2,000 rows, which fill a third: 232 against 166).
     """
     A, N = dout.shape
     if dout.dtype == torch.float32:
-        return (A + 128 * experts) * K >= 1 << 23
+        return (A + 128 * experts) * K >= 1 << 22
     return A <= 512 * experts and experts * K * N >= 1 << 25
 
 

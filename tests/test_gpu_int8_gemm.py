@@ -295,7 +295,7 @@ def test_which_gradient():
     assert moe_ops._int8_direct(dout, 4, 2048) and not moe_ops._int8_direct(dout, 3, 4096)
     assert not moe_ops._int8_direct(dout, 4, 2047)
     assert moe_ops._int8_direct(dout.float(), 4, 4096)
-    assert not moe_ops._int8_direct(dout.float(), 4, 2048)
+    assert not moe_ops._int8_direct(dout.float(), 4, 1024)
 
 
 def _held_weights(ws):
