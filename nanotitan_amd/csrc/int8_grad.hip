@@ -42,7 +42,7 @@ struct Int8Grad {
 };
 
 constexpr int64_t kGradMaxN = 1 << 22;
-constexpr int kGradBM = 128, kGradBN = 256, kGradWaves = 4;
+constexpr int kGradBM = 128, kGradWaves = 4;
 constexpr int kGradThreads = kGradWaves * kWave;
 
 // A row (a value of k) of the turned weights is 64 n, 8 chunks of 16 bytes; chunk c
@@ -103,8 +103,8 @@ __global__ void __launch_bounds__(kTermRows* kWave)
   }
 }
 
-template <typename T, int EPI>
-__global__ void __launch_bounds__(kGradThreads, 2) int8_grad_kernel(Int8Grad g) {
+template <typename T, int EPI, int BN>
+__global__ void __launch_bounds__(kGradThreads, BN == 256 ? 2 : 3) int8_grad_kernel(Int8Grad g) {
   typedef typename elem<T>::storage S;
   // terms of a value of dOut; none: rounded weights
   constexpr int TERMS = std::is_same<T, float>::value                      ? 3
@@ -113,8 +113,8 @@ __global__ void __launch_bounds__(kGradThreads, 2) int8_grad_kernel(Int8Grad g) 
   typedef std::conditional_t<(TERMS > 0), bf16, T> M;
   typedef typename mfma_op<M>::vec vec;
   const Int8Gemm& a = g.rows;
-  constexpr int BM = kGradBM, BN = kGradBN, WGN = 2;
-  constexpr int AB = BM / 2 / 16, CG = BN / 2 / 64;  // of a wave: 64 rows by 128 columns
+  // of a wave: 64 rows by half of the columns
+  constexpr int BM = kGradBM, WGN = 2, AB = BM / 2 / 16, CG = BN / 2 / 64;
   typedef OperandTile<BM, true, 64, kGradWaves> TA;
   constexpr int kA = TA::kBytes, kB = BN * 128;
   __shared__ __attribute__((aligned(1024))) char smem[2 * kA + kB];
@@ -145,7 +145,11 @@ __global__ void __launch_bounds__(kGradThreads, 2) int8_grad_kernel(Int8Grad g) 
   ta.init(g.pitch, wave, lane);
   FragReader<BM, true, AB, 64> fa;
   fa.init(wm * 64, lane);
-  // thread: 16 values of k, four n from n0 on
+  // of a block of 64 columns a wave turns all, or one of two waves half of each 16;
+  // thread: KT values of k, four n from n0 on
+  constexpr int kShare = kGradWaves * 64 / BN, KT = 16 / kShare;
+  typedef uint32_t Words __attribute__((ext_vector_type(KT / 4)));
+  const int block = wave / kShare, k_half = wave % kShare * KT;
   const int t4 = lane >> 4, g4 = lane >> 2 & 3, i4 = lane & 3, n0 = 16 * i4 + 4 * t4;
 
   for (int64_t logical = t_beg + wg / kXcd; logical < t_end; logical += nbx) {
@@ -159,20 +163,19 @@ __global__ void __launch_bounds__(kGradThreads, 2) int8_grad_kernel(Int8Grad g) 
     const int64_t left = (int64_t)__builtin_amdgcn_readfirstlane((int)r1) - row0;
     const int rows = (int)(left < BM ? left : BM);
     const int64_t col0 = (int64_t)nt * BN;
-    // this wave turns one block of 64 columns (none past the last)
-    const int64_t kb = col0 / kInt8Block + wave;
+    const int64_t kb = col0 / kInt8Block + block;  // (none past the last)
     const bool has = kb < kblocks;
 
-    uint4 w[4];
+    Words w[4];
     float4 s;
     auto fetch_weights = [&](int step) {
       const bool second = EPI == kGradTermsDual && step >= nk1;
       const int64_t nb = second ? step - nk1 : step;
       const int8_t* at = (second ? a.w2 : a.w) +
                          ((e * groups + nb) * kblocks + (has ? kb : kblocks - 1)) * 4096 +
-                         lane * 64;
+                         lane * 64 + k_half;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) w[i] = reinterpret_cast<const uint4*>(at)[i];
+      for (int i = 0; i < 4; ++i) w[i] = *reinterpret_cast<const Words*>(at + i * 16);
       if constexpr (TERMS == 0) {
         const int64_t n = nb * 64 + n0;
         const float* sc = a.w_scales + e * a.N + n;
@@ -198,22 +201,20 @@ __global__ void __launch_bounds__(kGradThreads, 2) int8_grad_kernel(Int8Grad g) 
     };
     auto turn = [&]() {
       const float sc[4] = {s.x, s.y, s.z, s.w};
-      uint32_t u[4][4];
+      uint32_t u[4][KT / 4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const uint32_t v[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
+      for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int d = 0; d < 4; ++d) u[i][d] = v[d] ^ 0x80808080u;
-      }
+        for (int d = 0; d < KT / 4; ++d) u[i][d] = w[i][d] ^ 0x80808080u;
 #pragma unroll
-      for (int j = 0; j < 16; ++j) {
+      for (int j = 0; j < KT; ++j) {
         float v[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i)
           v[i] = TERMS > 0 ? (float)(u[i][j / 4] >> (8 * (j % 4)) & 255u) - 128.f
                        : fmaf((float)(u[i][j / 4] >> (8 * (j % 4)) & 255u), sc[i],
                               -128.f * sc[i]);
-        const int k = wave * 64 + 16 * g4 + j;
+        const int k = block * 64 + 16 * g4 + k_half + j;
         *reinterpret_cast<uint2*>(turned + k * 128 +
                                   ((2 * i4 + (t4 >> 1)) ^ turned_swizzle(k)) * 16 +
                                   (t4 & 1) * 8) =
@@ -322,22 +323,36 @@ int run_grad(int dtype, int epi, Int8Grad g, hipStream_t s) {
       (to_terms && (g.aux == nullptr || g.next == nullptr || bad(a.out))) ||
       (epi == kGradSwiGLU && (g.aux2 == nullptr || g.next2 == nullptr || bad(g.terms2))))
     return NT_ERR_INVALID_ARG;
-  a.ntn = (int32_t)ceil_div(a.K, (int64_t)kGradBN);
+  // Half as wide where tiles of 256 columns (an expert's last one half full) are about as
+  // few as CUs: a step waits for its loads, and then twice as many run at a time (66
+  // tiles, 4,188 rows of terms, 2,048 to 512: 56 us for 80; 264, 512 to 2,048: 34 for 39;
+  // but 420, 871 rows, 4,096 to 14,336: 178 for 159, and 1,024 109 for 98).
+  const int64_t cus = device_cus(s);
+  const bool wide =
+      4 * (ceil_div(a.A, (int64_t)kGradBM) + a.E / 2) * ceil_div(a.K, (int64_t)256) > 5 * cus;
+  a.ntn = (int32_t)ceil_div(a.K, (int64_t)(wide ? 256 : 128));
   const int64_t tiles = (ceil_div(a.A, (int64_t)kGradBM) + a.E - 1) * a.ntn;
   if (tiles > INT32_MAX) return NT_ERR_TOO_LARGE;
-  const unsigned grid = (unsigned)std::min<int64_t>(tiles, 2 * (int64_t)device_cus(s));
+  const unsigned grid =
+      (unsigned)std::min<int64_t>(tiles, (wide ? 2 : 3) * cus);
   auto go = [&](auto type) {
     typedef typename decltype(type)::type T;
-    auto launch = [&](auto kernel) {
-      hipLaunchKernelGGL(kernel, dim3(grid), dim3(kGradThreads), 0, s, g);
+    auto launch = [&](auto epilogue) {
+      constexpr int EPI = decltype(epilogue)::value;
+      if (wide)
+        hipLaunchKernelGGL((int8_grad_kernel<T, EPI, 256>), dim3(grid), dim3(kGradThreads), 0, s,
+                           g);
+      else
+        hipLaunchKernelGGL((int8_grad_kernel<T, EPI, 128>), dim3(grid), dim3(kGradThreads), 0, s,
+                           g);
     };
     if constexpr (!std::is_same<T, float>::value) {
-      if (epi == kGradPlain) return launch(int8_grad_kernel<T, kGradPlain>);
+      if (epi == kGradPlain) return launch(std::integral_constant<int, kGradPlain>());
     }
-    if (epi == kGradGelu) launch(int8_grad_kernel<T, kGradGelu>);
-    else if (epi == kGradSwiGLU) launch(int8_grad_kernel<T, kGradSwiGLU>);
-    else if (epi == kGradTerms) launch(int8_grad_kernel<T, kGradTerms>);
-    else launch(int8_grad_kernel<T, kGradTermsDual>);
+    if (epi == kGradGelu) launch(std::integral_constant<int, kGradGelu>());
+    else if (epi == kGradSwiGLU) launch(std::integral_constant<int, kGradSwiGLU>());
+    else if (epi == kGradTerms) launch(std::integral_constant<int, kGradTerms>());
+    else launch(std::integral_constant<int, kGradTermsDual>());
   };
   if (dtype == NT_F32 && epi == kGradPlain) epi = kGradTerms;
   int8_by_type(dtype, go);

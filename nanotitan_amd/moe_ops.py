@@ -853,9 +853,9 @@ def _int8_direct(dout, experts, K):
     weights in 16 bits, at most 512 rows an expert and 2^25 weights or more (128 experts of 2,048 x
     768, 14,312 rows: 88 us against 111 + 104; 8 of 4,096 x 14,336, 1,000 rows: 338 against 300 +
     262, 8,192 rows: 1,331 against 301 + 1,022; 8 of 512 x 2,048, 4,096 rows: 54 against 9 + 28).
-    float32: where their tiles of 128 rows by 256 columns fill half of the chip (8 of 1,024 x
-    2,730, 8,192 rows: 228 us against 286; 1 of 4,096 x 4,096, 1,323 rows: 246 against 337; 8 of
-    1,024 x 4,096, 2,000 rows, which fill a third: 232 against 166).
+    float32: where tiles of 128 rows by 256 columns would fill half of the chip (8 of 1,024 x
+    2,730, 8,192 rows: 228 us against 286; 1 of 1,024 x 4,096, 4,096 rows: 183 against 243; below,
+    8 of 1,024 x 4,096, 2,000 rows: 163 against 160; 7 of 300 x 1,365, 5,003 rows: 72 against 65).
     """
     A, N = dout.shape
     if dout.dtype == torch.float32:
