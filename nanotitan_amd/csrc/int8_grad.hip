@@ -431,7 +431,7 @@ int nt_int8_grouped_gemm_dx_terms(int dtype, const int8_t* w, const int8_t* w2,
                                   hipStream_t stream) {
   Int8Grad g = make_grad(w, nullptr, offsets, terms, 0, E, A, K, N, dx);
   g.rows.w2 = w2, g.dout2 = terms2;
-  if ((w2 == nullptr) != (terms2 == nullptr)) return NT_ERR_INVALID_ARG;
+  if (w2 == nullptr && terms2 != nullptr) return NT_ERR_INVALID_ARG;
   return run_grad(dtype, w2 == nullptr ? kGradTerms : kGradTermsDual, g, stream);
 }
 

@@ -450,6 +450,56 @@ def test_gradient_rows_behind_the_last_stay():
         assert bool((t[rows:] == 7.0).all()) and not bool((t[:rows] == 7.0).all())
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("ffn", ["swiglu", "gelu"])
+def test_block_of_no_rows_and_of_a_sum(dtype, ffn):
+    """A gradient of no rows, and one that is a single value seen as all of them."""
+    t, f, d = TYPES[dtype], 96, 70
+    up = [_weights(2, d, f, i)[0] for i in range(2 if ffn == "swiglu" else 1)]
+    down = _weights(2, f, d, 5)[0]
+    block = int8_swiglu_ffn_fn if ffn == "swiglu" else int8_gelu_ffn_fn
+    for counts in ([0, 0], [0, 9]):
+        _, off = _offsets(counts)
+        x = _rand(sum(counts), d, dtype=t, seed=3).requires_grad_()
+        y = block(x, *up, down, off)
+        got, = torch.autograd.grad(y.sum(), x, retain_graph=True)
+        want, = torch.autograd.grad(y, x, torch.ones_like(y))
+        assert got.shape == x.shape and torch.equal(got, want)
+
+
+def test_gradient_of_wider_rows():
+    """Columns past the next multiple of 8 are not read."""
+    E, A, K, N = 2, 50, 90, 43
+    w, _, _ = _weights(E, K, N, 4)
+    _, off = _offsets([20, 30])
+    dout = _rand(A, N, dtype=torch.bfloat16, seed=1)
+    outs = []
+    for pitch in (48, 64, 136):
+        rows = torch.full((A, pitch), float("nan"), dtype=torch.bfloat16, device="cuda")
+        rows[:, :48] = 0.0
+        rows[:, :N] = dout
+        dx = torch.empty(A, K, dtype=torch.bfloat16, device="cuda")
+        capi.call("nt_int8_grouped_gemm_dx", capi.NT_BF16, w.codes.data_ptr(), w.scale.data_ptr(),
+                  off.data_ptr(), rows.data_ptr(), pitch, E, A, K, N, dx.data_ptr(),
+                  capi.current_stream())
+        outs.append(dx)
+    assert bool(outs[0].isfinite().all()) and all(torch.equal(o, outs[0]) for o in outs)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_gradient_of_malformed_offsets_stays_inside(dtype):
+    t, A, K, N = TYPES[dtype], 300, 130, 64
+    ext = moe_ops.get_hip_extension()
+    w, v = _weights(4, K, N, 0)[0], _weights(4, N, K, 1)[0]
+    dout, kept = _rand(A, N, dtype=t), _rand(A, K)
+    for off in ([-5, A + 9, 3, 2**31 - 1, 10], [A, 0, A, 0, A], [7, 7, 7, 7, 7]):
+        o = torch.tensor(off, dtype=torch.int32, device="cuda")
+        assert ext.int8_dx(dout, o, w.codes, w.scale, K).shape == (A, K)
+        terms = ext.int8_dx_gelu(dout, kept, o, w.codes, w.scale, v.scale, K)
+        assert ext.int8_dx_terms(terms, None, o, v.codes, v.scale, None, N, t).shape == (A, N)
+    torch.cuda.synchronize()
+
+
 def test_gradient_of_any_alignment_and_layout(direct):
     w, _, _ = _weights(1, 100, 64, 0)
     x = _rand(33, 100, dtype=torch.bfloat16).requires_grad_()
