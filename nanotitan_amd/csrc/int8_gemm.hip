@@ -29,17 +29,9 @@ namespace {
 
 // One k-step is SB = 64 or 128 integers of each operand row. Operands are copied to
 // LDS as they are, 1 KiB a load instruction: a lane's offset never changes, and what
-// tells instructions and steps apart is uniform.
-__device__ __forceinline__ void copy_to_lds(i32x4_t rsrc, uint32_t lane_off, uint32_t off,
-                                            uint32_t lds) {
-  asm volatile(
-      "s_mov_b32 m0, %3\n\t"
-      "s_nop 0\n\t"
-      "buffer_load_dwordx4 %0, %1, %2 offen lds"
-      :
-      : "v"(lane_off), "s"(rsrc), "s"(off), "s"(lds)
-      : "memory", "m0");
-}
+// tells instructions and steps apart is uniform. Both go into the vector offset: the
+// buffer's range does not cover a scalar one, and the last row block's and column
+// group's tiles reach past the integers.
 
 // The step's operands of `ROWS` rows (activations) or columns (weights): UNIT
 // operands (one; a group's four) for each of its SB / 64 blocks, then the next 16
@@ -65,10 +57,10 @@ struct OperandCopy {
 #pragma unroll
     for (int u = 0; u < kPer; ++u) {
       const uint32_t i = wave + u * NW;
-      copy_to_lds(r, lane_off,
-                  __builtin_amdgcn_readfirstlane(i / kGroup * group + kt * (kGroup * 1024) +
-                                                 i % kGroup * 1024),
-                  __builtin_amdgcn_readfirstlane(l0 + i * 1024u));
+      load16_to_lds(r, lane_off + __builtin_amdgcn_readfirstlane(
+                                      i / kGroup * group + kt * (kGroup * 1024) +
+                                      i % kGroup * 1024),
+                    __builtin_amdgcn_readfirstlane(l0 + i * 1024u));
     }
   }
 };
