@@ -54,22 +54,29 @@ template <typename T>
 constexpr int terms_of = std::is_same<T, float>::value ? 3 : 2;
 
 // Eight values of row `row` from column n on as TERMS planes of terms, each what those
-// before leave: a value of 2^-100 or more to 2^-17 by two, 2^-25 by three. (Of an
-// infinity the others are NaN: a gradient with one is no more finite as their sum.)
+// before leave: a value of 2^-100 or more to 2^-17 by two, 2^-25 by three. An infinity or
+// a NaN is its first term and leaves nothing; a finite value's first term is finite.
 template <int TERMS>
 __device__ __forceinline__ void put_terms(void* terms, int64_t row, int64_t rows, int64_t pitch,
                                           int64_t n, const float* values) {
+  constexpr float kInfinity = __builtin_inff(), kMost = int8_most<bf16>::value;
   float z[8];
 #pragma unroll
   for (int j = 0; j < 8; ++j) z[j] = values[j];
 #pragma unroll
   for (int i = 0; i < TERMS; ++i) {
     uint32_t w[4];
+    auto first = [&](int j) {  // (past the first term nothing is that large)
+      return i == 0 && fabsf(z[j]) < kInfinity ? fminf(fmaxf(z[j], -kMost), kMost) : z[j];
+    };
+    auto rest = [&](int j, uint32_t term) {
+      z[j] = fabsf(z[j]) < kInfinity ? z[j] - __uint_as_float(term) : 0.f;
+    };
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      w[j] = pack2<bf16>(z[2 * j], z[2 * j + 1]);
-      z[2 * j] -= __uint_as_float(w[j] << 16);
-      z[2 * j + 1] -= __uint_as_float(w[j] & 0xffff0000u);
+      w[j] = pack2<bf16>(first(2 * j), first(2 * j + 1));
+      rest(2 * j, w[j] << 16);
+      rest(2 * j + 1, w[j] & 0xffff0000u);
     }
     *reinterpret_cast<uint4*>(static_cast<uint16_t*>(terms) + (i * rows + row) * pitch + n) =
         make_uint4(w[0], w[1], w[2], w[3]);
