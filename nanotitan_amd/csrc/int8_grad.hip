@@ -5,7 +5,7 @@
 // on the 16-bit matrix cores. The weights are read as integers, a quarter of what
 // bringing them to 16 bits first would read and write, and turned on the way to LDS:
 // a thread's 64 bytes are 16 values of k for four neighbouring n, and it writes for
-// each k its four n. (v + 128) s - 128 s as one fused multiply-add rounds q s once.
+// each k its four n. (q + 128) s - 128 s as one fused multiply-add rounds q s once.
 //
 // Through a feed-forward block a gradient would round five times on the way: weights,
 // activation's gradient and product with it, weights, output; in float16 4.7e-4 of
@@ -206,8 +206,7 @@ __global__ void __launch_bounds__(kGradThreads, BN == 256 ? 2 : 3) int8_grad_ker
                           (kt % TURNS * a.A + row0) * g.pitch + nb * 64;
       ta.issue(d, ((rows - 1) * g.pitch + kv) * 2, lds, kv, wave);
     };
-    auto turn = [&]() {
-      const float sc[4] = {s.x, s.y, s.z, s.w};
+    auto turn_by = [&](auto&& value) {  // value(i, q + 128): of the integer q of column i
       uint32_t u[4][KT / 4];
 #pragma unroll
       for (int i = 0; i < 4; ++i)
@@ -217,15 +216,31 @@ __global__ void __launch_bounds__(kGradThreads, BN == 256 ? 2 : 3) int8_grad_ker
       for (int j = 0; j < KT; ++j) {
         float v[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          v[i] = TERMS > 0 ? (float)(u[i][j / 4] >> (8 * (j % 4)) & 255u) - 128.f
-                       : fmaf((float)(u[i][j / 4] >> (8 * (j % 4)) & 255u), sc[i],
-                              -128.f * sc[i]);
+        for (int i = 0; i < 4; ++i) v[i] = value(i, (float)(u[i][j / 4] >> (8 * (j % 4)) & 255u));
         const int k = block * 64 + 16 * g4 + k_half + j;
         *reinterpret_cast<uint2*>(turned + k * 128 +
                                   ((2 * i4 + (t4 >> 1)) ^ turned_swizzle(k)) * 16 +
                                   (t4 & 1) * 8) =
             make_uint2(pack2<M>(v[0], v[1]), pack2<M>(v[2], v[3]));
+      }
+    };
+    auto turn = [&]() {
+      if constexpr (TERMS > 0) {
+        turn_by([](int, float u) { return u - 128.f; });
+      } else {
+        // what int8_value gives: scales whose values pass the type's largest are rare
+        constexpr float kMost = int8_most<T>::value;
+        const float sc[4] = {s.x, s.y, s.z, s.w};
+        const bool large = sc[0] > kMost / 128 || sc[1] > kMost / 128 || sc[2] > kMost / 128 ||
+                           sc[3] > kMost / 128;
+        if (__any(large)) {
+          turn_by([&](int i, float u) {
+            const float v = (u - 128.f) * sc[i];
+            return v > kMost ? kMost : v < -kMost ? -kMost : v;  // (a NaN stays one)
+          });
+        } else {
+          turn_by([&](int i, float u) { return fmaf(u, sc[i], -128.f * sc[i]); });
+        }
       }
     };
 

@@ -57,3 +57,33 @@ def test_the_largest_float32_gradient(monkeypatch):
     # three terms hold 2^-25 of the value, their sum rounds once more
     assert bool(((got[:, 1] - dout[:, 0]).abs() <= 2.0**-23 * 3.4e38).all())
     assert torch.equal(got[:, 2], -got[:, 1])
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("A", [80, 6000])  # tiles of 128 and of 256 columns
+def test_the_direct_product_takes_the_weights_as_decoded(dtype, A):
+    """Rows of one 1 pick the weights out: rounded once to 16 bits, past the type's largest that,
+    a NaN channel NaN, as ``int8_weight_decode`` gives them."""
+    t, K, N = TYPES[dtype], 1500, 80
+    g = torch.Generator().manual_seed(1)
+    W = torch.randn(1, K, N, generator=g)
+    most = torch.finfo(t).max
+    W[0, :, 3] *= 1e-6
+    for n, big in ((10, 1.0), (11, 0.99), (33, 1.5)):
+        W[0, 7 + n, n] = big * most if n != 33 or t == torch.float16 else 3.4e38
+    W[0, 5, 70] = float("nan")
+    w = int8_weight(W.cuda())
+    off = torch.tensor([0, A], dtype=torch.int32, device="cuda")
+    dout = torch.zeros(A, N, dtype=t)
+    dout[torch.arange(A), torch.arange(A) % N] = 1.0
+    held = moe_ops.int8_weight_decode(w, t)[0].t()
+    ext = moe_ops.get_hip_extension()
+    got = ext.int8_dx(dout.cuda(), off, w.codes, w.scale, K)
+    # 0 * NaN: with the NaN channel every row is NaN; without it the rows are the weights
+    assert bool(got.isnan().all())
+    scale = w.scale.clone()
+    scale[0, 70] = 1.0
+    got = ext.int8_dx(dout.cuda(), off, w.codes, scale, K)
+    want = held.clone()
+    want[70] = 0.0  # (its integers are 0)
+    assert torch.equal(got, want.repeat(-(-A // N), 1)[:A])
