@@ -97,8 +97,9 @@ int nt_int8_linear_gelu(int dtype, const void* x, const int32_t* offsets, const 
  * f16 and bf16: the weights are the values held, rounded to dtype. Row r of dout is at
  * r * dout_pitch, a multiple of 8 from N on; columns from N to the next multiple of 8
  * are read and must be finite. dout is 16-byte aligned.
- * f32: dout stands for its terms (below) from nt_int8_terms with the weights' scales;
- * dout_pitch and w_scales are not read. */
+ * f32, and f16 and bf16 with dout_pitch 0: dout stands for its terms (below) with the
+ * weights' scales, which meet the integers themselves, so no weight is rounded; dout_pitch
+ * and w_scales are not read otherwise. */
 int nt_int8_grouped_gemm_dx(int dtype, const int8_t* w, const float* w_scales,
                             const int32_t* offsets, const void* dout, int64_t dout_pitch,
                             int32_t E, int64_t A, int64_t K, int64_t N, void* dx,
@@ -108,9 +109,11 @@ int nt_int8_grouped_gemm_dx(int dtype, const int8_t* w, const float* w_scales,
  * sums of bfloat16 numbers: two, to 2^-17, where gradients are f16 or bf16, three, to
  * 2^-25, where they are f32. [terms][A][nt_int8_pitch(N)], 16-byte aligned, columns
  * from N on zero to the next multiple of 16 (the rest is not written, nor read).
- * nt_int8_terms_bytes is their size (0: too large). nt_int8_terms makes them of float32
- * rows dout [A, N]. */
+ * nt_int8_terms_bytes is their size (0: too large). nt_int8_rows_terms makes them of rows
+ * dout [A, N] of dtype, nt_int8_terms of float32 ones. */
 size_t nt_int8_terms_bytes(int dtype, int64_t A, int64_t N);
+int nt_int8_rows_terms(int dtype, const void* dout, const int32_t* offsets, const float* w_scales,
+                       int32_t E, int64_t A, int64_t N, void* terms, hipStream_t stream);
 int nt_int8_terms(const float* dout, const int32_t* offsets, const float* w_scales, int32_t E,
                   int64_t A, int64_t N, void* terms, hipStream_t stream);
 

@@ -248,6 +248,8 @@ INT8_EXPORTS: dict[str, tuple[object, list[object]]] = {
     "nt_int8_grouped_gemm_dx": (
         c_int, [c_int, _P, _P, _P, _P, c_int64, c_int32, c_int64, c_int64, c_int64, _P, _P]),
     "nt_int8_terms_bytes": (c_size_t, [c_int, c_int64, c_int64]),
+    "nt_int8_rows_terms": (
+        c_int, [c_int, _P, _P, _P, c_int32, c_int64, c_int64, _P, _P]),
     "nt_int8_terms": (c_int, [_P, _P, _P, c_int32, c_int64, c_int64, _P, _P]),
     "nt_int8_grouped_gemm_dx_gelu": (
         c_int,

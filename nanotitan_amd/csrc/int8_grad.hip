@@ -7,18 +7,23 @@
 // a thread's 64 bytes are 16 values of k for four neighbouring n, and it writes for
 // each k its four n. (q + 128) s - 128 s as one fused multiply-add rounds q s once.
 //
-// Through a feed-forward block a gradient would round five times on the way: weights,
-// activation's gradient and product with it, weights, output; in float16 4.7e-4 of
-// the gradient, 2.1e-4 of that its output's. Three of these are taken out: what the
-// forward keeps and the epilogue are float32, the gradient of the hidden values goes
-// on as two bfloat16 terms, times the next weights' scales, and these weights are
-// their integers, exact in bfloat16. Both terms meet the same operands in LDS, a step
-// each, so the second costs matrix instructions but no weights (14,312 rows of 768 by
-// 128 experts' 2,048: 116 us with one rounded term, 150 with two).
+// Rounding weights to 16 bits is an error as large as the output's own: a product's
+// gradient is off by 2.9e-4 of its norm in float16 and 2.3e-3 in bfloat16, where the
+// output's rounding is 2.1e-4 and 1.7e-3, and float16 holds no weight past 65,504. So
+// dOut times the scales goes in as two bfloat16 terms (2^-17) and the weights are their
+// integers, exact in bfloat16: what is left is the output's rounding. Both terms meet the
+// same operands in LDS, a step each, so the second costs matrix instructions but no
+// weights (14,312 rows of 2,048 by 128 experts' 768: 93 us with rounded weights, 158 by
+// terms with the launch that makes them; 8,192 rows of 14,336 by 8 of 4,096: 1,056 and
+// 1,778). Rounded weights are the caller's choice.
 //
-// Gradients in float32 are three such terms everywhere: 24 bits, and no weight is
-// rounded. That is three 16-bit products where one in float32 has a 16th of their
-// rate (8 experts of 4,096 x 14,336, 8,192 rows: 2.7 ms, with float32 weights 5.4).
+// Through a feed-forward block there would be five such roundings: what the forward keeps
+// and the epilogue are float32, and the gradient of the hidden values goes on as terms for
+// the next weights.
+//
+// Gradients in float32 are three such terms everywhere: 24 bits. That is three 16-bit
+// products where one in float32 has a 16th of their rate (8 experts of 4,096 x 14,336,
+// 8,192 rows: 2.7 ms, with float32 weights 5.4).
 #include <algorithm>
 #include <type_traits>
 
@@ -29,7 +34,7 @@ namespace nt {
 namespace {
 
 // Terms, TermsDual: from terms and the weights' integers, out for one or two matrices;
-// Gelu, SwiGLU: to such terms (and in float32 from them).
+// Gelu, SwiGLU: to such terms.
 enum Int8GradEpilogue { kGradPlain, kGradGelu, kGradSwiGLU, kGradTerms, kGradTermsDual };
 
 struct Int8Grad {
@@ -83,10 +88,11 @@ __device__ __forceinline__ void put_terms(void* terms, int64_t row, int64_t rows
   }
 }
 
-// Terms of a float32 gradient times its experts' scales, a wave a row.
+// Terms of a gradient times its experts' scales, a wave a row.
 constexpr int kTermRows = 4;
+template <typename T>
 __global__ void __launch_bounds__(kTermRows* kWave)
-    int8_terms_kernel(const float* dout, const int32_t* offsets, const float* w_scales, int32_t E,
+    int8_terms_kernel(const void* dout, const int32_t* offsets, const float* w_scales, int32_t E,
                       int64_t A, int64_t N, void* terms) {
   const int64_t row = (int64_t)blockIdx.x * kTermRows +
                       __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
@@ -97,25 +103,27 @@ __global__ void __launch_bounds__(kTermRows* kWave)
     if (offsets[mid] <= row) lo = mid;
     else hi = mid - 1;
   }
-  const float *in = dout + row * N, *sc = w_scales + lo * N;
+  const auto* in = static_cast<const typename elem<T>::storage*>(dout) + row * N;
+  const float* sc = w_scales + lo * N;
   const int64_t pitch = int8_pitch(N), end = round_up(N, (int64_t)16);
   for (int64_t n = lane_id() * 8; n < end; n += kWave * 8) {
-    Some<float, 8> v, s;
+    Some<T, 8> v;
+    Some<float, 8> s;
     v.load(in, n, N);
     s.load(sc, n, N);
     float z[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) z[j] = v.v[j] * s.v[j];
-    put_terms<3>(terms, row, A, pitch, n, z);
+    for (int j = 0; j < 8; ++j) z[j] = elem<T>::load(v.v[j]) * s.v[j];
+    put_terms<terms_of<T>>(terms, row, A, pitch, n, z);
   }
 }
 
-template <typename T, int EPI, int BN>
+// IN: dout and dout2 are terms.
+template <typename T, int EPI, int BN, bool IN>
 __global__ void __launch_bounds__(kGradThreads, BN == 256 ? 2 : 3) int8_grad_kernel(Int8Grad g) {
   typedef typename elem<T>::storage S;
   // terms of a value of dOut; none: rounded weights
-  constexpr int TERMS = std::is_same<T, float>::value                      ? 3
-                        : EPI == kGradTerms || EPI == kGradTermsDual ? 2 : 0;
+  constexpr int TERMS = IN ? terms_of<T> : 0;
   constexpr int TURNS = TERMS > 0 ? TERMS : 1;  // steps of the same weights
   typedef std::conditional_t<(TERMS > 0), bf16, T> M;
   typedef typename mfma_op<M>::vec vec;
@@ -334,13 +342,14 @@ int run_grad(int dtype, int epi, Int8Grad g, hipStream_t s) {
   if (a.E < 1 || a.A < 0 || a.K < 1 || a.N < 1) return NT_ERR_INVALID_ARG;
   if (a.E > NT_MAX_EXPERTS) return NT_ERR_TOO_MANY_EXPERTS;
   if (a.K > kInt8MaxK || a.N > kGradMaxN || a.A > kInt8MaxRows) return NT_ERR_TOO_LARGE;
-  if (terms || dtype == NT_F32) g.pitch = int8_pitch(a.N);
+  const bool in = terms || dtype == NT_F32 || g.pitch == 0;
+  if (in) g.pitch = int8_pitch(a.N);
   if (g.pitch > kGradMaxN) return NT_ERR_TOO_LARGE;  // a tile's rows within 31 bits
   if (a.A == 0) return NT_OK;
   auto bad = [](const void* p) { return p == nullptr || reinterpret_cast<uintptr_t>(p) % 16 != 0; };
   const bool two = epi == kGradTermsDual;
   if (g.pitch < a.N || g.pitch % 8 != 0 || bad(g.dout) || bad(a.w) || a.out == nullptr ||
-      (a.offsets == nullptr && a.E != 1) || (!terms && dtype != NT_F32 && a.w_scales == nullptr) ||
+      (a.offsets == nullptr && a.E != 1) || (!in && a.w_scales == nullptr) ||
       (two && (bad(g.dout2) || bad(a.w2))) ||
       (to_terms && (g.aux == nullptr || g.next == nullptr || bad(a.out))) ||
       (epi == kGradSwiGLU && (g.aux2 == nullptr || g.next2 == nullptr || bad(g.terms2))))
@@ -359,24 +368,30 @@ int run_grad(int dtype, int epi, Int8Grad g, hipStream_t s) {
       (unsigned)std::min<int64_t>(tiles, (wide ? 2 : 3) * cus);
   auto go = [&](auto type) {
     typedef typename decltype(type)::type T;
-    auto launch = [&](auto epilogue) {
+    auto launch = [&](auto epilogue, auto input) {
       constexpr int EPI = decltype(epilogue)::value;
+      constexpr bool IN = decltype(input)::value;
       if (wide)
-        hipLaunchKernelGGL((int8_grad_kernel<T, EPI, 256>), dim3(grid), dim3(kGradThreads), 0, s,
-                           g);
+        hipLaunchKernelGGL((int8_grad_kernel<T, EPI, 256, IN>), dim3(grid), dim3(kGradThreads), 0,
+                           s, g);
       else
-        hipLaunchKernelGGL((int8_grad_kernel<T, EPI, 128>), dim3(grid), dim3(kGradThreads), 0, s,
-                           g);
+        hipLaunchKernelGGL((int8_grad_kernel<T, EPI, 128, IN>), dim3(grid), dim3(kGradThreads), 0,
+                           s, g);
     };
+    auto block = [&](auto input) {
+      if (epi == kGradGelu) launch(std::integral_constant<int, kGradGelu>(), input);
+      else launch(std::integral_constant<int, kGradSwiGLU>(), input);
+    };
+    if (epi == kGradTerms) return launch(std::integral_constant<int, kGradTerms>(), std::true_type());
+    if (epi == kGradTermsDual)
+      return launch(std::integral_constant<int, kGradTermsDual>(), std::true_type());
+    if (in) return block(std::true_type());
     if constexpr (!std::is_same<T, float>::value) {
-      if (epi == kGradPlain) return launch(std::integral_constant<int, kGradPlain>());
+      if (epi == kGradPlain) launch(std::integral_constant<int, kGradPlain>(), std::false_type());
+      else block(std::false_type());
     }
-    if (epi == kGradGelu) launch(std::integral_constant<int, kGradGelu>());
-    else if (epi == kGradSwiGLU) launch(std::integral_constant<int, kGradSwiGLU>());
-    else if (epi == kGradTerms) launch(std::integral_constant<int, kGradTerms>());
-    else launch(std::integral_constant<int, kGradTermsDual>());
   };
-  if (dtype == NT_F32 && epi == kGradPlain) epi = kGradTerms;
+  if (in && epi == kGradPlain) epi = kGradTerms;
   int8_by_type(dtype, go);
   return launch_status();
 }
@@ -403,8 +418,9 @@ size_t nt_int8_terms_bytes(int dtype, int64_t A, int64_t N) {
   return (size_t)((dtype == NT_F32 ? 3 : 2) * A * int8_pitch(N) * 2);
 }
 
-int nt_int8_terms(const float* dout, const int32_t* offsets, const float* w_scales, int32_t E,
-                  int64_t A, int64_t N, void* terms, hipStream_t stream) {
+int nt_int8_rows_terms(int dtype, const void* dout, const int32_t* offsets, const float* w_scales,
+                       int32_t E, int64_t A, int64_t N, void* terms, hipStream_t stream) {
+  if (!int8_float(dtype)) return NT_ERR_DTYPE;
   if (E < 1 || A < 0 || N < 1) return NT_ERR_INVALID_ARG;
   if (E > NT_MAX_EXPERTS) return NT_ERR_TOO_MANY_EXPERTS;
   if (N > kGradMaxN || A > kInt8MaxRows) return NT_ERR_TOO_LARGE;
@@ -412,9 +428,18 @@ int nt_int8_terms(const float* dout, const int32_t* offsets, const float* w_scal
   if (dout == nullptr || w_scales == nullptr || terms == nullptr ||
       reinterpret_cast<uintptr_t>(terms) % 16 != 0 || (offsets == nullptr && E != 1))
     return NT_ERR_INVALID_ARG;
-  hipLaunchKernelGGL(int8_terms_kernel, dim3((unsigned)ceil_div(A, (int64_t)kTermRows)),
-                     dim3(kTermRows * kWave), 0, stream, dout, offsets, w_scales, E, A, N, terms);
+  int8_by_type(dtype, [&](auto type) {
+    typedef typename decltype(type)::type T;
+    hipLaunchKernelGGL((int8_terms_kernel<T>), dim3((unsigned)ceil_div(A, (int64_t)kTermRows)),
+                       dim3(kTermRows * kWave), 0, stream, dout, offsets, w_scales, E, A, N,
+                       terms);
+  });
   return launch_status();
+}
+
+int nt_int8_terms(const float* dout, const int32_t* offsets, const float* w_scales, int32_t E,
+                  int64_t A, int64_t N, void* terms, hipStream_t stream) {
+  return nt_int8_rows_terms(NT_F32, dout, offsets, w_scales, E, A, N, terms, stream);
 }
 
 int nt_int8_grouped_gemm_dx(int dtype, const int8_t* w, const float* w_scales,

@@ -220,8 +220,8 @@ Tensor new_terms(const Tensor& like, int64_t A, int64_t N) {
                    like.options().dtype(at::kBFloat16));
 }
 
-// A gradient's rows for the products with the weights held: of 16-bit types of a
-// multiple of 8 values, aligned; of float32 their terms.
+// A gradient's rows for the products with the weights held: their terms (of float32
+// always), or rows of 16-bit types of a multiple of 8 values, aligned.
 struct GradIn {
   Weight w;
   const int32_t* off;
@@ -229,19 +229,19 @@ struct GradIn {
   Tensor rows;
 };
 GradIn check_dx(const Tensor& dout, const OptTensor& offsets, const Tensor& codes,
-                const Tensor& scales, int64_t K) {
+                const Tensor& scales, int64_t K, bool by_terms) {
   check_rows(dout, "dOut");
   const Weight w = check_weight(codes, scales, K, dout, "weight");
   const int32_t* off = check_offsets(offsets, dout, w.E);
   const int64_t A = dout.size(0), pitch = dout.size(1);
-  if (dout.scalar_type() == at::kFloat) {
+  if (by_terms || dout.scalar_type() == at::kFloat) {
     TORCH_CHECK(pitch == w.N, "dOut must have ", w.N, " columns, has ", pitch);
     c10::hip::HIPGuard guard(dout.get_device());
     Tensor terms = new_terms(dout, A, w.N);
-    check_status(nt_int8_terms(dout.data_ptr<float>(), off, w.scales, w.E, A, w.N,
-                               terms.data_ptr(), stream_of(dout)),
+    check_status(nt_int8_rows_terms(dtype_code(dout), dout.data_ptr(), off, w.scales, w.E, A, w.N,
+                                    terms.data_ptr(), stream_of(dout)),
                  "int8_terms");
-    return {w, off, A, pitch, terms};
+    return {w, off, A, 0, terms};
   }
   TORCH_CHECK(pitch == (w.N + 7) / 8 * 8 &&
                   reinterpret_cast<uintptr_t>(dout.data_ptr()) % 16 == 0,
@@ -258,9 +258,10 @@ void check_kept(const Tensor& t, int64_t rows, int64_t cols, const Tensor& like,
               " must be a contiguous [", rows, ", ", cols, "]");
 }
 
-// int8_dx(dOut, offsets, codes, scales, K) -> dOut @ W^T.
-Tensor int8_dx(Tensor dout, OptTensor offsets, Tensor codes, Tensor scales, int64_t K) {
-  const GradIn g = check_dx(dout, offsets, codes, scales, K);
+// int8_dx(dOut, offsets, codes, scales, K, by_terms) -> dOut @ W^T.
+Tensor int8_dx(Tensor dout, OptTensor offsets, Tensor codes, Tensor scales, int64_t K,
+               bool by_terms) {
+  const GradIn g = check_dx(dout, offsets, codes, scales, K, by_terms);
   c10::hip::HIPGuard guard(dout.get_device());
   Tensor dx = at::empty({g.A, K}, dout.options());
   check_status(nt_int8_grouped_gemm_dx(dtype_code(dout), g.w.codes, g.w.scales, g.off,
@@ -272,8 +273,8 @@ Tensor int8_dx(Tensor dout, OptTensor offsets, Tensor codes, Tensor scales, int6
 // The same and an activation's gradient, in terms for the up projections: (terms of
 // up or gate, of value).
 Tensor int8_dx_gelu(Tensor dout, Tensor slope, OptTensor offsets, Tensor codes, Tensor scales,
-                    Tensor up_scales, int64_t K) {
-  const GradIn g = check_dx(dout, offsets, codes, scales, K);
+                    Tensor up_scales, int64_t K, bool by_terms) {
+  const GradIn g = check_dx(dout, offsets, codes, scales, K, by_terms);
   check_kept(slope, g.A, K, dout, "gelu'");
   check_kept(up_scales, g.w.E, K, dout, "up scales");
   c10::hip::HIPGuard guard(dout.get_device());
@@ -287,8 +288,9 @@ Tensor int8_dx_gelu(Tensor dout, Tensor slope, OptTensor offsets, Tensor codes, 
 }
 std::tuple<Tensor, Tensor> int8_dx_swiglu(Tensor dout, Tensor gate, Tensor value,
                                           OptTensor offsets, Tensor codes, Tensor scales,
-                                          Tensor gate_scales, Tensor val_scales, int64_t K) {
-  const GradIn g = check_dx(dout, offsets, codes, scales, K);
+                                          Tensor gate_scales, Tensor val_scales, int64_t K,
+                                          bool by_terms) {
+  const GradIn g = check_dx(dout, offsets, codes, scales, K, by_terms);
   check_kept(gate, g.A, K, dout, "gate");
   check_kept(value, g.A, K, dout, "value");
   check_kept(gate_scales, g.w.E, K, dout, "gate scales");
@@ -385,9 +387,15 @@ void bind_int8(py::module& m) {
   m.def("int8_product", &int8_product, "Rows by 8-bit weights, grouped by expert");
   m.def("int8_swiglu_ffn", &int8_swiglu_ffn, "SwiGLU FFN on 8-bit weights -> (y, gate, value)");
   m.def("int8_gelu_ffn", &int8_gelu_ffn, "GELU FFN on 8-bit weights -> (y, gelu')");
-  m.def("int8_dx", &int8_dx, "Gradient rows by 8-bit weights, transposed");
-  m.def("int8_dx_gelu", &int8_dx_gelu, "Such a product times gelu' -> terms");
-  m.def("int8_dx_swiglu", &int8_dx_swiglu, "Such a product by SwiGLU's gradient -> (terms, terms)");
+  const auto by_terms = pybind11::arg("by_terms") = false;
+  using a = pybind11::arg;
+  m.def("int8_dx", &int8_dx, "Gradient rows by 8-bit weights, transposed", a("dout"), a("offsets"),
+        a("codes"), a("scales"), a("K"), by_terms);
+  m.def("int8_dx_gelu", &int8_dx_gelu, "Such a product times gelu' -> terms", a("dout"), a("slope"),
+        a("offsets"), a("codes"), a("scales"), a("up_scales"), a("K"), by_terms);
+  m.def("int8_dx_swiglu", &int8_dx_swiglu, "Such a product by SwiGLU's gradient -> (terms, terms)",
+        a("dout"), a("gate"), a("value"), a("offsets"), a("codes"), a("scales"), a("gate_scales"),
+        a("val_scales"), a("K"), by_terms);
   m.def("int8_dx_terms", &int8_dx_terms, "Terms by the integers of 8-bit weights, transposed");
   m.def("int8_moe_few_tokens", &int8_moe_few_tokens,
         "A whole MoE layer for few tokens on 8-bit weights -> (out, gates, topk)");

@@ -182,7 +182,8 @@ class Int8ExpertFFN(nn.Module):
     none. The weights are buffers: two a projection, ``<name>_codes`` and ``<name>_scale``, the
     float32 scales as the int32 of their bits, which a cast of the module to another float type
     leaves alone. ``cfg.ffn_checkpoint8`` does not apply: what the backward keeps is gate and
-    value, or gelu', in float32.
+    value, or gelu', in float32. ``cfg.int8_exact_gradient = False`` rounds the weights to 16
+    bits in a 16-bit gradient, which is faster (``int8_swiglu_ffn_fn``).
     """
 
     def __init__(self, experts):
@@ -210,7 +211,8 @@ class Int8ExpertFFN(nn.Module):
 
     def forward(self, packed_X, expert_offset):
         ffn = int8_swiglu_ffn_fn if len(self.names) == 3 else int8_gelu_ffn_fn
-        return ffn(packed_X, *self.weights(), expert_offset)
+        return ffn(packed_X, *self.weights(), expert_offset,
+                   getattr(self.cfg, "int8_exact_gradient", True))
 
 
 def moe_forward_from_logits(x_flat, logits, experts, num_experts, top_k):

@@ -849,7 +849,7 @@ def _int8_direct(dout, experts, K):
     """Whether the kernels that read 8-bit weights give dout @ W^T; else the weights go to
     dout's dtype first and to the product of that.
 
-    16-bit gradients: where reading and writing the weights costs more than the products gain from
+    16-bit gradients of weights rounded to 16 bits: where reading and writing the weights costs more than the products gain from
     weights in 16 bits, at most 512 rows an expert and 2^25 weights or more (128 experts of 2,048 x
     768, 14,312 rows: 88 us against 111 + 104; 8 of 4,096 x 14,336, 1,000 rows: 338 against 300 +
     262, 8,192 rows: 1,331 against 301 + 1,022; 8 of 512 x 2,048, 4,096 rows: 54 against 9 + 28).
@@ -871,9 +871,11 @@ def _aligned(t):
     return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
-def _int8_dx(dout, off, codes, scale, K):
+def _int8_dx(dout, off, codes, scale, K, exact):
     """dout @ W^T for the weights [E,K,N] that codes and scale hold."""
     ext = get_hip_extension()
+    if exact and dout.dtype != torch.float32:
+        return ext.int8_dx(dout.contiguous(), off, codes, scale, K, True)
     if _int8_direct(dout, scale.shape[0], K):
         return ext.int8_dx(_aligned(dout), off, codes, scale, K)
     W = ext.int8_weight_decode(codes, scale, K, dout.dtype)
@@ -883,38 +885,39 @@ def _int8_dx(dout, off, codes, scale, K):
 class Int8GroupedGEMM_FN(torch.autograd.Function):
     """X by frozen 8-bit weights; the gradient to X is dOut times the weights held, transposed.
 
-    The rounding of X is passed straight through. The backward's product takes the weights in
-    dOut's dtype (a rounding of 16-bit types, as small as the output's own).
+    The rounding of X is passed straight through. ``exact``: only the result is rounded to dOut's
+    dtype; else 16-bit gradients take the weights in dOut's dtype, which is a rounding as large
+    as the output's own, for three fifths of the time.
     """
 
     @staticmethod
-    def forward(ctx, X, expert_offset, weight):
+    def forward(ctx, X, expert_offset, weight, exact):
         ctx.save_for_backward(expert_offset, weight.codes, weight.scale)
-        ctx.shape = weight.shape
+        ctx.shape, ctx.exact = weight.shape, exact
         return get_hip_extension().int8_product(X, expert_offset, weight.codes, weight.scale)
 
     @staticmethod
     @_once_differentiable
     def backward(ctx, dout):
         off, codes, scale = ctx.saved_tensors
-        return _int8_dx(dout, off, codes, scale, ctx.shape[1]), None, None
+        return _int8_dx(dout, off, codes, scale, ctx.shape[1], ctx.exact), None, None, None
 
 
 class Int8SwiGLUFFN_FN(torch.autograd.Function):
     """SwiGLU FFN on frozen 8-bit weights, with the gradient to X.
 
     Keeps gate and value in float32; the rounding of X and of the hidden values is passed
-    straight through. Of 16-bit gradients the down projection's weights and the result are
-    rounded to their dtype, and nothing between.
+    straight through. ``exact``: only the result is rounded to a 16-bit dtype; else the down
+    projection's weights are too, for 5 to 20% less time in the backward.
     """
 
     @staticmethod
-    def forward(ctx, X, expert_offset, W_gate, W_val, W_out):
+    def forward(ctx, X, expert_offset, W_gate, W_val, W_out, exact):
         weights = (W_gate, W_val, W_out)
         held = [t for w in weights for t in (w.codes, w.scale)]
         y, gate, value = get_hip_extension().int8_swiglu_ffn(X, expert_offset, *held, True)
         ctx.save_for_backward(expert_offset, gate, value, *held)
-        ctx.shape = W_gate.shape
+        ctx.shape, ctx.exact = W_gate.shape, exact
         return y
 
     @staticmethod
@@ -923,20 +926,21 @@ class Int8SwiGLUFFN_FN(torch.autograd.Function):
         ext = get_hip_extension()
         off, gate, value, gc, gs, vc, vs, oc, os = ctx.saved_tensors
         E, d, f = ctx.shape
-        tg, tv = ext.int8_dx_swiglu(_aligned(dy), gate, value, off, oc, os, gs, vs, f)
+        dy = dy.contiguous() if ctx.exact else _aligned(dy)
+        tg, tv = ext.int8_dx_swiglu(dy, gate, value, off, oc, os, gs, vs, f, ctx.exact)
         dX = ext.int8_dx_terms(tg, tv, off, gc, gs, vc, d, dy.dtype)
-        return dX, None, None, None, None
+        return dX, None, None, None, None, None
 
 
 class Int8GeluFFN_FN(torch.autograd.Function):
-    """GELU FFN on frozen 8-bit weights, with the gradient to X; keeps gelu' in float32."""
+    """GELU FFN on frozen 8-bit weights, as Int8SwiGLUFFN_FN; keeps gelu' in float32."""
 
     @staticmethod
-    def forward(ctx, X, expert_offset, W_up, W_down):
+    def forward(ctx, X, expert_offset, W_up, W_down, exact):
         held = [t for w in (W_up, W_down) for t in (w.codes, w.scale)]
         y, slope = get_hip_extension().int8_gelu_ffn(X, expert_offset, *held, True)
         ctx.save_for_backward(expert_offset, slope, *held)
-        ctx.shape = W_up.shape
+        ctx.shape, ctx.exact = W_up.shape, exact
         return y
 
     @staticmethod
@@ -945,47 +949,52 @@ class Int8GeluFFN_FN(torch.autograd.Function):
         ext = get_hip_extension()
         off, slope, uc, us, dc, ds = ctx.saved_tensors
         E, d, f = ctx.shape
-        terms = ext.int8_dx_gelu(_aligned(dy), slope, off, dc, ds, us, f)
+        dy = dy.contiguous() if ctx.exact else _aligned(dy)
+        terms = ext.int8_dx_gelu(dy, slope, off, dc, ds, us, f, ctx.exact)
         dX = ext.int8_dx_terms(terms, None, off, uc, us, None, d, dy.dtype)
-        return dX, None, None, None
+        return dX, None, None, None, None
 
 
-def int8_grouped_gemm_fn(X, weight, expert_offset=None):
+def int8_grouped_gemm_fn(X, weight, expert_offset=None, exact_gradient=True):
     """X [A,K] by 8-bit weights [E,K,N], each row by its expert's: [A,N] in X's dtype.
 
     The rows of X are brought to 8 bits, the products are exact integer sums, scaled in float32
     and rounded once. Without ``expert_offset`` the weights are one linear layer's (E = 1).
-    Weights are frozen; X gets its gradient.
+    Weights are frozen; X gets its gradient, that of the weights held, rounded once. With
+    ``exact_gradient`` False a 16-bit gradient takes the weights rounded to its type first (past
+    its largest value: that), which is faster.
     """
     _check_int8(weight)
     if X.dim() != 2 or X.shape[1] != weight.shape[1]:
         raise RuntimeError(f"X {tuple(X.shape)} does not fit weights {tuple(weight.shape)}")
     X = X.contiguous()
     if _tracked(X):
-        return Int8GroupedGEMM_FN.apply(X, expert_offset, weight)
+        return Int8GroupedGEMM_FN.apply(X, expert_offset, weight, exact_gradient)
     return get_hip_extension().int8_product(X, expert_offset, weight.codes, weight.scale)
 
 
-def int8_swiglu_ffn_fn(X, W_gate, W_val, W_out, expert_offset=None):
+def int8_swiglu_ffn_fn(X, W_gate, W_val, W_out, expert_offset=None, exact_gradient=True):
     """silu(X W_gate) * (X W_val), then W_out, on 8-bit weights: [A,d] in X's dtype.
 
     X and the hidden values (from their values in X's dtype) are brought to 8 bits row by row;
-    gate and value stay in float32 up to the hidden values. X gets its gradient.
+    gate and value stay in float32 up to the hidden values. X gets its gradient, rounded once;
+    with ``exact_gradient`` False a 16-bit one takes the out projection's weights rounded to its
+    type (past its largest value: that), which is faster.
     """
     X = X.contiguous()
     _check_chain(X, W_gate, W_val, W_out)
     if _tracked(X):
-        return Int8SwiGLUFFN_FN.apply(X, expert_offset, W_gate, W_val, W_out)
+        return Int8SwiGLUFFN_FN.apply(X, expert_offset, W_gate, W_val, W_out, exact_gradient)
     return get_hip_extension().int8_swiglu_ffn(
         X, expert_offset, W_gate.codes, W_gate.scale, W_val.codes, W_val.scale, W_out.codes,
         W_out.scale, False)[0]
 
 
-def int8_gelu_ffn_fn(X, W_up, W_down, expert_offset=None):
+def int8_gelu_ffn_fn(X, W_up, W_down, expert_offset=None, exact_gradient=True):
     """gelu(X W_up) W_down (erf) on 8-bit weights, as int8_swiglu_ffn_fn."""
     X = X.contiguous()
     _check_chain(X, W_up, None, W_down)
     if _tracked(X):
-        return Int8GeluFFN_FN.apply(X, expert_offset, W_up, W_down)
+        return Int8GeluFFN_FN.apply(X, expert_offset, W_up, W_down, exact_gradient)
     return get_hip_extension().int8_gelu_ffn(X, expert_offset, W_up.codes, W_up.scale,
                                              W_down.codes, W_down.scale, False)[0]
