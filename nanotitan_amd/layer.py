@@ -255,6 +255,12 @@ def _plain_experts(experts) -> bool:
             and not nn.modules.module._has_any_global_hook())
 
 
+def _hung_on(module) -> bool:
+    """Whether hooks hang on a module, or a forward stands in place of its class's."""
+    return any((module._forward_hooks, module._forward_pre_hooks, module._backward_hooks,
+                module._backward_pre_hooks)) or "forward" in module.__dict__
+
+
 class HIPMoEBackend:
     """Reference CUDAMoEBackend dataflow (src/model/cuda_backend.py:11-81) on the HIP path."""
 
@@ -323,8 +329,13 @@ class MoE(nn.Module):
     def quantize_experts(self):
         """Puts the experts' weights into 8-bit integers, in place (``Int8ExpertFFN``): the module
         then has no expert parameters, and an optimizer made before still holds the old ones.
-        Hooks on the experts do not carry over. Returns self."""
+        Hooks on the experts, or a forward put in place of theirs, would be lost: it raises then.
+        Returns self."""
         if type(self.experts) is not Int8ExpertFFN:
+            if _hung_on(self.experts):
+                raise RuntimeError("quantize_experts replaces the experts: remove their hooks, or "
+                                   "the forward put in place of theirs, and add them to the new "
+                                   "ones")
             self.experts = Int8ExpertFFN(self.experts)
             self.moe_backend.experts = self.experts
         return self
