@@ -202,6 +202,7 @@ class Int8ExpertFFN(nn.Module):
             self.shapes[name] = w.shape
             self.register_buffer(f"{name}_codes", w.codes)
             self.register_buffer(f"{name}_scale", w.scale.view(torch.int32))
+        self.train(experts.training)
 
     def weights(self):
         """The projections' Int8Weights, as ``moe_few_tokens`` and the ``int8_*_ffn_fn`` take them."""
