@@ -76,6 +76,14 @@ int nt_int8_grouped_gemm_gelu(int dtype, const int8_t* x, const float* x_scales,
                               int32_t E, int64_t A, int64_t K, int64_t N, void* act,
                               float* act_grad, hipStream_t stream);
 
+/* How the products of these sizes are tiled on a chip of `cus` CUs, by the expected tiles
+ * of evenly spread experts: rows and columns (of SwiGLU both matrices' together) of a tile,
+ * or 0 and 0 where the weights are streamed. Of NT_INT8_GRADIENT K are the columns. No
+ * result depends on it. */
+enum { NT_INT8_PLAIN = 0, NT_INT8_SWIGLU = 1, NT_INT8_GELU = 2, NT_INT8_GRADIENT = 3 };
+int nt_int8_tile(int product, int32_t E, int64_t A, int64_t K, int64_t N, int32_t cus,
+                 int32_t* rows, int32_t* columns);
+
 /* The same three from rows x [A, K] of dtype, which they bring to 8 bits themselves:
  * the bits of nt_int8_rows and the product. The workspace (16-byte aligned, contents
  * arbitrary) is written before it is read: calls that cannot overlap may share one. */

@@ -209,6 +209,7 @@ EXPORTS: dict[str, tuple[object, list[object]]] = {
 
 # include/nanotitan_int8.h
 NT_INT8_MAX_K, NT_INT8_MAX_ROWS = 1 << 17, (1 << 24) - 1
+NT_INT8_PLAIN, NT_INT8_SWIGLU, NT_INT8_GELU, NT_INT8_GRADIENT = 0, 1, 2, 3
 INT8_EXPORTS: dict[str, tuple[object, list[object]]] = {
     "nt_int8_pitch": (c_int64, [c_int64]),
     "nt_int8_rows_bytes": (c_size_t, [c_int64, c_int64]),
@@ -231,6 +232,8 @@ INT8_EXPORTS: dict[str, tuple[object, list[object]]] = {
         c_int,
         [c_int, _P, _P, _P, _P, _P, c_int32, c_int64, c_int64, c_int64, _P, _P, _P],
     ),
+    "nt_int8_tile": (
+        c_int, [c_int, c_int32, c_int64, c_int64, c_int64, c_int32, _P, _P]),
     "nt_int8_linear_workspace_bytes": (c_size_t, [c_int64, c_int64]),
     "nt_int8_linear": (
         c_int,

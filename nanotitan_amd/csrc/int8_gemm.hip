@@ -300,26 +300,33 @@ int launch_tiles(Int8Gemm a, int per_cu, hipStream_t s) {
 // for a product (32,768 rows, 14,336 to 4,096: 1,793 -> 1,692 us, 8,192: 990 -> 940,
 // but 4,096: 442 -> 486; two matrices, 4,096 to 4,096: 969 -> 942 us, 2,048: 505 ->
 // 512).
+Int8Tile int8_tile(int epi, int64_t E, int64_t A, int64_t K, int64_t N, int64_t cus) {
+  const bool two = epi == kInt8SwiGLU;
+  const int64_t width = two ? 128 : 256;
+  auto tiles = [&](int64_t rows) {  // expected: an expert's last tile is half full
+    return (ceil_div(A, rows) + E / 2) * ceil_div(N, width);
+  };
+  const int64_t loads = ceil_div(A, 64) + E / 2;
+  if (A <= 24 * E || ((ceil_div(A, 128) + E / 2) * ceil_div(N, two ? 64 : 128) <= cus &&
+                      loads * N * (two ? 2 : 1) < 20000))
+    return {0, 0};
+  if (K >= (two ? 4096 : 8192) && tiles(256) >= 4 * cus) return {256, 256};
+  if (tiles(128) >= 3 * cus) return {128, 256};
+  return {128, 128};
+}
+
 template <typename T, int EPI>
 int launch_by_size(const Int8Gemm& a, hipStream_t s) {
   constexpr int dtype = std::is_same<T, float>::value ? NT_F32
                         : std::is_same<T, f16>::value ? NT_F16 : NT_BF16;
-  constexpr bool two = EPI == kInt8SwiGLU;
-  const int64_t cus = device_cus(s), width = two ? 128 : 256;
-  auto tiles = [&](int64_t rows) {  // expected: an expert's last tile is half full
-    return (ceil_div(a.A, rows) + a.E / 2) * ceil_div(a.N, width);
-  };
-  const int64_t loads = ceil_div(a.A, 64) + a.E / 2;
-  if (a.A <= 24 * (int64_t)a.E ||
-      ((ceil_div(a.A, 128) + a.E / 2) * ceil_div(a.N, two ? 64 : 128) <= cus &&
-       loads * a.N * (two ? 2 : 1) < 20000)) {
+  const Int8Tile tile = int8_tile(EPI, a.E, a.A, a.K, a.N, device_cus(s));
+  if (tile.rows == 0) {
     launch_int8_stream(a, EPI, dtype, s);
     return launch_status();
   }
-  if (a.K >= (two ? 4096 : 8192) && tiles(256) >= 4 * cus)
-    return launch_tiles<T, EPI, 256, 256, 4, 2, 3>(a, 1, s);
-  if (tiles(128) >= 3 * cus) return launch_tiles<T, EPI, 128, 256, 2, 2, 3>(a, 2, s);
-  if constexpr (two) return launch_tiles<T, EPI, 128, 128, 4, 1, 3>(a, 2, s);
+  if (tile.rows == 256) return launch_tiles<T, EPI, 256, 256, 4, 2, 3>(a, 1, s);
+  if (tile.cols == 256) return launch_tiles<T, EPI, 128, 256, 2, 2, 3>(a, 2, s);
+  if constexpr (EPI == kInt8SwiGLU) return launch_tiles<T, EPI, 128, 128, 4, 1, 3>(a, 2, s);
   else return launch_tiles<T, EPI, 128, 128, 2, 2, 3>(a, 3, s);
 }
 
@@ -368,6 +375,21 @@ int run_int8(int dtype, int epi, Int8Gemm a, hipStream_t s, void* ws = nullptr,
 using namespace nt;
 
 extern "C" {
+
+int nt_int8_tile(int product, int32_t E, int64_t A, int64_t K, int64_t N, int32_t cus,
+                 int32_t* rows, int32_t* columns) {
+  if (product < NT_INT8_PLAIN || product > NT_INT8_GRADIENT || cus < 1 || rows == nullptr ||
+      columns == nullptr)
+    return NT_ERR_INVALID_ARG;
+  Int8Gemm a = {};
+  a.E = E, a.A = A, a.K = K, a.N = N;
+  const int st = check_int8(NT_F32, a);
+  if (st != NT_OK) return st;
+  const Int8Tile tile = product == NT_INT8_GRADIENT ? int8_gradient_tile(E, A, K, cus)
+                                                    : int8_tile(product, E, A, K, N, cus);
+  *rows = tile.rows, *columns = tile.cols;
+  return NT_OK;
+}
 
 size_t nt_int8_linear_workspace_bytes(int64_t A, int64_t K) {
   if (A < 0 || A > kInt8MaxRows || K < 1 || K > kInt8MaxK) return 0;

@@ -8,7 +8,11 @@
 
 namespace nt {
 
-enum Int8Epilogue { kInt8Plain = 0, kInt8SwiGLU = 1, kInt8Gelu = 2 };
+enum Int8Epilogue {
+  kInt8Plain = NT_INT8_PLAIN,
+  kInt8SwiGLU = NT_INT8_SWIGLU,
+  kInt8Gelu = NT_INT8_GELU
+};
 
 struct Int8Gemm {
   const int8_t* x;          // rows of integers, and their scales [A]
@@ -23,6 +27,12 @@ struct Int8Gemm {
   float *out2, *out3;  // gate, value; gelu' (null: not written)
   int32_t ntn;
 };
+
+struct Int8Tile {
+  int32_t rows, cols;  // 0: no tiles, the weights are streamed
+};
+// int8_grad.hip: the tile of a gradient's product, K output columns.
+Int8Tile int8_gradient_tile(int64_t E, int64_t A, int64_t K, int64_t cus);
 
 // int8_few.hip: the product of few rows for each expert; and that of a few rows from
 // their values (false where it does not take them).

@@ -354,13 +354,8 @@ int run_grad(int dtype, int epi, Int8Grad g, hipStream_t s) {
       (to_terms && (g.aux == nullptr || g.next == nullptr || bad(a.out))) ||
       (epi == kGradSwiGLU && (g.aux2 == nullptr || g.next2 == nullptr || bad(g.terms2))))
     return NT_ERR_INVALID_ARG;
-  // Half as wide where tiles of 256 columns (an expert's last one half full) are about as
-  // few as CUs: a step waits for its loads, and then twice as many run at a time (66
-  // tiles, 4,188 rows of terms, 2,048 to 512: 56 us for 80; 264, 512 to 2,048: 34 for 39;
-  // but 420, 871 rows, 4,096 to 14,336: 178 for 159, and 1,024 109 for 98).
   const int64_t cus = device_cus(s);
-  const bool wide =
-      4 * (ceil_div(a.A, (int64_t)kGradBM) + a.E / 2) * ceil_div(a.K, (int64_t)256) > 5 * cus;
+  const bool wide = int8_gradient_tile(a.E, a.A, a.K, cus).cols == 256;
   a.ntn = (int32_t)ceil_div(a.K, (int64_t)(wide ? 256 : 128));
   const int64_t tiles = (ceil_div(a.A, (int64_t)kGradBM) + a.E - 1) * a.ntn;
   if (tiles > INT32_MAX) return NT_ERR_TOO_LARGE;
@@ -407,6 +402,16 @@ Int8Grad make_grad(const int8_t* w, const float* w_scales, const int32_t* offset
 }
 
 }  // namespace
+
+// Half as wide where tiles of 256 columns (an expert's last one half full) are about as
+// few as CUs: a step waits for its loads, and then twice as many run at a time (66
+// tiles, 4,188 rows of terms, 2,048 to 512: 56 us for 80; 264, 512 to 2,048: 34 for 39;
+// but 420, 871 rows, 4,096 to 14,336: 178 for 159, and 1,024 109 for 98).
+Int8Tile int8_gradient_tile(int64_t E, int64_t A, int64_t K, int64_t cus) {
+  const int64_t tiles = (ceil_div(A, (int64_t)kGradBM) + E / 2) * ceil_div(K, (int64_t)256);
+  return {kGradBM, 4 * tiles > 5 * cus ? 256 : 128};
+}
+
 }  // namespace nt
 
 using namespace nt;
