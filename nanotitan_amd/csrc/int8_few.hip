@@ -360,7 +360,7 @@ __global__ void __launch_bounds__(KW* kWave)
                      __hip_atomic_load(y, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT), sum);
         }
         if constexpr (kOwn)
-          static_cast<typename elem<X>::storage*>(arrive.out)[t * a.N + n] = to_bits<X>(sum);
+          static_cast<typename elem<X>::storage*>(arrive.out)[t * a.N + n] = rounded<X>(sum);
       }
     }
   }
@@ -556,7 +556,7 @@ __global__ void __launch_bounds__(256) int8_combine_kernel(const float* y, const
 #pragma unroll 4
   for (int j = 0; j < k; ++j)
     sum = fmaf(gates[t * k + j], y[(int64_t)inv[t * k + j] * d + c], sum);
-  static_cast<typename elem<T>::storage*>(out)[t * d + c] = to_bits<T>(sum);
+  static_cast<typename elem<T>::storage*>(out)[t * d + c] = rounded<T>(sum);
 }
 
 struct Layout {

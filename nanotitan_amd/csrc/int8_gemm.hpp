@@ -2,6 +2,8 @@
 // epilogues. Tiles of many rows: int8_gemm.hip; few rows: int8_few.hip.
 #pragma once
 
+#include <type_traits>
+
 #include "bits.hpp"
 #include "gelu.hpp"
 #include "int8.hpp"
@@ -97,21 +99,34 @@ __device__ __forceinline__ float normal_cdf<float>(float x, float& bell) {
   return 0.5f * erfcf(x * -0.70710678118654752f);
 }
 
+// A product or sum that goes on to T, rounded to float32 first. Without the bar the compiler
+// makes it and its rounding to float16 one operation in some columns of some kernels, and
+// one value in thousands then depends on the kernel that the batch's size chose.
+template <typename T>
+__device__ __forceinline__ float in_float32(float v) {
+  if constexpr (std::is_same<T, f16>::value) asm("" : "+v"(v));
+  return v;
+}
+template <typename T>
+__device__ __forceinline__ typename elem<T>::storage rounded(float v) {
+  return to_bits<T>(in_float32<T>(v));
+}
+
 // The outputs of one column from its scaled sums p (and p2, the value). What a backward
 // needs stays in float32: rounded to 16 bits it would be half of the gradient's error.
 template <typename T, int EPI>
 __device__ __forceinline__ void int8_epilogue(float p, float p2, typename elem<T>::storage& o,
                                               float& o2, float& o3) {
   if constexpr (EPI == kInt8Plain) {
-    o = to_bits<T>(p);
+    o = rounded<T>(p);
   } else if constexpr (EPI == kInt8SwiGLU) {
-    o = to_bits<T>(p * sigmoid_of<T>(p) * p2);
+    o = rounded<T>(p * sigmoid_of<T>(p) * p2);
     o2 = p;
     o3 = p2;
   } else {
     float bell;
     const float c = normal_cdf<T>(p, bell);
-    o = to_bits<T>(p * c);
+    o = rounded<T>(p * c);
     o2 = fmaf(p, bell * 0.39894228040143268f, c);
   }
 }

@@ -247,7 +247,9 @@ __global__ void __launch_bounds__(kGradThreads, BN == 256 ? 2 : 3) int8_grad_ker
             return v > kMost ? kMost : v < -kMost ? -kMost : v;  // (a NaN stays one)
           });
         } else {
-          turn_by([&](int i, float u) { return fmaf(u, sc[i], -128.f * sc[i]); });
+          turn_by([&](int i, float u) {
+            return in_float32<T>(fmaf(u, sc[i], -128.f * sc[i]));
+          });
         }
       }
     };
