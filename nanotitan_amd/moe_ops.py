@@ -787,11 +787,11 @@ def int8_weight(W):
     """W [E,K,N] (or [K,N], as one expert) as an Int8Weight: every channel's largest magnitude is 127.
 
     Each value goes to the nearest multiple of its channel's scale, ties to even. A channel with
-    an infinity or a NaN has a NaN scale.
+    an infinity or a NaN has a NaN scale. W gets no gradient.
     """
     if W.dim() == 2:
         W = W.unsqueeze(0)
-    codes, scale = get_hip_extension().int8_weight(W.detach().contiguous())
+    codes, scale = get_hip_extension().int8_weight(W.contiguous())
     return Int8Weight(codes, scale, tuple(W.shape))
 
 
@@ -808,9 +808,9 @@ def int8_rows(x):
     Row r's integer for column c is codes[r//16, c//64, c%64 // 16, r%16, c%16]; f is padded with
     zeros to 128, rows past the last hold anything. Times its row's scale it is the value's
     nearest multiple of the row's largest magnitude / 127 (ties to even). A row with an infinity
-    or a NaN has a NaN scale.
+    or a NaN has a NaN scale. Neither has a gradient.
     """
-    return get_hip_extension().int8_rows(x.detach().contiguous())
+    return get_hip_extension().int8_rows(x.contiguous())
 
 
 def int8_rows_decode(codes, scales, width, dtype):

@@ -8,6 +8,7 @@ import pytest
 import torch
 
 from nanotitan_amd.layer import MoE
+from nanotitan_amd.moe_ops import int8_rows, int8_weight
 
 pytestmark = pytest.mark.gpu
 
@@ -46,3 +47,14 @@ def test_copies_and_saved_modules():
             getattr(m.experts, f"{name}_codes").zero_()
         for again in (twin, other):
             assert torch.equal(again(x)[0], want[0]) and torch.equal(again.decode(x), want[1])
+
+
+def test_values_that_require_gradients():
+    """Parameters, transposed views of them too, go to 8 bits without a graph."""
+    p = torch.nn.Parameter(torch.randn(70, 130, device="cuda"))
+    for v in (p, p.t()):
+        w, (codes, scales) = int8_weight(v), int8_rows(v)
+        assert not (w.scale.requires_grad or scales.requires_grad)
+        plain = v.detach().clone()
+        assert torch.equal(w.codes, int8_weight(plain).codes)
+        assert torch.equal(codes, int8_rows(plain)[0])
