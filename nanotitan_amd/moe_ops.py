@@ -891,7 +891,7 @@ class Int8GroupedGEMM_FN(torch.autograd.Function):
     """
 
     @staticmethod
-    def forward(ctx, X, expert_offset, weight, exact):
+    def forward(ctx, X, expert_offset, weight, exact=True):
         ctx.save_for_backward(expert_offset, weight.codes, weight.scale)
         ctx.shape, ctx.exact = weight.shape, exact
         return get_hip_extension().int8_product(X, expert_offset, weight.codes, weight.scale)
@@ -912,7 +912,7 @@ class Int8SwiGLUFFN_FN(torch.autograd.Function):
     """
 
     @staticmethod
-    def forward(ctx, X, expert_offset, W_gate, W_val, W_out, exact):
+    def forward(ctx, X, expert_offset, W_gate, W_val, W_out, exact=True):
         weights = (W_gate, W_val, W_out)
         held = [t for w in weights for t in (w.codes, w.scale)]
         y, gate, value = get_hip_extension().int8_swiglu_ffn(X, expert_offset, *held, True)
@@ -936,7 +936,7 @@ class Int8GeluFFN_FN(torch.autograd.Function):
     """GELU FFN on frozen 8-bit weights, as Int8SwiGLUFFN_FN; keeps gelu' in float32."""
 
     @staticmethod
-    def forward(ctx, X, expert_offset, W_up, W_down, exact):
+    def forward(ctx, X, expert_offset, W_up, W_down, exact=True):
         held = [t for w in (W_up, W_down) for t in (w.codes, w.scale)]
         y, slope = get_hip_extension().int8_gelu_ffn(X, expert_offset, *held, True)
         ctx.save_for_backward(expert_offset, slope, *held)

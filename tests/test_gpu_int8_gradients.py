@@ -244,6 +244,14 @@ def test_rounded_weights_by_choice(dtype, size, direct, monkeypatch):
     assert torch.equal(a, b)
 
 
+def test_functions_without_the_choice_are_exact():
+    x, w, dout, off, gpu_off = _case(torch.bfloat16, "odd")
+    x.requires_grad_()
+    want, = torch.autograd.grad(int8_grouped_gemm_fn(x, w, gpu_off), x, dout)
+    got, = torch.autograd.grad(moe_ops.Int8GroupedGEMM_FN.apply(x, gpu_off, w), x, dout)
+    assert torch.equal(got, want)
+
+
 def test_the_module_takes_the_choice():
     cfg = SimpleNamespace(d_model=64, ffn_in=96, dtype=torch.bfloat16)
     with torch.device("cuda"):
