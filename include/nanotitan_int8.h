@@ -106,8 +106,8 @@ int nt_int8_linear_gelu(int dtype, const void* x, const int32_t* offsets, const 
  * r * dout_pitch, a multiple of 8 from N on; columns from N to the next multiple of 8
  * are read and must be finite. dout is 16-byte aligned.
  * f32, and f16 and bf16 with dout_pitch 0: dout stands for its terms (below) with the
- * weights' scales, which meet the integers themselves, so no weight is rounded; dout_pitch
- * and w_scales are not read otherwise. */
+ * weights' scales, which meet the integers themselves, so no weight is rounded; w_scales is
+ * not read then, nor dout_pitch of f32. */
 int nt_int8_grouped_gemm_dx(int dtype, const int8_t* w, const float* w_scales,
                             const int32_t* offsets, const void* dout, int64_t dout_pitch,
                             int32_t E, int64_t A, int64_t K, int64_t N, void* dx,
@@ -115,8 +115,9 @@ int nt_int8_grouped_gemm_dx(int dtype, const int8_t* w, const float* w_scales,
 
 /* Terms: a gradient [A, N] times the scales [E, N] of the weights that it will meet, as
  * sums of bfloat16 numbers: two, to 2^-17, where gradients are f16 or bf16, three, to
- * 2^-25, where they are f32. [terms][A][nt_int8_pitch(N)], 16-byte aligned, columns
- * from N on zero to the next multiple of 16 (the rest is not written, nor read).
+ * 2^-25, where they are f32 (a product with a scale below 2^-100: to fewer bits).
+ * [terms][A][nt_int8_pitch(N)], 16-byte aligned, columns from N on zero to the next
+ * multiple of 16 (the rest is not written, nor read).
  * nt_int8_terms_bytes is their size (0: too large). nt_int8_rows_terms makes them of rows
  * dout [A, N] of dtype, nt_int8_terms of float32 ones. */
 size_t nt_int8_terms_bytes(int dtype, int64_t A, int64_t N);

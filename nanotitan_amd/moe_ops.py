@@ -849,10 +849,11 @@ def _int8_direct(dout, experts, K):
     """Whether the kernels that read 8-bit weights give dout @ W^T; else the weights go to
     dout's dtype first and to the product of that.
 
-    16-bit gradients of weights rounded to 16 bits: where reading and writing the weights costs more than the products gain from
-    weights in 16 bits, at most 512 rows an expert and 2^25 weights or more (128 experts of 2,048 x
-    768, 14,312 rows: 88 us against 111 + 104; 8 of 4,096 x 14,336, 1,000 rows: 338 against 300 +
-    262, 8,192 rows: 1,331 against 301 + 1,022; 8 of 512 x 2,048, 4,096 rows: 54 against 9 + 28).
+    16-bit gradients of weights rounded to 16 bits: where reading and writing the weights costs
+    more than the products gain from weights in 16 bits, at most 512 rows an expert and 2^25
+    weights or more (128 experts of 2,048 x 768, 14,312 rows: 93 us against 241; 8 of 4,096 x
+    14,336, 1,000 rows: 286 against 486, 8,192 rows: 1,056 against 1,042; 1 of 1,024 x 4,096,
+    4,096 rows: 69 against 55).
     float32: where tiles of 128 rows by 256 columns would fill half of the chip (8 of 1,024 x
     2,730, 8,192 rows: 228 us against 286; 1 of 1,024 x 4,096, 4,096 rows: 183 against 243; below,
     8 of 1,024 x 4,096, 2,000 rows: 163 against 160; 7 of 300 x 1,365, 5,003 rows: 72 against 65).

@@ -96,6 +96,27 @@ def test_the_direct_product_takes_the_weights_as_decoded(dtype, A):
     assert torch.equal(got, want.repeat(-(-A // N), 1)[:A])
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+def test_gradients_as_small_as_the_terms_hold(dtype, monkeypatch):
+    """Products of gradient and scale of about 2^-100, each picked out by a row of one value."""
+    monkeypatch.setattr(moe_ops, "_int8_direct", lambda d, E, K: True)
+    t, K, N = TYPES[dtype], 100, 64
+    g = torch.Generator().manual_seed(1)
+    W = torch.randn(K, N, generator=g) * 2.0**-58  # scales of about 2^-64
+    w = int8_weight(W.cuda())
+    v = (torch.rand(N, generator=g) + 1.0) * 2.0**-36
+    dout = torch.diag(v.to(t)).cuda()
+    x = torch.zeros(N, K, dtype=t, device="cuda", requires_grad=True)
+    got, = torch.autograd.grad(int8_grouped_gemm_fn(x, w), x, dout)
+    held = int8_weight_decode(w, torch.float32)[0].double().t()
+    want = held * dout.double().sum(1, keepdim=True)
+    # the terms, and the roundings of dout s, of q s and of the sum; of bfloat16 the output's:
+    # 8 significant bits, so half of its last one is 2^-8 of the smallest value with that step
+    half = torch.finfo(t).eps / 2
+    rel = 2.0**-17 + half + 4 * U if t == torch.bfloat16 else 2.0**-25 + 6 * U
+    assert bool(((got.double() - want).abs() <= rel * want.abs()).all())
+
+
 # Rows an expert, and the widths: tiles of 128 columns, and of 256 with more than one a workgroup.
 SIZES = {"few": ([3, 0, 16, 1], 300, 265), "odd": ([200, 0, 3, 50], 77, 130),
          "tiles": ([128, 129, 0, 300], 130, 72), "many": ([900, 0, 2500, 2600], 3001, 90)}
