@@ -9,8 +9,8 @@
 // exact, so neither the split nor the batch shows in a result. HBM bounds it: 128 rows of
 // 8 experts, 4,096 to two times 14,336 (940 MB) 138 to 150 us, 6.3 to 6.8 TB/s where a
 // read alone reaches 7.1; one row, 4,096 to 14,336, 12 us. A batch that gathers at few
-// experts reads theirs again, from the caches (128 experts of 2,048 x 768, 3,072 rows:
-// 60 us, half of them at one expert 66, all 37; 8 of 4,096 x 14,336, 192 rows: 98, 99, 49).
+// experts reads theirs again, from the caches (128 experts of 2,048 x 768, 2,048 rows:
+// 51 us, half of them at one expert 56, all 28; 8 of 4,096 x 14,336, 192 rows: 98, 99, 49).
 //
 // A few short rows are brought to integers by every workgroup for itself, in LDS: a
 // launch that did it would take longer than all of the product.

@@ -17,7 +17,7 @@ def tile(product, E, A, K, N, cus=256):
 
 
 @pytest.mark.parametrize("product,E,A,K,N,want", [
-    (PLAIN, 8, 192, 4096, 14336, (0, 0)), (PLAIN, 128, 128 * 24, 2048, 768, (0, 0)),
+    (PLAIN, 8, 192, 4096, 14336, (0, 0)), (PLAIN, 64, 64 * 24, 2048, 768, (0, 0)),
     (PLAIN, 1, 64, 4096, 4096, (0, 0)), (PLAIN, 1, 400, 4096, 4096, (128, 128)),
     (PLAIN, 8, 61440, 2048, 512, (128, 256)), (PLAIN, 8, 4000, 4096, 4096, (128, 128)),
     (GELU, 128, 14312, 2048, 768, (128, 128)), (SWIGLU, 8, 61440, 512, 2048, (128, 256)),
